@@ -208,6 +208,86 @@ int32_t tl_qkv_append(tl_handle *h, int32_t seq, int32_t layer, int32_t pos0, in
  * logits may be NULL or a dev [V] buffer. */
 int32_t tl_lm_head_argmax(tl_handle *h, const float *x, int32_t *token, float *logit, float *logits);
 
+/* ---- serving operators ------------------------------------------------------- */
+
+/* A decoding step of many sequences over a paged KV cache.  No counterpart in
+ * the reference (its cache is one dense plane per sequence); the rotation, the
+ * INT8 cache and its scales follow tl_rope and tl_qkv_append.
+ *
+ * Each operator comes in two forms.  tl_x runs on the handle's stream and has
+ * completed when it returns.  tl_x_async queues its kernels on `stream` (a
+ * hipStream_t of the handle's device; NULL is its default stream) and returns:
+ * it allocates nothing, waits for nothing and can be captured into a HIP graph;
+ * the caller orders it with its own work there and keeps every buffer until it
+ * is done.  The arguments are checked in both forms as far as the host can see
+ * them; `stream`, `scratch` and `fault` are the async form's own.  What a call
+ * finds wrong on the device (a sequence, position, page or token id out of its
+ * range) is left out: nothing is read or written outside the buffers.  tl_x then
+ * returns TL_ERR_BAD_DESCRIPTOR after completing; tl_x_async sets *fault to 1
+ * (dev int32 or NULL; never cleared). */
+typedef enum tl_dtype { TL_F32 = 0, TL_BF16 = 1, TL_F16 = 2, TL_I8 = 3 } tl_dtype;
+
+/* A paged cache of one layer.  Position t of sequence s lies in page
+ * table[s * table_stride + t / page_size]; row t % page_size of KV head g in
+ * page p starts at element p * page_stride + (g * page_size + t % page_size) *
+ * head_dim of k and of v (both dev).  Table entries past a sequence's last
+ * position are never used.  Pages may be shared by sequences that only read
+ * them. */
+typedef struct tl_paged_cache {
+    void    *k, *v;             /* dev, 16-byte aligned */
+    const float *k_scale;       /* dev [n_kv_heads]: TL_I8 stands for k8 * k_scale; else NULL */
+    const float *v_scale;
+    const int32_t *table;       /* dev */
+    int64_t table_stride;       /* entries between sequences, >= max_pages */
+    int64_t page_stride;        /* elements, a multiple of 16 bytes; n_kv_heads * page_size * head_dim if dense */
+    int32_t dtype;              /* TL_I8, TL_BF16 or TL_F16 */
+    int32_t n_pages;
+    int32_t page_size;          /* positions: a power of two from 8 to 1024 */
+    int32_t n_kv_heads;
+    int32_t head_dim;           /* 64 or 128 */
+    int32_t n_seqs;
+    int32_t max_pages;          /* entries per sequence; max_pages * page_size <= 2^30 */
+} tl_paged_cache;
+
+/* Appends rows of Q|K|V projections [rows][(n_heads + 2 n_kv_heads) * head_dim]
+ * (dev, type act: TL_F32, TL_BF16 or TL_F16) to the cache: row r belongs to
+ * sequence row_seq[r] (row_seq NULL: r) at position row_pos[r]; q and k are
+ * rotated there with cos / sin [n_pos][head_dim] float32 (dev, TL:59-80), k and
+ * v are written to the cache (INT8: as tl_qkv_append does) and the rotated q to
+ * q_out (may be NULL, or qkv itself).  Steps are float32, each rounded; 16-bit
+ * results are rounded once.  Strides in elements; rows start 16-byte aligned.
+ * A negative row_seq is a padded row: it is skipped and its q_out left as it
+ * was.  Two rows of a call at one position of one sequence leave either row's
+ * values there. */
+int32_t tl_paged_append(tl_handle *h, const tl_paged_cache *cache, const void *qkv, int64_t qkv_stride, int32_t act,
+                        int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos,
+                        const float *cos, const float *sin, int32_t n_pos, void *q_out, int64_t q_stride);
+int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *cache, const void *qkv,
+                              int64_t qkv_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
+                              const int32_t *row_pos, const float *cos, const float *sin, int32_t n_pos, void *q_out,
+                              int64_t q_stride, int32_t *fault);
+
+/* Attention of one query row per token: row r of q [rows][n_heads * head_dim]
+ * (dev, type act) attends keys 0 .. row_pos[r] of sequence row_seq[r] (NULL: r),
+ * out[r] = softmax(scale q . k) . v in q's type; query head h reads KV head
+ * h / (n_heads / n_kv_heads).  Scores, probabilities and sums are float32 (not
+ * the INT8 probabilities of tl_attention).  A negative position has no keys: its
+ * row is zero.  A negative row_seq is a padded row, left as it was.  Keys of a
+ * page out of range are left out.  Several rows of one sequence at rising
+ * positions are causal attention.  Long rows are split over workgroups and
+ * joined; the parts pass through scratch (dev, 16-byte aligned, of
+ * tl_paged_attention_scratch bytes, one per call in flight; the handle's own in
+ * tl_paged_attention). */
+int32_t tl_paged_attention(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride, int32_t act,
+                           int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos, float scale,
+                           void *out, int64_t out_stride);
+int32_t tl_paged_attention_async(tl_handle *h, void *stream, const tl_paged_cache *cache, const void *q,
+                                 int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
+                                 const int32_t *row_pos, float scale, void *out, int64_t out_stride, void *scratch,
+                                 int64_t scratch_bytes, int32_t *fault);
+int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
+                                   int64_t *bytes);
+
 /* ---- composed path ---------------------------------------------------------- */
 
 /* Embedding rows for tokens [rows] (dev) into x [rows][D] (dev). */

@@ -58,6 +58,20 @@ class TlTimeline(C.Structure):
                 ("busy_us", C.c_double * 9), ("gap_us", C.c_double * 9), ("launches", C.c_int32 * 9)]
 
 
+# enum tl_dtype
+TL_F32, TL_BF16, TL_F16, TL_I8 = 0, 1, 2, 3
+
+
+class TlPagedCache(C.Structure):
+    """struct tl_paged_cache: one layer's paged KV cache."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("table", C.c_void_p),
+        ("table_stride", C.c_int64), ("page_stride", C.c_int64), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+        ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32),
+        ("max_pages", C.c_int32),
+    ]
+
+
 class TlError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{message} (status {status})")
@@ -74,6 +88,10 @@ _i64 = C.c_int64
 _i32p = C.POINTER(C.c_int32)
 _f32p = C.POINTER(C.c_float)
 _f64p = C.POINTER(C.c_double)
+_f32 = C.c_float
+_cachep = C.POINTER(TlPagedCache)
+_append = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64]
+_attend = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _i64]
 
 SIGNATURES = {
     "tl_create": (_i32, [C.POINTER(TlConfig), _i32, C.POINTER(_vp)]),
@@ -119,6 +137,11 @@ SIGNATURES = {
     "tl_generate": (_i32, [_vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _i32p, _i32p]),
     "tl_decode_batch": (_i32, [_vp, _i32, _vp, _vp, _i32, _vp]),
     "tl_capture_step": (_i32, [_vp, _i32, C.POINTER(TlCapture)]),
+    "tl_paged_append": (_i32, [_vp, *_append]),
+    "tl_paged_append_async": (_i32, [_vp, _vp, *_append, _vp]),
+    "tl_paged_attention": (_i32, [_vp, *_attend]),
+    "tl_paged_attention_async": (_i32, [_vp, _vp, *_attend, _vp, _i64, _vp]),
+    "tl_paged_attention_scratch": (_i32, [_vp, _cachep, _i32, _i32, C.POINTER(_i64)]),
     "tl_set_profiling": (_i32, [_vp, _i32]),
     "tl_get_profile": (_i32, [_vp, _i32, C.POINTER(C.c_int64), _f64p, _f64p]),
     "tl_decode_timeline": (_i32, [_vp, _i32, _i32, C.POINTER(TlTimeline)]),
@@ -180,6 +203,15 @@ def _fence(args) -> None:
             return
 
 
+def _current_device() -> int:
+    """The device a handle made now belongs to."""
+    try:
+        import torch
+    except ImportError:
+        return 0
+    return torch.cuda.current_device()
+
+
 def _addr(x) -> int | None:
     """Device or host address of a torch tensor, a NumPy array or an int."""
     if x is None:
@@ -206,6 +238,7 @@ class Runtime:
             raise (TlValueError if st == TL_ERR_BAD_DESCRIPTOR else TlError)(st, f"tl_create: {msg}")
         self.h = h
         self.max_seqs = max_seqs
+        self.device = _current_device()
 
     def close(self):
         if getattr(self, "h", None):

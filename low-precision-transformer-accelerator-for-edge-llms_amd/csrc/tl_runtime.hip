@@ -20,6 +20,7 @@
 
 #include "tl_int8.h"
 #include "tl_internal.h"
+#include "tl_serving.h"
 
 using namespace tl;
 
@@ -171,9 +172,15 @@ struct tl_handle {
     std::vector<int32_t> host_cursor;
     // pinned host words the device reads and writes: [0] the abort word the
     // token bookkeeping kernel checks every step, [1 + seq] the mirror of
-    // stopped[seq] it writes (1 EOS, 2 host abort)
+    // stopped[seq] it writes (1 EOS, 2 host abort), [1 + max_seqs] fault_host
     int32_t* ctl_host = nullptr;      // host view
     int32_t* ctl_dev = nullptr;       // device view of the same words
+    // the last of them: set by a serving operator's kernel that found something
+    // out of range (the operator's completing form clears and reads it)
+    int32_t* fault_host = nullptr;
+    int32_t* fault_dev = nullptr;
+    void* op_scratch = nullptr;       // scratch of the serving operators' completing forms, grown on demand
+    size_t op_scratch_cap = 0;        // bytes
     // pinned host words: argmax keys of the LM-head operator's workgroups,
     // written by the kernel, folded by the host
     unsigned long long* wg_keys_host = nullptr;   // host view, [vocab / 4]
@@ -1236,12 +1243,14 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
         // that the token bookkeeping kernel reads and writes every step
         void* hp = nullptr;
         void* dp = nullptr;
-        const size_t words = 1 + (size_t)max_seqs;
+        const size_t words = 2 + (size_t)max_seqs;
         if ((e = hipHostMalloc(&hp, sizeof(int32_t) * words, hipHostMallocMapped | hipHostMallocCoherent))) return bad(e);
         h->ctl_host = (int32_t*)hp;
         std::memset(hp, 0, sizeof(int32_t) * words);
         if ((e = hipHostGetDevicePointer(&dp, hp, 0))) return bad(e);
         h->ctl_dev = (int32_t*)dp;
+        h->fault_host = h->ctl_host + words - 1;
+        h->fault_dev = h->ctl_dev + words - 1;
         if ((e = hipHostMalloc(&hp, sizeof(unsigned long long) * (size_t)((c.vocab + 3) / 4),
                                hipHostMallocMapped | hipHostMallocCoherent)))
             return bad(e);
@@ -1278,6 +1287,7 @@ void tl_destroy(tl_handle* h) {
     for (void* p : h->allocs) (void)hipFree(p);
     for (auto e : h->watch_ev)
         if (e) (void)hipEventDestroy(e);
+    if (h->op_scratch) (void)hipFree(h->op_scratch);
     if (h->ctl_host) (void)hipHostFree(h->ctl_host);
     if (h->wg_keys_host) (void)hipHostFree(h->wg_keys_host);
     if (h->stream) (void)hipStreamDestroy(h->stream);
@@ -2258,6 +2268,231 @@ int32_t tl_decode_timeline(tl_handle* h, int32_t seq, int32_t n_steps, tl_timeli
         out->gap_us[k] *= inv;
         out->launches[k] = (int32_t)((out->launches[k] + done / 2) / std::max(done, 1));
     }
+    return TL_OK;
+}
+
+}  // extern "C"
+
+// ---- serving operators ----------------------------------------------------------
+
+namespace {
+
+// the handle's device for the length of a call: the serving operators take a
+// stream of it whatever device the calling thread is on
+struct OnDevice {
+    int was = -1;
+    hipError_t err = hipSuccess;
+    explicit OnDevice(int dev) {
+        int cur = 0;
+        if ((err = hipGetDevice(&cur)) != hipSuccess || cur == dev) return;
+        if ((err = hipSetDevice(dev)) == hipSuccess) was = cur;
+    }
+    ~OnDevice() {
+        if (was >= 0) (void)hipSetDevice(was);
+    }
+};
+
+// the completing form of a serving operator: launch(fault) on the handle's
+// stream, done on return; what the kernels left out is an error
+template <typename Launch>
+int32_t complete(tl_handle* h, int kclass, const char* what, Launch launch) {
+    *(volatile int32_t*)h->fault_host = 0;
+    {
+        Prof p(h, kclass, 0.0);
+        const int32_t r = check_launch(h, launch(), what);
+        if (r) return drained(h, r);
+    }
+    const int32_t r = finish(h);
+    if (r) return r;
+    if (*(volatile int32_t*)h->fault_host)
+        return fail(h, TL_ERR_BAD_DESCRIPTOR, std::string(what) + ": a sequence, position, page or token id is out of range");
+    return TL_OK;
+}
+
+// h->op_scratch of at least `bytes`.  Only completing calls use it, so no
+// queued work reads it when it is replaced.
+int32_t ensure_op_scratch(tl_handle* h, size_t bytes) {
+    if (bytes <= h->op_scratch_cap) return TL_OK;
+    if (h->op_scratch) {
+        (void)hipFree(h->op_scratch);
+        h->op_scratch = nullptr;
+        h->op_scratch_cap = 0;
+    }
+    TL_HIP(h, hipMalloc(&h->op_scratch, bytes));
+    h->op_scratch_cap = bytes;
+    return TL_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool act_type(int32_t t) { return t == TL_F32 || t == TL_BF16 || t == TL_F16; }
+int32_t type_size(int32_t t) { return t == TL_F32 ? 4 : t == TL_I8 ? 1 : 2; }
+
+// rows of `width` elements of type t: aligned starts, no overlap
+int32_t check_rows(tl_handle* h, const void* p, int64_t stride, int64_t width, int32_t t, const char* what) {
+    TL_REQ(h, aligned16(p), std::string(what) + " must be 16-byte aligned");
+    TL_REQ(h, stride >= width && stride * type_size(t) % 16 == 0,
+           std::string(what) + ": rows must not overlap and must start 16-byte aligned");
+    return TL_OK;
+}
+
+int32_t paged_cache_arg(tl_handle* h, const tl_paged_cache* c, PagedCache* out) {
+    TL_REQ(h, c && c->k && c->v && c->table, "null cache pointer");
+    TL_REQ(h, c->dtype == TL_I8 || c->dtype == TL_BF16 || c->dtype == TL_F16, "cache type must be INT8, bfloat16 or float16");
+    TL_REQ(h, c->dtype != TL_I8 || (c->k_scale && c->v_scale), "an INT8 cache needs k_scale and v_scale");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(h, TL_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return fail(h, TL_ERR_UNSUPPORTED, "page_size must be a power of two from 8 to 1024");
+    TL_REQ(h, c->n_pages >= 1 && c->n_kv_heads >= 1 && c->n_kv_heads <= 1024 && c->n_seqs >= 1 && c->max_pages >= 1,
+           "empty cache, or more than 1024 KV heads");
+    TL_REQ(h, (int64_t)c->max_pages * c->page_size <= (int64_t)1 << 30, "more than 2^30 positions per sequence");
+    TL_REQ(h, c->table_stride >= c->max_pages, "table_stride below max_pages");
+    TL_REQ(h, aligned16(c->k) && aligned16(c->v) && ((uintptr_t)c->table & 3) == 0, "the cache must be 16-byte aligned");
+    const int64_t page = (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
+    TL_REQ(h, c->page_stride >= page && c->page_stride * type_size(c->dtype) % 16 == 0,
+           "page_stride: pages must not overlap and must start 16-byte aligned");
+    TL_REQ(h, c->page_stride <= ((int64_t)1 << 60) / c->n_pages, "page_stride too large");
+    PagedCache o{};
+    o.g.table = c->table;
+    o.g.table_stride = c->table_stride;
+    o.g.page_stride = c->page_stride;
+    o.g.n_seqs = c->n_seqs;
+    o.g.max_pages = c->max_pages;
+    o.g.n_pages = c->n_pages;
+    o.g.page_shift = __builtin_ctz((unsigned)c->page_size);
+    o.g.n_kv = c->n_kv_heads;
+    o.g.head_dim = c->head_dim;
+    o.k = c->k;
+    o.v = c->v;
+    o.ks = c->k_scale;
+    o.vs = c->v_scale;
+    o.dtype = c->dtype;
+    *out = o;
+    return TL_OK;
+}
+
+// rows of an append or attention call
+int32_t check_paged_rows(tl_handle* h, int32_t act, int32_t rows, const int32_t* row_pos) {
+    TL_REQ(h, act_type(act), "activations must be float32, bfloat16 or float16");
+    TL_REQ(h, rows >= 0, "negative row count");
+    TL_REQ(h, row_pos || rows == 0, "null row_pos");
+    return TL_OK;
+}
+
+int32_t append_args(tl_handle* h, const tl_paged_cache* cache, const void* qkv, int64_t qkv_stride, int32_t act,
+                    int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, const float* cos,
+                    const float* sin, int32_t n_pos, void* q_out, int64_t q_stride, PagedAppendArgs* a) {
+    int32_t r = paged_cache_arg(h, cache, &a->c);
+    if (r || (r = check_paged_rows(h, act, rows, row_pos))) return r;
+    TL_REQ(h, n_heads >= 0 && n_heads <= 65536, "query head count out of range");
+    TL_REQ(h, cos && sin && n_pos >= 1 && aligned16(cos) && aligned16(sin), "RoPE tables missing or not 16-byte aligned");
+    TL_REQ(h, qkv || rows == 0, "null qkv");
+    const int64_t hd = cache->head_dim;
+    if ((r = check_rows(h, qkv, qkv_stride, (n_heads + 2 * (int64_t)cache->n_kv_heads) * hd, act, "qkv"))) return r;
+    if (q_out && (r = check_rows(h, q_out, q_stride, n_heads * hd, act, "q_out"))) return r;
+    TL_REQ(h, q_out != qkv || !q_out || q_stride == qkv_stride, "q_out on top of qkv needs the same stride");
+    a->qkv = qkv; a->qkv_stride = qkv_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
+    a->row_seq = row_seq; a->row_pos = row_pos; a->cos = cos; a->sin = sin; a->n_pos = n_pos;
+    a->q_out = q_out; a->q_stride = q_stride;
+    return TL_OK;
+}
+
+int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q, int64_t q_stride, int32_t act,
+                       int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, float scale,
+                       void* out, int64_t out_stride, PagedAttnArgs* a) {
+    int32_t r = paged_cache_arg(h, cache, &a->c);
+    if (r || (r = check_paged_rows(h, act, rows, row_pos))) return r;
+    TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
+           "query heads must be a multiple of the KV heads");
+    TL_REQ(h, (q && out) || rows == 0, "null q or out");
+    const int64_t width = (int64_t)n_heads * cache->head_dim;
+    if ((r = check_rows(h, q, q_stride, width, act, "q"))) return r;
+    if ((r = check_rows(h, out, out_stride, width, act, "out"))) return r;
+    a->q = q; a->q_stride = q_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
+    a->row_seq = row_seq; a->row_pos = row_pos; a->scale = scale; a->out = out; a->out_stride = out_stride;
+    a->splits = paged_attention_splits(a->c, rows, n_heads);
+    return TL_OK;
+}
+
+size_t attention_scratch_bytes(const PagedAttnArgs& a) {
+    return paged_attention_scratch(a.c, a.rows, a.n_heads, a.splits) * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t tl_paged_append(tl_handle* h, const tl_paged_cache* cache, const void* qkv, int64_t qkv_stride, int32_t act,
+                        int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos,
+                        const float* cos, const float* sin, int32_t n_pos, void* q_out, int64_t q_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAppendArgs a{};
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_out,
+                                  q_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.fault = h->fault_dev;
+    return complete(h, TL_K_OTHER, "tl_paged_append", [&] { return launch_paged_append(h->stream, a); });
+}
+
+int32_t tl_paged_append_async(tl_handle* h, void* stream, const tl_paged_cache* cache, const void* qkv,
+                              int64_t qkv_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t* row_seq,
+                              const int32_t* row_pos, const float* cos, const float* sin, int32_t n_pos, void* q_out,
+                              int64_t q_stride, int32_t* fault) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAppendArgs a{};
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_out,
+                                  q_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.fault = fault;
+    return check_launch(h, launch_paged_append((hipStream_t)stream, a), "tl_paged_append_async");
+}
+
+int32_t tl_paged_attention(tl_handle* h, const tl_paged_cache* cache, const void* q, int64_t q_stride, int32_t act,
+                           int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, float scale,
+                           void* out, int64_t out_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAttnArgs a{};
+    int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    if ((r = ensure_op_scratch(h, attention_scratch_bytes(a)))) return r;
+    a.scratch = (float*)h->op_scratch;
+    a.fault = h->fault_dev;
+    return complete(h, TL_K_ATTN, "tl_paged_attention", [&] { return launch_paged_attention(h->stream, a); });
+}
+
+int32_t tl_paged_attention_async(tl_handle* h, void* stream, const tl_paged_cache* cache, const void* q,
+                                 int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t* row_seq,
+                                 const int32_t* row_pos, float scale, void* out, int64_t out_stride, void* scratch,
+                                 int64_t scratch_bytes, int32_t* fault) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAttnArgs a{};
+    const int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
+    if (r) return r;
+    const size_t need = attention_scratch_bytes(a);
+    TL_REQ(h, need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= 0 && (size_t)scratch_bytes >= need),
+           "scratch missing, misaligned or smaller than tl_paged_attention_scratch says");
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.scratch = (float*)scratch;
+    a.fault = fault;
+    return check_launch(h, launch_paged_attention((hipStream_t)stream, a), "tl_paged_attention_async");
+}
+
+int32_t tl_paged_attention_scratch(tl_handle* h, const tl_paged_cache* cache, int32_t rows, int32_t n_heads,
+                                   int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedCache c;
+    const int32_t r = paged_cache_arg(h, cache, &c);
+    if (r) return r;
+    TL_REQ(h, bytes && rows >= 0, "bad scratch arguments");
+    TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
+           "query heads must be a multiple of the KV heads");
+    *bytes = (int64_t)(paged_attention_scratch(c, rows, n_heads, paged_attention_splits(c, rows, n_heads)) * sizeof(float));
     return TL_OK;
 }
 

@@ -1,0 +1,124 @@
+// tl_serving.h -- declarations of the serving operators (paged KV cache, 4-bit
+// projections, token log probabilities), shared by their kernels (tl_paged.hip,
+// tl_w4.hip, tl_score.hip) and the C++ runtime (tl_runtime.hip).  The index
+// arithmetic at the top is host code too: a CPU test compiles it by itself.
+#pragma once
+
+#include <stdint.h>
+
+#if defined(__HIPCC__)
+#define TL_HD __host__ __device__
+#else
+#define TL_HD
+#endif
+
+namespace tl {
+
+// The geometry of a paged cache: position t of sequence s lies in page
+// table[s][t / page_size], at row t % page_size of each KV head's block of that
+// page.  page_size is a power of two, at least 8.
+struct PagedGeom {
+    const int32_t* table;   // [n_seqs][table_stride]
+    int64_t table_stride;
+    int64_t page_stride;    // elements between pages
+    int32_t n_seqs, max_pages, n_pages;
+    int32_t page_shift;     // log2(page_size)
+    int32_t n_kv, head_dim;
+};
+
+// the page that holds position pos (0 <= pos < max_pages * page_size) of
+// sequence seq (0 <= seq < n_seqs), or -1 where the table's entry names none
+TL_HD inline int32_t paged_page(const PagedGeom& g, int32_t seq, int32_t pos) {
+    const int32_t p = g.table[(int64_t)seq * g.table_stride + (pos >> g.page_shift)];
+    return p >= 0 && p < g.n_pages ? p : -1;
+}
+
+// elements from the cache's base to row pos of KV head `head` in `page`: 64
+// bits, as a cache may hold more than 2^31 elements
+TL_HD inline int64_t paged_row(const PagedGeom& g, int32_t page, int32_t head, int32_t pos) {
+    const int32_t at = pos & ((1 << g.page_shift) - 1);
+    return (int64_t)page * g.page_stride + (((int64_t)head << g.page_shift) + at) * g.head_dim;
+}
+
+// What a row of an append or attention call names.  A row of a padded batch has
+// a negative sequence and is left alone; a row whose sequence or position lies
+// outside the cache is a fault and is left alone too.
+enum PagedRow : int { PAGED_ROW_OK = 0, PAGED_ROW_PADDING = 1, PAGED_ROW_FAULT = 2 };
+TL_HD inline PagedRow paged_row_kind(const PagedGeom& g, int32_t seq, int32_t pos) {
+    if (seq < 0) return PAGED_ROW_PADDING;
+    if (seq >= g.n_seqs) return PAGED_ROW_FAULT;
+    return pos < ((int64_t)g.max_pages << g.page_shift) ? PAGED_ROW_OK : PAGED_ROW_FAULT;
+}
+
+// The share of one row's keys 0 .. n - 1 that each of `splits` workgroups takes:
+// equal chunks of whole kPagedTile-key tiles, so that a short row uses few of
+// them (those whose chunk starts at or behind n do nothing).
+constexpr int32_t kPagedTile = 128;
+TL_HD inline int32_t paged_chunk(int32_t n, int32_t splits) {
+    const int32_t tiles = (int32_t)(((int64_t)n + kPagedTile - 1) / kPagedTile);
+    const int32_t per = (tiles + splits - 1) / splits;
+    return (per > 1 ? per : 1) * kPagedTile;
+}
+// ... and how many of them have keys
+TL_HD inline int32_t paged_active(int32_t n, int32_t splits) {
+    const int32_t c = paged_chunk(n, splits);
+    return (int32_t)(((int64_t)n + c - 1) / c);
+}
+
+}  // namespace tl
+
+#if defined(__HIPCC__)
+
+#include <hip/hip_runtime.h>
+
+namespace tl {
+
+enum DType : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2, DT_I8 = 3 };   // tl_dtype
+
+struct PagedCache {
+    PagedGeom g;
+    void* k;
+    void* v;
+    const float* ks;   // [n_kv] (DT_I8)
+    const float* vs;
+    int32_t dtype;
+};
+
+struct PagedAppendArgs {
+    PagedCache c;
+    const void* qkv;           // [rows][(n_heads + 2 n_kv) * head_dim], stride qkv_stride
+    int64_t qkv_stride;
+    int32_t act;               // DType of qkv and q_out
+    int32_t rows, n_heads;
+    const int32_t* row_seq;    // or null: row r is sequence r
+    const int32_t* row_pos;
+    const float* cos;          // [n_pos][head_dim]
+    const float* sin;
+    int32_t n_pos;
+    void* q_out;               // [rows][n_heads * head_dim], stride q_stride, or null
+    int64_t q_stride;
+    int32_t* fault;            // set to 1 where a row names no place in the cache, or null
+};
+hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a);
+
+struct PagedAttnArgs {
+    PagedCache c;
+    const void* q;             // [rows][n_heads * head_dim], stride q_stride
+    int64_t q_stride;
+    int32_t act;
+    int32_t rows, n_heads;
+    const int32_t* row_seq;
+    const int32_t* row_pos;
+    float scale;
+    void* out;                 // as q, stride out_stride
+    int64_t out_stride;
+    float* scratch;            // paged_attention_scratch() floats
+    int32_t splits;            // paged_attention_splits()
+    int32_t* fault;
+};
+int32_t paged_attention_splits(const PagedCache& c, int32_t rows, int32_t n_heads);
+size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, int32_t splits);   // floats
+hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
+
+}  // namespace tl
+#endif  // __HIPCC__

@@ -1,0 +1,207 @@
+"""Serving operators: a decoding step of many sequences over a paged KV cache.
+
+No counterpart in the reference, whose cache is one dense plane per sequence; the
+rotation and the INT8 cache follow its accelerator path (design_decisions A7/B2).
+
+Every call here queues its kernels on torch's current stream of the tensors'
+device and returns, as torch's own operations do (the ``_async`` entry points of
+include/tl_int8.h): results may be used by later work on that stream, and calls
+can be captured into a ``torch.cuda.CUDAGraph``.  Scratch memory comes from
+torch's allocator with each call, so calls on different streams and captured
+graphs share none.  Tensors are CUDA tensors of one device; float types are
+float32, bfloat16 and float16.
+
+What a call finds out of range on the device (a sequence, position, page or token
+id) it leaves out; ``check()`` tells.  Wrong types, shapes and layouts raise
+``TlValueError`` (a ``ValueError``) at once.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _native
+from ._native import Runtime, TlPagedCache, TlValueError
+
+_ACT = {torch.float32: _native.TL_F32, torch.bfloat16: _native.TL_BF16, torch.float16: _native.TL_F16}
+_CACHE = {torch.int8: _native.TL_I8, torch.bfloat16: _native.TL_BF16, torch.float16: _native.TL_F16}
+_HANDLES: dict[int, Runtime] = {}
+
+
+def _runtime(device: torch.device) -> Runtime:
+    """The operator handle of a device, made on first use."""
+    rt = _HANDLES.get(device.index)
+    if rt is None:
+        with torch.cuda.device(device):
+            rt = Runtime(dict(hidden=64, intermediate=64, n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, vocab=64,
+                              max_pos=64, rms_eps=1e-5, rope_theta=10000.0))
+        _HANDLES[device.index] = rt
+    return rt
+
+
+def _bad(message: str):
+    return TlValueError(_native.TL_ERR_BAD_DESCRIPTOR, message)
+
+
+def _rows(name: str, t, device, width: int | None = None, dtype=None) -> torch.Tensor:
+    """A matrix of float rows: elements of a row side by side, any row stride."""
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype not in _ACT or (dtype and t.dtype != dtype):
+        raise _bad(f"{name} must be a {dtype or 'float32, bfloat16 or float16'} tensor on {device}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (width is not None and t.shape[1] != width):
+        raise _bad(f"{name} must be [rows][{width or 'width'}] with adjacent elements")
+    return t
+
+
+def _ints(name: str, t, device, n: int) -> int:
+    """Address of n int32 values side by side."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1:
+        raise _bad(f"{name} must be a vector of int32 on {device}")
+    if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise _bad(f"{name} must hold one value for each of {n} rows")
+    return t.data_ptr()
+
+
+def _stride(t) -> int:
+    """Elements between rows (one row: any aligned stride will do)."""
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+
+
+class PagedCache:
+    """One layer's paged KV cache: pages [n_pages][n_kv_heads][page_size][head_dim] of
+    INT8 (with float32 scales per KV head), bfloat16 or float16, and the page table
+    [n_seqs][max_pages] int32.  The tensors stay the caller's: pages are handed out by
+    writing the table.  ``rope``: cos and sin [positions][head_dim] float32
+    (``build_rope_cache``), needed by ``append``.
+
+    Pages of 8 .. 1024 positions (a power of two), heads of 64 or 128.  Page blocks may lie
+    in a larger tensor (any stride of the first dimension that keeps 16-byte
+    alignment), the table in a wider one.
+    """
+
+    def __init__(self, k, v, table, k_scale=None, v_scale=None, rope=None, rt: Runtime | None = None):
+        if not isinstance(k, torch.Tensor) or not k.is_cuda or k.dtype not in _CACHE or k.dim() != 4:
+            raise _bad("k must be a CUDA tensor [n_pages][n_kv_heads][page_size][head_dim] of int8, bfloat16 or float16")
+        dev = k.device
+        n_pages, n_kv, page, hd = k.shape
+        for name, t in (("k", k), ("v", v)):
+            if not isinstance(t, torch.Tensor) or t.dtype != k.dtype or t.device != dev or t.shape != k.shape:
+                raise _bad("k and v must agree in type, shape and device")
+            if t.stride()[1:] != (page * hd, hd, 1) or (n_pages > 1 and t.stride(0) != k.stride(0)):
+                raise _bad(f"{name}: the blocks of a page must be dense, and k and v must have one page stride")
+        if not isinstance(table, torch.Tensor) or table.dtype != torch.int32 or table.device != dev or table.dim() != 2 \
+                or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise _bad(f"table must be [n_seqs][max_pages] int32 on {dev} with adjacent entries")
+        if (k.dtype == torch.int8) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
+            raise _bad("k_scale and v_scale go with an INT8 cache, and only with one")
+        for t in (k_scale, v_scale):
+            if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev
+                                  or t.shape != (n_kv,) or not t.is_contiguous()):
+                raise _bad(f"scales must be [n_kv_heads] float32 on {dev}")
+        if rope is not None:
+            for t in rope:
+                if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev or t.dim() != 2 \
+                        or t.shape[1] != hd or t.shape != rope[0].shape or not t.is_contiguous():
+                    raise _bad(f"rope must be cos and sin [positions][{hd}] float32 on {dev}")
+        self.rt = rt or _runtime(dev)
+        if self.rt.device != dev.index:
+            raise _bad("the handle belongs to another device")
+        self.k, self.v, self.table, self.k_scale, self.v_scale, self.rope = k, v, table, k_scale, v_scale, rope
+        self.device = dev
+        self.n_kv_heads, self.head_dim, self.n_seqs = n_kv, hd, table.shape[0]
+        self.fault = torch.zeros(1, dtype=torch.int32, device=dev)
+        ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        self.desc = TlPagedCache(
+            ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), ptr(table),
+            table.stride(0) if table.shape[0] > 1 else table.shape[1], k.stride(0) if n_pages > 1 else n_kv * page * hd,
+            _CACHE[k.dtype], n_pages, page, n_kv, hd, table.shape[0], table.shape[1])
+        self._desc = C.byref(self.desc)
+        self._scratch: dict[tuple[int, int], int] = {}
+        self._scratch_bytes(0, n_kv)   # the descriptor's own checks
+
+    def _scratch_bytes(self, rows: int, n_heads: int) -> int:
+        got = self._scratch.get((rows, n_heads))
+        if got is None:
+            n = C.c_int64()
+            self.rt.check(self.rt.lib.tl_paged_attention_scratch(self.rt.h, self._desc, rows, n_heads, C.byref(n)),
+                          "tl_paged_attention_scratch")
+            got = self._scratch[(rows, n_heads)] = n.value
+        return got
+
+    def _row_ids(self, row_seq, row_pos, rows: int):
+        if row_seq is None:
+            return None, _ints("row_pos", row_pos, self.device, rows)
+        return _ints("row_seq", row_seq, self.device, rows), _ints("row_pos", row_pos, self.device, rows)
+
+    def append(self, qkv, row_seq, row_pos, out=None):
+        """Rows of Q|K|V projections [rows][(n_heads + 2 n_kv_heads) * head_dim]: q and k rotated at
+        row_pos, k and v written to the cache at row_pos of sequence row_seq (None: row r
+        is sequence r; negative: a padded row, skipped).  Returns the rotated q (``out`` if
+        given; it may be the q part of qkv); a padded row of a new tensor is undefined."""
+        dev, hd = self.device, self.head_dim
+        _rows("qkv", qkv, dev)
+        if self.rope is None:
+            raise _bad("append needs the cache's rope tables")
+        rows, width = qkv.shape
+        n_heads = width // hd - 2 * self.n_kv_heads
+        if width % hd or n_heads < 0:
+            raise _bad("qkv must be [rows][(n_heads + 2 n_kv_heads) * head_dim]")
+        seq, pos = self._row_ids(row_seq, row_pos, rows)
+        if out is None:
+            out = torch.empty((rows, n_heads * hd), dtype=qkv.dtype, device=dev)
+        else:
+            _rows("out", out, dev, n_heads * hd, qkv.dtype)
+            if out.shape[0] != rows:
+                raise _bad("out must have a row for each of qkv's")
+        if rows == 0:
+            return out
+        cos, sin = self.rope
+        stride = _stride(qkv)
+        q_stride = stride if out.data_ptr() == qkv.data_ptr() and rows == 1 else _stride(out)
+        rt = self.rt
+        st = rt.lib.tl_paged_append_async(
+            rt.h, torch.cuda.current_stream(dev).cuda_stream, self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
+            rows, n_heads, seq, pos, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            out.data_ptr() if n_heads else None, q_stride, self.fault.data_ptr())
+        if st:
+            rt.check(st, "append")
+        return out
+
+    def attend(self, q, row_seq, row_pos, scale: float | None = None, out=None):
+        """Attention of one query row per token: row r of q [rows][n_heads * head_dim]
+        (rotated) over keys 0 .. row_pos[r] of sequence row_seq[r] (None: r); a
+        negative position gives zeros, a negative sequence leaves its row of ``out`` as it
+        was (undefined in a new tensor).  ``scale``: 1 / sqrt(head_dim) unless given."""
+        dev, hd = self.device, self.head_dim
+        _rows("q", q, dev)
+        rows, width = q.shape
+        n_heads = width // hd
+        if width % hd or n_heads == 0 or n_heads % self.n_kv_heads:
+            raise _bad("q must be [rows][n_heads * head_dim], n_heads a multiple of the KV heads")
+        seq, pos = self._row_ids(row_seq, row_pos, rows)
+        if out is None:
+            out = torch.empty((rows, width), dtype=q.dtype, device=dev)
+        else:
+            _rows("out", out, dev, width, q.dtype)
+            if out.shape[0] != rows:
+                raise _bad("out must have a row for each of q's")
+        if rows == 0:
+            return out
+        need = self._scratch_bytes(rows, n_heads)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rt = self.rt
+        st = rt.lib.tl_paged_attention_async(
+            rt.h, torch.cuda.current_stream(dev).cuda_stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows,
+            n_heads, seq, pos, 1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), _stride(out),
+            scratch.data_ptr() if need else None, need, self.fault.data_ptr())
+        if st:
+            rt.check(st, "attend")
+        return out
+
+    def check(self) -> None:
+        """Wait for the cache's calls on the current stream and raise if one of them met a
+        sequence, position or page out of range."""
+        if int(self.fault.item()):
+            self.fault.zero_()
+            raise _bad("a sequence, position or page is out of range")

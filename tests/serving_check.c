@@ -1,0 +1,149 @@
+/* Refusals and error paths of the serving operators, on the HIP runtime of
+ * host_paths_check.c (no GPU: kernels are counted, not run).  Every call that
+ * an argument rules out returns its status and a message, launches nothing and
+ * leaves the handle usable; a completing call whose launch fails returns an
+ * error with nothing left queued. */
+#define main host_paths_main
+#include "host_paths_check.c"
+#undef main
+
+static int checks, wrong;
+static tl_handle* H;
+
+static void expect(const char* what, int got, int want, long launches) {
+    checks++;
+    const int ok = got == want && ops == launches && (want == TL_OK || tl_last_error(H)[0]);
+    if (!ok) {
+        wrong++;
+        printf("%s: status %d, want %d; %ld launches, want %ld; \"%s\"\n", what, got, want, ops, launches, tl_last_error(H));
+    }
+    ops = 0;
+}
+
+enum { HD = 64, KV = 2, HEADS = 8, PAGE = 16, PAGES = 6, SEQS = 3, MAXP = 2 };
+static _Alignas(64) int8_t k_pages[PAGES * KV * PAGE * HD], v_pages[sizeof k_pages];
+static _Alignas(64) float ks[KV], vs[KV], qkv[4][(HEADS + 2 * KV) * HD], q[4][HEADS * HD], out[4][HEADS * HD];
+static _Alignas(64) float cs[64 * HD], sn[64 * HD];
+static int32_t table[SEQS * MAXP], seq[4], pos[4];
+
+static tl_paged_cache cache(void) {
+    const tl_paged_cache c = {k_pages, v_pages, ks, vs, table, MAXP, KV * PAGE * HD, TL_I8, PAGES, PAGE, KV, HD, SEQS, MAXP};
+    return c;
+}
+static int append(const tl_paged_cache* c) {
+    return tl_paged_append(H, c, qkv, (HEADS + 2 * KV) * HD, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, HEADS * HD);
+}
+static int attend(const tl_paged_cache* c) {
+    return tl_paged_attention(H, c, q, HEADS * HD, TL_F32, 4, HEADS, seq, pos, 0.125f, out, HEADS * HD);
+}
+static void both(const char* what, tl_paged_cache c, int want) {
+    expect(what, append(&c), want, 0);
+    expect(what, attend(&c), want, 0);
+}
+
+static void paged(void) {
+    tl_paged_cache c = cache();
+    const int64_t w = (HEADS + 2 * KV) * HD, qw = HEADS * HD;
+    int64_t need = -1;
+    expect("append", append(&c), TL_OK, 1);
+    expect("scratch", tl_paged_attention_scratch(H, &c, 4, HEADS, &need), TL_OK, 0);
+    expect("attention", attend(&c), TL_OK, need ? 2 : 1);
+    expect("no rows", tl_paged_append(H, &c, qkv, w, TL_F32, 0, HEADS, NULL, NULL, cs, sn, 64, q, qw), TL_OK, 0);
+    expect("no rows", tl_paged_attention(H, &c, q, qw, TL_F32, 0, HEADS, NULL, NULL, 1, out, qw), TL_OK, 0);
+    expect("no queries", tl_paged_append(H, &c, qkv, 2 * KV * HD, TL_F32, 4, 0, seq, pos, cs, sn, 64, NULL, 0), TL_OK, 1);
+    expect("in place", tl_paged_append(H, &c, qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, qkv, w), TL_OK, 1);
+#define WITH(what, change, want) do { tl_paged_cache x = cache(); change; both(what, x, want); } while (0)
+    WITH("null k", x.k = NULL, TL_ERR_BAD_DESCRIPTOR);
+    WITH("null table", x.table = NULL, TL_ERR_BAD_DESCRIPTOR);
+    WITH("no scales", x.k_scale = NULL, TL_ERR_BAD_DESCRIPTOR);
+    WITH("float32 cache", x.dtype = TL_F32, TL_ERR_BAD_DESCRIPTOR);
+    WITH("type", x.dtype = 9, TL_ERR_BAD_DESCRIPTOR);
+    WITH("head_dim", x.head_dim = 96, TL_ERR_UNSUPPORTED);
+    WITH("page 4", x.page_size = 4, TL_ERR_UNSUPPORTED);
+    WITH("page 24", x.page_size = 24, TL_ERR_UNSUPPORTED);
+    WITH("page 2048", x.page_size = 2048, TL_ERR_UNSUPPORTED);
+    WITH("page 0", x.page_size = 0, TL_ERR_UNSUPPORTED);
+    WITH("no pages", x.n_pages = 0, TL_ERR_BAD_DESCRIPTOR);
+    WITH("no KV heads", x.n_kv_heads = 0, TL_ERR_BAD_DESCRIPTOR);
+    WITH("no sequences", x.n_seqs = 0, TL_ERR_BAD_DESCRIPTOR);
+    WITH("no entries", x.max_pages = 0, TL_ERR_BAD_DESCRIPTOR);
+    WITH("too long", (x.max_pages = 1 << 27, x.table_stride = 1 << 27), TL_ERR_BAD_DESCRIPTOR);
+    WITH("table_stride", x.table_stride = MAXP - 1, TL_ERR_BAD_DESCRIPTOR);
+    WITH("misaligned k", x.k = k_pages + 8, TL_ERR_BAD_DESCRIPTOR);
+    WITH("misaligned v", x.v = v_pages + 1, TL_ERR_BAD_DESCRIPTOR);
+    WITH("short page_stride", x.page_stride -= 16, TL_ERR_BAD_DESCRIPTOR);
+    WITH("odd page_stride", x.page_stride += 8, TL_ERR_BAD_DESCRIPTOR);
+    WITH("huge page_stride", x.page_stride = (int64_t)1 << 60, TL_ERR_BAD_DESCRIPTOR);
+    expect("null cache", append(NULL), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("null cache", attend(NULL), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("null cache", tl_paged_attention_scratch(H, NULL, 4, HEADS, &need), TL_ERR_BAD_DESCRIPTOR, 0);
+#define APP(what, ...) expect("append: " what, tl_paged_append(H, &c, __VA_ARGS__), TL_ERR_BAD_DESCRIPTOR, 0)
+    APP("null qkv", NULL, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("int8 rows", qkv, w, TL_I8, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("negative rows", qkv, w, TL_F32, -1, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("negative heads", qkv, w, TL_F32, 4, -1, seq, pos, cs, sn, 64, q, qw);
+    APP("null pos", qkv, w, TL_F32, 4, HEADS, seq, NULL, cs, sn, 64, q, qw);
+    APP("null cos", qkv, w, TL_F32, 4, HEADS, seq, pos, NULL, sn, 64, q, qw);
+    APP("no table rows", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 0, q, qw);
+    APP("misaligned sin", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn + 1, 64, q, qw);
+    APP("overlapping rows", qkv, w - 4, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("odd stride", qkv, w + 1, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("odd 16-bit stride", qkv, w + 4, TL_F16, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("misaligned rows", &qkv[0][1], w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("misaligned q_out", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, &q[0][2], qw);
+    APP("short q_stride", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw - 4);
+    APP("in place, another stride", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, qkv, qw);
+#define ATT(what, ...) expect("attention: " what, tl_paged_attention(H, &c, __VA_ARGS__), TL_ERR_BAD_DESCRIPTOR, 0)
+    ATT("null q", NULL, qw, TL_F32, 4, HEADS, seq, pos, 1, out, qw);
+    ATT("null out", q, qw, TL_F32, 4, HEADS, seq, pos, 1, NULL, qw);
+    ATT("int8 rows", q, qw, TL_I8, 4, HEADS, seq, pos, 1, out, qw);
+    ATT("no heads", q, qw, TL_F32, 4, 0, seq, pos, 1, out, qw);
+    ATT("7 heads on 2", q, qw, TL_F32, 4, 7, seq, pos, 1, out, qw);
+    ATT("null pos", q, qw, TL_F32, 4, HEADS, seq, NULL, 1, out, qw);
+    ATT("negative rows", q, qw, TL_F32, -4, HEADS, seq, pos, 1, out, qw);
+    ATT("short stride", q, qw - 4, TL_F32, 4, HEADS, seq, pos, 1, out, qw);
+    ATT("misaligned out", q, qw, TL_F32, 4, HEADS, seq, pos, 1, &out[0][1], qw);
+    expect("scratch: null", tl_paged_attention_scratch(H, &c, 4, HEADS, NULL), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("scratch: heads", tl_paged_attention_scratch(H, &c, 4, 3, &need), TL_ERR_BAD_DESCRIPTOR, 0);
+
+    /* the form on the caller's stream: a long cache needs scratch */
+    tl_paged_cache l = cache();
+    static int32_t wide[SEQS * 512];
+    l.table = wide;
+    l.table_stride = l.max_pages = 512;
+    expect("long scratch", tl_paged_attention_scratch(H, &l, 1, HEADS, &need), TL_OK, 0);
+    checks++;
+    wrong += need <= 0;
+    void* s = aligned_alloc(64, (size_t)(need + 127) / 64 * 64);
+#define ASYNC(scr, n) tl_paged_attention_async(H, NULL, &l, q, qw, TL_F32, 1, HEADS, seq, pos, 1, out, qw, scr, n, NULL)
+    expect("async", ASYNC(s, need), TL_OK, 2);
+    expect("async, no scratch", ASYNC(NULL, need), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("async, short scratch", ASYNC(s, need - 1), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("async, misaligned scratch", ASYNC((char*)s + 4, need), TL_ERR_BAD_DESCRIPTOR, 0);
+    expect("async append", tl_paged_append_async(H, NULL, &c, qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw, NULL),
+           TL_OK, 1);
+    free(s);
+    queued = 0;   /* what the async calls queued */
+
+    /* a launch that fails */
+    for (long f = 1; f <= 2; f++) {
+        fail_at = f;
+        ops = 0;
+        const int r = tl_paged_attention(H, &l, q, qw, TL_F32, 1, HEADS, seq, pos, 1, out, qw);
+        fail_at = 0;
+        checks++;
+        wrong += r != TL_ERR_INTERNAL || queued != 0;
+        ops = 0;
+        expect("after a failed launch", tl_paged_attention(H, &l, q, qw, TL_F32, 1, HEADS, seq, pos, 1, out, qw), TL_OK, 2);
+    }
+    expect("null handle", tl_paged_attention_scratch(NULL, &c, 1, HEADS, &need), TL_ERR_BAD_DESCRIPTOR, 0);
+}
+
+int main(void) {
+    H = make(1024, 4);
+    ops = 0;
+    paged();
+    tl_destroy(H);
+    printf("%d checks, %d wrong\n", checks, wrong);
+    return wrong > 255 ? 255 : wrong;
+}

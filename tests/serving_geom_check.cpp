@@ -1,0 +1,70 @@
+// Index arithmetic of the paged cache (csrc/tl_serving.h) on the CPU: every table
+// lookup stays in the table, every row in its page and every page in the pool,
+// whatever the table holds; the chunks of a split row tile its keys.
+#include <cstdio>
+#include <cstdlib>
+#include <set>
+#include <vector>
+
+#include "tl_serving.h"
+
+using namespace tl;
+
+static int wrong;
+#define CHECK(c)                                              \
+    do {                                                      \
+        if (!(c)) {                                           \
+            wrong++;                                          \
+            if (wrong < 20) std::printf("line %d: %s\n", __LINE__, #c); \
+        }                                                     \
+    } while (0)
+
+int main() {
+    srand(1);
+    for (int shift = 3; shift <= 10; shift++) {
+        const int seqs = 3, max_pages = 5, n_pages = 7, n_kv = 3, hd = 64;
+        std::vector<int32_t> table(seqs * 9);
+        for (auto& e : table) e = rand() % 4 ? rand() % n_pages : (rand() % 2 ? -1 - rand() % 100 : n_pages + rand() % 1000);
+        table[4] = INT32_MIN;
+        table[5] = INT32_MAX;
+        PagedGeom g{table.data(), 9, (int64_t)n_kv * hd << shift, seqs, max_pages, n_pages, shift, n_kv, hd};
+        std::set<int64_t> seen;
+        for (int s = -2; s < seqs + 2; s++)
+            for (int64_t p = -2; p < ((int64_t)max_pages << shift) + 2; p++) {
+                const PagedRow k = paged_row_kind(g, s, (int32_t)p);
+                CHECK((k == PAGED_ROW_PADDING) == (s < 0));
+                CHECK((k == PAGED_ROW_FAULT) == (s >= seqs || (s >= 0 && p >= ((int64_t)max_pages << shift))));
+                if (k != PAGED_ROW_OK || p < 0) continue;
+                const int32_t e = table[s * 9 + (p >> shift)];
+                const int32_t page = paged_page(g, s, (int32_t)p);
+                CHECK(page == (e >= 0 && e < n_pages ? e : -1));
+                if (page < 0) continue;
+                for (int h = 0; h < n_kv; h++) {
+                    const int64_t at = paged_row(g, page, h, (int32_t)p);
+                    CHECK(at >= page * g.page_stride && at + hd <= (page + 1) * g.page_stride && at % hd == 0);
+                    CHECK(at == page * g.page_stride + ((int64_t)h * (1 << shift) + p % (1 << shift)) * hd);
+                }
+            }
+    }
+    // offsets past 2^31 elements and past 2^32 bytes
+    {
+        int32_t entry = 999999;
+        PagedGeom g{&entry, 1, (int64_t)8 * 1024 * 128, 1, 1, 1000000, 10, 8, 128};
+        CHECK(paged_page(g, 0, 1023) == 999999);
+        CHECK(paged_row(g, 999999, 7, 1023) == 999999ll * 1048576 + (7ll * 1024 + 1023) * 128);
+        CHECK(paged_row_kind(g, 0, INT32_MAX) == PAGED_ROW_FAULT);
+        g.max_pages = 1 << 20;
+        CHECK(paged_row_kind(g, 0, (1 << 30) - 1) == PAGED_ROW_OK && paged_row_kind(g, 0, 1 << 30) == PAGED_ROW_FAULT);
+    }
+    // chunks: whole tiles, all keys in exactly one chunk, no more chunks than splits
+    for (int splits : {1, 2, 3, 7, 32, 255, 256})
+        for (int64_t n : {1ll, 2ll, 127ll, 128ll, 129ll, 1000ll, 2047ll, 2048ll, 40000ll, 131071ll, 1ll << 30}) {
+            const int32_t c = paged_chunk((int32_t)n, splits), act = paged_active((int32_t)n, splits);
+            CHECK(c % kPagedTile == 0 && c > 0);
+            CHECK(act >= 1 && act <= splits);
+            CHECK((int64_t)(act - 1) * c < n && (int64_t)act * c >= n);
+        }
+    CHECK(paged_active(0, 5) == 0);
+    std::printf("%d wrong\n", wrong);
+    return wrong ? 1 : 0;
+}

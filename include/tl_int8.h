@@ -288,6 +288,48 @@ int32_t tl_paged_attention_async(tl_handle *h, void *stream, const tl_paged_cach
 int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
                                    int64_t *bytes);
 
+/* Projection of m rows with 4-bit weights: y[m][n] = residual[m][n] + sum_k
+ * x[m][k] w[n][k], w[n][k] = q s[n][k / group], q from -8 to 7, x, residual
+ * and y of type act (TL_F32, TL_BF16, TL_F16), residual may be NULL.  q [n][k / 2] bytes:
+ * column 2 j of a row is the low nibble of byte j, 2 j + 1 the high one, two's
+ * complement.  scales [n][k / group] of scale_dtype (a float type); group 32, 64
+ * or 128, k a multiple of it, at most 1024 groups.  All dev; strides in elements,
+ * x's rows and q 16-byte aligned.  A row of x is taken as integers of 2^-30 of
+ * its largest magnitude, products are exact, sums float32; an infinity or NaN in a
+ * row of x makes the whole row of y NaN.  Few rows (a decoding step) are what it is
+ * made for; any number is right.  scratch as in tl_paged_attention_async. */
+int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const uint8_t *q,
+                     const void *scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k,
+                     const void *residual, int64_t res_stride, void *y, int64_t y_stride);
+int32_t tl_linear_w4_async(tl_handle *h, void *stream, const void *x, int64_t x_stride, int32_t act, int32_t m,
+                           const uint8_t *q, const void *scales, int32_t scale_dtype, int32_t group, int32_t n,
+                           int32_t k, const void *residual, int64_t res_stride, void *y, int64_t y_stride,
+                           void *scratch, int64_t scratch_bytes);
+int32_t tl_linear_w4_scratch(tl_handle *h, int32_t m, int32_t n, int32_t k, int32_t group, int64_t *bytes);
+/* Offline quantizer for it, as tl_quantize_weight_rows: w [rows][n] float32 (finite), per group
+ * s = max|w| / 7 in float32, rounded to scale_dtype (1, and zero weights, where that is 0),
+ * q = clip(rne(w / s), -8, 7). */
+int32_t tl_quantize_w4_rows(tl_handle *h, const float *w, int32_t rows, int32_t n, int32_t group,
+                            int32_t scale_dtype, uint8_t *q, void *scales);
+
+/* Log probabilities from logits [rows][vocab] of type dtype (TL_F32, TL_BF16,
+ * TL_F16; any row stride, aligned as its type): logprob[r] = log softmax of row r
+ * at targets[r] (negative: none, 0; vocab or more: NaN and a fault), entropy[r] (may be
+ * NULL) = - sum p ln p in nats, and the `top` (0 .. 32, at most vocab) most probable ids in
+ * descending order, the lower id first among equal logits, with their log
+ * probabilities: top_ids, top_logprobs [rows][top].  Outputs int32 and float32, all dev.  A
+ * logit of minus infinity has probability 0.  A row without a finite maximum or with a
+ * NaN has no distribution: its log probabilities and entropy are NaN, NaN logits are
+ * no alternatives, and where too few are left the id is -1.  vocab at most 2^28. */
+int32_t tl_token_logprobs(tl_handle *h, const void *logits, int64_t stride, int32_t dtype, int32_t rows,
+                          int32_t vocab, const int32_t *targets, int32_t top, float *logprob, float *entropy,
+                          int32_t *top_ids, float *top_logprobs);
+int32_t tl_token_logprobs_async(tl_handle *h, void *stream, const void *logits, int64_t stride, int32_t dtype,
+                                int32_t rows, int32_t vocab, const int32_t *targets, int32_t top, float *logprob,
+                                float *entropy, int32_t *top_ids, float *top_logprobs, void *scratch,
+                                int64_t scratch_bytes, int32_t *fault);
+int32_t tl_token_logprobs_scratch(tl_handle *h, int32_t rows, int32_t vocab, int32_t top, int64_t *bytes);
+
 /* ---- composed path ---------------------------------------------------------- */
 
 /* Embedding rows for tokens [rows] (dev) into x [rows][D] (dev). */

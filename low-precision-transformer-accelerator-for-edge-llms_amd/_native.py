@@ -91,6 +91,8 @@ _f64p = C.POINTER(C.c_double)
 _f32 = C.c_float
 _cachep = C.POINTER(TlPagedCache)
 _append = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64]
+_w4 = [_vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64]
+_logprobs = [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]
 _attend = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _i64]
 
 SIGNATURES = {
@@ -142,6 +144,13 @@ SIGNATURES = {
     "tl_paged_attention": (_i32, [_vp, *_attend]),
     "tl_paged_attention_async": (_i32, [_vp, _vp, *_attend, _vp, _i64, _vp]),
     "tl_paged_attention_scratch": (_i32, [_vp, _cachep, _i32, _i32, C.POINTER(_i64)]),
+    "tl_linear_w4": (_i32, [_vp, *_w4]),
+    "tl_linear_w4_async": (_i32, [_vp, _vp, *_w4, _vp, _i64]),
+    "tl_linear_w4_scratch": (_i32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "tl_quantize_w4_rows": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "tl_token_logprobs": (_i32, [_vp, *_logprobs]),
+    "tl_token_logprobs_async": (_i32, [_vp, _vp, *_logprobs, _vp, _i64, _vp]),
+    "tl_token_logprobs_scratch": (_i32, [_vp, _i32, _i32, _i32, C.POINTER(_i64)]),
     "tl_set_profiling": (_i32, [_vp, _i32]),
     "tl_get_profile": (_i32, [_vp, _i32, C.POINTER(C.c_int64), _f64p, _f64p]),
     "tl_decode_timeline": (_i32, [_vp, _i32, _i32, C.POINTER(TlTimeline)]),

@@ -17,8 +17,9 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(OUT_DIR, "libtl_int8.so")
-SOURCES = ["tl_kernels.hip", "tl_decode.hip", "tl_gemm.hip", "tl_float.hip", "tl_paged.hip", "tl_runtime.hip"]
-HEADERS = ["tl_internal.h", "tl_device.h", "tl_serving.h", os.path.join(ROOT, "include", "tl_int8.h")]
+SOURCES = ["tl_kernels.hip", "tl_decode.hip", "tl_gemm.hip", "tl_float.hip", "tl_paged.hip", "tl_w4.hip", "tl_score.hip",
+           "tl_runtime.hip"]
+HEADERS = ["tl_internal.h", "tl_device.h", "tl_serving.h", "tl_rows.h", os.path.join(ROOT, "include", "tl_int8.h")]
 
 # -ffp-contract=off: float32 math rounds exactly where the source (and the
 # oracle) rounds.  The packed-fp32 target feature is switched off for the

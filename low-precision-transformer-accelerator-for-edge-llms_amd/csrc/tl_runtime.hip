@@ -1264,6 +1264,7 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
     if ((e = init_decode_kernels())) return bad(e);
     if ((e = init_gemm_pk_kernels())) return bad(e);
     if ((e = init_skinny_kernels())) return bad(e);
+    if ((e = init_w4_kernels())) return bad(e);
     if (const char* env = std::getenv("TL_BATCH_O_FUSE")) h->o_fuse = env[0] != '0';
     if (const char* env = std::getenv("TL_BATCH_KSLICE")) h->batch_kslice = env[0] != '0';
     if (const char* env = std::getenv("TL_BATCH_QKV_KSLICE")) h->qkv_kslice = env[0] != '0';
@@ -2327,6 +2328,12 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool act_type(int32_t t) { return t == TL_F32 || t == TL_BF16 || t == TL_F16; }
 int32_t type_size(int32_t t) { return t == TL_F32 ? 4 : t == TL_I8 ? 1 : 2; }
 
+int32_t check_scratch(tl_handle* h, const void* p, int64_t bytes, size_t need) {
+    TL_REQ(h, need == 0 || (p && aligned16(p) && bytes >= 0 && (size_t)bytes >= need),
+           "scratch missing, misaligned or smaller than the operator's _scratch call says");
+    return TL_OK;
+}
+
 // rows of `width` elements of type t: aligned starts, no overlap
 int32_t check_rows(tl_handle* h, const void* p, int64_t stride, int64_t width, int32_t t, const char* what) {
     TL_REQ(h, aligned16(p), std::string(what) + " must be 16-byte aligned");
@@ -2413,6 +2420,39 @@ int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q,
     return TL_OK;
 }
 
+int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const uint8_t* q,
+                const void* scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual,
+                int64_t res_stride, void* y, int64_t y_stride, W4Args* a) {
+    TL_REQ(h, act_type(act) && act_type(scale_dtype), "types must be float32, bfloat16 or float16");
+    TL_REQ(h, m >= 0 && n >= 1 && k >= 1, "empty projection");
+    if (!w4_supported(k, group))
+        return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
+    TL_REQ(h, q && scales && aligned16(q) && (uintptr_t)scales % type_size(scale_dtype) == 0, "weights missing or misaligned");
+    TL_REQ(h, (x && y) || m == 0, "null x or y");
+    const int32_t r = check_rows(h, x, x_stride, k, act, "x");
+    if (r) return r;
+    TL_REQ(h, y_stride >= n && (uintptr_t)y % type_size(act) == 0, "y: rows must not overlap and must be aligned");
+    TL_REQ(h, !residual || (res_stride >= n && (uintptr_t)residual % type_size(act) == 0),
+           "residual: rows must not overlap and must be aligned");
+    a->x = x; a->x_stride = x_stride; a->act = act; a->m = m; a->n = n; a->k = k; a->group = group;
+    a->q = q; a->scales = scales; a->scale_dtype = scale_dtype;
+    a->residual = residual; a->res_stride = res_stride; a->y = y; a->y_stride = y_stride;
+    return TL_OK;
+}
+
+int32_t logprobs_args(tl_handle* h, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
+                      const int32_t* targets, int32_t top, float* logprob, float* entropy, int32_t* top_ids,
+                      float* top_logprobs, LogprobsArgs* a) {
+    TL_REQ(h, act_type(dtype), "logits must be float32, bfloat16 or float16");
+    TL_REQ(h, rows >= 0 && vocab >= 1 && vocab <= 1 << 28, "row count or vocabulary out of range");
+    TL_REQ(h, top >= 0 && top <= kMaxTop && top <= vocab, "top must be 0 .. 32 and at most the vocabulary");
+    TL_REQ(h, rows == 0 || (logits && targets && logprob && (top == 0 || (top_ids && top_logprobs))), "null pointer");
+    TL_REQ(h, stride >= vocab && (uintptr_t)logits % type_size(dtype) == 0, "logits: rows must not overlap and must be aligned");
+    a->logits = logits; a->stride = stride; a->dtype = dtype; a->rows = rows; a->vocab = vocab; a->top = top;
+    a->targets = targets; a->logprob = logprob; a->entropy = entropy; a->top_ids = top_ids; a->top_logprobs = top_logprobs;
+    return TL_OK;
+}
+
 size_t attention_scratch_bytes(const PagedAttnArgs& a) {
     return paged_attention_scratch(a.c, a.rows, a.n_heads, a.splits) * sizeof(float);
 }
@@ -2473,9 +2513,8 @@ int32_t tl_paged_attention_async(tl_handle* h, void* stream, const tl_paged_cach
     PagedAttnArgs a{};
     const int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
     if (r) return r;
-    const size_t need = attention_scratch_bytes(a);
-    TL_REQ(h, need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= 0 && (size_t)scratch_bytes >= need),
-           "scratch missing, misaligned or smaller than tl_paged_attention_scratch says");
+    const int32_t bad = check_scratch(h, scratch, scratch_bytes, attention_scratch_bytes(a));
+    if (bad) return bad;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
     a.scratch = (float*)scratch;
@@ -2493,6 +2532,96 @@ int32_t tl_paged_attention_scratch(tl_handle* h, const tl_paged_cache* cache, in
     TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
            "query heads must be a multiple of the KV heads");
     *bytes = (int64_t)(paged_attention_scratch(c, rows, n_heads, paged_attention_splits(c, rows, n_heads)) * sizeof(float));
+    return TL_OK;
+}
+
+int32_t tl_linear_w4(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const uint8_t* q,
+                     const void* scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual,
+                     int64_t res_stride, void* y, int64_t y_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    W4Args a{};
+    int32_t r = w4_args(h, x, x_stride, act, m, q, scales, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    if ((r = ensure_op_scratch(h, w4_scratch(m, n, k, group)))) return r;
+    a.scratch = h->op_scratch;
+    return complete(h, TL_K_OTHER, "tl_linear_w4", [&] { return launch_linear_w4(h->stream, a); });
+}
+
+int32_t tl_linear_w4_async(tl_handle* h, void* stream, const void* x, int64_t x_stride, int32_t act, int32_t m,
+                           const uint8_t* q, const void* scales, int32_t scale_dtype, int32_t group, int32_t n,
+                           int32_t k, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
+                           void* scratch, int64_t scratch_bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    W4Args a{};
+    int32_t r = w4_args(h, x, x_stride, act, m, q, scales, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
+    if (r || (r = check_scratch(h, scratch, scratch_bytes, w4_scratch(m, n, k, group)))) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.scratch = scratch;
+    return check_launch(h, launch_linear_w4((hipStream_t)stream, a), "tl_linear_w4_async");
+}
+
+int32_t tl_linear_w4_scratch(tl_handle* h, int32_t m, int32_t n, int32_t k, int32_t group, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes && m >= 0 && n >= 1 && k >= 1, "bad scratch arguments");
+    if (!w4_supported(k, group))
+        return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
+    *bytes = (int64_t)w4_scratch(m, n, k, group);
+    return TL_OK;
+}
+
+int32_t tl_quantize_w4_rows(tl_handle* h, const float* w, int32_t rows, int32_t n, int32_t group, int32_t scale_dtype,
+                            uint8_t* q, void* scales) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, rows >= 0 && n >= 1, "empty weights");
+    TL_REQ(h, act_type(scale_dtype), "scales must be float32, bfloat16 or float16");
+    if (!w4_supported(n, group))
+        return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
+    TL_REQ(h, w && q && scales && aligned16(w) && ((uintptr_t)q & 3) == 0 && (uintptr_t)scales % type_size(scale_dtype) == 0,
+           "null or misaligned pointer");
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    return complete(h, TL_K_OTHER, "tl_quantize_w4_rows",
+                    [&] { return launch_quantize_w4(h->stream, w, rows, n, group, scale_dtype, q, scales); });
+}
+
+int32_t tl_token_logprobs(tl_handle* h, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
+                          const int32_t* targets, int32_t top, float* logprob, float* entropy, int32_t* top_ids,
+                          float* top_logprobs) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    LogprobsArgs a{};
+    int32_t r = logprobs_args(h, logits, stride, dtype, rows, vocab, targets, top, logprob, entropy, top_ids, top_logprobs, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    if ((r = ensure_op_scratch(h, logprobs_scratch(rows, vocab, top)))) return r;
+    a.scratch = h->op_scratch;
+    a.fault = h->fault_dev;
+    return complete(h, TL_K_OTHER, "tl_token_logprobs", [&] { return launch_token_logprobs(h->stream, a); });
+}
+
+int32_t tl_token_logprobs_async(tl_handle* h, void* stream, const void* logits, int64_t stride, int32_t dtype,
+                                int32_t rows, int32_t vocab, const int32_t* targets, int32_t top, float* logprob,
+                                float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
+                                int64_t scratch_bytes, int32_t* fault) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    LogprobsArgs a{};
+    int32_t r = logprobs_args(h, logits, stride, dtype, rows, vocab, targets, top, logprob, entropy, top_ids, top_logprobs, &a);
+    if (r || (r = check_scratch(h, scratch, scratch_bytes, logprobs_scratch(rows, vocab, top)))) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.scratch = scratch;
+    a.fault = fault;
+    return check_launch(h, launch_token_logprobs((hipStream_t)stream, a), "tl_token_logprobs_async");
+}
+
+int32_t tl_token_logprobs_scratch(tl_handle* h, int32_t rows, int32_t vocab, int32_t top, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes && rows >= 0 && vocab >= 1 && vocab <= 1 << 28, "bad scratch arguments");
+    TL_REQ(h, top >= 0 && top <= kMaxTop && top <= vocab, "top must be 0 .. 32 and at most the vocabulary");
+    *bytes = (int64_t)logprobs_scratch(rows, vocab, top);
     return TL_OK;
 }
 

@@ -120,5 +120,47 @@ int32_t paged_attention_splits(const PagedCache& c, int32_t rows, int32_t n_head
 size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, int32_t splits);   // floats
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
 
+// 4-bit weights: q [n][k / 2] bytes, column 2 j of a row in byte j's low nibble
+// and 2 j + 1 in its high one, each a two's complement number -8 .. 7; scales
+// [n][k / group] of scale_dtype
+struct W4Args {
+    const void* x;             // [m][k] of act, stride x_stride
+    int64_t x_stride;
+    int32_t act;
+    int32_t m, n, k, group;
+    const uint8_t* q;
+    const void* scales;
+    int32_t scale_dtype;
+    const void* residual;      // [m][n] of act, stride res_stride, or null
+    int64_t res_stride;
+    void* y;                   // [m][n] of act, stride y_stride
+    int64_t y_stride;
+    void* scratch;             // w4_scratch() bytes, 16-byte aligned
+};
+bool w4_supported(int32_t k, int32_t group);
+size_t w4_scratch(int32_t m, int32_t n, int32_t k, int32_t group);
+hipError_t launch_linear_w4(hipStream_t s, const W4Args& a);
+hipError_t launch_quantize_w4(hipStream_t s, const float* w, int32_t rows, int32_t k, int32_t group, int32_t scale_dtype,
+                              uint8_t* q, void* scales);
+hipError_t init_w4_kernels();
+
+// log probabilities, entropy and top alternatives of rows of logits
+struct LogprobsArgs {
+    const void* logits;        // [rows][vocab] of dtype, stride `stride`, any alignment of the type
+    int64_t stride;
+    int32_t dtype;
+    int32_t rows, vocab, top;
+    const int32_t* targets;    // [rows]; negative: none
+    float* logprob;            // [rows]
+    float* entropy;            // [rows] or null
+    int32_t* top_ids;          // [rows][top]
+    float* top_logprobs;       // [rows][top]
+    void* scratch;             // logprobs_scratch() bytes, 16-byte aligned
+    int32_t* fault;            // set to 1 by a target from vocab on, or null
+};
+constexpr int32_t kMaxTop = 32;
+size_t logprobs_scratch(int32_t rows, int32_t vocab, int32_t top);
+hipError_t launch_token_logprobs(hipStream_t s, const LogprobsArgs& a);
+
 }  // namespace tl
 #endif  // __HIPCC__

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -205,3 +206,127 @@ class PagedCache:
         if int(self.fault.item()):
             self.fault.zero_()
             raise _bad("a sequence, position or page is out of range")
+
+
+class W4Linear:
+    """A projection with 4-bit weights: y = x w^T (+ residual), w[n][k] = q[n][k] *
+    scales[n][k // group].  q [n][k / 2] uint8 holds two weights of -8 .. 7 (two's
+    complement) in a byte, the even column in the low nibble; scales [n][k / group] are
+    float32, bfloat16 or float16; group is 32, 64 or 128."""
+
+    def __init__(self, q, scales, rt: Runtime | None = None):
+        if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.uint8 or q.dim() != 2 or not q.is_contiguous():
+            raise _bad("q must be a contiguous CUDA tensor [n][k / 2] of uint8")
+        if not isinstance(scales, torch.Tensor) or scales.device != q.device or scales.dtype not in _ACT \
+                or scales.dim() != 2 or scales.shape[0] != q.shape[0] or not scales.is_contiguous():
+            raise _bad(f"scales must be contiguous [n][k / group] float32, bfloat16 or float16 on {q.device}")
+        self.device = q.device
+        self.n, self.k = q.shape[0], 2 * q.shape[1]
+        if scales.shape[1] == 0 or self.k % scales.shape[1]:
+            raise _bad("scales must hold one value for each group of a row")
+        self.group = self.k // scales.shape[1]
+        self.rt = rt or _runtime(q.device)
+        if self.rt.device != q.device.index:
+            raise _bad("the handle belongs to another device")
+        self.q, self.scales = q, scales
+        self._scratch: dict[int, int] = {}
+        self._scratch_bytes(1)   # the library's own checks of k and group
+
+    @classmethod
+    def from_float(cls, w, group: int = 128, scale_dtype=torch.float16, rt: Runtime | None = None) -> "W4Linear":
+        """Quantize float32 weights [n][k] (tl_quantize_w4_rows)."""
+        if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype != torch.float32 or w.dim() != 2:
+            raise _bad("w must be a CUDA tensor [n][k] of float32")
+        if scale_dtype not in _ACT:
+            raise _bad("scales are float32, bfloat16 or float16")
+        n, k = w.shape
+        if group not in (32, 64, 128) or k % group:
+            raise _bad("group must be 32, 64 or 128 and divide k")
+        rt = rt or _runtime(w.device)
+        w = w.contiguous()
+        q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+        scales = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
+        rt.call("tl_quantize_w4_rows", w, n, k, group, _ACT[scale_dtype], q, scales)
+        return cls(q, scales, rt)
+
+    def _scratch_bytes(self, rows: int) -> int:
+        got = self._scratch.get(rows)
+        if got is None:
+            n = C.c_int64()
+            self.rt.check(self.rt.lib.tl_linear_w4_scratch(self.rt.h, rows, self.n, self.k, self.group, C.byref(n)),
+                          "tl_linear_w4_scratch")
+            got = self._scratch[rows] = n.value
+        return got
+
+    def __call__(self, x, residual=None, out=None):
+        """x [rows][k] -> [rows][n] in x's type; ``out`` may be ``residual``."""
+        dev = self.device
+        _rows("x", x, dev, self.k)
+        rows = x.shape[0]
+        if out is None:
+            out = torch.empty((rows, self.n), dtype=x.dtype, device=dev)
+        else:
+            _rows("out", out, dev, self.n, x.dtype)
+        if residual is not None:
+            _rows("residual", residual, dev, self.n, x.dtype)
+        if out.shape[0] != rows or (residual is not None and residual.shape[0] != rows):
+            raise _bad("out and residual must have a row for each of x's")
+        if rows == 0:
+            return out
+        need = self._scratch_bytes(rows)
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rt = self.rt
+        st = rt.lib.tl_linear_w4_async(
+            rt.h, torch.cuda.current_stream(dev).cuda_stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows,
+            self.q.data_ptr(), self.scales.data_ptr(), _ACT[self.scales.dtype], self.group, self.n, self.k,
+            None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),
+            out.data_ptr(), _stride(out), scratch.data_ptr() if need else None, need)
+        if st:
+            rt.check(st, "W4Linear")
+        return out
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor        # [rows] float32
+    entropy: torch.Tensor        # [rows] float32, nats
+    top_ids: torch.Tensor        # [rows][top] int32
+    top_logprobs: torch.Tensor   # [rows][top] float32
+
+
+_LOGPROBS_SCRATCH: dict[tuple[int, int, int], int] = {}
+
+
+def token_logprobs(logits, targets, top: int = 0, rt: Runtime | None = None) -> TokenLogprobs:
+    """Of each row of logits [rows][vocab]: the log probability of targets[row] (int32; negative:
+    none, 0; an id past the vocabulary gives NaN), the entropy, and the ``top`` (up to 32)
+    most probable ids, the lower one first among equal logits."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise _bad("logits must be a CUDA tensor")
+    dev = logits.device
+    _rows("logits", logits, dev)
+    rows, vocab = logits.shape
+    ids = _ints("targets", targets, dev, rows)
+    if not 0 <= top <= min(32, vocab) or vocab == 0:
+        raise _bad("top must be 0 .. 32 and at most the vocabulary")
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    best = torch.empty((2, rows, top), dtype=torch.int32, device=dev)
+    got = TokenLogprobs(stats[0], stats[1], best[0], best[1].view(torch.float32))
+    if rows == 0:
+        return got
+    rt = rt or _runtime(dev)
+    if rt.device != dev.index:
+        raise _bad("the handle belongs to another device")
+    need = _LOGPROBS_SCRATCH.get((rows, vocab, top))
+    if need is None:
+        n = C.c_int64()
+        rt.check(rt.lib.tl_token_logprobs_scratch(rt.h, rows, vocab, top, C.byref(n)), "tl_token_logprobs_scratch")
+        need = _LOGPROBS_SCRATCH[(rows, vocab, top)] = n.value
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    at, ib = stats.data_ptr(), best.data_ptr()
+    st = rt.lib.tl_token_logprobs_async(
+        rt.h, torch.cuda.current_stream(dev).cuda_stream, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+        _ACT[logits.dtype], rows, vocab, ids, top, at, at + 4 * rows, ib, ib + 4 * rows * top,
+        scratch.data_ptr() if need else None, need, None)
+    if st:
+        rt.check(st, "token_logprobs")
+    return got

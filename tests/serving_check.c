@@ -139,10 +139,104 @@ static void paged(void) {
     expect("null handle", tl_paged_attention_scratch(NULL, &c, 1, HEADS, &need), TL_ERR_BAD_DESCRIPTOR, 0);
 }
 
+static void linear_w4(void) {
+    static _Alignas(64) uint8_t w[32 * 128];
+    static _Alignas(64) float x[4][256], y[4][32], r[4][32], sc[32 * 8], wf[32 * 256];
+    int64_t need;
+    expect("w4 scratch", tl_linear_w4_scratch(H, 4, 32, 256, 64, &need), TL_OK, 0);
+#define W4(xx, xs, act, m, q, s, st, grp, n, k, rr, rs, yy, ys) \
+    tl_linear_w4(H, xx, xs, act, m, q, s, st, grp, n, k, rr, rs, yy, ys)
+    const int bad = TL_ERR_BAD_DESCRIPTOR, uns = TL_ERR_UNSUPPORTED;
+    const int ok = W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, r, 32, y, 32);
+    checks++;
+    wrong += ok != TL_OK || ops < 1;
+    ops = 0;
+    expect("no rows", W4(x, 256, TL_F32, 0, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), TL_OK, 0);
+    expect("int8 rows", W4(x, 256, TL_I8, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("scale type", W4(x, 256, TL_F32, 4, w, sc, TL_I8, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("negative rows", W4(x, 256, TL_F32, -1, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("no columns", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 0, 256, NULL, 0, y, 32), bad, 0);
+    expect("k 0", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 0, NULL, 0, y, 32), bad, 0);
+    expect("k 200", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 200, NULL, 0, y, 32), uns, 0);
+    expect("group 16", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 16, 32, 256, NULL, 0, y, 32), uns, 0);
+    expect("group 0", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 0, 32, 256, NULL, 0, y, 32), uns, 0);
+    expect("many groups", W4(x, 65536, TL_F32, 4, w, sc, TL_F32, 32, 32, 65536, NULL, 0, y, 32), uns, 0);
+    expect("null q", W4(x, 256, TL_F32, 4, NULL, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("misaligned q", W4(x, 256, TL_F32, 4, w + 8, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("misaligned scales", W4(x, 256, TL_F32, 4, w, (char*)sc + 2, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("null x", W4(NULL, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("null y", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, NULL, 32), bad, 0);
+    expect("short x", W4(x, 252, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("odd x", W4(x, 257, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("misaligned x", W4(&x[0][1], 256, TL_F32, 3, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("short y", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 31), bad, 0);
+    expect("misaligned y", W4(x, 256, TL_F32, 3, w, sc, TL_F32, 64, 32, 256, NULL, 0, (char*)y + 2, 32), bad, 0);
+    expect("short residual", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, r, 31, y, 32), bad, 0);
+    expect("scratch null", tl_linear_w4_scratch(H, 4, 32, 256, 64, NULL), bad, 0);
+    expect("scratch group", tl_linear_w4_scratch(H, 4, 32, 256, 48, &need), uns, 0);
+    expect("quantize", tl_quantize_w4_rows(H, wf, 32, 256, 64, TL_F32, w, sc), TL_OK, 1);
+    expect("quantize no rows", tl_quantize_w4_rows(H, wf, 0, 256, 64, TL_F32, w, sc), TL_OK, 0);
+    expect("quantize null", tl_quantize_w4_rows(H, NULL, 32, 256, 64, TL_F32, w, sc), bad, 0);
+    expect("quantize group", tl_quantize_w4_rows(H, wf, 32, 256, 40, TL_F32, w, sc), uns, 0);
+    expect("quantize type", tl_quantize_w4_rows(H, wf, 32, 256, 64, TL_I8, w, sc), bad, 0);
+    expect("quantize misaligned", tl_quantize_w4_rows(H, wf + 1, 31, 256, 64, TL_F32, w, sc), bad, 0);
+    /* scratch of the form on the caller's stream, where the shape needs it */
+    static float big[40][256], out[40][32];
+    expect("w4 scratch", tl_linear_w4_scratch(H, 40, 32, 256, 32, &need), TL_OK, 0);
+    if (need > 0) {
+        expect("async, no scratch", tl_linear_w4_async(H, NULL, big, 256, TL_F32, 40, w, sc, TL_F32, 32, 32, 256, NULL, 0,
+                                                       out, 32, NULL, need), bad, 0);
+        expect("async, short scratch", tl_linear_w4_async(H, NULL, big, 256, TL_F32, 40, w, sc, TL_F32, 32, 32, 256, NULL, 0,
+                                                          out, 32, big, need - 1), bad, 0);
+    }
+}
+
+static void logprobs(void) {
+    static _Alignas(64) float x[2][20000], lp[2], h[2], tl[2][8];
+    static int32_t t[2], ids[2][8];
+    const int bad = TL_ERR_BAD_DESCRIPTOR;
+    int64_t need;
+#define LP(x, st, dt, rows, v, t, top, lp, h, ids, tl) tl_token_logprobs(H, x, st, dt, rows, v, t, top, lp, h, ids[0], tl[0])
+    expect("logprobs, one part", LP(x, 20000, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), TL_OK, 1);
+    expect("logprobs", LP(x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids, tl), TL_OK, 2);
+    expect("odd stride", LP((char*)x + 2, 19999, TL_F16, 2, 5000, t, 8, lp, h, ids, tl), TL_OK, 1);
+    expect("no rows", LP(x, 20000, TL_F32, 0, 20000, t, 8, lp, h, ids, tl), TL_OK, 0);
+    expect("no entropy", LP(x, 20000, TL_F32, 2, 5000, t, 8, lp, NULL, ids, tl), TL_OK, 1);
+    expect("no alternatives", tl_token_logprobs(H, x, 20000, TL_F32, 2, 5000, t, 0, lp, h, NULL, NULL), TL_OK, 1);
+    expect("null logits", LP(NULL, 20000, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("null targets", LP(x, 20000, TL_F32, 2, 5000, NULL, 8, lp, h, ids, tl), bad, 0);
+    expect("null logprob", LP(x, 20000, TL_F32, 2, 5000, t, 8, NULL, h, ids, tl), bad, 0);
+    expect("null ids", tl_token_logprobs(H, x, 20000, TL_F32, 2, 5000, t, 8, lp, h, NULL, tl[0]), bad, 0);
+    expect("int8 logits", LP(x, 20000, TL_I8, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("top 33", LP(x, 20000, TL_F32, 2, 5000, t, 33, lp, h, ids, tl), bad, 0);
+    expect("top -1", LP(x, 20000, TL_F32, 2, 5000, t, -1, lp, h, ids, tl), bad, 0);
+    expect("top above vocab", LP(x, 20000, TL_F32, 2, 7, t, 8, lp, h, ids, tl), bad, 0);
+    expect("vocab 0", LP(x, 20000, TL_F32, 2, 0, t, 0, lp, h, ids, tl), bad, 0);
+    expect("vocab above 2^28", LP(x, 1 << 30, TL_F32, 2, (1 << 28) + 1, t, 0, lp, h, ids, tl), bad, 0);
+    expect("overlapping rows", LP(x, 4999, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("misaligned", LP((char*)x + 2, 20000, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("negative rows", LP(x, 20000, TL_F32, -2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("scratch", tl_token_logprobs_scratch(H, 2, 20000, 8, &need), TL_OK, 0);
+    static char s[4096];
+    char* a = (char*)(((uintptr_t)s + 63) & ~(uintptr_t)63);
+    checks++;
+    wrong += need <= 0 || need > 2048;
+#define AS(scr, n) tl_token_logprobs_async(H, NULL, x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids[0], tl[0], scr, n, NULL)
+    expect("async", AS(a, need), TL_OK, 2);
+    expect("async, no scratch", AS(NULL, need), bad, 0);
+    expect("async, short scratch", AS(a, need - 1), bad, 0);
+    expect("async, misaligned scratch", AS(a + 8, need), bad, 0);
+    expect("scratch null", tl_token_logprobs_scratch(H, 2, 20000, 8, NULL), bad, 0);
+    expect("scratch top", tl_token_logprobs_scratch(H, 2, 20, 21, &need), bad, 0);
+    queued = 0;
+}
+
 int main(void) {
     H = make(1024, 4);
     ops = 0;
     paged();
+    linear_w4();
+    logprobs();
     tl_destroy(H);
     printf("%d checks, %d wrong\n", checks, wrong);
     return wrong > 255 ? 255 : wrong;

@@ -54,7 +54,7 @@ def test_paged_cache_layout_matches_header(tmp_path):
 
 
 @pytest.mark.skipif(_hipcc() is None, reason="hipcc is needed to compile the kernels")
-@pytest.mark.parametrize("src", ["tl_paged.hip"])
+@pytest.mark.parametrize("src", ["tl_paged.hip", "tl_w4.hip", "tl_score.hip"])
 def test_no_mfma_runs_under_a_narrowed_exec(src, tmp_path):
     hits = exposed_mfmas(_asm(os.path.join(CSRC, src), str(tmp_path)))
     assert hits == [], f"MFMAs under a narrowed EXEC with no skip in {src}: {hits[:10]}"

@@ -220,11 +220,22 @@ int32_t tl_lm_head_argmax(tl_handle *h, const float *x, int32_t *token, float *l
  * it allocates nothing, waits for nothing and can be captured into a HIP graph;
  * the caller orders it with its own work there and keeps every buffer until it
  * is done.  The arguments are checked in both forms as far as the host can see
- * them; `stream`, `scratch` and `fault` are the async form's own.  What a call
+ * them; `stream`, `scratch`, `counters` and `fault` are the async form's own.
+ *   scratch   dev, 16-byte aligned, of at least the bytes the operator's _scratch
+ *             call gives for the same sizes; its contents do not matter.  Calls
+ *             that may run at the same time need one each.
+ *   counters  dev, TL_OP_COUNTERS int32 that are zero when the kernels start, and
+ *             are zero again when they are done; one each for calls that may
+ *             run at the same time, graphs that hold them included.  With them
+ *             the parts of a result are joined by the workgroup that finishes
+ *             last, without them (NULL) by a second kernel, to the same bits.
+ *   fault     dev int32 or NULL.
+ * What a call
  * finds wrong on the device (a sequence, position, page or token id out of its
  * range) is left out: nothing is read or written outside the buffers.  tl_x then
  * returns TL_ERR_BAD_DESCRIPTOR after completing; tl_x_async sets *fault to 1
- * (dev int32 or NULL; never cleared). */
+ * (and never clears it). */
+#define TL_OP_COUNTERS 16384
 typedef enum tl_dtype { TL_F32 = 0, TL_BF16 = 1, TL_F16 = 2, TL_I8 = 3 } tl_dtype;
 
 /* A paged cache of one layer.  Position t of sequence s lies in page
@@ -274,17 +285,16 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
  * the INT8 probabilities of tl_attention).  A negative position has no keys: its
  * row is zero.  A negative row_seq is a padded row, left as it was.  Keys of a
  * page out of range are left out.  Several rows of one sequence at rising
- * positions are causal attention.  Long rows are split over workgroups and
- * joined; the parts pass through scratch (dev, 16-byte aligned, of
- * tl_paged_attention_scratch bytes, one per call in flight; the handle's own in
- * tl_paged_attention). */
+ * positions are causal attention.  The keys are shared out evenly over the GPU
+ * whatever the rows' lengths; the parts of a row that was split are joined, in the
+ * order of its keys. */
 int32_t tl_paged_attention(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride, int32_t act,
                            int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos, float scale,
                            void *out, int64_t out_stride);
 int32_t tl_paged_attention_async(tl_handle *h, void *stream, const tl_paged_cache *cache, const void *q,
                                  int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
                                  const int32_t *row_pos, float scale, void *out, int64_t out_stride, void *scratch,
-                                 int64_t scratch_bytes, int32_t *fault);
+                                 int64_t scratch_bytes, int32_t *counters, int32_t *fault);
 int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
                                    int64_t *bytes);
 
@@ -297,7 +307,7 @@ int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, in
  * x's rows and q 16-byte aligned.  A row of x is taken as integers of 2^-30 of
  * its largest magnitude, products are exact, sums float32; an infinity or NaN in a
  * row of x makes the whole row of y NaN.  Few rows (a decoding step) are what it is
- * made for; any number is right.  scratch as in tl_paged_attention_async. */
+ * made for; any number is right. */
 int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const uint8_t *q,
                      const void *scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k,
                      const void *residual, int64_t res_stride, void *y, int64_t y_stride);
@@ -327,7 +337,7 @@ int32_t tl_token_logprobs(tl_handle *h, const void *logits, int64_t stride, int3
 int32_t tl_token_logprobs_async(tl_handle *h, void *stream, const void *logits, int64_t stride, int32_t dtype,
                                 int32_t rows, int32_t vocab, const int32_t *targets, int32_t top, float *logprob,
                                 float *entropy, int32_t *top_ids, float *top_logprobs, void *scratch,
-                                int64_t scratch_bytes, int32_t *fault);
+                                int64_t scratch_bytes, int32_t *counters, int32_t *fault);
 int32_t tl_token_logprobs_scratch(tl_handle *h, int32_t rows, int32_t vocab, int32_t top, int64_t *bytes);
 
 /* ---- composed path ---------------------------------------------------------- */

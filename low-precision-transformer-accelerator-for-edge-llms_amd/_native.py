@@ -60,6 +60,7 @@ class TlTimeline(C.Structure):
 
 # enum tl_dtype
 TL_F32, TL_BF16, TL_F16, TL_I8 = 0, 1, 2, 3
+TL_OP_COUNTERS = 16384
 
 
 class TlPagedCache(C.Structure):
@@ -142,14 +143,14 @@ SIGNATURES = {
     "tl_paged_append": (_i32, [_vp, *_append]),
     "tl_paged_append_async": (_i32, [_vp, _vp, *_append, _vp]),
     "tl_paged_attention": (_i32, [_vp, *_attend]),
-    "tl_paged_attention_async": (_i32, [_vp, _vp, *_attend, _vp, _i64, _vp]),
+    "tl_paged_attention_async": (_i32, [_vp, _vp, *_attend, _vp, _i64, _vp, _vp]),
     "tl_paged_attention_scratch": (_i32, [_vp, _cachep, _i32, _i32, C.POINTER(_i64)]),
     "tl_linear_w4": (_i32, [_vp, *_w4]),
     "tl_linear_w4_async": (_i32, [_vp, _vp, *_w4, _vp, _i64]),
     "tl_linear_w4_scratch": (_i32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_i64)]),
     "tl_quantize_w4_rows": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "tl_token_logprobs": (_i32, [_vp, *_logprobs]),
-    "tl_token_logprobs_async": (_i32, [_vp, _vp, *_logprobs, _vp, _i64, _vp]),
+    "tl_token_logprobs_async": (_i32, [_vp, _vp, *_logprobs, _vp, _i64, _vp, _vp]),
     "tl_token_logprobs_scratch": (_i32, [_vp, _i32, _i32, _i32, C.POINTER(_i64)]),
     "tl_set_profiling": (_i32, [_vp, _i32]),
     "tl_get_profile": (_i32, [_vp, _i32, C.POINTER(C.c_int64), _f64p, _f64p]),

@@ -179,6 +179,7 @@ struct tl_handle {
     // out of range (the operator's completing form clears and reads it)
     int32_t* fault_host = nullptr;
     int32_t* fault_dev = nullptr;
+    int32_t* op_counters = nullptr;   // [kOpCounters], zero between the serving operators' calls
     void* op_scratch = nullptr;       // scratch of the serving operators' completing forms, grown on demand
     size_t op_scratch_cap = 0;        // bytes
     // pinned host words: argmax keys of the LM-head operator's workgroups,
@@ -1197,7 +1198,7 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
         (e = dalloc(h, &h->stopped, (size_t)max_seqs)) ||
         (e = dalloc(h, &h->racc, h->racc_cap = (size_t)std::min(32, h->max_rows) * D)) ||
         (e = dalloc(h, &h->qacc, h->qacc_cap = (size_t)std::min(32, max_seqs) * h->QKV)) ||
-        (e = dalloc(h, &h->pf_sink, 1)) ||
+        (e = dalloc(h, &h->pf_sink, 1)) || (e = dalloc(h, &h->op_counters, (size_t)kOpCounters)) ||
         (e = dalloc(h, &h->qmax, (size_t)kQmaxStride * R)) ||
         (e = dalloc(h, &h->tokens_out, (size_t)max_seqs * c.max_pos)) ||
         (e = dalloc(h, &h->logit_out, (size_t)max_seqs * c.max_pos)) ||
@@ -1223,6 +1224,7 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
         (e = hipMemsetAsync(h->eos_id, 0xFF, sizeof(int32_t) * max_seqs, h->stream)) ||
         (e = hipMemsetAsync(h->stopped, 0, sizeof(int32_t) * max_seqs, h->stream)) ||
         (e = hipMemsetAsync(h->tile_ctr, 0, sizeof(unsigned) * kSkinnyTiles, h->stream)) ||
+        (e = hipMemsetAsync(h->op_counters, 0, sizeof(int32_t) * kOpCounters, h->stream)) ||
         (e = hipMemsetAsync(h->racc, 0, sizeof(int32_t) * h->racc_cap, h->stream)) ||
         (e = hipMemsetAsync(h->qacc, 0, sizeof(int32_t) * h->qacc_cap, h->stream)) ||
         (e = hipMemsetAsync(h->qmax, 0, sizeof(unsigned) * kQmaxStride * R, h->stream)))
@@ -2357,7 +2359,7 @@ int32_t paged_cache_arg(tl_handle* h, const tl_paged_cache* c, PagedCache* out) 
     const int64_t page = (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
     TL_REQ(h, c->page_stride >= page && c->page_stride * type_size(c->dtype) % 16 == 0,
            "page_stride: pages must not overlap and must start 16-byte aligned");
-    TL_REQ(h, c->page_stride <= ((int64_t)1 << 60) / c->n_pages, "page_stride too large");
+    TL_REQ(h, c->page_stride * type_size(c->dtype) < (int64_t)1 << 32, "pages of 4 GiB or more");
     PagedCache o{};
     o.g.table = c->table;
     o.g.table_stride = c->table_stride;
@@ -2411,12 +2413,13 @@ int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q,
     TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
            "query heads must be a multiple of the KV heads");
     TL_REQ(h, (q && out) || rows == 0, "null q or out");
+    if (!paged_countable(a->c.g, rows, (n_heads / cache->n_kv_heads + 7) / 8 * cache->n_kv_heads))
+        return fail(h, TL_ERR_UNSUPPORTED, "2^31 or more tiles of 128 keys over all rows and KV heads, as long as the table allows");
     const int64_t width = (int64_t)n_heads * cache->head_dim;
     if ((r = check_rows(h, q, q_stride, width, act, "q"))) return r;
     if ((r = check_rows(h, out, out_stride, width, act, "out"))) return r;
     a->q = q; a->q_stride = q_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
     a->row_seq = row_seq; a->row_pos = row_pos; a->scale = scale; a->out = out; a->out_stride = out_stride;
-    a->splits = paged_attention_splits(a->c, rows, n_heads);
     return TL_OK;
 }
 
@@ -2454,7 +2457,7 @@ int32_t logprobs_args(tl_handle* h, const void* logits, int64_t stride, int32_t 
 }
 
 size_t attention_scratch_bytes(const PagedAttnArgs& a) {
-    return paged_attention_scratch(a.c, a.rows, a.n_heads, a.splits) * sizeof(float);
+    return a.rows > 0 ? paged_attention_scratch(a.c, a.rows, a.n_heads) : 0;
 }
 
 }  // namespace
@@ -2501,6 +2504,7 @@ int32_t tl_paged_attention(tl_handle* h, const tl_paged_cache* cache, const void
     TL_HIP(h, on.err);
     if ((r = ensure_op_scratch(h, attention_scratch_bytes(a)))) return r;
     a.scratch = (float*)h->op_scratch;
+    a.counters = h->op_counters;
     a.fault = h->fault_dev;
     return complete(h, TL_K_ATTN, "tl_paged_attention", [&] { return launch_paged_attention(h->stream, a); });
 }
@@ -2508,7 +2512,7 @@ int32_t tl_paged_attention(tl_handle* h, const tl_paged_cache* cache, const void
 int32_t tl_paged_attention_async(tl_handle* h, void* stream, const tl_paged_cache* cache, const void* q,
                                  int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t* row_seq,
                                  const int32_t* row_pos, float scale, void* out, int64_t out_stride, void* scratch,
-                                 int64_t scratch_bytes, int32_t* fault) {
+                                 int64_t scratch_bytes, int32_t* counters, int32_t* fault) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     PagedAttnArgs a{};
     const int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
@@ -2518,6 +2522,7 @@ int32_t tl_paged_attention_async(tl_handle* h, void* stream, const tl_paged_cach
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
     a.scratch = (float*)scratch;
+    a.counters = counters;
     a.fault = fault;
     return check_launch(h, launch_paged_attention((hipStream_t)stream, a), "tl_paged_attention_async");
 }
@@ -2531,7 +2536,7 @@ int32_t tl_paged_attention_scratch(tl_handle* h, const tl_paged_cache* cache, in
     TL_REQ(h, bytes && rows >= 0, "bad scratch arguments");
     TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
            "query heads must be a multiple of the KV heads");
-    *bytes = (int64_t)(paged_attention_scratch(c, rows, n_heads, paged_attention_splits(c, rows, n_heads)) * sizeof(float));
+    *bytes = rows > 0 ? (int64_t)paged_attention_scratch(c, rows, n_heads) : 0;
     return TL_OK;
 }
 
@@ -2598,6 +2603,7 @@ int32_t tl_token_logprobs(tl_handle* h, const void* logits, int64_t stride, int3
     TL_HIP(h, on.err);
     if ((r = ensure_op_scratch(h, logprobs_scratch(rows, vocab, top)))) return r;
     a.scratch = h->op_scratch;
+    a.counters = h->op_counters;
     a.fault = h->fault_dev;
     return complete(h, TL_K_OTHER, "tl_token_logprobs", [&] { return launch_token_logprobs(h->stream, a); });
 }
@@ -2605,7 +2611,7 @@ int32_t tl_token_logprobs(tl_handle* h, const void* logits, int64_t stride, int3
 int32_t tl_token_logprobs_async(tl_handle* h, void* stream, const void* logits, int64_t stride, int32_t dtype,
                                 int32_t rows, int32_t vocab, const int32_t* targets, int32_t top, float* logprob,
                                 float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch,
-                                int64_t scratch_bytes, int32_t* fault) {
+                                int64_t scratch_bytes, int32_t* counters, int32_t* fault) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     LogprobsArgs a{};
     int32_t r = logprobs_args(h, logits, stride, dtype, rows, vocab, targets, top, logprob, entropy, top_ids, top_logprobs, &a);
@@ -2613,6 +2619,7 @@ int32_t tl_token_logprobs_async(tl_handle* h, void* stream, const void* logits, 
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
     a.scratch = scratch;
+    a.counters = counters;
     a.fault = fault;
     return check_launch(h, launch_token_logprobs((hipStream_t)stream, a), "tl_token_logprobs_async");
 }

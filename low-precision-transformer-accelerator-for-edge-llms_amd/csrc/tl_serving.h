@@ -50,19 +50,37 @@ TL_HD inline PagedRow paged_row_kind(const PagedGeom& g, int32_t seq, int32_t po
     return pos < ((int64_t)g.max_pages << g.page_shift) ? PAGED_ROW_OK : PAGED_ROW_FAULT;
 }
 
-// The share of one row's keys 0 .. n - 1 that each of `splits` workgroups takes:
-// equal chunks of whole kPagedTile-key tiles, so that a short row uses few of
-// them (those whose chunk starts at or behind n do nothing).
+// Attention shares out tiles of kPagedTile keys.  Row r has paged_tiles(n) of them
+// for each of its head blocks (a row without keys one, for its zeros); all tiles
+// of a call, in the order row, head block, key, are dealt to the workgroups in
+// runs that differ in length by at most one, whatever the rows' lengths are.
 constexpr int32_t kPagedTile = 128;
-TL_HD inline int32_t paged_chunk(int32_t n, int32_t splits) {
-    const int32_t tiles = (int32_t)(((int64_t)n + kPagedTile - 1) / kPagedTile);
-    const int32_t per = (tiles + splits - 1) / splits;
-    return (per > 1 ? per : 1) * kPagedTile;
+TL_HD inline int32_t paged_tiles(int32_t n) { return n > 0 ? (int32_t)(((int64_t)n + kPagedTile - 1) / kPagedTile) : 1; }
+
+struct PagedShare {
+    int32_t per;   // tiles of every workgroup
+    int32_t rem;   // the first rem have one more
+    TL_HD int32_t start(int32_t w) const { return w * per + (w < rem ? w : rem); }
+    TL_HD int32_t owner(int32_t tile) const {
+        const int32_t longer = rem * (per + 1);
+        return tile < longer ? (int32_t)((uint32_t)tile / (uint32_t)(per + 1))
+                             : rem + (int32_t)((uint32_t)(tile - longer) / (uint32_t)per);
+    }
+};
+TL_HD inline PagedShare paged_share(int32_t tiles, int32_t workgroups) {
+    const int32_t per = (int32_t)((uint32_t)tiles / (uint32_t)workgroups);
+    return PagedShare{per, tiles - per * workgroups};
 }
-// ... and how many of them have keys
-TL_HD inline int32_t paged_active(int32_t n, int32_t splits) {
-    const int32_t c = paged_chunk(n, splits);
-    return (int32_t)(((int64_t)n + c - 1) / c);
+// A workgroup leaves at most two parts of rows that others share with it: one at
+// the start of its run (0) and one at the end (1).
+TL_HD inline int32_t paged_part(const PagedShare& s, int32_t w, int32_t unit_start) {
+    return 2 * w + (unit_start > s.start(w) ? 1 : 0);
+}
+// whether a call's tiles can be counted in 31 bits, were every row as long as the
+// table allows
+inline bool paged_countable(const PagedGeom& g, int32_t rows, int32_t head_blocks) {
+    const int64_t most = paged_tiles((int32_t)((int64_t)g.max_pages << g.page_shift));
+    return most * head_blocks <= INT32_MAX / (rows > 0 ? rows : 1);
 }
 
 }  // namespace tl
@@ -112,12 +130,13 @@ struct PagedAttnArgs {
     float scale;
     void* out;                 // as q, stride out_stride
     int64_t out_stride;
-    float* scratch;            // paged_attention_scratch() floats
-    int32_t splits;            // paged_attention_splits()
+    float* scratch;            // paged_attention_scratch() bytes
+    int32_t* counters;         // kOpCounters zeros, left zero, or null: parts are joined by a second kernel
     int32_t* fault;
 };
-int32_t paged_attention_splits(const PagedCache& c, int32_t rows, int32_t n_heads);
-size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, int32_t splits);   // floats
+constexpr int32_t kOpCounters = 16384;
+int32_t paged_attention_workgroups(const PagedCache& c, int32_t rows, int32_t n_heads);
+size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads);
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
 
 // 4-bit weights: q [n][k / 2] bytes, column 2 j of a row in byte j's low nibble
@@ -156,6 +175,7 @@ struct LogprobsArgs {
     int32_t* top_ids;          // [rows][top]
     float* top_logprobs;       // [rows][top]
     void* scratch;             // logprobs_scratch() bytes, 16-byte aligned
+    int32_t* counters;         // as PagedAttnArgs::counters
     int32_t* fault;            // set to 1 by a target from vocab on, or null
 };
 constexpr int32_t kMaxTop = 32;

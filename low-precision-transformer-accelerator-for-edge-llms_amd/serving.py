@@ -6,9 +6,9 @@ rotation and the INT8 cache follow its accelerator path (design_decisions A7/B2)
 Every call here queues its kernels on torch's current stream of the tensors'
 device and returns, as torch's own operations do (the ``_async`` entry points of
 include/tl_int8.h): results may be used by later work on that stream, and calls
-can be captured into a ``torch.cuda.CUDAGraph``.  Scratch memory comes from
-torch's allocator with each call, so calls on different streams and captured
-graphs share none.  Tensors are CUDA tensors of one device; float types are
+can be captured into a ``torch.cuda.CUDAGraph``.  Scratch memory
+is torch's, kept for each stream, and a captured graph has its own, so calls on
+different streams and graphs share none.  Tensors are CUDA tensors of one device; float types are
 float32, bfloat16 and float16.
 
 What a call finds out of range on the device (a sequence, position, page or token
@@ -29,6 +29,7 @@ from ._native import Runtime, TlPagedCache, TlValueError
 _ACT = {torch.float32: _native.TL_F32, torch.bfloat16: _native.TL_BF16, torch.float16: _native.TL_F16}
 _CACHE = {torch.int8: _native.TL_I8, torch.bfloat16: _native.TL_BF16, torch.float16: _native.TL_F16}
 _HANDLES: dict[int, Runtime] = {}
+_WORKSPACES: dict[tuple[int, int], "_Workspace"] = {}
 
 
 def _runtime(device: torch.device) -> Runtime:
@@ -40,6 +41,38 @@ def _runtime(device: torch.device) -> Runtime:
                               max_pos=64, rms_eps=1e-5, rope_theta=10000.0))
         _HANDLES[device.index] = rt
     return rt
+
+
+def _stream(dev: torch.device) -> int:
+    """The current stream of a device, without the object torch.cuda.current_stream makes."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+class _Workspace:
+    """Scratch and zeroed counters of the calls on one stream, which run one after another."""
+
+    def __init__(self, dev: torch.device):
+        self.counters = torch.zeros(_native.TL_OP_COUNTERS, dtype=torch.int32, device=dev)
+        self.scratch = torch.empty(0, dtype=torch.uint8, device=dev)
+
+
+def _workspace(dev: torch.device, stream: int, need: int):
+    """(scratch address, counters address) for a call on a stream, and what keeps the scratch.
+    While the stream is captured the scratch is the graph's own and there are no counters, as
+    the graph may run beside other calls."""
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _workspace(dev, stream, need)
+    if torch._C._cuda_isCurrentStreamCapturing():
+        own = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        return own.data_ptr() if need else None, None, own
+    ws = _WORKSPACES.get((dev.index, stream))
+    if ws is None:
+        ws = _WORKSPACES[(dev.index, stream)] = _Workspace(dev)
+    if ws.scratch.shape[0] < need:
+        # (the allocator gives the old block to this stream's later work only)
+        ws.scratch = torch.empty(need + need // 4, dtype=torch.uint8, device=dev)
+    return ws.scratch.data_ptr(), ws.counters.data_ptr(), ws
 
 
 def _bad(message: str):
@@ -162,7 +195,7 @@ class PagedCache:
         q_stride = stride if out.data_ptr() == qkv.data_ptr() and rows == 1 else _stride(out)
         rt = self.rt
         st = rt.lib.tl_paged_append_async(
-            rt.h, torch.cuda.current_stream(dev).cuda_stream, self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
+            rt.h, _stream(dev), self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
             rows, n_heads, seq, pos, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
             out.data_ptr() if n_heads else None, q_stride, self.fault.data_ptr())
         if st:
@@ -190,12 +223,12 @@ class PagedCache:
         if rows == 0:
             return out
         need = self._scratch_bytes(rows, n_heads)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rt = self.rt
+        rt, stream = self.rt, _stream(dev)
+        scratch, counters, keep = _workspace(dev, stream, need)
         st = rt.lib.tl_paged_attention_async(
-            rt.h, torch.cuda.current_stream(dev).cuda_stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows,
+            rt.h, stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows,
             n_heads, seq, pos, 1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), _stride(out),
-            scratch.data_ptr() if need else None, need, self.fault.data_ptr())
+            scratch, need, counters, self.fault.data_ptr())
         if st:
             rt.check(st, "attend")
         return out
@@ -274,13 +307,13 @@ class W4Linear:
         if rows == 0:
             return out
         need = self._scratch_bytes(rows)
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rt = self.rt
+        rt, stream = self.rt, _stream(dev)
+        scratch, _, keep = _workspace(dev, stream, need) if need else (None, None, None)
         st = rt.lib.tl_linear_w4_async(
-            rt.h, torch.cuda.current_stream(dev).cuda_stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows,
+            rt.h, stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows,
             self.q.data_ptr(), self.scales.data_ptr(), _ACT[self.scales.dtype], self.group, self.n, self.k,
             None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),
-            out.data_ptr(), _stride(out), scratch.data_ptr() if need else None, need)
+            out.data_ptr(), _stride(out), scratch, need)
         if st:
             rt.check(st, "W4Linear")
         return out
@@ -321,12 +354,12 @@ def token_logprobs(logits, targets, top: int = 0, rt: Runtime | None = None) -> 
         n = C.c_int64()
         rt.check(rt.lib.tl_token_logprobs_scratch(rt.h, rows, vocab, top, C.byref(n)), "tl_token_logprobs_scratch")
         need = _LOGPROBS_SCRATCH[(rows, vocab, top)] = n.value
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    at, ib = stats.data_ptr(), best.data_ptr()
+    at, ib, stream = stats.data_ptr(), best.data_ptr(), _stream(dev)
+    scratch, counters, keep = _workspace(dev, stream, need)
     st = rt.lib.tl_token_logprobs_async(
-        rt.h, torch.cuda.current_stream(dev).cuda_stream, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+        rt.h, stream, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
         _ACT[logits.dtype], rows, vocab, ids, top, at, at + 4 * rows, ib, ib + 4 * rows * top,
-        scratch.data_ptr() if need else None, need, None)
+        scratch, need, counters, None)
     if st:
         rt.check(st, "token_logprobs")
     return got

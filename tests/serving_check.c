@@ -47,7 +47,7 @@ static void paged(void) {
     int64_t need = -1;
     expect("append", append(&c), TL_OK, 1);
     expect("scratch", tl_paged_attention_scratch(H, &c, 4, HEADS, &need), TL_OK, 0);
-    expect("attention", attend(&c), TL_OK, need ? 2 : 1);
+    expect("attention", attend(&c), TL_OK, 1);
     expect("no rows", tl_paged_append(H, &c, qkv, w, TL_F32, 0, HEADS, NULL, NULL, cs, sn, 64, q, qw), TL_OK, 0);
     expect("no rows", tl_paged_attention(H, &c, q, qw, TL_F32, 0, HEADS, NULL, NULL, 1, out, qw), TL_OK, 0);
     expect("no queries", tl_paged_append(H, &c, qkv, 2 * KV * HD, TL_F32, 4, 0, seq, pos, cs, sn, 64, NULL, 0), TL_OK, 1);
@@ -73,7 +73,7 @@ static void paged(void) {
     WITH("misaligned v", x.v = v_pages + 1, TL_ERR_BAD_DESCRIPTOR);
     WITH("short page_stride", x.page_stride -= 16, TL_ERR_BAD_DESCRIPTOR);
     WITH("odd page_stride", x.page_stride += 8, TL_ERR_BAD_DESCRIPTOR);
-    WITH("huge page_stride", x.page_stride = (int64_t)1 << 60, TL_ERR_BAD_DESCRIPTOR);
+    WITH("huge page_stride", x.page_stride = (int64_t)1 << 32, TL_ERR_BAD_DESCRIPTOR);
     expect("null cache", append(NULL), TL_ERR_BAD_DESCRIPTOR, 0);
     expect("null cache", attend(NULL), TL_ERR_BAD_DESCRIPTOR, 0);
     expect("null cache", tl_paged_attention_scratch(H, NULL, 4, HEADS, &need), TL_ERR_BAD_DESCRIPTOR, 0);
@@ -103,6 +103,10 @@ static void paged(void) {
     ATT("negative rows", q, qw, TL_F32, -4, HEADS, seq, pos, 1, out, qw);
     ATT("short stride", q, qw - 4, TL_F32, 4, HEADS, seq, pos, 1, out, qw);
     ATT("misaligned out", q, qw, TL_F32, 4, HEADS, seq, pos, 1, &out[0][1], qw);
+    tl_paged_cache deep = cache();
+    deep.max_pages = 1 << 26;   /* 2^30 positions: 2^22 tiles */
+    deep.table_stride = 1 << 26;
+    expect("too many tiles", tl_paged_attention(H, &deep, q, qw, TL_F32, 300, HEADS, seq, pos, 1, out, qw), TL_ERR_UNSUPPORTED, 0);
     expect("scratch: null", tl_paged_attention_scratch(H, &c, 4, HEADS, NULL), TL_ERR_BAD_DESCRIPTOR, 0);
     expect("scratch: heads", tl_paged_attention_scratch(H, &c, 4, 3, &need), TL_ERR_BAD_DESCRIPTOR, 0);
 
@@ -115,7 +119,7 @@ static void paged(void) {
     checks++;
     wrong += need <= 0;
     void* s = aligned_alloc(64, (size_t)(need + 127) / 64 * 64);
-#define ASYNC(scr, n) tl_paged_attention_async(H, NULL, &l, q, qw, TL_F32, 1, HEADS, seq, pos, 1, out, qw, scr, n, NULL)
+#define ASYNC(scr, n) tl_paged_attention_async(H, NULL, &l, q, qw, TL_F32, 1, HEADS, seq, pos, 1, out, qw, scr, n, NULL, NULL)
     expect("async", ASYNC(s, need), TL_OK, 2);
     expect("async, no scratch", ASYNC(NULL, need), TL_ERR_BAD_DESCRIPTOR, 0);
     expect("async, short scratch", ASYNC(s, need - 1), TL_ERR_BAD_DESCRIPTOR, 0);
@@ -221,7 +225,7 @@ static void logprobs(void) {
     char* a = (char*)(((uintptr_t)s + 63) & ~(uintptr_t)63);
     checks++;
     wrong += need <= 0 || need > 2048;
-#define AS(scr, n) tl_token_logprobs_async(H, NULL, x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids[0], tl[0], scr, n, NULL)
+#define AS(scr, n) tl_token_logprobs_async(H, NULL, x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids[0], tl[0], scr, n, NULL, NULL)
     expect("async", AS(a, need), TL_OK, 2);
     expect("async, no scratch", AS(NULL, need), bad, 0);
     expect("async, short scratch", AS(a, need - 1), bad, 0);

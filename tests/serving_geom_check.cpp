@@ -1,6 +1,7 @@
 // Index arithmetic of the paged cache (csrc/tl_serving.h) on the CPU: every table
 // lookup stays in the table, every row in its page and every page in the pool,
-// whatever the table holds; the chunks of a split row tile its keys.
+// whatever the table holds; the workgroups' shares tile the keys.
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <set>
@@ -56,15 +57,39 @@ int main() {
         g.max_pages = 1 << 20;
         CHECK(paged_row_kind(g, 0, (1 << 30) - 1) == PAGED_ROW_OK && paged_row_kind(g, 0, 1 << 30) == PAGED_ROW_FAULT);
     }
-    // chunks: whole tiles, all keys in exactly one chunk, no more chunks than splits
-    for (int splits : {1, 2, 3, 7, 32, 255, 256})
-        for (int64_t n : {1ll, 2ll, 127ll, 128ll, 129ll, 1000ll, 2047ll, 2048ll, 40000ll, 131071ll, 1ll << 30}) {
-            const int32_t c = paged_chunk((int32_t)n, splits), act = paged_active((int32_t)n, splits);
-            CHECK(c % kPagedTile == 0 && c > 0);
-            CHECK(act >= 1 && act <= splits);
-            CHECK((int64_t)(act - 1) * c < n && (int64_t)act * c >= n);
+    // shares: every tile has one owner, runs follow one another and differ by at most one; a workgroup leaves
+    // at most one part in each of its two places
+    for (int w : {1, 2, 3, 7, 64, 255, 768})
+        for (int64_t tiles : {1ll, 2ll, 63ll, 64ll, 65ll, 767ll, 768ll, 769ll, 5000ll, (1ll << 31) - 1}) {
+            const PagedShare s = paged_share((int32_t)tiles, w);
+            CHECK(s.start(0) == 0 && s.start(w) == tiles);
+            for (int i = 0; i < w; i++) {
+                const int64_t n = s.start(i + 1) - s.start(i);
+                CHECK(n == s.per || n == s.per + 1);
+                if (n == 0) continue;
+                CHECK(s.owner(s.start(i)) == i && s.owner(s.start(i + 1) - 1) == i);
+            }
+            if (tiles > 5000) continue;
+            srand(w);
+            std::set<int> parts;
+            for (int64_t unit = 0; unit < tiles;) {
+                const int64_t end = std::min<int64_t>(tiles, unit + 1 + rand() % 40);
+                const int w0 = s.owner(unit), w1 = s.owner(end - 1);
+                for (int i = w0; i <= w1 && w0 != w1; i++) {
+                    const int p = paged_part(s, i, unit);
+                    CHECK(p / 2 == i && parts.insert(p).second);
+                }
+                unit = end;
+            }
         }
-    CHECK(paged_active(0, 5) == 0);
+    CHECK(paged_tiles(-3) == 1 && paged_tiles(0) == 1 && paged_tiles(1) == 1 && paged_tiles(128) == 1 && paged_tiles(129) == 2);
+    CHECK(paged_tiles(1 << 30) == 1 << 23);
+    PagedGeom g{};
+    g.max_pages = 1 << 20;
+    g.page_shift = 10;
+    CHECK(paged_countable(g, 1, 255) && paged_countable(g, 255, 1) && !paged_countable(g, 256, 1) && !paged_countable(g, 2, 128));
+    g.max_pages = 1;
+    CHECK(paged_countable(g, 1 << 20, 100) && !paged_countable(g, 1 << 20, 1 << 9));
     std::printf("%d wrong\n", wrong);
     return wrong ? 1 : 0;
 }

@@ -298,29 +298,35 @@ int32_t tl_paged_attention_async(tl_handle *h, void *stream, const tl_paged_cach
 int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
                                    int64_t *bytes);
 
-/* Projection of m rows with 4-bit weights: y[m][n] = residual[m][n] + sum_k
- * x[m][k] w[n][k], w[n][k] = q s[n][k / group], q from -8 to 7, x, residual
- * and y of type act (TL_F32, TL_BF16, TL_F16), residual may be NULL.  q [n][k / 2] bytes:
- * column 2 j of a row is the low nibble of byte j, 2 j + 1 the high one, two's
- * complement.  scales [n][k / group] of scale_dtype (a float type); group 32, 64
- * or 128, k a multiple of it, at most 1024 groups.  All dev; strides in elements,
- * x's rows and q 16-byte aligned.  A row of x is taken as integers of 2^-30 of
- * its largest magnitude, products are exact, sums float32; an infinity or NaN in a
- * row of x makes the whole row of y NaN.  Few rows (a decoding step) are what it is
- * made for; any number is right. */
-int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const uint8_t *q,
-                     const void *scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k,
-                     const void *residual, int64_t res_stride, void *y, int64_t y_stride);
-int32_t tl_linear_w4_async(tl_handle *h, void *stream, const void *x, int64_t x_stride, int32_t act, int32_t m,
-                           const uint8_t *q, const void *scales, int32_t scale_dtype, int32_t group, int32_t n,
-                           int32_t k, const void *residual, int64_t res_stride, void *y, int64_t y_stride,
-                           void *scratch, int64_t scratch_bytes);
-int32_t tl_linear_w4_scratch(tl_handle *h, int32_t m, int32_t n, int32_t k, int32_t group, int64_t *bytes);
-/* Offline quantizer for it, as tl_quantize_weight_rows: w [rows][n] float32 (finite), per group
+/* Projections with 4-bit weights: w[n][k] = q s[n][k / group], q from -8 to 7.  q
+ * [n][k / 2] bytes: column 2 j of a row is the low nibble of byte j, 2 j + 1 the
+ * high one, two's complement; scales [n][k / group] of scale_dtype (TL_F32, TL_BF16 or
+ * TL_F16); group 32, 64 or 128, k a multiple of it, at most 1024 groups. */
+/* Offline quantizer, as tl_quantize_weight_rows: w [rows][n] float32 (dev, finite), per group
  * s = max|w| / 7 in float32, rounded to scale_dtype (1, and zero weights, where that is 0),
  * q = clip(rne(w / s), -8, 7). */
 int32_t tl_quantize_w4_rows(tl_handle *h, const float *w, int32_t rows, int32_t n, int32_t group,
                             int32_t scale_dtype, uint8_t *q, void *scales);
+/* q and scales (dev) into the order the kernels read, once per weight matrix: packed
+ * (dev, 16-byte aligned) takes tl_w4_packed_bytes, about as many as they; they are not
+ * needed afterwards. */
+int32_t tl_w4_packed_bytes(tl_handle *h, int32_t n, int32_t k, int32_t group, int32_t scale_dtype, int64_t *bytes);
+int32_t tl_pack_w4(tl_handle *h, const uint8_t *q, const void *scales, int32_t scale_dtype, int32_t group, int32_t n,
+                   int32_t k, void *packed);
+/* y[m][n] = residual[m][n] + sum_k x[m][k] w[n][k], x, residual and y of type act
+ * (TL_F32, TL_BF16, TL_F16), residual may be NULL or y.  All dev; strides in elements, x's
+ * rows 16-byte aligned.  A row of x is taken as integers of 2^-30 of its largest
+ * magnitude, products are exact, sums float32; an infinity or NaN in a row of x makes
+ * its whole row of y NaN.  Few rows (a decoding step) are what it is made for; up to
+ * 2^20 are right. */
+int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
+                     int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void *residual,
+                     int64_t res_stride, void *y, int64_t y_stride);
+int32_t tl_linear_w4_async(tl_handle *h, void *stream, const void *x, int64_t x_stride, int32_t act, int32_t m,
+                           const void *packed, int32_t scale_dtype, int32_t group, int32_t n, int32_t k,
+                           const void *residual, int64_t res_stride, void *y, int64_t y_stride, void *scratch,
+                           int64_t scratch_bytes);
+int32_t tl_linear_w4_scratch(tl_handle *h, int32_t m, int32_t k, int64_t *bytes);
 
 /* Log probabilities from logits [rows][vocab] of type dtype (TL_F32, TL_BF16,
  * TL_F16; any row stride, aligned as its type): logprob[r] = log softmax of row r

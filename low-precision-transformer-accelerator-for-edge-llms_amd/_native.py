@@ -92,7 +92,7 @@ _f64p = C.POINTER(C.c_double)
 _f32 = C.c_float
 _cachep = C.POINTER(TlPagedCache)
 _append = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64]
-_w4 = [_vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64]
+_w4 = [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64]
 _logprobs = [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]
 _attend = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _i64]
 
@@ -147,7 +147,9 @@ SIGNATURES = {
     "tl_paged_attention_scratch": (_i32, [_vp, _cachep, _i32, _i32, C.POINTER(_i64)]),
     "tl_linear_w4": (_i32, [_vp, *_w4]),
     "tl_linear_w4_async": (_i32, [_vp, _vp, *_w4, _vp, _i64]),
-    "tl_linear_w4_scratch": (_i32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "tl_linear_w4_scratch": (_i32, [_vp, _i32, _i32, C.POINTER(_i64)]),
+    "tl_w4_packed_bytes": (_i32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "tl_pack_w4": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "tl_quantize_w4_rows": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "tl_token_logprobs": (_i32, [_vp, *_logprobs]),
     "tl_token_logprobs_async": (_i32, [_vp, _vp, *_logprobs, _vp, _i64, _vp, _vp]),

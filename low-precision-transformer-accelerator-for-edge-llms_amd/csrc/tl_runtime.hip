@@ -2423,22 +2423,30 @@ int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q,
     return TL_OK;
 }
 
-int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const uint8_t* q,
-                const void* scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual,
-                int64_t res_stride, void* y, int64_t y_stride, W4Args* a) {
-    TL_REQ(h, act_type(act) && act_type(scale_dtype), "types must be float32, bfloat16 or float16");
-    TL_REQ(h, m >= 0 && n >= 1 && k >= 1, "empty projection");
+// the shape of 4-bit weights
+int32_t w4_shape(tl_handle* h, int32_t n, int32_t k, int32_t group, int32_t scale_dtype) {
+    TL_REQ(h, act_type(scale_dtype), "scales must be float32, bfloat16 or float16");
+    TL_REQ(h, n >= 1 && k >= 1, "empty weights");
     if (!w4_supported(k, group))
         return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
-    TL_REQ(h, q && scales && aligned16(q) && (uintptr_t)scales % type_size(scale_dtype) == 0, "weights missing or misaligned");
-    TL_REQ(h, (x && y) || m == 0, "null x or y");
-    const int32_t r = check_rows(h, x, x_stride, k, act, "x");
+    return TL_OK;
+}
+
+int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const void* packed,
+                int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual, int64_t res_stride, void* y,
+                int64_t y_stride, W4Args* a) {
+    int32_t r = w4_shape(h, n, k, group, scale_dtype);
     if (r) return r;
+    TL_REQ(h, act_type(act), "rows must be float32, bfloat16 or float16");
+    TL_REQ(h, m >= 0 && m <= 1 << 20, "row count outside 0 .. 2^20");
+    TL_REQ(h, packed && aligned16(packed), "packed weights missing or misaligned");
+    TL_REQ(h, (x && y) || m == 0, "null x or y");
+    if ((r = check_rows(h, x, x_stride, k, act, "x"))) return r;
     TL_REQ(h, y_stride >= n && (uintptr_t)y % type_size(act) == 0, "y: rows must not overlap and must be aligned");
     TL_REQ(h, !residual || (res_stride >= n && (uintptr_t)residual % type_size(act) == 0),
            "residual: rows must not overlap and must be aligned");
     a->x = x; a->x_stride = x_stride; a->act = act; a->m = m; a->n = n; a->k = k; a->group = group;
-    a->q = q; a->scales = scales; a->scale_dtype = scale_dtype;
+    a->packed = packed; a->scale_dtype = scale_dtype;
     a->residual = residual; a->res_stride = res_stride; a->y = y; a->y_stride = y_stride;
     return TL_OK;
 }
@@ -2540,50 +2548,69 @@ int32_t tl_paged_attention_scratch(tl_handle* h, const tl_paged_cache* cache, in
     return TL_OK;
 }
 
-int32_t tl_linear_w4(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const uint8_t* q,
-                     const void* scales, int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual,
-                     int64_t res_stride, void* y, int64_t y_stride) {
+int32_t tl_linear_w4(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const void* packed,
+                     int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void* residual, int64_t res_stride,
+                     void* y, int64_t y_stride) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     W4Args a{};
-    int32_t r = w4_args(h, x, x_stride, act, m, q, scales, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
+    int32_t r = w4_args(h, x, x_stride, act, m, packed, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
     if (r) return r;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
-    if ((r = ensure_op_scratch(h, w4_scratch(m, n, k, group)))) return r;
+    if ((r = ensure_op_scratch(h, w4_scratch(m, k)))) return r;
     a.scratch = h->op_scratch;
     return complete(h, TL_K_OTHER, "tl_linear_w4", [&] { return launch_linear_w4(h->stream, a); });
 }
 
 int32_t tl_linear_w4_async(tl_handle* h, void* stream, const void* x, int64_t x_stride, int32_t act, int32_t m,
-                           const uint8_t* q, const void* scales, int32_t scale_dtype, int32_t group, int32_t n,
-                           int32_t k, const void* residual, int64_t res_stride, void* y, int64_t y_stride,
-                           void* scratch, int64_t scratch_bytes) {
+                           const void* packed, int32_t scale_dtype, int32_t group, int32_t n, int32_t k,
+                           const void* residual, int64_t res_stride, void* y, int64_t y_stride, void* scratch,
+                           int64_t scratch_bytes) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     W4Args a{};
-    int32_t r = w4_args(h, x, x_stride, act, m, q, scales, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
-    if (r || (r = check_scratch(h, scratch, scratch_bytes, w4_scratch(m, n, k, group)))) return r;
+    int32_t r = w4_args(h, x, x_stride, act, m, packed, scale_dtype, group, n, k, residual, res_stride, y, y_stride, &a);
+    if (r || (r = check_scratch(h, scratch, scratch_bytes, w4_scratch(m, k)))) return r;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
     a.scratch = scratch;
     return check_launch(h, launch_linear_w4((hipStream_t)stream, a), "tl_linear_w4_async");
 }
 
-int32_t tl_linear_w4_scratch(tl_handle* h, int32_t m, int32_t n, int32_t k, int32_t group, int64_t* bytes) {
+int32_t tl_linear_w4_scratch(tl_handle* h, int32_t m, int32_t k, int64_t* bytes) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
-    TL_REQ(h, bytes && m >= 0 && n >= 1 && k >= 1, "bad scratch arguments");
-    if (!w4_supported(k, group))
-        return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
-    *bytes = (int64_t)w4_scratch(m, n, k, group);
+    TL_REQ(h, bytes && m >= 0 && m <= 1 << 20 && k >= 1 && k <= 1 << 17, "bad scratch arguments");
+    *bytes = (int64_t)w4_scratch(m, k);
     return TL_OK;
+}
+
+int32_t tl_w4_packed_bytes(tl_handle* h, int32_t n, int32_t k, int32_t group, int32_t scale_dtype, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes, "null pointer");
+    const int32_t r = w4_shape(h, n, k, group, scale_dtype);
+    if (r) return r;
+    *bytes = w4_packed_bytes(n, k, group, scale_dtype);
+    return TL_OK;
+}
+
+int32_t tl_pack_w4(tl_handle* h, const uint8_t* q, const void* scales, int32_t scale_dtype, int32_t group, int32_t n,
+                   int32_t k, void* packed) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    const int32_t r = w4_shape(h, n, k, group, scale_dtype);
+    if (r) return r;
+    TL_REQ(h, q && scales && packed && aligned16(packed) && ((uintptr_t)q & 3) == 0 &&
+                  (uintptr_t)scales % type_size(scale_dtype) == 0, "null or misaligned pointer");
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    return complete(h, TL_K_OTHER, "tl_pack_w4",
+                    [&] { return launch_pack_w4(h->stream, q, scales, scale_dtype, group, n, k, packed); });
 }
 
 int32_t tl_quantize_w4_rows(tl_handle* h, const float* w, int32_t rows, int32_t n, int32_t group, int32_t scale_dtype,
                             uint8_t* q, void* scales) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
-    TL_REQ(h, rows >= 0 && n >= 1, "empty weights");
-    TL_REQ(h, act_type(scale_dtype), "scales must be float32, bfloat16 or float16");
-    if (!w4_supported(n, group))
-        return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
+    TL_REQ(h, rows >= 0, "negative row count");
+    const int32_t r = w4_shape(h, 1, n, group, scale_dtype);
+    if (r) return r;
     TL_REQ(h, w && q && scales && aligned16(w) && ((uintptr_t)q & 3) == 0 && (uintptr_t)scales % type_size(scale_dtype) == 0,
            "null or misaligned pointer");
     const OnDevice on(h->device);

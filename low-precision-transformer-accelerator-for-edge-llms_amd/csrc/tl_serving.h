@@ -139,16 +139,16 @@ int32_t paged_attention_workgroups(const PagedCache& c, int32_t rows, int32_t n_
 size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads);
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
 
-// 4-bit weights: q [n][k / 2] bytes, column 2 j of a row in byte j's low nibble
-// and 2 j + 1 in its high one, each a two's complement number -8 .. 7; scales
-// [n][k / group] of scale_dtype
+// Projections with 4-bit weights.  Packed weights (launch_pack_w4) hold, for each
+// 16 rows and 128 columns, 1 KiB in the order a wavefront's lanes take it, rows and
+// columns behind the last ones zero, and behind all of them the scales
+// [16 rows][group][row] of scale_dtype.
 struct W4Args {
     const void* x;             // [m][k] of act, stride x_stride
     int64_t x_stride;
     int32_t act;
     int32_t m, n, k, group;
-    const uint8_t* q;
-    const void* scales;
+    const void* packed;
     int32_t scale_dtype;
     const void* residual;      // [m][n] of act, stride res_stride, or null
     int64_t res_stride;
@@ -157,8 +157,13 @@ struct W4Args {
     void* scratch;             // w4_scratch() bytes, 16-byte aligned
 };
 bool w4_supported(int32_t k, int32_t group);
-size_t w4_scratch(int32_t m, int32_t n, int32_t k, int32_t group);
+int64_t w4_packed_bytes(int32_t n, int32_t k, int32_t group, int32_t scale_dtype);
+size_t w4_scratch(int32_t m, int32_t k);
 hipError_t launch_linear_w4(hipStream_t s, const W4Args& a);
+// q [n][k / 2] bytes: column 2 j of a row in byte j's low nibble, 2 j + 1 in its
+// high one, each a two's complement number -8 .. 7; scales [n][k / group]
+hipError_t launch_pack_w4(hipStream_t s, const uint8_t* q, const void* scales, int32_t scale_dtype, int32_t group,
+                          int32_t n, int32_t k, void* packed);
 hipError_t launch_quantize_w4(hipStream_t s, const float* w, int32_t rows, int32_t k, int32_t group, int32_t scale_dtype,
                               uint8_t* q, void* scales);
 hipError_t init_w4_kernels();

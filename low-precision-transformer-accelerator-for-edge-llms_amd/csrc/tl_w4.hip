@@ -2,18 +2,23 @@
 //
 // y[m][n] = (residual +) sum_g s[n][g] sum_{k in g} w[n][k] x[m][k], w in -8 .. 7.
 //
-// The inner sums run on v_mfma_i32_16x16x64_i8, exactly: a nibble becomes the
-// INT8 number 16 w by a mask (and a shift for the low one), and a row of x
-// becomes four base-256 digits, each -128 .. 127.  The row is scaled by a power
-// of two so that its largest magnitude lies in [2^29, 2^30) and rounded to an
-// integer v; the digits are the bytes of (v + 0x808080) ^ 0x808080.  A value is
-// off by at most 2^-30 of its row's largest, whatever its type; products and
-// sums of 128 are exact in INT32, and only the sum over groups (each times its
-// scale) rounds, in float32.
+// The inner sums run on the INT8 matrix instructions, exactly.  A nibble becomes
+// the INT8 number 16 w by a mask (and a shift for the low one).  A row of x becomes
+// four base-256 digits, each -128 .. 127: it is scaled by a power of two so that
+// its largest magnitude lies in [2^29, 2^30) and rounded to integers v, whose
+// digits are the bytes of (v + 0x808080) ^ 0x808080.  So a value is off by at most
+// 2^-30 of its row's largest, whatever its type; products and sums over a group
+// are exact in INT32, and only the sum over groups, each times its scale, rounds,
+// in float32.  The 16 columns of a product are four rows of x with four digits.
 //
-// A matrix product has 16 columns, a row of x takes four of them (its digits),
-// times the groups in the product's 128 weights: with groups of 64 or 32 each
-// group has columns of its own that are zero in the others' places.
+// What bounds it: the weights, k / 2 bytes a row, read once; of the rest the
+// latency from the first load to the result.  They stream in the order of the
+// lanes' registers, 1 KiB for 16 rows by 128 columns, 8 KiB in flight in each
+// wavefront; the digits of up to 16 rows of x wait in LDS.  Queued back to back, one
+// row by 5632 x 2048 takes 7.7 us, by 32000 x 2048 (group 32, float32 scales) 12.5,
+// by 14336 x 8192 15.7 (3.9 TB/s); 13 rows by 2048 x 5632 14.7, 16 by 32000 x 2048
+// 20.9.  With the weights in the rows' own order, where a load's pieces lie k / 2
+// bytes apart, the second took 20.9.
 #include <algorithm>
 
 #include "tl_rows.h"
@@ -22,188 +27,328 @@ namespace tl {
 namespace {
 
 constexpr int kW4Waves = 8;
-constexpr int kW4MaxGroups = 1024;   // group scales of a row held in LDS
+constexpr int kW4Threads = 64 * kW4Waves;
+constexpr int kW4MaxGroups = 1024;
+constexpr int64_t kW4EnoughWaves = 1024;
+constexpr int kW4Ahead = 8;          // 1 KiB weight blocks in flight per wavefront
 constexpr int kBadRow = INT32_MIN;   // exponent of a row with an infinity or NaN
-constexpr int kZeros = 128;          // bytes of zeros the unused columns read
+constexpr int kW4Lds = 152 * 1024;   // of a workgroup's 160 KiB
 
-__host__ __device__ inline int w4_blocks(int k) { return 2 * ((k + 255) / 256); }   // 128-weight blocks, in pairs
-// bytes of one digit of a row, shifted 16 per digit so that columns differ in LDS bank
-__host__ __device__ inline int w4_digit_stride(int k) { return w4_blocks(k) * 128 + 16; }
+__host__ __device__ inline int w4_blocks(int k) { return (k + 127) / 128; }
+__host__ __device__ inline int w4_tiles(int n) { return (n + 15) / 16; }
+__host__ __device__ inline int w4_groups(int k, int group) { return w4_blocks(k) * (128 / group); }   // with the padding's
+
+// The digits of `cols / 4` rows of x (cols: 4, 8 or 16), in the order the products
+// take them: for 64 columns of x, lane group g and column of the product 16 bytes,
+// those of x's columns 32 c + 8 g + 2 i + parity at 8 c + 4 parity + i.
+__host__ __device__ inline int w4_frag(int k64, int g, int col, int cols) { return ((k64 * 4 + g) * cols + col) * 16; }
+__host__ __device__ inline size_t w4_frag_bytes(int k, int cols) { return (size_t)w4_blocks(k) * 128 * cols; }
 
 // four integers (of columns k, k + 2, k + 4, k + 6) to one dword per digit
-TL_DEV void digits4(const int v[4], unsigned d[4]) {
-    unsigned u[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) u[i] = ((unsigned)v[i] + 0x00808080u) ^ 0x00808080u;
-    const unsigned a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
-    const unsigned c = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), e = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+TL_DEV void digits4(int v0, int v1, int v2, int v3, unsigned d[4]) {
+    const unsigned u0 = ((unsigned)v0 + 0x00808080u) ^ 0x00808080u, u1 = ((unsigned)v1 + 0x00808080u) ^ 0x00808080u;
+    const unsigned u2 = ((unsigned)v2 + 0x00808080u) ^ 0x00808080u, u3 = ((unsigned)v3 + 0x00808080u) ^ 0x00808080u;
+    const unsigned a = __builtin_amdgcn_perm(u1, u0, 0x05010400u), b = __builtin_amdgcn_perm(u3, u2, 0x05010400u);
+    const unsigned c = __builtin_amdgcn_perm(u1, u0, 0x07030602u), e = __builtin_amdgcn_perm(u3, u2, 0x07030602u);
     d[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
     d[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
     d[2] = __builtin_amdgcn_perm(e, c, 0x05040100u);
     d[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
 }
 
-// The digits of one row of x at base[digit][block][column parity][lane group]
-// [16]: byte j of lane group g in block b is column 128 b + 32 g + 2 j + parity,
-// as the low and high nibbles of a lane's 16 weight bytes come.  Columns from k
-// on are zero.  Returns the power of two the row was scaled by (kBadRow: not
-// finite).  The whole workgroup takes part; red: a word per wavefront.
-template <typename P>
-TL_DEV int row_digits(const W4Args& a, int64_t row, P base, unsigned* red) {
-    const int nt = blockDim.x;
-    const int64_t at = row * a.x_stride;
-    unsigned mx = 0;
-    for (int i = threadIdx.x * 4; i < a.k; i += nt * 4) {
-        const v4f v = load4(a.x, at + i, a.act);
-#pragma unroll
-        for (int j = 0; j < 4; j++) mx = max(mx, __float_as_uint(fabsf(v[j])));
-    }
+// Digits of rows row0 .. row0 + rows - 1 of x (rows <= 4) to base; columns from k on
+// are zero.  exps[r]: the power of two the row was scaled by (kBadRow: not finite).
+// The whole workgroup takes part; mx: a word per row.
+TL_DEV void rows_digits(const W4Args& a, int row0, int rows, char* base, int cols, unsigned* mx, int* exps) {
+    const int tid = threadIdx.x;
+    const int units = a.k >> 3, padded = w4_blocks(a.k) * 16;   // of 8 columns
+    if (tid < rows) mx[tid] = 0u;
+    __syncthreads();
     // magnitudes order as their bits do, infinity and NaN above the numbers
+    for (int r = 0; r < rows; r++) {
+        unsigned m = 0;
+        for (int u = tid; u < units; u += kW4Threads) {
+            const int64_t at = (row0 + r) * a.x_stride + 8 * u;
+            const v4f x0 = load4(a.x, at, a.act), x1 = load4(a.x, at + 4, a.act);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, o));
-    __syncthreads();
-    if (lane_id() == 0) red[threadIdx.x >> 6] = mx;
-    __syncthreads();
-    for (int i = 0; i < nt >> 6; i++) mx = max(mx, red[i]);
-    const bool bad = mx >= 0x7F800000u;
-    const int e = bad || mx == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(mx));
-    const int ds = w4_digit_stride(a.k);
-    for (int i = threadIdx.x * 8; i < w4_blocks(a.k) * 128; i += nt * 8) {
-        v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
-        if (i < a.k && !bad) {   // k is a multiple of 32
-            x0 = load4(a.x, at + i, a.act);
-            x1 = load4(a.x, at + i + 4, a.act);
+            for (int j = 0; j < 4; j++) m = max(m, max(__float_as_uint(fabsf(x0[j])), __float_as_uint(fabsf(x1[j]))));
         }
-        int v[2][4];
+        m = max(m, (unsigned)dpp<kDppXor1>((int)m));
+        m = max(m, (unsigned)dpp<kDppXor2>((int)m));
+        m = max(m, (unsigned)dpp<kDppHalfMirror>((int)m));
+        m = max(m, (unsigned)dpp<kDppRowMirror>((int)m));
+        if ((tid & 15) == 0) atomicMax(&mx[r], m);
+    }
+    __syncthreads();
+    for (int r = 0; r < rows; r++) {
+        const unsigned m = mx[r];
+        const bool bad = m >= 0x7F800000u;
+        const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
+        if (tid == 0) exps[r] = bad ? kBadRow : e;
+        for (int u = tid; u < padded; u += kW4Threads) {
+            v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+            if (u < units && !bad) {
+                const int64_t at = (row0 + r) * a.x_stride + 8 * u;
+                x0 = load4(a.x, at, a.act);
+                x1 = load4(a.x, at + 4, a.act);
+            }
+            int v[8];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            v[j][0] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x0[j], e));
-            v[j][1] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x0[2 + j], e));
-            v[j][2] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x1[j], e));
-            v[j][3] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x1[2 + j], e));
-        }
-        const int to = (i >> 7) * 128 + ((i >> 5) & 3) * 16 + ((i >> 3) & 3) * 4;
+            for (int j = 0; j < 4; j++) {
+                v[j] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x0[j], e));
+                v[4 + j] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x1[j], e));
+            }
+            unsigned even[4], odd[4];
+            digits4(v[0], v[2], v[4], v[6], even);
+            digits4(v[1], v[3], v[5], v[7], odd);
+            char* to = base + 8 * (u >> 2 & 1);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            unsigned d[4];
-            digits4(v[j], d);
-#pragma unroll
-            for (int c = 0; c < 4; c++) *(unsigned*)(base + c * ds + to + 64 * j) = d[c];
+            for (int d = 0; d < 4; d++)
+                *(v2i*)(to + w4_frag(u >> 3, u & 3, 4 * r + d, cols)) = v2i{(int)even[d], (int)odd[d]};
         }
     }
-    return bad ? kBadRow : e;
 }
 
-// scratch of a call: zeros, the rows' exponents, the rows' digits
-__host__ __device__ inline size_t w4_exp_off() { return kZeros; }
-__host__ __device__ inline size_t w4_digit_off(int m) { return kZeros + ((size_t)m * 4 + 15) / 16 * 16; }
+// n pieces from memory to LDS by the whole workgroup, four loads of a thread in
+// flight; put(v, i) stores piece i
+template <typename V, typename Put>
+TL_DEV void to_lds(const V* from, int n, Put put) {
+    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * kW4Threads) {
+        const V a = from[i0], b = from[min(i0 + kW4Threads, n - 1)], c = from[min(i0 + 2 * kW4Threads, n - 1)],
+                d = from[min(i0 + 3 * kW4Threads, n - 1)];
+        put(a, i0);
+        if (i0 + kW4Threads < n) put(b, i0 + kW4Threads);
+        if (i0 + 2 * kW4Threads < n) put(c, i0 + 2 * kW4Threads);
+        if (i0 + 3 * kW4Threads < n) put(d, i0 + 3 * kW4Threads);
+    }
+}
 
-__global__ __launch_bounds__(512) void w4_digits_kernel(W4Args a) {
-    __shared__ unsigned red[8];
+// scratch of a call: the rows' exponents, the digits of each four rows
+__host__ __device__ inline size_t w4_digit_off(int m) { return ((size_t)m * 4 + 15) / 16 * 16; }
+
+__global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
+    __shared__ unsigned mx[1];
     const int row = blockIdx.x;
     char* s = (char*)a.scratch;
-    if (row == 0 && threadIdx.x < kZeros / 4) ((unsigned*)s)[threadIdx.x] = 0u;
-    const int e = row_digits(a, row, s + w4_digit_off(a.m) + (size_t)row * 4 * w4_digit_stride(a.k), red);
-    if (threadIdx.x == 0) ((int*)(s + w4_exp_off()))[row] = e;
+    // one row at its place among its four
+    char* base = s + w4_digit_off(a.m) + (row >> 2) * w4_frag_bytes(a.k, 16) + (row & 3) * 64;
+    rows_digits(a, row, 1, base, 16, mx, (int*)s + row);
 }
 
-// Workgroup (16 weight rows, tile of x rows): its wavefronts share out the pairs
-// of 128-weight blocks of the rows; CB column blocks of 16.
-template <int CB>
-__global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args a, int lq) {
+struct W4Shape {
+    int32_t split;       // wavefronts that share a tile of 16 weight rows: 1, 2, 4 or 8
+    int32_t cols;        // columns of a product in use by the digits' layout
+};
+
+constexpr int kW4Chunk = 8;   // blocks of 128 columns whose digits are in LDS at a time (COPY)
+
+// Workgroup (8 / split tiles of 16 weight rows, 4 CB rows of x).  LQ: log2 of the
+// groups in 128 columns.  Up to four rows of x each workgroup converts to digits
+// itself (COPY false); of more, it copies what w4_digits_kernel left in scratch,
+// 1024 columns at a time, the next ones on their way while these are used.
+template <int CB, int LQ, bool COPY>
+__global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a, W4Shape sh) {
     extern __shared__ __align__(16) char lds[];
-    const int ng = a.k / a.group, nblk = w4_blocks(a.k);
-    const int q_n = 1 << lq;                           // groups in a block
-    const int cols = 4 << lq;                          // columns of one row of x
-    const int mt = (CB * 16) >> (2 + lq);              // rows of x in a tile
-    const int m0 = blockIdx.y * mt, n0 = blockIdx.x * 16;
+    constexpr int Q = 1 << LQ;
+    const int nblk = w4_blocks(a.k), groups = nblk << LQ;
     const int lane = lane_id(), wave = wave_id(), col = lane & 15, g = lane >> 4;
+    const int tiles = w4_tiles(a.n), per = kW4Waves / sh.split;
+    const int part = wave % sh.split;
+    const int tile = blockIdx.x * per + wave / sh.split;
+    const int m0 = blockIdx.y * (4 * CB);
 
-    // the first weights, on their way while the scales are laid out
-    const int64_t row_bytes = a.k >> 1;
-    const uint8_t* wrow = a.q + (int64_t)min(n0 + col, a.n - 1) * row_bytes;
-    auto load = [&](int blk) {
-        const int64_t at = blk * 64 + g * 16;
-        return at < row_bytes ? __builtin_nontemporal_load((const v4i*)(wrow + at)) : v4i{0, 0, 0, 0};
+    // the first weights, on their way while digits and scales are laid out
+    const char* w = (const char*)a.packed + ((int64_t)min(tile, tiles - 1) * nblk) * 1024 + lane * 16;
+    v4i ring[kW4Ahead];
+    auto load = [&](int i) {   // the i-th block of this wavefront
+        const int blk = min(part + i * sh.split, nblk - 1);
+        return __builtin_nontemporal_load((const v4i*)(w + (int64_t)blk * 1024));
     };
-    const int pairs = nblk >> 1;
-    v4i next[2] = {};
-    if (wave < pairs) {
-        next[0] = load(2 * wave);
-        next[1] = load(2 * wave + 1);
-    }
-
-    // scales as float32, [group][16 rows], zeros behind the last group
-    float* s_w = (float*)lds;
-    for (int i = threadIdx.x; i < 16 * nblk * q_n; i += 64 * kW4Waves) {
-        const int r = i / (nblk * q_n), gr = i - r * (nblk * q_n);
-        s_w[gr * 16 + r] = gr < ng ? load1(a.scales, (int64_t)min(n0 + r, a.n - 1) * ng + gr, a.scale_dtype) : 0.0f;
-    }
-    float* red = s_w + 16 * nblk * q_n;                // [wave][16 rows][mt]
-
-    // where this lane reads each column block's digits: its column's row and digit,
-    // or zeros where its column is another group's or past the last row
-    const char* scr = (const char*)a.scratch;
-    const int ds = w4_digit_stride(a.k);
-    const char* b_at[CB];
-    int b_step[CB];
 #pragma unroll
-    for (int c = 0; c < CB; c++) {
-        const int cc = c * 16 + col, m = m0 + (cc >> (2 + lq)), d = (cc >> lq) & 3;
-        const bool mine = m < a.m && (g >> (2 - lq)) == (cc & (q_n - 1));
-        b_at[c] = mine ? scr + w4_digit_off(a.m) + ((size_t)m * 4 + d) * ds + g * 16 : scr;
-        b_step[c] = mine ? 128 : 0;
+    for (int i = 0; i < kW4Ahead; i++) ring[i] = load(i);
+
+    // scales of the workgroup's tiles as float32 [tile][group][16 rows]
+    float* s_scale = (float*)lds;
+    {
+        const char* sc = (const char*)a.packed + (int64_t)tiles * nblk * 1024;
+        const int64_t from = (int64_t)blockIdx.x * per * groups * 16;
+        const int n4 = min(per, tiles - (int)blockIdx.x * per) * groups * 4;
+        if (a.scale_dtype == DT_F32)
+            to_lds((const v4f*)((const float*)sc + from), n4, [&](v4f v, int i) { *(v4f*)(s_scale + 4 * i) = v; });
+        else
+            to_lds((const v2i*)((const uint16_t*)sc + from), n4,
+                   [&](v2i v, int i) { *(v4f*)(s_scale + 4 * i) = unpack4(v, a.scale_dtype); });
     }
+    char* next = lds + (size_t)per * groups * 64;
+    float* red = (float*)next;                     // [wave][16 rows][4 CB]
+    next += kW4Waves * 16 * 4 * CB * 4;
+    unsigned* s_mx = (unsigned*)next;
+    int* s_exp = (int*)next + 16;
+    next += 128;
+    char* digits = next;
+    const char* scr = (const char*)a.scratch + w4_digit_off(a.m) + (size_t)blockIdx.y * CB * w4_frag_bytes(a.k, 16);
+
+    // COPY: a chunk's digits, [CB][blocks] of 2 KiB; a thread's share of the next one
+    constexpr int kBlockBytes = 128 * 16, kShare = kW4Chunk * kBlockBytes / (kW4Threads * 16);
+    const int64_t fcb = COPY ? kW4Chunk * kBlockBytes : 0;
+    v4i share[CB][kShare];
+    auto fetch = [&](int chunk) {
+        const int rest = (nblk - chunk * kW4Chunk) * (kBlockBytes / 16);   // pieces of a row block from the chunk on
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+#pragma unroll
+            for (int j = 0; j < kShare; j++)
+                share[c][j] = ((const v4i*)(scr + c * w4_frag_bytes(a.k, 16) + (int64_t)chunk * kW4Chunk * kBlockBytes))
+                    [min((int)threadIdx.x + j * kW4Threads, rest - 1)];
+    };
+    auto put = [&](int chunk) {
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+#pragma unroll
+            for (int j = 0; j < kShare; j++)
+                ((v4i*)(digits + ((chunk & 1) * CB + c) * fcb))[threadIdx.x + j * kW4Threads] = share[c][j];
+    };
+    if constexpr (COPY) {
+        if (threadIdx.x < 4 * CB) s_exp[threadIdx.x] = m0 + (int)threadIdx.x < a.m ? ((const int*)a.scratch)[m0 + threadIdx.x] : 0;
+        fetch(0);
+        put(0);
+    } else {
+        rows_digits(a, m0, min(4, a.m - m0), digits, sh.cols, s_mx, s_exp);
+    }
+    __syncthreads();
+
     v4f acc[CB];
 #pragma unroll
     for (int c = 0; c < CB; c++) acc[c] = v4f{0, 0, 0, 0};
-    __syncthreads();
+    // A digit's sums enter times 256^(digit - 3) and 2^-32: 2^-22 of the result for rows
+    // around 1, so that no partial sum overflows whose result does not
+    const float place = __builtin_amdgcn_ldexpf(1.0f, 8 * (col & 3) - 56);
+    const int mine = (nblk - part + sh.split - 1) / sh.split;   // blocks of this wavefront
+    const float* scale = s_scale + (wave / sh.split) * groups * 16 + 4 * g;
+    const int frag = w4_frag(0, g, col & (sh.cols - 1), sh.cols);
+    const int f64 = 4 * sh.cols * 16;              // bytes of 64 columns' digits
 
-    for (int p = wave; p < pairs; p += kW4Waves) {
-        const v4i cur[2] = {next[0], next[1]};
-        if (p + kW4Waves < pairs) {
-            next[0] = load(2 * (p + kW4Waves));
-            next[1] = load(2 * (p + kW4Waves) + 1);
+    auto block = [&](v4i q, int blk, const char* base) {
+        const v4i lo = (q << 4) & (int)0xF0F0F0F0, hi = q & (int)0xF0F0F0F0;
+        v4f sc[Q];
+#pragma unroll
+        for (int j = 0; j < Q; j++) sc[j] = *(const v4f*)(scale + ((blk << LQ) + j) * 16);
+#pragma unroll
+        for (int c = 0; c < CB; c++) {
+            const char* f = base + c * fcb + frag;
+            v4i t = {0, 0, 0, 0};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const v4i b = *(const v4i*)(f + h * f64);
+                const v4i aw = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
+                if constexpr (LQ < 2) {
+                    if (LQ == 1) t = v4i{0, 0, 0, 0};
+                    t = __builtin_amdgcn_mfma_i32_16x16x64_i8(aw, b, t, 0, 0, 0);
+                    if (LQ == 1 || h == 1)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            acc[c][i] = __builtin_fmaf((float)t[i] * place, sc[LQ == 1 ? h : 0][i], acc[c][i]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const long aa = __builtin_bit_cast(long, v2i{aw[2 * e], aw[2 * e + 1]});
+                        const long bb = __builtin_bit_cast(long, v2i{b[2 * e], b[2 * e + 1]});
+                        const v4i u = __builtin_amdgcn_mfma_i32_16x16x32_i8(aa, bb, v4i{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            acc[c][i] = __builtin_fmaf((float)u[i] * place, sc[(2 * h + e) & (Q - 1)][i], acc[c][i]);
+                    }
+                }
+            }
         }
+    };
+    if constexpr (COPY) {
+        // every wavefront goes through all chunks, as they meet at each
+        const int chunks = (nblk + kW4Chunk - 1) / kW4Chunk, each = kW4Chunk / sh.split;   // its blocks in a chunk
+        fetch(min(1, chunks - 1));
+        for (int i0 = 0; i0 < chunks * each; i0 += kW4Ahead) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int blk = 2 * p + h;
-            const v4i lo = (cur[h] << 4) & (int)0xF0F0F0F0, hi = cur[h] & (int)0xF0F0F0F0;
-            const v4f sc = *(const v4f*)(s_w + ((blk << lq) + (col & (q_n - 1))) * 16 + 4 * g);
+            for (int s = 0; s < kW4Ahead; s++) {
+                const int i = i0 + s;
+                if (i >= chunks * each) break;
+                const int ch = i / each;
+                if (i > 0 && (s & (each - 1)) == 0) {
+                    // (the buffer's last readers were done before the chunk in between began)
+                    put(ch);
+                    __syncthreads();
+                    if (ch + 1 < chunks) fetch(ch + 1);
+                }
+                if (i < mine) {
+                    const int blk = part + i * sh.split;
+                    const v4i q = ring[s];
+                    ring[s] = load(i + kW4Ahead);
+                    block(q, blk, digits + (ch & 1) * CB * fcb + (blk - ch * kW4Chunk) * kBlockBytes);
+                }
+            }
+        }
+    } else {
+        for (int i0 = 0; i0 < mine; i0 += kW4Ahead) {
 #pragma unroll
-            for (int c = 0; c < CB; c++) {
-                const char* b = b_at[c] + (int64_t)blk * b_step[c];
-                v4i t = {0, 0, 0, 0};
-                t = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, *(const v4i*)b, t, 0, 0, 0);
-                t = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, *(const v4i*)(b + 64), t, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[c][i] = __builtin_fmaf((float)t[i], sc[i], acc[c][i]);
+            for (int s = 0; s < kW4Ahead; s++) {
+                if (i0 + s >= mine) break;
+                const v4i q = ring[s];
+                ring[s] = load(i0 + s + kW4Ahead);   // (behind the last block: the last again)
+                const int blk = part + (i0 + s) * sh.split;
+                block(q, blk, digits + (int64_t)blk * 2 * f64);
             }
         }
     }
 
-    // columns of a row of x: its digits, times 256^digit, and its groups
+    // a row of x: its digits' columns; then the wavefronts of a tile
 #pragma unroll
-    for (int c = 0; c < CB; c++) {
-        const float w = __builtin_amdgcn_ldexpf(1.0f, 8 * ((col >> lq) & 3));
+    for (int c = 0; c < CB; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v = acc[c][i] * w;
-            for (int o = 1; o < cols; o <<= 1) v += lane_xor_rt(v, o);
-            if ((col & (cols - 1)) == 0) red[(wave * 16 + 4 * g + i) * mt + ((c * 16 + col) >> (2 + lq))] = v;
+            float v = acc[c][i];
+            v += lane_xor<1>(v);
+            v += lane_xor<2>(v);
+            if ((col & 3) == 0) red[(wave * 16 + 4 * g + i) * (4 * CB) + 4 * c + (col >> 2)] = v;
         }
-    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * mt; i += 64 * kW4Waves) {
-        const int r = i & 15, m = i >> 4;
-        if (n0 + r >= a.n || m0 + m >= a.m) continue;
+    for (int i = threadIdx.x; i < per * 16 * 4 * CB; i += kW4Threads) {
+        const int r = i & 15, m = (i >> 4) % (4 * CB), t = (i >> 4) / (4 * CB);
+        const int64_t nn = ((int64_t)blockIdx.x * per + t) * 16 + r;
+        if (nn >= a.n || m0 + m >= a.m) continue;
         float v = 0.0f;
+        for (int p = 0; p < sh.split; p++) v += red[((t * sh.split + p) * 16 + r) * (4 * CB) + m];
+        const int e = s_exp[m];
+        v = e == kBadRow ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v, 52 - e);   // 2^e x, 2^4 w, 2^-56
+        if (a.residual) v += load1(a.residual, (m0 + m) * a.res_stride + nn, a.act);
+        store1(a.y, (m0 + m) * a.y_stride + nn, a.act, v);
+    }
+}
+
+// one 16-byte piece of the packed weights, or four scales, per thread
+__global__ __launch_bounds__(256) void pack_w4_kernel(const uint8_t* q, const void* scales, int dt, int group, int n, int k,
+                                                      char* packed) {
+    const int nblk = w4_blocks(k), tiles = w4_tiles(n), groups = w4_groups(k, group), ng = k / group;
+    const int64_t pieces = (int64_t)tiles * nblk * 64, quads = (int64_t)tiles * groups * 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces + quads; i += (int64_t)gridDim.x * 256) {
+        if (i < pieces) {
+            const int lane = (int)(i & 63), blk = (int)((i >> 6) % nblk);
+            const int64_t row = (i >> 6) / nblk * 16 + (lane & 15);
+            v4i v = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kW4Waves; w++) v += red[(w * 16 + r) * mt + m];
-        const int e = ((const int*)(scr + w4_exp_off()))[m0 + m];
-        v = e == kBadRow ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(v, -e - 4);   // the weights came as 16 w
-        if (a.residual) v += load1(a.residual, (int64_t)(m0 + m) * a.res_stride + n0 + r, a.act);
-        store1(a.y, (int64_t)(m0 + m) * a.y_stride + n0 + r, a.act, v);
+            for (int j = 0; j < 4; j++) {
+                const int byte = blk * 64 + 16 * j + 4 * (lane >> 4);
+                if (row < n && byte < k / 2) v[j] = *(const int*)(q + row * (k / 2) + byte);
+            }
+            *(v4i*)(packed + i * 16) = v;
+        } else {
+            const int64_t s = i - pieces;
+            const int64_t row = s / (groups * 4) * 16 + 4 * (s & 3);
+            const int gr = (int)((s >> 2) % groups);
+            v4f v = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (row + j < n && gr < ng) v[j] = load1(scales, (row + j) * ng + gr, dt);
+            store4(packed + pieces * 16, s * 4, dt, v);
+        }
     }
 }
 
@@ -241,37 +386,94 @@ __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* w, int64_
     if (at % group == 0) store1(scales, at / group, dt, s);
 }
 
+int log2_groups(int32_t group) { return group == 128 ? 0 : group == 64 ? 1 : 2; }
+
+// LDS of a workgroup: scales, sums, exponents, digits
+size_t w4_lds(const W4Args& a, int split, int cb, size_t digits) {
+    return (size_t)(kW4Waves / split) * w4_groups(a.k, a.group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 128 + digits;
+}
+size_t w4_chunk_lds(int cb) { return (size_t)2 * cb * kW4Chunk * 128 * 16; }
+
 }  // namespace
 
 bool w4_supported(int32_t k, int32_t group) {
     return (group == 32 || group == 64 || group == 128) && k > 0 && k % group == 0 && k / group <= kW4MaxGroups;
 }
 
-size_t w4_scratch(int32_t m, int32_t n, int32_t k, int32_t group) {
-    (void)n;
-    (void)group;
-    return w4_digit_off(m) + (size_t)m * 4 * w4_digit_stride(k);
+int64_t w4_packed_bytes(int32_t n, int32_t k, int32_t group, int32_t scale_dtype) {
+    return (int64_t)w4_tiles(n) * (w4_blocks(k) * 1024ll + w4_groups(k, group) * 16ll * (scale_dtype == DT_F32 ? 4 : 2));
 }
 
-static size_t w4_lds(int32_t k, int lq, int mt) {
-    return ((size_t)16 * (w4_blocks(k) << lq) + (size_t)kW4Waves * 16 * mt) * sizeof(float);
+size_t w4_scratch(int32_t m, int32_t k) {
+    return m <= 0 ? 0 : w4_digit_off(m) + ((size_t)m + 3) / 4 * w4_frag_bytes(k, 16);
 }
 
 hipError_t launch_linear_w4(hipStream_t s, const W4Args& a) {
     if (a.m <= 0 || a.n <= 0) return hipSuccess;
-    TL_KLAUNCH(w4_digits_kernel, dim3(a.m), dim3(512), 0, s, a);
-    const int lq = a.group == 128 ? 0 : a.group == 64 ? 1 : 2;
-    auto go = [&](auto cbt) {
+    const int tiles = w4_tiles(a.n), cbs = (a.m + 3) / 4;
+    W4Shape sh;
+    sh.cols = a.m == 1 ? 4 : a.m == 2 ? 8 : 16;
+    // Up to four rows each workgroup converts them itself where their digits fit in 64
+    // KiB: one kernel.  One row by 32000 x 2048: 12.5 us, 19.2 through scratch; four by
+    // 5632 x 2048: 9.8, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch 21.7.
+    const bool convert = cbs == 1 && w4_frag_bytes(a.k, sh.cols) <= 64 * 1024;
+    int cb = 1;
+    size_t digits;
+    if (convert) {
+        digits = w4_frag_bytes(a.k, sh.cols);
+        // wavefronts per tile: enough of them for 4 on each CU (one row by 14336 x 8192
+        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9)
+        sh.split = 1;
+        while (sh.split < kW4Waves && ((int64_t)tiles * sh.split < kW4EnoughWaves || w4_lds(a, sh.split, 1, digits) > (size_t)kW4Lds))
+            sh.split *= 2;
+    } else {
+        sh.cols = 16;
+        // What a workgroup moves through its CU: 16 CB bytes of digits and 8 of weights per
+        // tile and column of x, in as many rounds as 256 CUs need (16 rows by 32000 x 2048:
+        // 20.9 us; counted with 512 at once 24.1)
+        int64_t best = INT64_MAX;
+        for (int c : {4, 2, 1}) {
+            if (c > 1 && c / 2 >= cbs) continue;   // rows to spare
+            for (int split = 1; split <= kW4Waves; split *= 2) {
+                if (w4_lds(a, split, c, w4_chunk_lds(c)) > (size_t)kW4Lds) continue;
+                const int per = kW4Waves / split;
+                const int64_t wgs = (int64_t)((tiles + per - 1) / per) * ((cbs + c - 1) / c);
+                const int64_t cost = (wgs + 255) / 256 * (2 * c + per);
+                if (cost < best) {
+                    best = cost;
+                    cb = c;
+                    sh.split = split;
+                }
+            }
+        }
+        digits = w4_chunk_lds(cb);
+        TL_KLAUNCH(w4_digits_kernel, dim3(a.m), dim3(kW4Threads), 0, s, a);
+    }
+    const int per = kW4Waves / sh.split;
+    const dim3 grid((tiles + per - 1) / per, (cbs + cb - 1) / cb), block(kW4Threads);
+    const size_t lds = w4_lds(a, sh.split, cb, digits);
+    auto go = [&](auto cbt, auto copyt) {
         constexpr int CB = decltype(cbt)::value;
-        const int mt = (CB * 16) >> (2 + lq);
-        const dim3 grid((a.n + 15) / 16, (a.m + mt - 1) / mt);
-        TL_KLAUNCH((w4_kernel<CB>), grid, dim3(64 * kW4Waves), w4_lds(a.k, lq, mt), s, a, lq);
+        constexpr bool COPY = decltype(copyt)::value;
+        switch (log2_groups(a.group)) {
+            case 0: TL_KLAUNCH((w4_kernel<CB, 0, COPY>), grid, block, lds, s, a, sh); break;
+            case 1: TL_KLAUNCH((w4_kernel<CB, 1, COPY>), grid, block, lds, s, a, sh); break;
+            default: TL_KLAUNCH((w4_kernel<CB, 2, COPY>), grid, block, lds, s, a, sh); break;
+        }
     };
-    const int cb = ((a.m << (2 + lq)) + 15) / 16;
-    if (cb <= 1) go(std::integral_constant<int, 1>{});
-    else if (cb <= 2) go(std::integral_constant<int, 2>{});
-    else if (cb <= 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 8>{});
+    using std::integral_constant;
+    if (convert) go(integral_constant<int, 1>{}, std::false_type{});
+    else if (cb == 1) go(integral_constant<int, 1>{}, std::true_type{});
+    else if (cb == 2) go(integral_constant<int, 2>{}, std::true_type{});
+    else go(integral_constant<int, 4>{}, std::true_type{});
+    return hipGetLastError();
+}
+
+hipError_t launch_pack_w4(hipStream_t s, const uint8_t* q, const void* scales, int32_t scale_dtype, int32_t group,
+                          int32_t n, int32_t k, void* packed) {
+    const int64_t work = (int64_t)w4_tiles(n) * (w4_blocks(k) * 64ll + w4_groups(k, group) * 4ll);
+    TL_KLAUNCH(pack_w4_kernel, dim3((unsigned)std::min<int64_t>(8192, (work + 255) / 256)), dim3(256), 0, s, q, scales,
+               scale_dtype, group, n, k, (char*)packed);
     return hipGetLastError();
 }
 
@@ -284,16 +486,18 @@ hipError_t launch_quantize_w4(hipStream_t s, const float* w, int32_t rows, int32
     return hipGetLastError();
 }
 
-hipError_t init_w4_kernels() {
+template <int CB, bool COPY>
+static hipError_t init_w4() {
     hipError_t e = hipSuccess;
-    auto big = [&](const void* f) {
-        if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    };
-    big((const void*)w4_kernel<1>);
-    big((const void*)w4_kernel<2>);
-    big((const void*)w4_kernel<4>);
-    big((const void*)w4_kernel<8>);
+    for (const void* f : {(const void*)w4_kernel<CB, 0, COPY>, (const void*)w4_kernel<CB, 1, COPY>, (const void*)w4_kernel<CB, 2, COPY>})
+        if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kW4Lds);
     return e;
+}
+
+hipError_t init_w4_kernels() {
+    hipError_t e;
+    if ((e = init_w4<1, false>()) || (e = init_w4<1, true>()) || (e = init_w4<2, true>()) || (e = init_w4<4, true>())) return e;
+    return hipSuccess;
 }
 
 }  // namespace tl

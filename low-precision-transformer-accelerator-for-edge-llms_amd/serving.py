@@ -241,11 +241,28 @@ class PagedCache:
             raise _bad("a sequence, position or page is out of range")
 
 
+def quantize_w4(w, group: int = 128, scale_dtype=torch.float16, rt: Runtime | None = None):
+    """4-bit weights of float32 ones [n][k] (tl_quantize_w4_rows): (q, scales) for ``W4Linear``."""
+    if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype != torch.float32 or w.dim() != 2:
+        raise _bad("w must be a CUDA tensor [n][k] of float32")
+    if scale_dtype not in _ACT:
+        raise _bad("scales are float32, bfloat16 or float16")
+    n, k = w.shape
+    if group not in (32, 64, 128) or k == 0 or k % group:
+        raise _bad("group must be 32, 64 or 128 and divide k")
+    rt = rt or _runtime(w.device)
+    q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
+    rt.call("tl_quantize_w4_rows", w.contiguous(), n, k, group, _ACT[scale_dtype], q, scales)
+    return q, scales
+
+
 class W4Linear:
     """A projection with 4-bit weights: y = x w^T (+ residual), w[n][k] = q[n][k] *
     scales[n][k // group].  q [n][k / 2] uint8 holds two weights of -8 .. 7 (two's
     complement) in a byte, the even column in the low nibble; scales [n][k / group] are
-    float32, bfloat16 or float16; group is 32, 64 or 128."""
+    float32, bfloat16 or float16; group is 32, 64 or 128.  Both are packed here, once, into
+    the order the kernels read, and not kept."""
 
     def __init__(self, q, scales, rt: Runtime | None = None):
         if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.uint8 or q.dim() != 2 or not q.is_contiguous():
@@ -258,36 +275,26 @@ class W4Linear:
         if scales.shape[1] == 0 or self.k % scales.shape[1]:
             raise _bad("scales must hold one value for each group of a row")
         self.group = self.k // scales.shape[1]
-        self.rt = rt or _runtime(q.device)
-        if self.rt.device != q.device.index:
+        self.scale_dtype = _ACT[scales.dtype]
+        self.rt = rt = rt or _runtime(q.device)
+        if rt.device != q.device.index:
             raise _bad("the handle belongs to another device")
-        self.q, self.scales = q, scales
+        n = C.c_int64()
+        rt.check(rt.lib.tl_w4_packed_bytes(rt.h, self.n, self.k, self.group, self.scale_dtype, C.byref(n)), "W4Linear")
+        self.packed = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        rt.call("tl_pack_w4", q, scales, self.scale_dtype, self.group, self.n, self.k, self.packed)
         self._scratch: dict[int, int] = {}
-        self._scratch_bytes(1)   # the library's own checks of k and group
 
     @classmethod
     def from_float(cls, w, group: int = 128, scale_dtype=torch.float16, rt: Runtime | None = None) -> "W4Linear":
-        """Quantize float32 weights [n][k] (tl_quantize_w4_rows)."""
-        if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype != torch.float32 or w.dim() != 2:
-            raise _bad("w must be a CUDA tensor [n][k] of float32")
-        if scale_dtype not in _ACT:
-            raise _bad("scales are float32, bfloat16 or float16")
-        n, k = w.shape
-        if group not in (32, 64, 128) or k % group:
-            raise _bad("group must be 32, 64 or 128 and divide k")
-        rt = rt or _runtime(w.device)
-        w = w.contiguous()
-        q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
-        scales = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
-        rt.call("tl_quantize_w4_rows", w, n, k, group, _ACT[scale_dtype], q, scales)
-        return cls(q, scales, rt)
+        """Quantize and pack float32 weights [n][k]."""
+        return cls(*quantize_w4(w, group, scale_dtype, rt), rt)
 
     def _scratch_bytes(self, rows: int) -> int:
         got = self._scratch.get(rows)
         if got is None:
             n = C.c_int64()
-            self.rt.check(self.rt.lib.tl_linear_w4_scratch(self.rt.h, rows, self.n, self.k, self.group, C.byref(n)),
-                          "tl_linear_w4_scratch")
+            self.rt.check(self.rt.lib.tl_linear_w4_scratch(self.rt.h, rows, self.k, C.byref(n)), "tl_linear_w4_scratch")
             got = self._scratch[rows] = n.value
         return got
 
@@ -308,12 +315,11 @@ class W4Linear:
             return out
         need = self._scratch_bytes(rows)
         rt, stream = self.rt, _stream(dev)
-        scratch, _, keep = _workspace(dev, stream, need) if need else (None, None, None)
+        scratch, _, keep = _workspace(dev, stream, need)
         st = rt.lib.tl_linear_w4_async(
-            rt.h, stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows,
-            self.q.data_ptr(), self.scales.data_ptr(), _ACT[self.scales.dtype], self.group, self.n, self.k,
-            None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),
-            out.data_ptr(), _stride(out), scratch, need)
+            rt.h, stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows, self.packed.data_ptr(), self.scale_dtype,
+            self.group, self.n, self.k, None if residual is None else residual.data_ptr(),
+            0 if residual is None else _stride(residual), out.data_ptr(), _stride(out), scratch, need)
         if st:
             rt.check(st, "W4Linear")
         return out

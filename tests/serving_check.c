@@ -146,53 +146,64 @@ static void paged(void) {
 static void linear_w4(void) {
     static _Alignas(64) uint8_t w[32 * 128];
     static _Alignas(64) float x[4][256], y[4][32], r[4][32], sc[32 * 8], wf[32 * 256];
-    int64_t need;
-    expect("w4 scratch", tl_linear_w4_scratch(H, 4, 32, 256, 64, &need), TL_OK, 0);
-#define W4(xx, xs, act, m, q, s, st, grp, n, k, rr, rs, yy, ys) \
-    tl_linear_w4(H, xx, xs, act, m, q, s, st, grp, n, k, rr, rs, yy, ys)
     const int bad = TL_ERR_BAD_DESCRIPTOR, uns = TL_ERR_UNSUPPORTED;
-    const int ok = W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, r, 32, y, 32);
-    checks++;
-    wrong += ok != TL_OK || ops < 1;
-    ops = 0;
-    expect("no rows", W4(x, 256, TL_F32, 0, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), TL_OK, 0);
-    expect("int8 rows", W4(x, 256, TL_I8, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("scale type", W4(x, 256, TL_F32, 4, w, sc, TL_I8, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("negative rows", W4(x, 256, TL_F32, -1, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("no columns", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 0, 256, NULL, 0, y, 32), bad, 0);
-    expect("k 0", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 0, NULL, 0, y, 32), bad, 0);
-    expect("k 200", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 200, NULL, 0, y, 32), uns, 0);
-    expect("group 16", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 16, 32, 256, NULL, 0, y, 32), uns, 0);
-    expect("group 0", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 0, 32, 256, NULL, 0, y, 32), uns, 0);
-    expect("many groups", W4(x, 65536, TL_F32, 4, w, sc, TL_F32, 32, 32, 65536, NULL, 0, y, 32), uns, 0);
-    expect("null q", W4(x, 256, TL_F32, 4, NULL, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("misaligned q", W4(x, 256, TL_F32, 4, w + 8, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("misaligned scales", W4(x, 256, TL_F32, 4, w, (char*)sc + 2, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("null x", W4(NULL, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("null y", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, NULL, 32), bad, 0);
-    expect("short x", W4(x, 252, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("odd x", W4(x, 257, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("misaligned x", W4(&x[0][1], 256, TL_F32, 3, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("short y", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, NULL, 0, y, 31), bad, 0);
-    expect("misaligned y", W4(x, 256, TL_F32, 3, w, sc, TL_F32, 64, 32, 256, NULL, 0, (char*)y + 2, 32), bad, 0);
-    expect("short residual", W4(x, 256, TL_F32, 4, w, sc, TL_F32, 64, 32, 256, r, 31, y, 32), bad, 0);
-    expect("scratch null", tl_linear_w4_scratch(H, 4, 32, 256, 64, NULL), bad, 0);
-    expect("scratch group", tl_linear_w4_scratch(H, 4, 32, 256, 48, &need), uns, 0);
+    int64_t need = 0, size = 0;
+    expect("packed bytes", tl_w4_packed_bytes(H, 32, 256, 64, TL_F32, &size), TL_OK, 0);
+    void* wp = aligned_alloc(64, (size_t)(size + 63) / 64 * 64);
+    expect("pack", tl_pack_w4(H, w, sc, TL_F32, 64, 32, 256, wp), TL_OK, 1);
+    expect("pack null", tl_pack_w4(H, NULL, sc, TL_F32, 64, 32, 256, wp), bad, 0);
+    expect("pack null out", tl_pack_w4(H, w, sc, TL_F32, 64, 32, 256, NULL), bad, 0);
+    expect("pack misaligned", tl_pack_w4(H, w, sc, TL_F32, 64, 32, 256, (char*)wp + 8), bad, 0);
+    expect("pack misaligned q", tl_pack_w4(H, w + 2, sc, TL_F32, 64, 32, 256, wp), bad, 0);
+    expect("pack misaligned scales", tl_pack_w4(H, w, (char*)sc + 2, TL_F32, 64, 32, 256, wp), bad, 0);
+    expect("pack group", tl_pack_w4(H, w, sc, TL_F32, 48, 32, 256, wp), uns, 0);
+    expect("pack no rows", tl_pack_w4(H, w, sc, TL_F32, 64, 0, 256, wp), bad, 0);
+    expect("pack scale type", tl_pack_w4(H, w, sc, TL_I8, 64, 32, 256, wp), bad, 0);
+    expect("packed bytes null", tl_w4_packed_bytes(H, 32, 256, 64, TL_F32, NULL), bad, 0);
+    expect("packed bytes group", tl_w4_packed_bytes(H, 32, 256, 16, TL_F32, &size), uns, 0);
+#define W4(xx, xs, act, m, p, st, grp, n, k, rr, rs, yy, ys) tl_linear_w4(H, xx, xs, act, m, p, st, grp, n, k, rr, rs, yy, ys)
+    expect("w4", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, r, 32, y, 32), TL_OK, 1);
+    expect("no rows", W4(x, 256, TL_F32, 0, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), TL_OK, 0);
+    expect("int8 rows", W4(x, 256, TL_I8, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("scale type", W4(x, 256, TL_F32, 4, wp, TL_I8, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("negative rows", W4(x, 256, TL_F32, -1, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("too many rows", W4(x, 256, TL_F32, (1 << 20) + 1, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("no columns", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 0, 256, NULL, 0, y, 32), bad, 0);
+    expect("k 0", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 0, NULL, 0, y, 32), bad, 0);
+    expect("k 200", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 200, NULL, 0, y, 32), uns, 0);
+    expect("group 16", W4(x, 256, TL_F32, 4, wp, TL_F32, 16, 32, 256, NULL, 0, y, 32), uns, 0);
+    expect("group 0", W4(x, 256, TL_F32, 4, wp, TL_F32, 0, 32, 256, NULL, 0, y, 32), uns, 0);
+    expect("many groups", W4(x, 65536, TL_F32, 4, wp, TL_F32, 32, 32, 65536, NULL, 0, y, 32), uns, 0);
+    expect("null weights", W4(x, 256, TL_F32, 4, NULL, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("misaligned weights", W4(x, 256, TL_F32, 4, (char*)wp + 8, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("null x", W4(NULL, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("null y", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, NULL, 32), bad, 0);
+    expect("short x", W4(x, 252, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("odd x", W4(x, 257, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("misaligned x", W4(&x[0][1], 256, TL_F32, 3, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("short y", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 31), bad, 0);
+    expect("misaligned y", W4(x, 256, TL_F32, 3, wp, TL_F32, 64, 32, 256, NULL, 0, (char*)y + 2, 32), bad, 0);
+    expect("short residual", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, r, 31, y, 32), bad, 0);
+    expect("scratch null", tl_linear_w4_scratch(H, 4, 256, NULL), bad, 0);
+    expect("scratch rows", tl_linear_w4_scratch(H, -4, 256, &need), bad, 0);
     expect("quantize", tl_quantize_w4_rows(H, wf, 32, 256, 64, TL_F32, w, sc), TL_OK, 1);
     expect("quantize no rows", tl_quantize_w4_rows(H, wf, 0, 256, 64, TL_F32, w, sc), TL_OK, 0);
     expect("quantize null", tl_quantize_w4_rows(H, NULL, 32, 256, 64, TL_F32, w, sc), bad, 0);
     expect("quantize group", tl_quantize_w4_rows(H, wf, 32, 256, 40, TL_F32, w, sc), uns, 0);
     expect("quantize type", tl_quantize_w4_rows(H, wf, 32, 256, 64, TL_I8, w, sc), bad, 0);
     expect("quantize misaligned", tl_quantize_w4_rows(H, wf + 1, 31, 256, 64, TL_F32, w, sc), bad, 0);
-    /* scratch of the form on the caller's stream, where the shape needs it */
-    static float big[40][256], out[40][32];
-    expect("w4 scratch", tl_linear_w4_scratch(H, 40, 32, 256, 32, &need), TL_OK, 0);
-    if (need > 0) {
-        expect("async, no scratch", tl_linear_w4_async(H, NULL, big, 256, TL_F32, 40, w, sc, TL_F32, 32, 32, 256, NULL, 0,
-                                                       out, 32, NULL, need), bad, 0);
-        expect("async, short scratch", tl_linear_w4_async(H, NULL, big, 256, TL_F32, 40, w, sc, TL_F32, 32, 32, 256, NULL, 0,
-                                                          out, 32, big, need - 1), bad, 0);
-    }
+    /* the form on the caller's stream */
+    static _Alignas(64) float big[40][256], out[40][32];
+    expect("w4 scratch", tl_linear_w4_scratch(H, 40, 256, &need), TL_OK, 0);
+    char* s = aligned_alloc(64, (size_t)(need + 127) / 64 * 64);
+#define AW(scr, n) tl_linear_w4_async(H, NULL, big, 256, TL_F32, 40, wp, TL_F32, 64, 32, 256, NULL, 0, out, 32, scr, n)
+    expect("async", AW(s, need), TL_OK, 2);
+    expect("async, no scratch", AW(NULL, need), bad, 0);
+    expect("async, short scratch", AW(s, need - 1), bad, 0);
+    expect("async, misaligned scratch", AW(s + 4, need), bad, 0);
+    queued = 0;
+    free(s);
+    free(wp);
 }
 
 static void logprobs(void) {

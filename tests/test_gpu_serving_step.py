@@ -28,11 +28,10 @@ def test_steps(act, cache, tol, captured):
     start = [14, 0, 31, 5, 0]
     live = [0, 1, 2, 3, -1]                       # the last row pads the batch
 
-    def linear(n, k):
-        return serving.W4Linear.from_float(torch.randn(n, k, generator=g).cuda() / math.sqrt(k), 64, torch.float16)
-
-    wqkv, wo, head = linear((heads + 2 * kv) * hd, d), linear(d, heads * hd), linear(vocab, d)
-    w = [dense(x.q.cpu(), x.scales.cpu()) for x in (wqkv, wo, head)]
+    weights = [serving.quantize_w4(torch.randn(n, k, generator=g).cuda() / math.sqrt(k), 64, torch.float16)
+               for n, k in (((heads + 2 * kv) * hd, d), (d, heads * hd), (vocab, d))]
+    wqkv, wo, head = (serving.W4Linear(*p) for p in weights)
+    w = [dense(q.cpu(), s.cpu()) for q, s in weights]
     cos, sin = (torch.from_numpy(t) for t in build_rope_cache(128, hd, 10000.0))
     k = torch.zeros(24, kv, page, hd, dtype=dt[cache], device="cuda")
     table = torch.full((4, 5), -1, dtype=torch.int32, device="cuda")

@@ -54,7 +54,8 @@ def reference(x, q, scales, act, residual=None):
     ("f32", "f16", 128, 1, 5632, 2048), ("bf16", "bf16", 32, 13, 2048, 5632), ("f16", "f32", 64, 16, 300, 2112),
     ("f32", "f32", 32, 8, 40, 8192), ("f32", "f16", 128, 33, 70, 1280), ("bf16", "f32", 64, 100, 31, 704),
     ("f32", "f32", 128, 1, 20, 131072), ("f16", "bf16", 32, 2, 9, 32768), ("f32", "f16", 128, 32, 64, 256),
-    ("f32", "f16", 64, 7, 2000, 2048),
+    ("f32", "f16", 64, 7, 2000, 2048), ("f32", "f32", 128, 16, 8000, 2048), ("bf16", "f16", 32, 5, 20000, 512),
+    ("f32", "bf16", 64, 4, 333, 4096), ("f32", "f16", 128, 3, 33, 16384), ("f16", "f16", 32, 6, 48, 16416),
 ])
 def test_linear(serving, act, scale, group, m, n, k):
     """One row and many, widths and columns off the tiles, every group and type, strided rows, with and without a
@@ -102,6 +103,24 @@ def test_exact_integers(serving):
     assert (got[7] == 0).all()
 
 
+def test_range(serving):
+    """Scales and rows near the ends of float32's range: results that fit are right, larger ones infinite, never
+    not a number."""
+    g = torch.Generator().manual_seed(9)
+    q, _ = weights(g, 64, 256, 64, "f32")
+    s = (2.0 ** torch.linspace(-125, 127, 64)).float()[:, None].expand(64, 4).contiguous()
+    x = torch.randn(6, 256, generator=g) * torch.tensor([1, 1e30, 1e-30, 1e-8, 1e8, 2e-38])[:, None]
+    got = serving.W4Linear(q.cuda(), s.cuda())(x.cuda()).cpu().double()
+    want, tol = reference(x, q, s, "f32")
+    # the sums are kept as y 2^(e - 52), 2^e times the row's largest in [2^29, 2^30): each of the 4 groups' additions
+    # may lose 2^-150 there, up to 2^-150 2^52 max|x| / 2^29 = 2^-127 max|x| of y, for each of 4 digits
+    tol = tol + 16 * 2.0 ** -127 * x.double().abs().amax(1, keepdim=True)
+    big = want.abs() > 3.5e38
+    assert not torch.isnan(got).any() and (got[big] == torch.sign(want[big]) * float("inf")).all()
+    fits = want.abs() < 3.3e38
+    assert ((got - want).abs() <= tol)[fits].all()
+
+
 def test_special_values(serving):
     """An infinity or NaN makes its row NaN and no other; infinite and NaN scales reach their output."""
     g = torch.Generator().manual_seed(2)
@@ -125,20 +144,23 @@ def test_quantizer(serving, scale, group):
     w[3, :group] = 0
     w[4, group:2 * group] = 1e-30
     w[5, 0] = 3e38
-    lin = serving.W4Linear.from_float(w.cuda(), group, DT[scale])
+    got_q, got_s = serving.quantize_w4(w.cuda(), group, DT[scale])
     v = w.view(37, -1, group)
     s = (v.abs().amax(-1) / np.float32(7)).float()
     s = (s.clamp_max(65504.0) if scale == "f16" else s).to(DT[scale])
     zero = s == 0
     s = torch.where(zero, torch.ones_like(s), s)
     want = torch.where(zero[..., None], torch.zeros_like(v), (v / s.float()[..., None]).round().clamp(-8, 7))
-    assert torch.equal(lin.scales.cpu(), s.view(37, -1))
-    q = lin.q.cpu().to(torch.int64)
+    assert torch.equal(got_s.cpu(), s.view(37, -1))
+    q = got_q.cpu().to(torch.int64)
     got = torch.stack([q & 15, q >> 4], -1).view(37, -1)
     got = torch.where(got > 7, got - 16, got)
     assert torch.equal(got, want.view(37, -1).to(torch.int64))
+    x = torch.randn(3, 384, generator=g).cuda()
+    same = serving.W4Linear.from_float(w.cuda(), group, DT[scale])(x)
+    assert torch.equal(same, serving.W4Linear(got_q, got_s)(x))
     # within half a step of a weight, except where +-8 is clipped (the scales are rounded down)
-    err = (dense(lin.q.cpu(), lin.scales.cpu()).view_as(v) - v.double()).abs()
+    err = (dense(got_q.cpu(), got_s.cpu()).view_as(v) - v.double()).abs()
     inside = ~zero[..., None] & ((v / s.float()[..., None]).abs() <= 7.4)
     assert (err[inside] <= (0.5 + 1e-5) * s.double()[..., None].expand_as(err)[inside]).all()
 
@@ -152,7 +174,7 @@ def test_completing_form_and_graph(serving):
     want = lin(x)
     rt = runtime()
     y = torch.zeros_like(want)
-    rt.call("tl_linear_w4", x, 1024, 0, 9, lin.q, lin.scales, 1, 64, 200, 1024, None, 0, y, 200)
+    rt.call("tl_linear_w4", x, 1024, 0, 9, lin.packed, 1, 64, 200, 1024, None, 0, y, 200)
     assert torch.equal(y, want)
     rt.close()
     graphs = []
@@ -190,7 +212,7 @@ def test_refusals(serving):
                 lambda: lin(x, residual=torch.zeros(2, 24, dtype=torch.float16, device="cuda")),
                 lambda: lin(torch.zeros(2, 259, device="cuda")[:, 3:]), lambda: lin(x.t().contiguous().t()),
                 lambda: serving.W4Linear.from_float(x, 48), lambda: serving.W4Linear.from_float(x.half()),
-                lambda: serving.W4Linear.from_float(x, 64, torch.float64)):
+                lambda: serving.quantize_w4(x, 64, torch.float64), lambda: serving.quantize_w4(x.cpu())):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
     assert lin(x[:0]).shape == (0, 24)

@@ -347,9 +347,10 @@ def token_logprobs(logits, targets, top: int = 0, rt: Runtime | None = None) -> 
     ids = _ints("targets", targets, dev, rows)
     if not 0 <= top <= min(32, vocab) or vocab == 0:
         raise _bad("top must be 0 .. 32 and at most the vocabulary")
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev)
-    best = torch.empty((2, rows, top), dtype=torch.int32, device=dev)
-    got = TokenLogprobs(stats[0], stats[1], best[0], best[1].view(torch.float32))
+    logprob, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
+    best = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    best_lp = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    got = TokenLogprobs(logprob, entropy, best, best_lp)
     if rows == 0:
         return got
     rt = rt or _runtime(dev)
@@ -360,12 +361,12 @@ def token_logprobs(logits, targets, top: int = 0, rt: Runtime | None = None) -> 
         n = C.c_int64()
         rt.check(rt.lib.tl_token_logprobs_scratch(rt.h, rows, vocab, top, C.byref(n)), "tl_token_logprobs_scratch")
         need = _LOGPROBS_SCRATCH[(rows, vocab, top)] = n.value
-    at, ib, stream = stats.data_ptr(), best.data_ptr(), _stream(dev)
+    stream = _stream(dev)
     scratch, counters, keep = _workspace(dev, stream, need)
     st = rt.lib.tl_token_logprobs_async(
         rt.h, stream, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
-        _ACT[logits.dtype], rows, vocab, ids, top, at, at + 4 * rows, ib, ib + 4 * rows * top,
-        scratch, need, counters, None)
+        _ACT[logits.dtype], rows, vocab, ids, top, logprob.data_ptr(), entropy.data_ptr(),
+        best.data_ptr(), best_lp.data_ptr(), scratch, need, counters, None)
     if st:
         rt.check(st, "token_logprobs")
     return got

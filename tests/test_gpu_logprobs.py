@@ -162,6 +162,40 @@ def test_graph(serving):
         check(got, data, ids, 9)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab,top", [
+    ("f32", 1, 32000, 5), ("bf16", 20, 32000, 32), ("f32", 70, 16001, 20), ("f16", 130, 16385, 3), ("bf16", 300, 16500, 32),
+    ("f32", 3, 300007, 0)])
+def test_joined_in_place_or_not(serving, dtype, rows, vocab, top):
+    """Rows whose parts the last workgroup joins and rows joined by a kernel of their own: a captured call, which has
+    no counters, gives the same bits."""
+    rng = np.random.default_rng(rows)
+    t = torch.from_numpy((rng.standard_normal((rows, vocab)) * 2).astype(np.float32)).to(DT[dtype])
+    t[rows // 2, ::3] = 1.5           # more equal logits than a part's room for candidates
+    t[rows // 3, 50:] = -float("inf")
+    targets = rng.integers(0, vocab, rows).astype(np.int32)
+    x, ids = t.cuda(), torch.from_numpy(targets).cuda()
+    first = serving.token_logprobs(x, ids, top)
+    check(first, t.float().numpy(), targets, top)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = serving.token_logprobs(x, ids, top)
+    for _ in range(3):
+        graph.replay()
+        again = serving.token_logprobs(x, ids, top)
+        torch.cuda.synchronize()
+        for a, b, c in zip(first, captured, again):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_large_logits(serving):
+    """Rows far from zero, on both sides of where the difference to the maximum is taken first."""
+    rng = np.random.default_rng(8)
+    shifts = [0, 90, -90, 4090, 4101, -4090, -4110, 65504, -1e5, 3e7, -3e7, 1e12, 3.4e38, -3.4e38]
+    x = np.stack([rng.standard_normal(9000) * 2 + s for s in shifts]).astype(np.float32)
+    targets = rng.integers(0, 9000, len(x)).astype(np.int32)
+    check(serving.token_logprobs(torch.from_numpy(x).cuda(), torch.from_numpy(targets).cuda(), 12), x, targets, 12)
+
+
 def test_engine_score_tokens():
     """A prompt scored by the engine: its tokens' log probabilities are those of the engine's own logits."""
     import oracle

@@ -20,7 +20,11 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 // A workgroup takes 256 units of one row: a unit is four rotated pairs (d ..
 // d + 3 and their partners half a head on), or eight values of v.  Nothing is
 // read twice from memory; the row's cos and sin are shared by its heads through
-// the cache.
+// the cache.  What bounds it: from one row to some hundreds the chain of loads and
+// the launch (3.5 us for 1 row as for 61); 2048 rows of 32 + 2 x 8 heads of 128 in
+// float16 take 11.5 us (3.0 TB/s).  A row's values are loaded before its place is
+// known, and the activations' type is the compiler's: with the type looked at per
+// load, loads wait for each other, 12.7 us.
 // ---------------------------------------------------------------------------
 TL_DEV void cache_store4(void* base, int64_t i, int dt, v4f v, float s) {
     if (dt != DT_I8) {
@@ -33,9 +37,21 @@ TL_DEV void cache_store4(void* base, int64_t i, int dt, v4f v, float s) {
     *(unsigned*)((int8_t*)base + i) = w;
 }
 
+template <int ACT>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     const PagedGeom& g = a.c.g;
     const int row = blockIdx.x;
+    const int hd = g.head_dim, half = hd >> 1, quads = half >> 2;
+    const int n_rot = (a.n_heads + g.n_kv) * quads;
+    const int u = blockIdx.y * 256 + threadIdx.x;
+    const bool rotate = u < n_rot;
+    const int head = rotate ? u / quads : a.n_heads + g.n_kv, w = (u - n_rot) * 8;   // (v: the head's place from w)
+    const int d = rotate ? (u - head * quads) * 4 : w;
+    if (!rotate && w >= g.n_kv * hd) return;
+    if (head < a.n_heads && !a.q_out) return;
+    // the values, on their way while the row's place is looked up
+    const int64_t at = (int64_t)row * a.qkv_stride + (int64_t)head * hd + d;
+    const v4f x1 = load4(a.qkv, at, ACT), x2 = load4(a.qkv, at + (rotate ? half : 4), ACT);
     const int seq = a.row_seq ? a.row_seq[row] : row;
     const int pos = a.row_pos[row];
     const PagedRow kind = paged_row_kind(g, seq, pos);
@@ -43,18 +59,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     // a position needs its rotation and, for k and v, its page
     const int page = kind == PAGED_ROW_OK && pos >= 0 && pos < a.n_pos ? paged_page(g, seq, pos) : -1;
     if (page < 0) {
-        if (a.fault && threadIdx.x == 0 && blockIdx.y == 0) *a.fault = 1;
+        if (a.fault) *a.fault = 1;
         return;
     }
-    const int hd = g.head_dim, half = hd >> 1, quads = half >> 2;
-    const int n_rot = (a.n_heads + g.n_kv) * quads;
-    const int u = blockIdx.y * 256 + threadIdx.x;
-    const int64_t in = (int64_t)row * a.qkv_stride;
-    if (u < n_rot) {
-        const int head = u / quads, d = (u - head * quads) * 4;
-        if (head < a.n_heads && !a.q_out) return;
-        const int64_t at = in + (int64_t)head * hd + d;
-        const v4f x1 = load4(a.qkv, at, a.act), x2 = load4(a.qkv, at + half, a.act);
+    if (rotate) {
         const float* c = a.cos + (int64_t)pos * hd + d;
         const float* s = a.sin + (int64_t)pos * hd + d;
         const v4f c1 = *(const v4f*)c, c2 = *(const v4f*)(c + half), s1 = *(const v4f*)s, s2 = *(const v4f*)(s + half);
@@ -66,8 +74,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         }
         if (head < a.n_heads) {
             const int64_t to = (int64_t)row * a.q_stride + (int64_t)head * hd + d;
-            store4(a.q_out, to, a.act, y1);
-            store4(a.q_out, to + half, a.act, y2);
+            store4(a.q_out, to, ACT, y1);
+            store4(a.q_out, to + half, ACT, y2);
         } else {
             const int kvh = head - a.n_heads;
             const float sk = a.c.dtype == DT_I8 ? a.c.ks[kvh] : 1.0f;
@@ -77,14 +85,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         }
         return;
     }
-    const int w = (u - n_rot) * 8;
-    if (w >= g.n_kv * hd) return;
-    const int kvh = w / hd, d = w - kvh * hd;
-    const int64_t at = in + (int64_t)(a.n_heads + g.n_kv) * hd + w;
+    const int kvh = w / hd;
     const float sv = a.c.dtype == DT_I8 ? a.c.vs[kvh] : 1.0f;
-    const int64_t to = paged_row(g, page, kvh, pos) + d;
-    cache_store4(a.c.v, to, a.c.dtype, load4(a.qkv, at, a.act), sv);
-    cache_store4(a.c.v, to + 4, a.c.dtype, load4(a.qkv, at + 4, a.act), sv);
+    const int64_t to = paged_row(g, page, kvh, pos) + (w - kvh * hd);
+    cache_store4(a.c.v, to, a.c.dtype, x1, sv);
+    cache_store4(a.c.v, to + 4, a.c.dtype, x2, sv);
 }
 
 // ---------------------------------------------------------------------------
@@ -832,7 +837,10 @@ int32_t head_blocks(int32_t n_heads, int32_t n_kv) { return (n_heads / n_kv + 7)
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a) {
     if (a.rows <= 0) return hipSuccess;
     const int units = (a.n_heads + a.c.g.n_kv) * (a.c.g.head_dim / 8) + a.c.g.n_kv * a.c.g.head_dim / 8;
-    TL_KLAUNCH(paged_append_kernel, dim3(a.rows, (units + 255) / 256), dim3(256), 0, s, a);
+    const dim3 grid(a.rows, (units + 255) / 256), block(256);
+    if (a.act == DT_F32) TL_KLAUNCH((paged_append_kernel<DT_F32>), grid, block, 0, s, a);
+    else if (a.act == DT_BF16) TL_KLAUNCH((paged_append_kernel<DT_BF16>), grid, block, 0, s, a);
+    else TL_KLAUNCH((paged_append_kernel<DT_F16>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 

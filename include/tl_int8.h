@@ -318,7 +318,7 @@ int32_t tl_pack_w4(tl_handle *h, const uint8_t *q, const void *scales, int32_t s
  * rows 16-byte aligned.  A row of x is taken as integers of 2^-30 of its largest
  * magnitude, products are exact, sums float32; an infinity or NaN in a row of x makes
  * its whole row of y NaN.  Few rows (a decoding step) are what it is made for; up to
- * 2^20 are right. */
+ * 2^17 are right.  n at most 2^24, n k below 2^35. */
 int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
                      int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void *residual,
                      int64_t res_stride, void *y, int64_t y_stride);

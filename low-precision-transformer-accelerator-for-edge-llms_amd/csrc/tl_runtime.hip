@@ -2382,7 +2382,7 @@ int32_t paged_cache_arg(tl_handle* h, const tl_paged_cache* c, PagedCache* out) 
 // rows of an append or attention call
 int32_t check_paged_rows(tl_handle* h, int32_t act, int32_t rows, const int32_t* row_pos) {
     TL_REQ(h, act_type(act), "activations must be float32, bfloat16 or float16");
-    TL_REQ(h, rows >= 0, "negative row count");
+    TL_REQ(h, rows >= 0 && rows < 1 << 24, "row count outside 0 .. 2^24 - 1");
     TL_REQ(h, row_pos || rows == 0, "null row_pos");
     return TL_OK;
 }
@@ -2427,6 +2427,7 @@ int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q,
 int32_t w4_shape(tl_handle* h, int32_t n, int32_t k, int32_t group, int32_t scale_dtype) {
     TL_REQ(h, act_type(scale_dtype), "scales must be float32, bfloat16 or float16");
     TL_REQ(h, n >= 1 && k >= 1, "empty weights");
+    TL_REQ(h, n <= 1 << 24 && (int64_t)n * k < (int64_t)1 << 35, "more than 2^24 rows or 2^35 weights");
     if (!w4_supported(k, group))
         return fail(h, TL_ERR_UNSUPPORTED, "group must be 32, 64 or 128 and k a multiple of it, at most 1024 groups");
     return TL_OK;
@@ -2438,7 +2439,7 @@ int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int3
     int32_t r = w4_shape(h, n, k, group, scale_dtype);
     if (r) return r;
     TL_REQ(h, act_type(act), "rows must be float32, bfloat16 or float16");
-    TL_REQ(h, m >= 0 && m <= 1 << 20, "row count outside 0 .. 2^20");
+    TL_REQ(h, m >= 0 && m <= 1 << 17, "row count outside 0 .. 2^17");
     TL_REQ(h, packed && aligned16(packed), "packed weights missing or misaligned");
     TL_REQ(h, (x && y) || m == 0, "null x or y");
     if ((r = check_rows(h, x, x_stride, k, act, "x"))) return r;
@@ -2457,6 +2458,8 @@ int32_t logprobs_args(tl_handle* h, const void* logits, int64_t stride, int32_t 
     TL_REQ(h, act_type(dtype), "logits must be float32, bfloat16 or float16");
     TL_REQ(h, rows >= 0 && vocab >= 1 && vocab <= 1 << 28, "row count or vocabulary out of range");
     TL_REQ(h, top >= 0 && top <= kMaxTop && top <= vocab, "top must be 0 .. 32 and at most the vocabulary");
+    if (logprobs_workgroups(rows, vocab, top) >= 1 << 24)
+        return fail(h, TL_ERR_UNSUPPORTED, "2^24 or more parts of 8192 logits over all rows");
     TL_REQ(h, rows == 0 || (logits && targets && logprob && (top == 0 || (top_ids && top_logprobs))), "null pointer");
     TL_REQ(h, stride >= vocab && (uintptr_t)logits % type_size(dtype) == 0, "logits: rows must not overlap and must be aligned");
     a->logits = logits; a->stride = stride; a->dtype = dtype; a->rows = rows; a->vocab = vocab; a->top = top;
@@ -2578,7 +2581,7 @@ int32_t tl_linear_w4_async(tl_handle* h, void* stream, const void* x, int64_t x_
 
 int32_t tl_linear_w4_scratch(tl_handle* h, int32_t m, int32_t k, int64_t* bytes) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
-    TL_REQ(h, bytes && m >= 0 && m <= 1 << 20 && k >= 1 && k <= 1 << 17, "bad scratch arguments");
+    TL_REQ(h, bytes && m >= 0 && m <= 1 << 17 && k >= 1 && k <= 1 << 17, "bad scratch arguments");
     *bytes = (int64_t)w4_scratch(m, k);
     return TL_OK;
 }
@@ -2609,7 +2612,7 @@ int32_t tl_quantize_w4_rows(tl_handle* h, const float* w, int32_t rows, int32_t 
                             uint8_t* q, void* scales) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     TL_REQ(h, rows >= 0, "negative row count");
-    const int32_t r = w4_shape(h, 1, n, group, scale_dtype);
+    const int32_t r = w4_shape(h, std::max(rows, 1), n, group, scale_dtype);
     if (r) return r;
     TL_REQ(h, w && q && scales && aligned16(w) && ((uintptr_t)q & 3) == 0 && (uintptr_t)scales % type_size(scale_dtype) == 0,
            "null or misaligned pointer");

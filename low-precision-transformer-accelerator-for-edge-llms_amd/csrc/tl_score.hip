@@ -461,6 +461,8 @@ Cut cut_of(int32_t rows, int32_t vocab, int32_t top) {
 
 }  // namespace
 
+int64_t logprobs_workgroups(int32_t rows, int32_t vocab, int32_t top) { return (int64_t)rows * cut_of(rows, vocab, top).parts; }
+
 size_t logprobs_scratch(int32_t rows, int32_t vocab, int32_t top) {
     const Cut c = cut_of(rows, vocab, top);
     return c.parts <= 1 ? 0 : (size_t)rows * c.parts * (2 + kept_of(top)) * 8;

@@ -184,6 +184,7 @@ struct LogprobsArgs {
     int32_t* fault;            // set to 1 by a target from vocab on, or null
 };
 constexpr int32_t kMaxTop = 32;
+int64_t logprobs_workgroups(int32_t rows, int32_t vocab, int32_t top);
 size_t logprobs_scratch(int32_t rows, int32_t vocab, int32_t top);
 hipError_t launch_token_logprobs(hipStream_t s, const LogprobsArgs& a);
 

@@ -80,6 +80,7 @@ static void paged(void) {
 #define APP(what, ...) expect("append: " what, tl_paged_append(H, &c, __VA_ARGS__), TL_ERR_BAD_DESCRIPTOR, 0)
     APP("null qkv", NULL, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
     APP("int8 rows", qkv, w, TL_I8, 4, HEADS, seq, pos, cs, sn, 64, q, qw);
+    APP("too many rows", qkv, w, TL_F32, 1 << 24, HEADS, seq, pos, cs, sn, 64, q, qw);
     APP("negative rows", qkv, w, TL_F32, -1, HEADS, seq, pos, cs, sn, 64, q, qw);
     APP("negative heads", qkv, w, TL_F32, 4, -1, seq, pos, cs, sn, 64, q, qw);
     APP("null pos", qkv, w, TL_F32, 4, HEADS, seq, NULL, cs, sn, 64, q, qw);
@@ -157,6 +158,8 @@ static void linear_w4(void) {
     expect("pack misaligned q", tl_pack_w4(H, w + 2, sc, TL_F32, 64, 32, 256, wp), bad, 0);
     expect("pack misaligned scales", tl_pack_w4(H, w, (char*)sc + 2, TL_F32, 64, 32, 256, wp), bad, 0);
     expect("pack group", tl_pack_w4(H, w, sc, TL_F32, 48, 32, 256, wp), uns, 0);
+    expect("pack too many rows", tl_pack_w4(H, w, sc, TL_F32, 64, (1 << 24) + 1, 256, wp), bad, 0);
+    expect("pack too many weights", tl_pack_w4(H, w, sc, TL_F32, 64, 1 << 24, 4096, wp), bad, 0);
     expect("pack no rows", tl_pack_w4(H, w, sc, TL_F32, 64, 0, 256, wp), bad, 0);
     expect("pack scale type", tl_pack_w4(H, w, sc, TL_I8, 64, 32, 256, wp), bad, 0);
     expect("packed bytes null", tl_w4_packed_bytes(H, 32, 256, 64, TL_F32, NULL), bad, 0);
@@ -167,7 +170,7 @@ static void linear_w4(void) {
     expect("int8 rows", W4(x, 256, TL_I8, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
     expect("scale type", W4(x, 256, TL_F32, 4, wp, TL_I8, 64, 32, 256, NULL, 0, y, 32), bad, 0);
     expect("negative rows", W4(x, 256, TL_F32, -1, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
-    expect("too many rows", W4(x, 256, TL_F32, (1 << 20) + 1, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
+    expect("too many rows", W4(x, 256, TL_F32, (1 << 17) + 1, wp, TL_F32, 64, 32, 256, NULL, 0, y, 32), bad, 0);
     expect("no columns", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 0, 256, NULL, 0, y, 32), bad, 0);
     expect("k 0", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 0, NULL, 0, y, 32), bad, 0);
     expect("k 200", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 200, NULL, 0, y, 32), uns, 0);
@@ -213,7 +216,8 @@ static void logprobs(void) {
     int64_t need;
 #define LP(x, st, dt, rows, v, t, top, lp, h, ids, tl) tl_token_logprobs(H, x, st, dt, rows, v, t, top, lp, h, ids[0], tl[0])
     expect("logprobs, one part", LP(x, 20000, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), TL_OK, 1);
-    expect("logprobs", LP(x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids, tl), TL_OK, 2);
+    expect("logprobs, joined in place", LP(x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids, tl), TL_OK, 1);
+    expect("logprobs, a join", LP(x, 20000, TL_F32, 600, 20000, t, 8, lp, h, ids, tl), TL_OK, 2);
     expect("odd stride", LP((char*)x + 2, 19999, TL_F16, 2, 5000, t, 8, lp, h, ids, tl), TL_OK, 1);
     expect("no rows", LP(x, 20000, TL_F32, 0, 20000, t, 8, lp, h, ids, tl), TL_OK, 0);
     expect("no entropy", LP(x, 20000, TL_F32, 2, 5000, t, 8, lp, NULL, ids, tl), TL_OK, 1);
@@ -230,12 +234,14 @@ static void logprobs(void) {
     expect("vocab above 2^28", LP(x, 1 << 30, TL_F32, 2, (1 << 28) + 1, t, 0, lp, h, ids, tl), bad, 0);
     expect("overlapping rows", LP(x, 4999, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
     expect("misaligned", LP((char*)x + 2, 20000, TL_F32, 2, 5000, t, 8, lp, h, ids, tl), bad, 0);
+    expect("too many rows", LP(x, 5000, TL_F32, 1 << 24, 5000, t, 8, lp, h, ids, tl), TL_ERR_UNSUPPORTED, 0);
+    expect("too many parts", LP(x, 20000, TL_F32, 1 << 23, 20000, t, 8, lp, h, ids, tl), TL_ERR_UNSUPPORTED, 0);
     expect("negative rows", LP(x, 20000, TL_F32, -2, 5000, t, 8, lp, h, ids, tl), bad, 0);
     expect("scratch", tl_token_logprobs_scratch(H, 2, 20000, 8, &need), TL_OK, 0);
     static char s[4096];
     char* a = (char*)(((uintptr_t)s + 63) & ~(uintptr_t)63);
     checks++;
-    wrong += need <= 0 || need > 2048;
+    wrong += need <= 0 || need > 4000;
 #define AS(scr, n) tl_token_logprobs_async(H, NULL, x, 20000, TL_F32, 2, 20000, t, 8, lp, h, ids[0], tl[0], scr, n, NULL, NULL)
     expect("async", AS(a, need), TL_OK, 2);
     expect("async, no scratch", AS(NULL, need), bad, 0);

@@ -146,6 +146,42 @@ def test_attention(serving, act, cache, heads, kv, hd, page, positions):
             assert (got[i] == 0).all()
 
 
+@pytest.mark.parametrize("rows,longest,cache,kv,heads", [
+    (65, 700, "i8", 2, 8), (130, 300, "f16", 1, 16), (257, 260, "i8", 1, 9), (600, 150, "bf16", 2, 4),
+    (20, 12000, "f16", 1, 8)])       # the last: one row of 94 parts among short ones
+def test_attention_many_rows(serving, rows, longest, cache, kv, heads):
+    """Rows past one lane each and past one workgroup's threads, padded ones and ones without keys among them; parts
+    joined in place and, captured, by a kernel of their own."""
+    seqs = min(rows, 24)
+    lengths = [longest if i == seqs // 2 else 1 + (i * 37) % min(longest, 140) for i in range(seqs)]
+    built = build(cache, kv, 64, 16, lengths, seed=rows, stale=0.0)
+    c = make(serving, built)
+    g = built[4]
+    seq = [i % seqs if i % 11 != 3 else -1 for i in range(rows)]
+    pos = [-1 if i % 13 == 5 else lengths[s] - 1 - (i // seqs) % lengths[s] for i, s in enumerate(seq)]
+    q = torch.randn(rows, heads * 64, generator=g)
+    ids = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (seq, pos)]
+    want, tol = attention_reference(q, built, seq, pos, 16, 0.125, "f32", cache)
+    qd = q.cuda()
+    out = torch.full((rows, heads * 64), 5.0, device="cuda")
+    c.attend(qd, *ids, out=out)
+    graph = torch.cuda.CUDAGraph()
+    captured = torch.full((rows, heads * 64), 5.0, device="cuda")
+    with torch.cuda.graph(graph):
+        c.attend(qd, *ids, out=captured)
+    for _ in range(3):
+        graph.replay()
+        c.attend(qd, *ids, out=out)
+        c.check()
+        for o in (out, captured):
+            got = o.cpu().double()
+            for r in range(rows):
+                if seq[r] < 0:
+                    assert (got[r] == 5.0).all()
+                    got[r] = 0
+            assert torch.isfinite(got).all() and ((got - want).abs() <= tol + 1e-300).all()
+
+
 def test_attention_completing_form_and_causal_rows(serving):
     """tl_paged_attention (the handle's stream and scratch) gives the same bits; several rows of one sequence
     at rising positions are causal attention; padded rows stay as they were."""

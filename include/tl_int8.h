@@ -227,14 +227,14 @@ int32_t tl_lm_head_argmax(tl_handle *h, const float *x, int32_t *token, float *l
  *   counters  dev, TL_OP_COUNTERS int32 that are zero when the kernels start, and
  *             are zero again when they are done; one each for calls that may
  *             run at the same time, graphs that hold them included.  With them
- *             the parts of a result are joined by the workgroup that finishes
- *             last, without them (NULL) by a second kernel, to the same bits.
+ *             the parts of a result may be joined by the workgroup that finishes
+ *             last, without them (NULL) a second kernel does it: attention's
+ *             sums of parts then round in another order.
  *   fault     dev int32 or NULL.
- * What a call
- * finds wrong on the device (a sequence, position, page or token id out of its
- * range) is left out: nothing is read or written outside the buffers.  tl_x then
- * returns TL_ERR_BAD_DESCRIPTOR after completing; tl_x_async sets *fault to 1
- * (and never clears it). */
+ * What a call finds wrong on the device (a sequence, position, page or token id
+ * out of its range) is left out: nothing is read or written outside the buffers.
+ * tl_x then returns TL_ERR_BAD_DESCRIPTOR after completing; tl_x_async sets *fault
+ * to 1 (and never clears it).  Up to 2^24 - 1 rows (tl_linear_w4: 2^17). */
 #define TL_OP_COUNTERS 16384
 typedef enum tl_dtype { TL_F32 = 0, TL_BF16 = 1, TL_F16 = 2, TL_I8 = 3 } tl_dtype;
 
@@ -336,7 +336,8 @@ int32_t tl_linear_w4_scratch(tl_handle *h, int32_t m, int32_t k, int64_t *bytes)
  * probabilities: top_ids, top_logprobs [rows][top].  Outputs int32 and float32, all dev.  A
  * logit of minus infinity has probability 0.  A row without a finite maximum or with a
  * NaN has no distribution: its log probabilities and entropy are NaN, NaN logits are
- * no alternatives, and where too few are left the id is -1.  vocab at most 2^28. */
+ * no alternatives, and where too few are left the id is -1.  vocab at most 2^28;
+ * below 2^24 parts of up to 8192 logits over all rows. */
 int32_t tl_token_logprobs(tl_handle *h, const void *logits, int64_t stride, int32_t dtype, int32_t rows,
                           int32_t vocab, const int32_t *targets, int32_t top, float *logprob, float *entropy,
                           int32_t *top_ids, float *top_logprobs);

@@ -200,6 +200,13 @@ def load_library() -> C.CDLL:
         fn = getattr(L, name)
         fn.restype = res
         fn.argtypes = args
+    # calls that only queue work keep the interpreter lock: threads may share their handle
+    held = C.PyDLL(LIB_PATH)
+    for name in SIGNATURES:
+        if name.endswith("_async"):
+            fn = getattr(held, name)
+            fn.restype, fn.argtypes = SIGNATURES[name]
+            setattr(L, name, fn)
     _lib = L
     return L
 

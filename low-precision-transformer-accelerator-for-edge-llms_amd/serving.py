@@ -6,10 +6,12 @@ rotation and the INT8 cache follow its accelerator path (design_decisions A7/B2)
 Every call here queues its kernels on torch's current stream of the tensors'
 device and returns, as torch's own operations do (the ``_async`` entry points of
 include/tl_int8.h): results may be used by later work on that stream, and calls
-can be captured into a ``torch.cuda.CUDAGraph``.  Scratch memory
-is torch's, kept for each stream, and a captured graph has its own, so calls on
-different streams and graphs share none.  Tensors are CUDA tensors of one device; float types are
-float32, bfloat16 and float16.
+can be captured into a ``torch.cuda.CUDAGraph`` (but the first on a device).  Scratch
+memory is torch's, kept for each stream, and a captured graph has its own, so calls
+on different streams and graphs share none; threads may call at the same time.  A
+captured call joins the parts of a long row in another order than a queued one does,
+so attention may differ between them in the last place.  Tensors are CUDA tensors of
+one device; float types are float32, bfloat16 and float16.
 
 What a call finds out of range on the device (a sequence, position, page or token
 id) it leaves out; ``check()`` tells.  Wrong types, shapes and layouts raise
@@ -37,6 +39,8 @@ def _runtime(device: torch.device) -> Runtime:
     rt = _HANDLES.get(device.index)
     if rt is None:
         with torch.cuda.device(device):
+            if torch._C._cuda_isCurrentStreamCapturing():
+                raise _bad("the first call on a device cannot be captured: make it once before")
             rt = Runtime(dict(hidden=64, intermediate=64, n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, vocab=64,
                               max_pos=64, rms_eps=1e-5, rope_theta=10000.0))
         _HANDLES[device.index] = rt
@@ -68,11 +72,13 @@ def _workspace(dev: torch.device, stream: int, need: int):
         return own.data_ptr() if need else None, None, own
     ws = _WORKSPACES.get((dev.index, stream))
     if ws is None:
-        ws = _WORKSPACES[(dev.index, stream)] = _Workspace(dev)
-    if ws.scratch.shape[0] < need:
-        # (the allocator gives the old block to this stream's later work only)
-        ws.scratch = torch.empty(need + need // 4, dtype=torch.uint8, device=dev)
-    return ws.scratch.data_ptr(), ws.counters.data_ptr(), ws
+        ws = _WORKSPACES.setdefault((dev.index, stream), _Workspace(dev))
+    scratch = ws.scratch
+    if scratch.shape[0] < need:
+        # (the allocator gives the old block to this stream's later work only, and not
+        # before another thread's call that holds it is queued)
+        scratch = ws.scratch = torch.empty(need + need // 4, dtype=torch.uint8, device=dev)
+    return scratch.data_ptr(), ws.counters.data_ptr(), scratch
 
 
 def _bad(message: str):

@@ -105,3 +105,72 @@ def test_steps(act, cache, tol, captured):
         assert torch.isfinite(logits).all() and (att[4] == 0).all()
     c.check()
     assert worst < tol, worst
+
+
+def test_threads_and_streams():
+    """Threads that call at the same time, on streams of their own and on one they share, with sizes that make the
+    shared workspace grow: every call gives what it gives alone."""
+    import threading
+    from lpta import serving
+    g = torch.Generator().manual_seed(2)
+    lin = serving.W4Linear(*serving.quantize_w4(torch.randn(256, 512, generator=g).cuda()))
+    k, v = (torch.randn(260, 1, 16, 64, generator=g).half().cuda() for _ in range(2))
+    table = torch.arange(260, dtype=torch.int32, device="cuda").view(2, 130)
+    cache = serving.PagedCache(k, v, table)
+    jobs = []
+    for n in range(4):
+        x = torch.randn(3 + 5 * n, 512, generator=g).cuda()
+        logits = torch.randn(4 + 9 * n, 20000 + 7777 * n, generator=g).cuda()
+        ids = torch.randint(0, 20000, (len(logits),), generator=g, dtype=torch.int32).cuda()
+        q = torch.randn(1 + n, 256, generator=g).cuda()
+        seq = torch.arange(1 + n, dtype=torch.int32, device="cuda") % 2
+        pos = torch.full((1 + n,), 900 + 300 * n, dtype=torch.int32, device="cuda")
+
+        def job(x=x, logits=logits, ids=ids, q=q, seq=seq, pos=pos, n=n):
+            return [lin(x), *serving.token_logprobs(logits, ids, 3 * n), cache.attend(q, seq, pos)]
+        jobs.append(job)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    shared = torch.cuda.Stream()
+    for own in (False, True):
+        got, errors = [[] for _ in jobs], []
+
+        def work(n):
+            try:
+                stream = torch.cuda.Stream() if own else shared
+                with torch.cuda.stream(stream):
+                    for _ in range(20):
+                        got[n].append(jobs[n]())
+                stream.synchronize()
+            except Exception as e:   # noqa: BLE001
+                errors.append(e)
+        threads = [threading.Thread(target=work, args=(n,)) for n in range(len(jobs))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not errors
+        for n in range(len(jobs)):
+            for again in got[n]:
+                assert all(torch.equal(a, b) for a, b in zip(again, want[n])), (own, n)
+    cache.check()
+
+
+def test_first_call_is_not_captured(monkeypatch):
+    """The call that would make a device's handle is refused while its stream is captured."""
+    from lpta import serving
+    x = torch.randn(2, 100, device="cuda")
+    ids = torch.zeros(2, dtype=torch.int32, device="cuda")
+    want = serving.token_logprobs(x, ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with monkeypatch.context() as m:
+            m.setattr(serving, "_HANDLES", {})
+            with pytest.raises(ValueError, match="captured"):
+                serving.token_logprobs(x, ids)
+        got = serving.token_logprobs(x, ids)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got.logprob, want.logprob)

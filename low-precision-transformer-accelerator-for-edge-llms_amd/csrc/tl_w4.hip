@@ -14,10 +14,13 @@
 // What bounds it: the weights, k / 2 bytes a row, read once; of the rest the
 // latency from the first load to the result.  They stream in the order of the
 // lanes' registers, 1 KiB for 16 rows by 128 columns, 8 KiB in flight in each
-// wavefront; the digits of up to 16 rows of x wait in LDS.  Queued back to back, one
-// row by 5632 x 2048 takes 7.7 us, by 32000 x 2048 (group 32, float32 scales) 12.5,
-// by 14336 x 8192 15.7 (3.9 TB/s); 13 rows by 2048 x 5632 14.7, 16 by 32000 x 2048
-// 20.9.  With the weights in the rows' own order, where a load's pieces lie k / 2
+// wavefront; the digits of up to 16 rows of x wait in LDS.  Rows of x, scales and the
+// first weights are asked for together, and a row stays in registers from the search
+// for its largest magnitude to its digits (loaded twice: four rows by 5632 x 2048 9.8
+// us, now 8.5).  Queued back to back, one row by 5632 x 2048 takes 7.7 us (6.1 in a
+// graph), by 32000 x 2048 (group 32, float32 scales) 11.8, by 14336 x 8192 14.9 (4.1
+// TB/s); 13 rows by 2048 x 5632 14.4 (5 of them the digits' kernel), 16 by 32000 x
+// 2048 20.5.  With the weights in the rows' own order, where a load's pieces lie k / 2
 // bytes apart, the second took 20.9.
 #include <algorithm>
 
@@ -56,83 +59,127 @@ TL_DEV void digits4(int v0, int v1, int v2, int v3, unsigned d[4]) {
     d[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
 }
 
-// Digits of rows row0 .. row0 + rows - 1 of x (rows <= 4) to base; columns from k on
-// are zero.  exps[r]: the power of two the row was scaled by (kBadRow: not finite).
-// The whole workgroup takes part; mx: a word per row.
-TL_DEV void rows_digits(const W4Args& a, int row0, int rows, char* base, int cols, unsigned* mx, int* exps) {
-    const int tid = threadIdx.x;
-    const int units = a.k >> 3, padded = w4_blocks(a.k) * 16;   // of 8 columns
-    if (tid < rows) mx[tid] = 0u;
-    __syncthreads();
-    // magnitudes order as their bits do, infinity and NaN above the numbers
-    for (int r = 0; r < rows; r++) {
-        unsigned m = 0;
-        for (int u = tid; u < units; u += kW4Threads) {
-            const int64_t at = (row0 + r) * a.x_stride + 8 * u;
-            const v4f x0 = load4(a.x, at, a.act), x1 = load4(a.x, at + 4, a.act);
-#pragma unroll
-            for (int j = 0; j < 4; j++) m = max(m, max(__float_as_uint(fabsf(x0[j])), __float_as_uint(fabsf(x1[j]))));
-        }
-        m = max(m, (unsigned)dpp<kDppXor1>((int)m));
-        m = max(m, (unsigned)dpp<kDppXor2>((int)m));
-        m = max(m, (unsigned)dpp<kDppHalfMirror>((int)m));
-        m = max(m, (unsigned)dpp<kDppRowMirror>((int)m));
-        if ((tid & 15) == 0) atomicMax(&mx[r], m);
-    }
-    __syncthreads();
-    for (int r = 0; r < rows; r++) {
-        const unsigned m = mx[r];
-        const bool bad = m >= 0x7F800000u;
-        const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
-        if (tid == 0) exps[r] = bad ? kBadRow : e;
-        for (int u = tid; u < padded; u += kW4Threads) {
-            v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
-            if (u < units && !bad) {
-                const int64_t at = (row0 + r) * a.x_stride + 8 * u;
-                x0 = load4(a.x, at, a.act);
-                x1 = load4(a.x, at + 4, a.act);
-            }
-            int v[8];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                v[j] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x0[j], e));
-                v[4 + j] = (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x1[j], e));
-            }
-            unsigned even[4], odd[4];
-            digits4(v[0], v[2], v[4], v[6], even);
-            digits4(v[1], v[3], v[5], v[7], odd);
-            char* to = base + 8 * (u >> 2 & 1);
-#pragma unroll
-            for (int d = 0; d < 4; d++)
-                *(v2i*)(to + w4_frag(u >> 3, u & 3, 4 * r + d, cols)) = v2i{(int)even[d], (int)odd[d]};
-        }
-    }
-}
+// Rows row0 .. row0 + rows - 1 of x (rows <= 4) to digits, by a whole workgroup that
+// keeps them in registers between the search for their largest magnitudes and the
+// conversion: kSlots units of 8 columns per thread, slot j of row j / per.
+constexpr int kSlots = 4;
+__host__ __device__ inline int w4_slots(int rows, int k) { return rows * ((w4_blocks(k) * 16 + kW4Threads - 1) / kW4Threads); }
 
-// n pieces from memory to LDS by the whole workgroup, four loads of a thread in
-// flight; put(v, i) stores piece i
-template <typename V, typename Put>
-TL_DEV void to_lds(const V* from, int n, Put put) {
-    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * kW4Threads) {
-        const V a = from[i0], b = from[min(i0 + kW4Threads, n - 1)], c = from[min(i0 + 2 * kW4Threads, n - 1)],
-                d = from[min(i0 + 3 * kW4Threads, n - 1)];
-        put(a, i0);
-        if (i0 + kW4Threads < n) put(b, i0 + kW4Threads);
-        if (i0 + 2 * kW4Threads < n) put(c, i0 + 2 * kW4Threads);
-        if (i0 + 3 * kW4Threads < n) put(d, i0 + 3 * kW4Threads);
+struct RowUnits {
+    v4i raw[kSlots][2];
+
+    TL_DEV void load(const W4Args& a, int row0, int rows) {
+        const int units = a.k >> 3, per = (w4_blocks(a.k) * 16 + kW4Threads - 1) / kW4Threads;
+#pragma unroll
+        for (int j = 0; j < kSlots; j++) {
+            const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
+            raw[j][0] = raw[j][1] = v4i{0, 0, 0, 0};
+            if (r >= rows || u >= units) continue;
+            const int64_t at = (row0 + r) * a.x_stride + 8 * u;
+            if (a.act == DT_F32) {
+                raw[j][0] = *(const v4i*)((const float*)a.x + at);
+                raw[j][1] = *(const v4i*)((const float*)a.x + at + 4);
+            } else {
+                raw[j][0] = *(const v4i*)((const uint16_t*)a.x + at);
+            }
+        }
     }
-}
+
+    // digits to base, zero from column k on; exps[r]: the power of two the row was scaled by
+    // (kBadRow: not finite).  mx: a word per row, zero.  Ends without a barrier.
+    TL_DEV void digits(const W4Args& a, int rows, char* base, int cols, unsigned* mx, int* exps) {
+        const int padded = w4_blocks(a.k) * 16, per = (padded + kW4Threads - 1) / kW4Threads;
+        v4f x[kSlots][2];
+#pragma unroll
+        for (int j = 0; j < kSlots; j++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                x[j][h] = a.act == DT_F32 ? __builtin_bit_cast(v4f, raw[j][h])
+                                          : unpack4(v2i{raw[j][0][2 * h], raw[j][0][2 * h + 1]}, a.act);
+        // magnitudes order as their bits do, infinity and NaN above the numbers
+#pragma unroll
+        for (int j = 0; j < kSlots; j++) {
+            const int r = j / per;
+            if (r >= rows) break;
+            unsigned m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(fabsf(x[j][i >> 2][i & 3])));
+            m = max(m, (unsigned)dpp<kDppXor1>((int)m));
+            m = max(m, (unsigned)dpp<kDppXor2>((int)m));
+            m = max(m, (unsigned)dpp<kDppHalfMirror>((int)m));
+            m = max(m, (unsigned)dpp<kDppRowMirror>((int)m));
+            if ((threadIdx.x & 15) == 0) atomicMax(&mx[r], m);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSlots; j++) {
+            const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
+            if (r >= rows) break;
+            const unsigned m = mx[r];
+            const bool bad = m >= 0x7F800000u;
+            const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
+            if (u == 0) exps[r] = bad ? kBadRow : e;
+            if (u < padded) put(x[j][0], x[j][1], e, bad, r, u, base, cols);
+        }
+    }
+
+    static TL_DEV void put(v4f x0, v4f x1, int e, bool bad, int r, int u, char* base, int cols) {
+        int v[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[j] = bad ? 0 : (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x0[j], e));
+            v[4 + j] = bad ? 0 : (int)__builtin_rintf(__builtin_amdgcn_ldexpf(x1[j], e));
+        }
+        unsigned even[4], odd[4];
+        digits4(v[0], v[2], v[4], v[6], even);
+        digits4(v[1], v[3], v[5], v[7], odd);
+        char* to = base + 8 * (u >> 2 & 1);
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+            *(v2i*)(to + w4_frag(u >> 3, u & 3, 4 * r + d, cols)) = v2i{(int)even[d], (int)odd[d]};
+    }
+};
 
 // scratch of a call: the rows' exponents, the digits of each four rows
 __host__ __device__ inline size_t w4_digit_off(int m) { return ((size_t)m * 4 + 15) / 16 * 16; }
 
 __global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
     __shared__ unsigned mx[1];
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x;
     char* s = (char*)a.scratch;
     // one row at its place among its four
     char* base = s + w4_digit_off(a.m) + (row >> 2) * w4_frag_bytes(a.k, 16) + (row & 3) * 64;
-    rows_digits(a, row, 1, base, 16, mx, (int*)s + row);
+    if (tid == 0) mx[0] = 0u;
+    RowUnits x;
+    if (w4_slots(1, a.k) <= kSlots) {
+        x.load(a, row, 1);
+        __syncthreads();
+        x.digits(a, 1, base, 16, mx, (int*)s + row);
+        return;
+    }
+    // longer rows are read twice
+    __syncthreads();
+    const int units = a.k >> 3, padded = w4_blocks(a.k) * 16;
+    unsigned m = 0;
+    for (int u = tid; u < units; u += kW4Threads) {
+        const v4f x0 = load4(a.x, row * a.x_stride + 8 * u, a.act), x1 = load4(a.x, row * a.x_stride + 8 * u + 4, a.act);
+#pragma unroll
+        for (int j = 0; j < 4; j++) m = max(m, max(__float_as_uint(fabsf(x0[j])), __float_as_uint(fabsf(x1[j]))));
+    }
+    atomicMax(&mx[0], m);
+    __syncthreads();
+    m = mx[0];
+    const bool bad = m >= 0x7F800000u;
+    const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
+    if (tid == 0) ((int*)s)[row] = bad ? kBadRow : e;
+    for (int u = tid; u < padded; u += kW4Threads) {
+        v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+        if (u < units) {
+            x0 = load4(a.x, row * a.x_stride + 8 * u, a.act);
+            x1 = load4(a.x, row * a.x_stride + 8 * u + 4, a.act);
+        }
+        RowUnits::put(x0, x1, e, bad, 0, u, base, 16);
+    }
 }
 
 struct W4Shape {
@@ -140,6 +187,7 @@ struct W4Shape {
     int32_t cols;        // columns of a product in use by the digits' layout
 };
 
+constexpr int kFirst = 4;     // fours of scales of a thread that are loaded ahead
 constexpr int kW4Chunk = 8;   // blocks of 128 columns whose digits are in LDS at a time (COPY)
 
 // Workgroup (8 / split tiles of 16 weight rows, 4 CB rows of x).  LQ: log2 of the
@@ -157,7 +205,28 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     const int tile = blockIdx.x * per + wave / sh.split;
     const int m0 = blockIdx.y * (4 * CB);
 
-    // the first weights, on their way while digits and scales are laid out
+    // everything the workgroup starts with, on its way at once: its rows of x, the first
+    // scales, the first weights
+    RowUnits x;
+    if constexpr (!COPY) x.load(a, m0, min(4, a.m - m0));
+
+    // scales of the workgroup's tiles as float32 [tile][group][16 rows]
+    float* s_scale = (float*)lds;
+    const int n4 = min(per, tiles - (int)blockIdx.x * per) * groups * 4;   // fours of them
+    const bool wide = a.scale_dtype == DT_F32;
+    const char* sc = (const char*)a.packed + (int64_t)tiles * nblk * 1024 + (int64_t)blockIdx.x * per * groups * 16 * (wide ? 4 : 2);
+    v4i first[kFirst];
+#pragma unroll
+    for (int j = 0; j < kFirst; j++) {
+        const int i = min((int)threadIdx.x + j * kW4Threads, n4 - 1);
+        if (wide) {
+            first[j] = ((const v4i*)sc)[i];
+        } else {
+            const v2i v = ((const v2i*)sc)[i];
+            first[j] = v4i{v[0], v[1], 0, 0};
+        }
+    }
+
     const char* w = (const char*)a.packed + ((int64_t)min(tile, tiles - 1) * nblk) * 1024 + lane * 16;
     v4i ring[kW4Ahead];
     auto load = [&](int i) {   // the i-th block of this wavefront
@@ -167,18 +236,9 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
 #pragma unroll
     for (int i = 0; i < kW4Ahead; i++) ring[i] = load(i);
 
-    // scales of the workgroup's tiles as float32 [tile][group][16 rows]
-    float* s_scale = (float*)lds;
-    {
-        const char* sc = (const char*)a.packed + (int64_t)tiles * nblk * 1024;
-        const int64_t from = (int64_t)blockIdx.x * per * groups * 16;
-        const int n4 = min(per, tiles - (int)blockIdx.x * per) * groups * 4;
-        if (a.scale_dtype == DT_F32)
-            to_lds((const v4f*)((const float*)sc + from), n4, [&](v4f v, int i) { *(v4f*)(s_scale + 4 * i) = v; });
-        else
-            to_lds((const v2i*)((const uint16_t*)sc + from), n4,
-                   [&](v2i v, int i) { *(v4f*)(s_scale + 4 * i) = unpack4(v, a.scale_dtype); });
-    }
+    auto put_scales = [&](v4i v, int i) {
+        *(v4f*)(s_scale + 4 * i) = wide ? __builtin_bit_cast(v4f, v) : unpack4(v2i{v[0], v[1]}, a.scale_dtype);
+    };
     char* next = lds + (size_t)per * groups * 64;
     float* red = (float*)next;                     // [wave][16 rows][4 CB]
     next += kW4Waves * 16 * 4 * CB * 4;
@@ -211,10 +271,17 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     if constexpr (COPY) {
         if (threadIdx.x < 4 * CB) s_exp[threadIdx.x] = m0 + (int)threadIdx.x < a.m ? ((const int*)a.scratch)[m0 + threadIdx.x] : 0;
         fetch(0);
-        put(0);
     } else {
-        rows_digits(a, m0, min(4, a.m - m0), digits, sh.cols, s_mx, s_exp);
+        if (threadIdx.x < 4) s_mx[threadIdx.x] = 0u;
+        __syncthreads();
+        x.digits(a, min(4, a.m - m0), digits, sh.cols, s_mx, s_exp);
     }
+#pragma unroll
+    for (int j = 0; j < kFirst; j++)
+        if ((int)threadIdx.x + j * kW4Threads < n4) put_scales(first[j], threadIdx.x + j * kW4Threads);
+    for (int i = threadIdx.x + kFirst * kW4Threads; i < n4; i += kW4Threads)
+        put_scales(wide ? ((const v4i*)sc)[i] : v4i{((const v2i*)sc)[i][0], ((const v2i*)sc)[i][1], 0, 0}, i);
+    if constexpr (COPY) put(0);
     __syncthreads();
 
     v4f acc[CB];
@@ -414,15 +481,17 @@ hipError_t launch_linear_w4(hipStream_t s, const W4Args& a) {
     W4Shape sh;
     sh.cols = a.m == 1 ? 4 : a.m == 2 ? 8 : 16;
     // Up to four rows each workgroup converts them itself where their digits fit in 64
-    // KiB: one kernel.  One row by 32000 x 2048: 12.5 us, 19.2 through scratch; four by
-    // 5632 x 2048: 9.8, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch 21.7.
-    const bool convert = cbs == 1 && w4_frag_bytes(a.k, sh.cols) <= 64 * 1024;
+    // KiB: one kernel.  One row by 32000 x 2048: 11.8 us, 19.2 through scratch; four by
+    // 5632 x 2048: 8.5, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch
+    // 20.8.  More rows would be converted by too many: 16 by 5632 x 2048 16.1, 10.7.
+    const bool convert = cbs == 1 && w4_frag_bytes(a.k, sh.cols) <= 64 * 1024 && w4_slots(a.m, a.k) <= kSlots;
     int cb = 1;
     size_t digits;
     if (convert) {
         digits = w4_frag_bytes(a.k, sh.cols);
         // wavefronts per tile: enough of them for 4 on each CU (one row by 14336 x 8192
-        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9)
+        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9;
+        // each measured before the rows stayed in registers)
         sh.split = 1;
         while (sh.split < kW4Waves && ((int64_t)tiles * sh.split < kW4EnoughWaves || w4_lds(a, sh.split, 1, digits) > (size_t)kW4Lds))
             sh.split *= 2;

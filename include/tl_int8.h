@@ -268,8 +268,8 @@ typedef struct tl_paged_cache {
  * q_out (may be NULL, or qkv itself).  Steps are float32, each rounded; 16-bit
  * results are rounded once.  Strides in elements; rows start 16-byte aligned.
  * A negative row_seq is a padded row: it is skipped and its q_out left as it
- * was.  Two rows of a call at one position of one sequence leave either row's
- * values there. */
+ * was.  Two rows of a call at one position of one sequence leave a mixture of
+ * both there. */
 int32_t tl_paged_append(tl_handle *h, const tl_paged_cache *cache, const void *qkv, int64_t qkv_stride, int32_t act,
                         int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos,
                         const float *cos, const float *sin, int32_t n_pos, void *q_out, int64_t q_stride);
@@ -287,7 +287,7 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
  * page out of range are left out.  Several rows of one sequence at rising
  * positions are causal attention.  The keys are shared out evenly over the GPU
  * whatever the rows' lengths; the parts of a row that was split are joined, in the
- * order of its keys. */
+ * order of its keys.  out may be q. */
 int32_t tl_paged_attention(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride, int32_t act,
                            int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos, float scale,
                            void *out, int64_t out_stride);
@@ -314,7 +314,8 @@ int32_t tl_w4_packed_bytes(tl_handle *h, int32_t n, int32_t k, int32_t group, in
 int32_t tl_pack_w4(tl_handle *h, const uint8_t *q, const void *scales, int32_t scale_dtype, int32_t group, int32_t n,
                    int32_t k, void *packed);
 /* y[m][n] = residual[m][n] + sum_k x[m][k] w[n][k], x, residual and y of type act
- * (TL_F32, TL_BF16, TL_F16), residual may be NULL or y.  All dev; strides in elements, x's
+ * (TL_F32, TL_BF16, TL_F16), residual may be NULL or y; x and y must not
+ * overlap.  All dev; strides in elements, x's
  * rows 16-byte aligned.  A row of x is taken as integers of 2^-30 of its largest
  * magnitude, products are exact, sums float32; an infinity or NaN in a row of x makes
  * its whole row of y NaN.  Few rows (a decoding step) are what it is made for; up to

@@ -2344,6 +2344,16 @@ int32_t check_rows(tl_handle* h, const void* p, int64_t stride, int64_t width, i
     return TL_OK;
 }
 
+// Rows that are written are those that are read (in place) or apart from them.
+int32_t check_apart(tl_handle* h, const void* in, int64_t in_stride, int64_t in_width, const void* out, int64_t out_stride,
+                    int64_t out_width, int32_t t, int32_t rows, bool in_place, const char* what) {
+    const int64_t e = type_size(t);
+    if (in_place && in == out && (in_stride == out_stride || rows <= 1)) return TL_OK;
+    TL_REQ(h, rows_apart(in, in_stride * e, in_width * e, out, out_stride * e, out_width * e, rows),
+           std::string(what) + " overlap");
+    return TL_OK;
+}
+
 int32_t paged_cache_arg(tl_handle* h, const tl_paged_cache* c, PagedCache* out) {
     TL_REQ(h, c && c->k && c->v && c->table, "null cache pointer");
     TL_REQ(h, c->dtype == TL_I8 || c->dtype == TL_BF16 || c->dtype == TL_F16, "cache type must be INT8, bfloat16 or float16");
@@ -2399,6 +2409,8 @@ int32_t append_args(tl_handle* h, const tl_paged_cache* cache, const void* qkv, 
     if ((r = check_rows(h, qkv, qkv_stride, (n_heads + 2 * (int64_t)cache->n_kv_heads) * hd, act, "qkv"))) return r;
     if (q_out && (r = check_rows(h, q_out, q_stride, n_heads * hd, act, "q_out"))) return r;
     TL_REQ(h, q_out != qkv || !q_out || q_stride == qkv_stride, "q_out on top of qkv needs the same stride");
+    if (q_out && (r = check_apart(h, qkv, qkv_stride, (n_heads + 2 * (int64_t)cache->n_kv_heads) * hd, q_out, q_stride,
+                                  n_heads * hd, act, rows, true, "qkv and q_out"))) return r;
     a->qkv = qkv; a->qkv_stride = qkv_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
     a->row_seq = row_seq; a->row_pos = row_pos; a->cos = cos; a->sin = sin; a->n_pos = n_pos;
     a->q_out = q_out; a->q_stride = q_stride;
@@ -2418,6 +2430,7 @@ int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q,
     const int64_t width = (int64_t)n_heads * cache->head_dim;
     if ((r = check_rows(h, q, q_stride, width, act, "q"))) return r;
     if ((r = check_rows(h, out, out_stride, width, act, "out"))) return r;
+    if ((r = check_apart(h, q, q_stride, width, out, out_stride, width, act, rows, true, "q and out"))) return r;
     a->q = q; a->q_stride = q_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
     a->row_seq = row_seq; a->row_pos = row_pos; a->scale = scale; a->out = out; a->out_stride = out_stride;
     return TL_OK;
@@ -2446,6 +2459,8 @@ int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int3
     TL_REQ(h, y_stride >= n && (uintptr_t)y % type_size(act) == 0, "y: rows must not overlap and must be aligned");
     TL_REQ(h, !residual || (res_stride >= n && (uintptr_t)residual % type_size(act) == 0),
            "residual: rows must not overlap and must be aligned");
+    if ((r = check_apart(h, x, x_stride, k, y, y_stride, n, act, m, false, "x and y"))) return r;
+    if (residual && (r = check_apart(h, residual, res_stride, n, y, y_stride, n, act, m, true, "residual and y"))) return r;
     a->x = x; a->x_stride = x_stride; a->act = act; a->m = m; a->n = n; a->k = k; a->group = group;
     a->packed = packed; a->scale_dtype = scale_dtype;
     a->residual = residual; a->res_stride = res_stride; a->y = y; a->y_stride = y_stride;

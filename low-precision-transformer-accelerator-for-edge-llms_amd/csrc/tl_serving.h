@@ -83,6 +83,17 @@ inline bool paged_countable(const PagedGeom& g, int32_t rows, int32_t head_block
     return most * head_blocks <= INT32_MAX / (rows > 0 ? rows : 1);
 }
 
+// Whether two sets of rows (bytes: strides s, widths w) share no byte: one behind the
+// other, or, with one stride, side by side in each row of a wider matrix.
+inline bool rows_apart(const void* p, int64_t sp, int64_t wp, const void* q, int64_t sq, int64_t wq, int64_t rows) {
+    if (rows <= 0) return true;
+    const int64_t d = (int64_t)((uintptr_t)q - (uintptr_t)p);   // of q's rows from p's
+    if (d >= (rows - 1) * sp + wp || -d >= (rows - 1) * sq + wq) return true;
+    if (rows == 1 || sp != sq || sp <= 0) return false;
+    const int64_t at = (d % sp + sp) % sp;
+    return at >= wp && at + wq <= sp;
+}
+
 }  // namespace tl
 
 #if defined(__HIPCC__)

@@ -11,7 +11,8 @@ memory is torch's, kept for each stream, and a captured graph has its own, so ca
 on different streams and graphs share none; threads may call at the same time.  A
 captured call joins the parts of a long row in another order than a queued one does,
 so attention may differ between them in the last place.  Tensors are CUDA tensors of
-one device; float types are float32, bfloat16 and float16.
+one device; float types are float32, bfloat16 and float16.  Nothing here is
+differentiable: results carry no gradient.
 
 What a call finds out of range on the device (a sequence, position, page or token
 id) it leaves out; ``check()`` tells.  Wrong types, shapes and layouts raise
@@ -212,7 +213,7 @@ class PagedCache:
         """Attention of one query row per token: row r of q [rows][n_heads * head_dim]
         (rotated) over keys 0 .. row_pos[r] of sequence row_seq[r] (None: r); a
         negative position gives zeros, a negative sequence leaves its row of ``out`` as it
-        was (undefined in a new tensor).  ``scale``: 1 / sqrt(head_dim) unless given."""
+        was (undefined in a new tensor).  ``out`` may be q.  ``scale``: 1 / sqrt(head_dim) unless given."""
         dev, hd = self.device, self.head_dim
         _rows("q", q, dev)
         rows, width = q.shape
@@ -305,7 +306,7 @@ class W4Linear:
         return got
 
     def __call__(self, x, residual=None, out=None):
-        """x [rows][k] -> [rows][n] in x's type; ``out`` may be ``residual``."""
+        """x [rows][k] -> [rows][n] in x's type; ``out`` may be ``residual``, not x."""
         dev = self.device
         _rows("x", x, dev, self.k)
         rows = x.shape[0]

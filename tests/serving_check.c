@@ -94,6 +94,8 @@ static void paged(void) {
     APP("misaligned q_out", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, &q[0][2], qw);
     APP("short q_stride", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, q, qw - 4);
     APP("in place, another stride", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, qkv, qw);
+    APP("q_out on k", qkv, w, TL_F32, 4, HEADS, seq, pos, cs, sn, 64, &qkv[0][2 * HD], w);
+    APP("q_out a row on", qkv, w, TL_F32, 3, HEADS, seq, pos, cs, sn, 64, &qkv[1][0], w);
 #define ATT(what, ...) expect("attention: " what, tl_paged_attention(H, &c, __VA_ARGS__), TL_ERR_BAD_DESCRIPTOR, 0)
     ATT("null q", NULL, qw, TL_F32, 4, HEADS, seq, pos, 1, out, qw);
     ATT("null out", q, qw, TL_F32, 4, HEADS, seq, pos, 1, NULL, qw);
@@ -104,6 +106,9 @@ static void paged(void) {
     ATT("negative rows", q, qw, TL_F32, -4, HEADS, seq, pos, 1, out, qw);
     ATT("short stride", q, qw - 4, TL_F32, 4, HEADS, seq, pos, 1, out, qw);
     ATT("misaligned out", q, qw, TL_F32, 4, HEADS, seq, pos, 1, &out[0][1], qw);
+    ATT("out a row on", q, qw, TL_F32, 3, HEADS, seq, pos, 1, &q[1][0], qw);
+    ATT("out on q, another stride", q, qw, TL_F32, 2, HEADS, seq, pos, 1, q, qw + 4);
+    expect("out is q", tl_paged_attention(H, &c, q, qw, TL_F32, 4, HEADS, seq, pos, 1, q, qw), TL_OK, 1);
     tl_paged_cache deep = cache();
     deep.max_pages = 1 << 26;   /* 2^30 positions: 2^22 tiles */
     deep.table_stride = 1 << 26;
@@ -187,6 +192,11 @@ static void linear_w4(void) {
     expect("short y", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, y, 31), bad, 0);
     expect("misaligned y", W4(x, 256, TL_F32, 3, wp, TL_F32, 64, 32, 256, NULL, 0, (char*)y + 2, 32), bad, 0);
     expect("short residual", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, r, 31, y, 32), bad, 0);
+    expect("y on x", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, NULL, 0, x, 256), bad, 0);
+    expect("y in x's rows", W4(x, 256, TL_F32, 2, wp, TL_F32, 64, 32, 128, NULL, 0, &x[0][128], 256), TL_OK, 1);
+    expect("y and x meet", W4(x, 256, TL_F32, 2, wp, TL_F32, 64, 32, 128, NULL, 0, &x[0][127], 256), bad, 0);
+    expect("residual is y", W4(x, 256, TL_F32, 4, wp, TL_F32, 64, 32, 256, y, 32, y, 32), TL_OK, 1);
+    expect("residual shifted", W4(x, 256, TL_F32, 2, wp, TL_F32, 64, 32, 256, (char*)y + 4, 32, y, 32), bad, 0);
     expect("scratch null", tl_linear_w4_scratch(H, 4, 256, NULL), bad, 0);
     expect("scratch rows", tl_linear_w4_scratch(H, -4, 256, &need), bad, 0);
     expect("quantize", tl_quantize_w4_rows(H, wf, 32, 256, 64, TL_F32, w, sc), TL_OK, 1);

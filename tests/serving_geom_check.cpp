@@ -90,6 +90,22 @@ int main() {
     CHECK(paged_countable(g, 1, 255) && paged_countable(g, 255, 1) && !paged_countable(g, 256, 1) && !paged_countable(g, 2, 128));
     g.max_pages = 1;
     CHECK(paged_countable(g, 1 << 20, 100) && !paged_countable(g, 1 << 20, 1 << 9));
+    // rows that share no byte, against the bytes themselves
+    srand(5);
+    for (int i = 0; i < 200000; i++) {
+        const int64_t rows = rand() % 4, wp = 1 + rand() % 6, wq = 1 + rand() % 6, sp = wp + rand() % 9;
+        const int64_t sq = rand() % 2 && sp >= wq ? sp : wq + rand() % 9, at = rand() % 70;
+        char bytes[256] = {};
+        const char *p = bytes + 64, *q = bytes + 30 + at;
+        bool apart = true;
+        for (int64_t r = 0; r < rows; r++) for (int64_t b = 0; b < wp; b++) bytes[64 + r * sp + b] = 1;
+        for (int64_t r = 0; r < rows; r++) for (int64_t b = 0; b < wq; b++) apart &= !q[r * sq + b];
+        const bool said = rows_apart(p, sp, wp, q, sq, wq, rows);
+        CHECK(!said || apart);
+        if (rows <= 1) CHECK(said == apart);
+        // side by side within each row
+        if (sp == sq && q >= p + wp && q + wq <= p + sp) CHECK(said);
+    }
     std::printf("%d wrong\n", wrong);
     return wrong ? 1 : 0;
 }

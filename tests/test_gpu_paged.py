@@ -243,6 +243,24 @@ def test_attention_faults_are_left_out(serving):
     rt.close()
 
 
+def test_attention_in_place_and_scales(serving):
+    """out = q gives the bits of another out, whole rows and split ones; scales of zero and below."""
+    built = build("f16", 2, 64, 16, [5000, 90, 300], seed=6)
+    c = make(serving, built)
+    q = torch.randn(3, 24 * 64, generator=built[4])
+    pos = torch.tensor([4999, 89, -1], dtype=torch.int32, device="cuda")
+    for scale in (0.125, 0.0, -0.2):
+        x = q.cuda()
+        out = c.attend(x, None, pos, scale=scale)
+        want, tol = attention_reference(q, built, [0, 1, 2], [4999, 89, -1], 16, scale, "f32", "f16")
+        assert ((out.cpu().double() - want).abs() <= tol + 1e-300).all()
+        assert c.attend(x, None, pos, scale=scale, out=x) is x and torch.equal(x, out)
+    wide = torch.randn(3, 2 * 24 * 64, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        c.attend(wide[:, :24 * 64], None, pos, out=wide[:, 64:25 * 64])
+    c.attend(wide[:, :24 * 64], None, pos, out=wide[:, 24 * 64:])
+
+
 def test_attention_extreme_scores(serving):
     """Scores far apart (all weight on one key), equal scores (plain means), a zero query, tiny and huge
     queries, and attended infinities and NaN."""

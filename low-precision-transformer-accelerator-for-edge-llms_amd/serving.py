@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import NamedTuple
 
 import torch
@@ -33,18 +34,21 @@ _ACT = {torch.float32: _native.TL_F32, torch.bfloat16: _native.TL_BF16, torch.fl
 _CACHE = {torch.int8: _native.TL_I8, torch.bfloat16: _native.TL_BF16, torch.float16: _native.TL_F16}
 _HANDLES: dict[int, Runtime] = {}
 _WORKSPACES: dict[tuple[int, int], "_Workspace"] = {}
+_COMPLETING = threading.Lock()   # one call at a time on a handle's own stream
 
 
 def _runtime(device: torch.device) -> Runtime:
     """The operator handle of a device, made on first use."""
     rt = _HANDLES.get(device.index)
     if rt is None:
-        with torch.cuda.device(device):
+        with _COMPLETING, torch.cuda.device(device):
+            if device.index in _HANDLES:
+                return _HANDLES[device.index]
             if torch._C._cuda_isCurrentStreamCapturing():
                 raise _bad("the first call on a device cannot be captured: make it once before")
             rt = Runtime(dict(hidden=64, intermediate=64, n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, vocab=64,
                               max_pos=64, rms_eps=1e-5, rope_theta=10000.0))
-        _HANDLES[device.index] = rt
+            _HANDLES[device.index] = rt
     return rt
 
 
@@ -260,7 +264,8 @@ def quantize_w4(w, group: int = 128, scale_dtype=torch.float16, rt: Runtime | No
     rt = rt or _runtime(w.device)
     q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
-    rt.call("tl_quantize_w4_rows", w.contiguous(), n, k, group, _ACT[scale_dtype], q, scales)
+    with _COMPLETING:
+        rt.call("tl_quantize_w4_rows", w.contiguous(), n, k, group, _ACT[scale_dtype], q, scales)
     return q, scales
 
 
@@ -289,7 +294,8 @@ class W4Linear:
         n = C.c_int64()
         rt.check(rt.lib.tl_w4_packed_bytes(rt.h, self.n, self.k, self.group, self.scale_dtype, C.byref(n)), "W4Linear")
         self.packed = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        rt.call("tl_pack_w4", q, scales, self.scale_dtype, self.group, self.n, self.k, self.packed)
+        with _COMPLETING:
+            rt.call("tl_pack_w4", q, scales, self.scale_dtype, self.group, self.n, self.k, self.packed)
         self._scratch: dict[int, int] = {}
 
     @classmethod

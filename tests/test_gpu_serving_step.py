@@ -117,6 +117,7 @@ def test_threads_and_streams():
     k, v = (torch.randn(260, 1, 16, 64, generator=g).half().cuda() for _ in range(2))
     table = torch.arange(260, dtype=torch.int32, device="cuda").view(2, 130)
     cache = serving.PagedCache(k, v, table)
+    dense_w = torch.randn(96, 512, generator=g).cuda()
     jobs = []
     for n in range(4):
         x = torch.randn(3 + 5 * n, 512, generator=g).cuda()
@@ -127,7 +128,8 @@ def test_threads_and_streams():
         pos = torch.full((1 + n,), 900 + 300 * n, dtype=torch.int32, device="cuda")
 
         def job(x=x, logits=logits, ids=ids, q=q, seq=seq, pos=pos, n=n):
-            return [lin(x), *serving.token_logprobs(logits, ids, 3 * n), cache.attend(q, seq, pos)]
+            made = serving.W4Linear.from_float(dense_w, 64)
+            return [lin(x), made(x), *serving.token_logprobs(logits, ids, 3 * n), cache.attend(q, seq, pos)]
         jobs.append(job)
     want = [job() for job in jobs]
     torch.cuda.synchronize()

@@ -58,6 +58,7 @@ def reference(x, q, scales, act, residual=None):
     ("f32", "bf16", 64, 4, 333, 4096), ("f32", "f16", 128, 3, 33, 16384), ("f16", "f16", 32, 6, 48, 16416),
     ("f32", "f16", 128, 1, 40, 16384), ("bf16", "f32", 64, 2, 40, 8192), ("f16", "f16", 32, 2, 24, 8224),
     ("f32", "bf16", 128, 1, 24, 16512), ("bf16", "f16", 64, 21, 50, 20480), ("f32", "f16", 32, 300, 70, 1056),
+    ("bf16", "f16", 32, 1, 16400, 4096), ("f16", "f32", 32, 5, 16400, 2080),   # more scales than a first round of loads
 ])
 def test_linear(serving, act, scale, group, m, n, k):
     """One row and many, widths and columns off the tiles, every group and type, strided rows, with and without a

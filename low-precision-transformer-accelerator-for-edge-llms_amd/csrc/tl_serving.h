@@ -4,7 +4,10 @@
 // arithmetic at the top is host code too: a CPU test compiles it by itself.
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
+
+#include <initializer_list>
 
 #if defined(__HIPCC__)
 #define TL_HD __host__ __device__
@@ -94,6 +97,101 @@ inline bool rows_apart(const void* p, int64_t sp, int64_t wp, const void* q, int
     return at >= wp && at + wq <= sp;
 }
 
+// Projections with 4-bit weights: sizes, the plan of a call, and where its pieces lie.
+//
+// Weights come in tiles of 16 rows and blocks of 128 columns.  Scratch of a call
+// (w4_scratch() bytes): the exponents of its rows of x, then the digits of each four
+// rows ("row block"), w4_frag_bytes(k, 16) bytes.
+constexpr int32_t kW4Waves = 8, kW4Threads = 64 * kW4Waves;
+constexpr int32_t kW4MaxGroups = 1024;
+constexpr int64_t kW4EnoughWaves = 1024;
+constexpr int64_t kW4Lds = 152 * 1024;   // of a workgroup's 160 KiB
+constexpr int32_t kW4Slots = 4;          // units of 8 columns of x that a thread keeps in registers
+constexpr int32_t kW4Chunk = 8;          // blocks of 128 columns whose digits are in LDS at a time
+
+TL_HD inline int32_t w4_blocks(int32_t k) { return (k + 127) / 128; }
+TL_HD inline int32_t w4_tiles(int32_t n) { return (n + 15) / 16; }
+TL_HD inline int32_t w4_row_blocks(int32_t m) { return (m + 3) / 4; }
+TL_HD inline int32_t w4_groups(int32_t k, int32_t group) { return w4_blocks(k) * (128 / group); }   // with the padding's
+TL_HD inline int64_t w4_frag_bytes(int32_t k, int32_t cols) { return (int64_t)w4_blocks(k) * 128 * cols; }
+TL_HD inline int64_t w4_digit_off(int32_t m) { return ((int64_t)m * 4 + 15) / 16 * 16; }
+// units of all of `rows` rows that a thread takes
+TL_HD inline int32_t w4_slots(int32_t rows, int32_t k) { return rows * ((w4_blocks(k) * 16 + kW4Threads - 1) / kW4Threads); }
+// The row block that workgroup row y takes as its c-th of cb.  Where cb does not divide
+// the row blocks, the last workgroup row has some to spare: they stand for the last one
+// again, and their results go nowhere.
+TL_HD inline int32_t w4_row_block(int32_t y, int32_t cb, int32_t c, int32_t m) {
+    const int32_t b = y * cb + c, last = w4_row_blocks(m) - 1;
+    return b < last ? b : last;
+}
+inline size_t w4_scratch(int32_t m, int32_t k) {
+    return m <= 0 ? 0 : (size_t)(w4_digit_off(m) + w4_row_blocks(m) * w4_frag_bytes(k, 16));
+}
+
+struct W4Plan {
+    bool convert;          // one kernel that turns x into digits itself (up to four rows)
+    int32_t cb;            // row blocks of a workgroup: 1, 2 or 4
+    int32_t split;         // wavefronts that share a tile of 16 weight rows: 1, 2, 4 or 8
+    int32_t cols;          // columns of a product in use by the digits' layout
+    int32_t grid_x, grid_y;
+    int64_t lds;           // bytes of a workgroup
+};
+
+// LDS of a workgroup: scales, sums, exponents, digits
+inline int64_t w4_lds(int32_t k, int32_t group, int32_t split, int32_t cb, int64_t digits) {
+    return (int64_t)(kW4Waves / split) * w4_groups(k, group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 128 + digits;
+}
+
+inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {
+    const int32_t tiles = w4_tiles(n), cbs = w4_row_blocks(m);
+    W4Plan p{};
+    p.cols = m == 1 ? 4 : m == 2 ? 8 : 16;
+    // Up to four rows each workgroup converts them itself where their digits fit in 64
+    // KiB: one kernel.  One row by 32000 x 2048: 11.8 us, 19.2 through scratch; four by
+    // 5632 x 2048: 8.5, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch
+    // 20.8.  More rows would be converted by too many: 16 by 5632 x 2048 16.1, 10.7.
+    p.convert = cbs == 1 && w4_frag_bytes(k, p.cols) <= 64 * 1024 && w4_slots(m, k) <= kW4Slots;
+    p.cb = 1;
+    int64_t digits;
+    if (p.convert) {
+        digits = w4_frag_bytes(k, p.cols);
+        // wavefronts per tile: enough of them for 4 on each CU (one row by 14336 x 8192
+        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9;
+        // each measured before the rows stayed in registers)
+        p.split = 1;
+        while (p.split < kW4Waves && ((int64_t)tiles * p.split < kW4EnoughWaves || w4_lds(k, group, p.split, 1, digits) > kW4Lds))
+            p.split *= 2;
+    } else {
+        p.cols = 16;
+        // What a workgroup moves through its CU: 16 CB bytes of digits and 8 of weights per
+        // tile and column of x, in as many rounds as 256 CUs need (16 rows by 32000 x 2048:
+        // 20.9 us; counted with 512 at once 24.1)
+        int64_t best = INT64_MAX;
+        digits = 0;
+        for (int32_t c : {4, 2, 1}) {
+            if (c > 1 && c / 2 >= cbs) continue;   // all of another workgroup row to spare
+            const int64_t chunk = (int64_t)2 * c * kW4Chunk * 128 * 16;
+            for (int32_t split = 1; split <= kW4Waves; split *= 2) {
+                if (w4_lds(k, group, split, c, chunk) > kW4Lds) continue;
+                const int32_t per = kW4Waves / split;
+                const int64_t wgs = (int64_t)((tiles + per - 1) / per) * ((cbs + c - 1) / c);
+                const int64_t cost = (wgs + 255) / 256 * (2 * c + per);
+                if (cost < best) {
+                    best = cost;
+                    p.cb = c;
+                    p.split = split;
+                    digits = chunk;
+                }
+            }
+        }
+    }
+    const int32_t per = kW4Waves / p.split;
+    p.grid_x = (tiles + per - 1) / per;
+    p.grid_y = (cbs + p.cb - 1) / p.cb;
+    p.lds = w4_lds(k, group, p.split, p.cb, digits);
+    return p;
+}
+
 }  // namespace tl
 
 #if defined(__HIPCC__)
@@ -169,7 +267,6 @@ struct W4Args {
 };
 bool w4_supported(int32_t k, int32_t group);
 int64_t w4_packed_bytes(int32_t n, int32_t k, int32_t group, int32_t scale_dtype);
-size_t w4_scratch(int32_t m, int32_t k);
 hipError_t launch_linear_w4(hipStream_t s, const W4Args& a);
 // q [n][k / 2] bytes: column 2 j of a row in byte j's low nibble, 2 j + 1 in its
 // high one, each a two's complement number -8 .. 7; scales [n][k / group]

@@ -29,23 +29,13 @@
 namespace tl {
 namespace {
 
-constexpr int kW4Waves = 8;
-constexpr int kW4Threads = 64 * kW4Waves;
-constexpr int kW4MaxGroups = 1024;
-constexpr int64_t kW4EnoughWaves = 1024;
 constexpr int kW4Ahead = 8;          // 1 KiB weight blocks in flight per wavefront
 constexpr int kBadRow = INT32_MIN;   // exponent of a row with an infinity or NaN
-constexpr int kW4Lds = 152 * 1024;   // of a workgroup's 160 KiB
-
-__host__ __device__ inline int w4_blocks(int k) { return (k + 127) / 128; }
-__host__ __device__ inline int w4_tiles(int n) { return (n + 15) / 16; }
-__host__ __device__ inline int w4_groups(int k, int group) { return w4_blocks(k) * (128 / group); }   // with the padding's
 
 // The digits of `cols / 4` rows of x (cols: 4, 8 or 16), in the order the products
 // take them: for 64 columns of x, lane group g and column of the product 16 bytes,
 // those of x's columns 32 c + 8 g + 2 i + parity at 8 c + 4 parity + i.
-__host__ __device__ inline int w4_frag(int k64, int g, int col, int cols) { return ((k64 * 4 + g) * cols + col) * 16; }
-__host__ __device__ inline size_t w4_frag_bytes(int k, int cols) { return (size_t)w4_blocks(k) * 128 * cols; }
+TL_DEV int w4_frag(int k64, int g, int col, int cols) { return ((k64 * 4 + g) * cols + col) * 16; }
 
 // four integers (of columns k, k + 2, k + 4, k + 6) to one dword per digit
 TL_DEV void digits4(int v0, int v1, int v2, int v3, unsigned d[4]) {
@@ -61,17 +51,14 @@ TL_DEV void digits4(int v0, int v1, int v2, int v3, unsigned d[4]) {
 
 // Rows row0 .. row0 + rows - 1 of x (rows <= 4) to digits, by a whole workgroup that
 // keeps them in registers between the search for their largest magnitudes and the
-// conversion: kSlots units of 8 columns per thread, slot j of row j / per.
-constexpr int kSlots = 4;
-__host__ __device__ inline int w4_slots(int rows, int k) { return rows * ((w4_blocks(k) * 16 + kW4Threads - 1) / kW4Threads); }
-
+// conversion: kW4Slots units of 8 columns per thread, slot j of row j / per.
 struct RowUnits {
-    v4i raw[kSlots][2];
+    v4i raw[kW4Slots][2];
 
     TL_DEV void load(const W4Args& a, int row0, int rows) {
         const int units = a.k >> 3, per = (w4_blocks(a.k) * 16 + kW4Threads - 1) / kW4Threads;
 #pragma unroll
-        for (int j = 0; j < kSlots; j++) {
+        for (int j = 0; j < kW4Slots; j++) {
             const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
             raw[j][0] = raw[j][1] = v4i{0, 0, 0, 0};
             if (r >= rows || u >= units) continue;
@@ -89,16 +76,16 @@ struct RowUnits {
     // (kBadRow: not finite).  mx: a word per row, zero.  Ends without a barrier.
     TL_DEV void digits(const W4Args& a, int rows, char* base, int cols, unsigned* mx, int* exps) {
         const int padded = w4_blocks(a.k) * 16, per = (padded + kW4Threads - 1) / kW4Threads;
-        v4f x[kSlots][2];
+        v4f x[kW4Slots][2];
 #pragma unroll
-        for (int j = 0; j < kSlots; j++)
+        for (int j = 0; j < kW4Slots; j++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
                 x[j][h] = a.act == DT_F32 ? __builtin_bit_cast(v4f, raw[j][h])
                                           : unpack4(v2i{raw[j][0][2 * h], raw[j][0][2 * h + 1]}, a.act);
         // magnitudes order as their bits do, infinity and NaN above the numbers
 #pragma unroll
-        for (int j = 0; j < kSlots; j++) {
+        for (int j = 0; j < kW4Slots; j++) {
             const int r = j / per;
             if (r >= rows) break;
             unsigned m = 0;
@@ -112,7 +99,7 @@ struct RowUnits {
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kSlots; j++) {
+        for (int j = 0; j < kW4Slots; j++) {
             const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
             if (r >= rows) break;
             const unsigned m = mx[r];
@@ -140,9 +127,6 @@ struct RowUnits {
     }
 };
 
-// scratch of a call: the rows' exponents, the digits of each four rows
-__host__ __device__ inline size_t w4_digit_off(int m) { return ((size_t)m * 4 + 15) / 16 * 16; }
-
 __global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
     __shared__ unsigned mx[1];
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -151,7 +135,7 @@ __global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
     char* base = s + w4_digit_off(a.m) + (row >> 2) * w4_frag_bytes(a.k, 16) + (row & 3) * 64;
     if (tid == 0) mx[0] = 0u;
     RowUnits x;
-    if (w4_slots(1, a.k) <= kSlots) {
+    if (w4_slots(1, a.k) <= kW4Slots) {
         x.load(a, row, 1);
         __syncthreads();
         x.digits(a, 1, base, 16, mx, (int*)s + row);
@@ -188,7 +172,6 @@ struct W4Shape {
 };
 
 constexpr int kFirst = 4;     // fours of scales of a thread that are loaded ahead
-constexpr int kW4Chunk = 8;   // blocks of 128 columns whose digits are in LDS at a time (COPY)
 
 // Workgroup (8 / split tiles of 16 weight rows, 4 CB rows of x).  LQ: log2 of the
 // groups in 128 columns.  Up to four rows of x each workgroup converts to digits
@@ -246,7 +229,7 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     int* s_exp = (int*)next + 16;
     next += 128;
     char* digits = next;
-    const char* scr = (const char*)a.scratch + w4_digit_off(a.m) + (size_t)blockIdx.y * CB * w4_frag_bytes(a.k, 16);
+    const char* scr = (const char*)a.scratch + w4_digit_off(a.m);
 
     // COPY: a chunk's digits, [CB][blocks] of 2 KiB; a thread's share of the next one
     constexpr int kBlockBytes = 128 * 16, kShare = kW4Chunk * kBlockBytes / (kW4Threads * 16);
@@ -258,7 +241,8 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
         for (int c = 0; c < CB; c++)
 #pragma unroll
             for (int j = 0; j < kShare; j++)
-                share[c][j] = ((const v4i*)(scr + c * w4_frag_bytes(a.k, 16) + (int64_t)chunk * kW4Chunk * kBlockBytes))
+                share[c][j] = ((const v4i*)(scr + w4_row_block(blockIdx.y, CB, c, a.m) * w4_frag_bytes(a.k, 16) +
+                                            (int64_t)chunk * kW4Chunk * kBlockBytes))
                     [min((int)threadIdx.x + j * kW4Threads, rest - 1)];
     };
     auto put = [&](int chunk) {
@@ -455,12 +439,6 @@ __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* w, int64_
 
 int log2_groups(int32_t group) { return group == 128 ? 0 : group == 64 ? 1 : 2; }
 
-// LDS of a workgroup: scales, sums, exponents, digits
-size_t w4_lds(const W4Args& a, int split, int cb, size_t digits) {
-    return (size_t)(kW4Waves / split) * w4_groups(a.k, a.group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 128 + digits;
-}
-size_t w4_chunk_lds(int cb) { return (size_t)2 * cb * kW4Chunk * 128 * 16; }
-
 }  // namespace
 
 bool w4_supported(int32_t k, int32_t group) {
@@ -471,56 +449,13 @@ int64_t w4_packed_bytes(int32_t n, int32_t k, int32_t group, int32_t scale_dtype
     return (int64_t)w4_tiles(n) * (w4_blocks(k) * 1024ll + w4_groups(k, group) * 16ll * (scale_dtype == DT_F32 ? 4 : 2));
 }
 
-size_t w4_scratch(int32_t m, int32_t k) {
-    return m <= 0 ? 0 : w4_digit_off(m) + ((size_t)m + 3) / 4 * w4_frag_bytes(k, 16);
-}
-
 hipError_t launch_linear_w4(hipStream_t s, const W4Args& a) {
     if (a.m <= 0 || a.n <= 0) return hipSuccess;
-    const int tiles = w4_tiles(a.n), cbs = (a.m + 3) / 4;
-    W4Shape sh;
-    sh.cols = a.m == 1 ? 4 : a.m == 2 ? 8 : 16;
-    // Up to four rows each workgroup converts them itself where their digits fit in 64
-    // KiB: one kernel.  One row by 32000 x 2048: 11.8 us, 19.2 through scratch; four by
-    // 5632 x 2048: 8.5, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch
-    // 20.8.  More rows would be converted by too many: 16 by 5632 x 2048 16.1, 10.7.
-    const bool convert = cbs == 1 && w4_frag_bytes(a.k, sh.cols) <= 64 * 1024 && w4_slots(a.m, a.k) <= kSlots;
-    int cb = 1;
-    size_t digits;
-    if (convert) {
-        digits = w4_frag_bytes(a.k, sh.cols);
-        // wavefronts per tile: enough of them for 4 on each CU (one row by 14336 x 8192
-        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9;
-        // each measured before the rows stayed in registers)
-        sh.split = 1;
-        while (sh.split < kW4Waves && ((int64_t)tiles * sh.split < kW4EnoughWaves || w4_lds(a, sh.split, 1, digits) > (size_t)kW4Lds))
-            sh.split *= 2;
-    } else {
-        sh.cols = 16;
-        // What a workgroup moves through its CU: 16 CB bytes of digits and 8 of weights per
-        // tile and column of x, in as many rounds as 256 CUs need (16 rows by 32000 x 2048:
-        // 20.9 us; counted with 512 at once 24.1)
-        int64_t best = INT64_MAX;
-        for (int c : {4, 2, 1}) {
-            if (c > 1 && c / 2 >= cbs) continue;   // rows to spare
-            for (int split = 1; split <= kW4Waves; split *= 2) {
-                if (w4_lds(a, split, c, w4_chunk_lds(c)) > (size_t)kW4Lds) continue;
-                const int per = kW4Waves / split;
-                const int64_t wgs = (int64_t)((tiles + per - 1) / per) * ((cbs + c - 1) / c);
-                const int64_t cost = (wgs + 255) / 256 * (2 * c + per);
-                if (cost < best) {
-                    best = cost;
-                    cb = c;
-                    sh.split = split;
-                }
-            }
-        }
-        digits = w4_chunk_lds(cb);
-        TL_KLAUNCH(w4_digits_kernel, dim3(a.m), dim3(kW4Threads), 0, s, a);
-    }
-    const int per = kW4Waves / sh.split;
-    const dim3 grid((tiles + per - 1) / per, (cbs + cb - 1) / cb), block(kW4Threads);
-    const size_t lds = w4_lds(a, sh.split, cb, digits);
+    const W4Plan p = w4_plan(a.m, a.n, a.k, a.group);
+    if (!p.convert) TL_KLAUNCH(w4_digits_kernel, dim3(a.m), dim3(kW4Threads), 0, s, a);
+    const W4Shape sh{p.split, p.cols};
+    const dim3 grid(p.grid_x, p.grid_y), block(kW4Threads);
+    const size_t lds = p.lds;
     auto go = [&](auto cbt, auto copyt) {
         constexpr int CB = decltype(cbt)::value;
         constexpr bool COPY = decltype(copyt)::value;
@@ -531,9 +466,9 @@ hipError_t launch_linear_w4(hipStream_t s, const W4Args& a) {
         }
     };
     using std::integral_constant;
-    if (convert) go(integral_constant<int, 1>{}, std::false_type{});
-    else if (cb == 1) go(integral_constant<int, 1>{}, std::true_type{});
-    else if (cb == 2) go(integral_constant<int, 2>{}, std::true_type{});
+    if (p.convert) go(integral_constant<int, 1>{}, std::false_type{});
+    else if (p.cb == 1) go(integral_constant<int, 1>{}, std::true_type{});
+    else if (p.cb == 2) go(integral_constant<int, 2>{}, std::true_type{});
     else go(integral_constant<int, 4>{}, std::true_type{});
     return hipGetLastError();
 }

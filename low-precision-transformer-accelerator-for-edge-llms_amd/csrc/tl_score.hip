@@ -312,9 +312,9 @@ __global__ __launch_bounds__(kThreads, TILES == 1 ? 4 : 7) void logprobs_kernel(
             // infinity): all of them.  Then of the equal ones, or of minus infinity, as many
             // as are missing, lowest index first.
             unsigned nth = order_bits(-__builtin_inff());
-            auto bits = [&](int t, int j) {   // 0: no logit
+            auto bits = [&](int t, int j) {   // 0: no logit (a tile behind the part's last has the next part's indices)
                 const int i = first + t * kRun + j;
-                return x[t][j] == x[t][j] && (unsigned)i < (unsigned)a.vocab ? order_bits(x[t][j]) : 0u;
+                return t < live && x[t][j] == x[t][j] && (unsigned)i < (unsigned)a.vocab ? order_bits(x[t][j]) : 0u;
             };
             if (n > kList) {
                 nth = 0;

@@ -77,6 +77,7 @@ void    tl_destroy(tl_handle *h);
 const char *tl_last_error(const tl_handle *h);   /* h may be NULL: last tl_create failure */
 const char *tl_status_string(int32_t status);
 int32_t tl_get_config(const tl_handle *h, tl_config *cfg);
+int32_t tl_get_device(const tl_handle *h, int32_t *device);   /* HIP device the handle was made on */
 int32_t tl_sync(tl_handle *h);
 
 /* Layer weights in TL:249-267 order q,k,v,o,gate,up,down; w[i] is [N_i][K_i]

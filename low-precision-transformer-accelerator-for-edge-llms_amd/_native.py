@@ -102,6 +102,7 @@ SIGNATURES = {
     "tl_last_error": (C.c_char_p, [_vp]),
     "tl_status_string": (C.c_char_p, [_i32]),
     "tl_get_config": (_i32, [_vp, C.POINTER(TlConfig)]),
+    "tl_get_device": (_i32, [_vp, C.POINTER(_i32)]),
     "tl_sync": (_i32, [_vp]),
     "tl_load_layer": (_i32, [_vp, _i32, _vp * 7, _vp * 7, _vp, _vp, _i32]),
     "tl_load_lm_head": (_i32, [_vp, _vp, _vp, _vp, _i32]),
@@ -222,15 +223,6 @@ def _fence(args) -> None:
             return
 
 
-def _current_device() -> int:
-    """The device a handle made now belongs to."""
-    try:
-        import torch
-    except ImportError:
-        return 0
-    return torch.cuda.current_device()
-
-
 def _addr(x) -> int | None:
     """Device or host address of a torch tensor, a NumPy array or an int."""
     if x is None:
@@ -257,7 +249,9 @@ class Runtime:
             raise (TlValueError if st == TL_ERR_BAD_DESCRIPTOR else TlError)(st, f"tl_create: {msg}")
         self.h = h
         self.max_seqs = max_seqs
-        self.device = _current_device()
+        dev = _i32()
+        self.check(self.lib.tl_get_device(h, C.byref(dev)), "tl_get_device")
+        self.device = dev.value
 
     def close(self):
         if getattr(self, "h", None):

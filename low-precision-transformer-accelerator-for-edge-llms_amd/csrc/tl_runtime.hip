@@ -1303,6 +1303,12 @@ int32_t tl_get_config(const tl_handle* h, tl_config* cfg) {
     return TL_OK;
 }
 
+int32_t tl_get_device(const tl_handle* h, int32_t* device) {
+    if (!h || !device) return TL_ERR_BAD_DESCRIPTOR;
+    *device = h->device;
+    return TL_OK;
+}
+
 int32_t tl_sync(tl_handle* h) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     return finish(h);

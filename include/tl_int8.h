@@ -19,7 +19,11 @@
  *     name ends in _async.  Device inputs must therefore be complete when a
  *     call is made: a caller that wrote them on another stream synchronizes
  *     that stream first.
- *   - A handle is not thread safe: one host thread per handle.
+ *   - A handle is not thread safe: one host thread per handle, but for the calls
+ *     whose name ends in _async and those that give the sizes of their buffers
+ *     (_scratch, tl_w4_packed_bytes), which any number may make meanwhile.
+ *     tl_last_error gives the calling thread's copy of the latest message, good
+ *     until the thread asks again.
  *   - Matrices are row-major; weights are [N][K] int8 (one output channel per
  *     K-contiguous row, docs/design_decisions.txt B3) with one float32 scale
  *     per output channel (A10, B1).

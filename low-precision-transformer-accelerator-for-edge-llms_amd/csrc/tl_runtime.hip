@@ -191,7 +191,7 @@ struct tl_handle {
 
     std::vector<void*> allocs;
     std::string err;
-
+    mutable std::mutex err_mutex;   // calls that only queue work may fail on several threads at once
 
     bool batch_kslice = true;             // up to 32 rows: K-sliced down GEMM folded by the next RMSNorm
                                           // row prologue (TL_BATCH_KSLICE=0 turns it off)
@@ -235,8 +235,12 @@ struct tl_handle {
 namespace {
 
 int fail(tl_handle* h, int32_t code, const std::string& msg) {
-    if (h) h->err = msg;
-    else g_create_error = msg;
+    if (h) {
+        const std::lock_guard<std::mutex> lock(h->err_mutex);
+        h->err = msg;
+    } else {
+        g_create_error = msg;
+    }
     return code;
 }
 
@@ -1135,7 +1139,14 @@ const char* tl_status_string(int32_t s) {
     }
 }
 
-const char* tl_last_error(const tl_handle* h) { return h ? h->err.c_str() : g_create_error.c_str(); }
+const char* tl_last_error(const tl_handle* h) {
+    if (!h) return g_create_error.c_str();
+    // the calling thread's copy: another thread's call may fail meanwhile
+    thread_local std::string copy;
+    const std::lock_guard<std::mutex> lock(h->err_mutex);
+    copy = h->err;
+    return copy.c_str();
+}
 
 int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
     if (!cfg || !out) return fail(nullptr, TL_ERR_BAD_DESCRIPTOR, "null argument");

@@ -321,10 +321,12 @@ int32_t tl_pack_w4(tl_handle *h, const uint8_t *q, const void *scales, int32_t s
 /* y[m][n] = residual[m][n] + sum_k x[m][k] w[n][k], x, residual and y of type act
  * (TL_F32, TL_BF16, TL_F16), residual may be NULL or y; x and y must not
  * overlap.  All dev; strides in elements, x's
- * rows 16-byte aligned.  A row of x is taken as integers of 2^-30 of its largest
- * magnitude, products are exact, sums float32; an infinity or NaN in a row of x makes
- * its whole row of y NaN.  Few rows (a decoding step) are what it is made for; up to
- * 2^17 are right.  n at most 2^24, n k below 2^35. */
+ * rows 16-byte aligned.  Each 128 columns of a row of x (from a multiple of 128) are
+ * taken as integers of 2^-30 of their largest magnitude, products are exact, sums
+ * float32: a value far below another of its 128 has fewer bits than float32, one 3000
+ * times smaller some 18.  An infinity or NaN in a row of x makes its whole row of y
+ * NaN.  Few rows (a decoding step) are what it is made for; up to 2^17 are right.  n at
+ * most 2^24, n k below 2^35. */
 int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
                      int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void *residual,
                      int64_t res_stride, void *y, int64_t y_stride);

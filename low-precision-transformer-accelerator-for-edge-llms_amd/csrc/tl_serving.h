@@ -100,8 +100,9 @@ inline bool rows_apart(const void* p, int64_t sp, int64_t wp, const void* q, int
 // Projections with 4-bit weights: sizes, the plan of a call, and where its pieces lie.
 //
 // Weights come in tiles of 16 rows and blocks of 128 columns.  Scratch of a call
-// (w4_scratch() bytes): the exponents of its rows of x, then the digits of each four
-// rows ("row block"), w4_frag_bytes(k, 16) bytes.
+// (w4_scratch() bytes): the exponents of its rows of x; of each four rows ("row block")
+// the exponents of their blocks, w4_bexp_bytes(k) bytes; then the row blocks' digits,
+// w4_frag_bytes(k, 16) bytes each.
 constexpr int32_t kW4Waves = 8, kW4Threads = 64 * kW4Waves;
 constexpr int32_t kW4MaxGroups = 1024;
 constexpr int64_t kW4EnoughWaves = 1024;
@@ -114,7 +115,11 @@ TL_HD inline int32_t w4_tiles(int32_t n) { return (n + 15) / 16; }
 TL_HD inline int32_t w4_row_blocks(int32_t m) { return (m + 3) / 4; }
 TL_HD inline int32_t w4_groups(int32_t k, int32_t group) { return w4_blocks(k) * (128 / group); }   // with the padding's
 TL_HD inline int64_t w4_frag_bytes(int32_t k, int32_t cols) { return (int64_t)w4_blocks(k) * 128 * cols; }
-TL_HD inline int64_t w4_digit_off(int32_t m) { return ((int64_t)m * 4 + 15) / 16 * 16; }
+TL_HD inline int64_t w4_bexp_bytes(int32_t k) { return (int64_t)w4_blocks(k) * 8; }   // int16 [block][row]
+TL_HD inline int64_t w4_bexp_off(int32_t m) { return ((int64_t)m * 4 + 15) / 16 * 16; }
+TL_HD inline int64_t w4_digit_off(int32_t m, int32_t k) {
+    return w4_bexp_off(m) + (w4_row_blocks(m) * w4_bexp_bytes(k) + 15) / 16 * 16;
+}
 // units of all of `rows` rows that a thread takes
 TL_HD inline int32_t w4_slots(int32_t rows, int32_t k) { return rows * ((w4_blocks(k) * 16 + kW4Threads - 1) / kW4Threads); }
 // The row block that workgroup row y takes as its c-th of cb.  Where cb does not divide
@@ -125,7 +130,7 @@ TL_HD inline int32_t w4_row_block(int32_t y, int32_t cb, int32_t c, int32_t m) {
     return b < last ? b : last;
 }
 inline size_t w4_scratch(int32_t m, int32_t k) {
-    return m <= 0 ? 0 : (size_t)(w4_digit_off(m) + w4_row_blocks(m) * w4_frag_bytes(k, 16));
+    return m <= 0 ? 0 : (size_t)(w4_digit_off(m, k) + w4_row_blocks(m) * w4_frag_bytes(k, 16));
 }
 
 struct W4Plan {
@@ -137,27 +142,29 @@ struct W4Plan {
     int64_t lds;           // bytes of a workgroup
 };
 
-// LDS of a workgroup: scales, sums, exponents, digits
+// LDS of a workgroup: scales, sums, exponents of rows and blocks, digits
 inline int64_t w4_lds(int32_t k, int32_t group, int32_t split, int32_t cb, int64_t digits) {
-    return (int64_t)(kW4Waves / split) * w4_groups(k, group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 128 + digits;
+    return (int64_t)(kW4Waves / split) * w4_groups(k, group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 192 +
+           (cb * w4_bexp_bytes(k) + 15) / 16 * 16 + digits;
 }
 
 inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {
     const int32_t tiles = w4_tiles(n), cbs = w4_row_blocks(m);
     W4Plan p{};
     p.cols = m == 1 ? 4 : m == 2 ? 8 : 16;
-    // Up to four rows each workgroup converts them itself where their digits fit in 64
-    // KiB: one kernel.  One row by 32000 x 2048: 11.8 us, 19.2 through scratch; four by
-    // 5632 x 2048: 8.5, 11.0; three by 8192 x 8192 (128 KiB): 28.4, through scratch
-    // 20.8.  More rows would be converted by too many: 16 by 5632 x 2048 16.1, 10.7.
-    p.convert = cbs == 1 && w4_frag_bytes(k, p.cols) <= 64 * 1024 && w4_slots(m, k) <= kW4Slots;
+    // Up to four rows each workgroup converts them itself where its registers hold them
+    // (their digits are 64 KiB then at most): one kernel.  One row by 32000 x 2048: 11.8 us,
+    // 18.3 through scratch; by 14336 x 8192: 14.5, 28.3; four by 5632 x 2048: 7.9, 10.3.
+    // More rows would be converted by too many: 16 by 5632 x 2048 16.1, 10.7.
+    p.convert = cbs == 1 && w4_slots(m, k) <= kW4Slots;
     p.cb = 1;
     int64_t digits;
     if (p.convert) {
         digits = w4_frag_bytes(k, p.cols);
         // wavefronts per tile: enough of them for 4 on each CU (one row by 14336 x 8192
-        // 15.8 us, with half of them 20.3; by 32000 x 2048 12.5, with twice of them 13.9;
-        // each measured before the rows stayed in registers)
+        // 14.5 us, with half of them 19.6; by 5632 x 2048 5.8 in a graph, with half of them
+        // 6.3, with twice 6.8; four by 5632 x 2048 7.9, with twice 8.9.  Two rows by 8192 x
+        // 8192 would rather have twice: 11.8 us for 14.0)
         p.split = 1;
         while (p.split < kW4Waves && ((int64_t)tiles * p.split < kW4EnoughWaves || w4_lds(k, group, p.split, 1, digits) > kW4Lds))
             p.split *= 2;

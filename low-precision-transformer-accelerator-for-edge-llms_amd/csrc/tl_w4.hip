@@ -3,25 +3,28 @@
 // y[m][n] = (residual +) sum_g s[n][g] sum_{k in g} w[n][k] x[m][k], w in -8 .. 7.
 //
 // The inner sums run on the INT8 matrix instructions, exactly.  A nibble becomes
-// the INT8 number 16 w by a mask (and a shift for the low one).  A row of x becomes
-// four base-256 digits, each -128 .. 127: it is scaled by a power of two so that
-// its largest magnitude lies in [2^29, 2^30) and rounded to integers v, whose
-// digits are the bytes of (v + 0x808080) ^ 0x808080.  So a value is off by at most
-// 2^-30 of its row's largest, whatever its type; products and sums over a group
-// are exact in INT32, and only the sum over groups, each times its scale, rounds,
+// the INT8 number 16 w by a mask (and a shift for the low one).  128 columns of a row
+// of x become four base-256 digits, each -128 .. 127: they are scaled by a power of two
+// of their own so that their largest magnitude lies in [2^29, 2^30) and rounded to
+// integers v, whose digits are the bytes of (v + 0x808080) ^ 0x808080.  So a value is
+// off by at most 2^-30 of the largest of its 128 columns, whatever its type (with one
+// power for a whole row, an outlier took bits from all of it: 4096 columns with one of
+// 30000 times the rest lost a factor of 80 against float32); products and sums over a
+// group are exact in INT32, and only the sum over groups, each times its scale, rounds,
 // in float32.  The 16 columns of a product are four rows of x with four digits.
 //
 // What bounds it: the weights, k / 2 bytes a row, read once; of the rest the
 // latency from the first load to the result.  They stream in the order of the
 // lanes' registers, 1 KiB for 16 rows by 128 columns, 8 KiB in flight in each
 // wavefront; the digits of up to 16 rows of x wait in LDS.  Rows of x, scales and the
-// first weights are asked for together, and a row stays in registers from the search
-// for its largest magnitude to its digits (loaded twice: four rows by 5632 x 2048 9.8
-// us, now 8.5).  Queued back to back, one row by 5632 x 2048 takes 7.7 us (6.1 in a
-// graph), by 32000 x 2048 (group 32, float32 scales) 11.8, by 14336 x 8192 14.9 (4.1
-// TB/s); 13 rows by 2048 x 5632 14.4 (5 of them the digits' kernel), 16 by 32000 x
-// 2048 20.5.  With the weights in the rows' own order, where a load's pieces lie k / 2
-// bytes apart, the second took 20.9.
+// first weights are asked for together, and a block of x turns to digits as soon as it
+// is there: only the sums need to know the whole row's largest magnitude (with one
+// power of two for a row, and a barrier before its digits, four rows by 5632 x 2048
+// took 8.5 us, now 7.9).  Queued back to back, one row by 5632 x 2048 takes 7.8 us (5.8
+// in a graph), by 32000 x 2048 (group 32, float32 scales) 11.8, by 14336 x 8192 14.5
+// (4.1 TB/s); 13 rows by 2048 x 5632 14.5, 16 by 32000 x 2048 20.8.  With the weights
+// in the rows' own order, where a load's pieces lie k / 2 bytes apart, the second took
+// 20.9.
 #include <algorithm>
 
 #include "tl_rows.h"
@@ -49,20 +52,22 @@ TL_DEV void digits4(int v0, int v1, int v2, int v3, unsigned d[4]) {
     d[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
 }
 
-// Rows row0 .. row0 + rows - 1 of x (rows <= 4) to digits, by a whole workgroup that
-// keeps them in registers between the search for their largest magnitudes and the
-// conversion: kW4Slots units of 8 columns per thread, slot j of row j / per.
+// Rows of x to digits by a whole workgroup: kW4Slots units of 8 columns per thread.  A
+// block of 128 columns (16 adjacent threads) takes the power of two that brings its
+// largest magnitude to [2^29, 2^30), so that none waits for another.
 struct RowUnits {
     v4i raw[kW4Slots][2];
 
-    TL_DEV void load(const W4Args& a, int row0, int rows) {
-        const int units = a.k >> 3, per = (w4_blocks(a.k) * 16 + kW4Threads - 1) / kW4Threads;
+    // slot j: unit u0 + threadIdx.x + (j % per) * kW4Threads of row row0 + j / per, zeros
+    // behind the rows and the columns
+    TL_DEV void load(const W4Args& a, int row0, int rows, int per, int u0) {
+        const int units = a.k >> 3;
 #pragma unroll
         for (int j = 0; j < kW4Slots; j++) {
-            const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
+            const int r = j / per, u = u0 + threadIdx.x + (j - r * per) * kW4Threads;
             raw[j][0] = raw[j][1] = v4i{0, 0, 0, 0};
             if (r >= rows || u >= units) continue;
-            const int64_t at = (row0 + r) * a.x_stride + 8 * u;
+            const int64_t at = (row0 + r) * a.x_stride + 8 * (int64_t)u;
             if (a.act == DT_F32) {
                 raw[j][0] = *(const v4i*)((const float*)a.x + at);
                 raw[j][1] = *(const v4i*)((const float*)a.x + at + 4);
@@ -72,45 +77,58 @@ struct RowUnits {
         }
     }
 
-    // digits to base, zero from column k on; exps[r]: the power of two the row was scaled by
-    // (kBadRow: not finite).  mx: a word per row, zero.  Ends without a barrier.
-    TL_DEV void digits(const W4Args& a, int rows, char* base, int cols, unsigned* mx, int* exps) {
-        const int padded = w4_blocks(a.k) * 16, per = (padded + kW4Threads - 1) / kW4Threads;
-        v4f x[kW4Slots][2];
-#pragma unroll
-        for (int j = 0; j < kW4Slots; j++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                x[j][h] = a.act == DT_F32 ? __builtin_bit_cast(v4f, raw[j][h])
-                                          : unpack4(v2i{raw[j][0][2 * h], raw[j][0][2 * h + 1]}, a.act);
-        // magnitudes order as their bits do, infinity and NaN above the numbers
+    // digits to base, zero from column k on; bexp[4 block + row]: the blocks' powers of two;
+    // most[j * kW4Waves + wave]: the largest magnitude (as bits) of the wavefront's slot j,
+    // not less than what is there if `more`
+    TL_DEV void digits(const W4Args& a, int rows, int per, int u0, char* base, int cols, int16_t* bexp, unsigned* most,
+                       bool more) {
+        const int padded = w4_blocks(a.k) * 16;
 #pragma unroll
         for (int j = 0; j < kW4Slots; j++) {
-            const int r = j / per;
+            const int r = j / per, u = u0 + threadIdx.x + (j - r * per) * kW4Threads;
             if (r >= rows) break;
+            v4f x[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                x[h] = a.act == DT_F32 ? __builtin_bit_cast(v4f, raw[j][h])
+                                       : unpack4(v2i{raw[j][0][2 * h], raw[j][0][2 * h + 1]}, a.act);
+            // magnitudes order as their bits do, infinity and NaN above the numbers
             unsigned m = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(fabsf(x[j][i >> 2][i & 3])));
+            for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(fabsf(x[i >> 2][i & 3])));
             m = max(m, (unsigned)dpp<kDppXor1>((int)m));
             m = max(m, (unsigned)dpp<kDppXor2>((int)m));
             m = max(m, (unsigned)dpp<kDppHalfMirror>((int)m));
             m = max(m, (unsigned)dpp<kDppRowMirror>((int)m));
-            if ((threadIdx.x & 15) == 0) atomicMax(&mx[r], m);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kW4Slots; j++) {
-            const int r = j / per, u = threadIdx.x + (j - r * per) * kW4Threads;
-            if (r >= rows) break;
-            const unsigned m = mx[r];
-            const bool bad = m >= 0x7F800000u;
-            const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
-            if (u == 0) exps[r] = bad ? kBadRow : e;
-            if (u < padded) put(x[j][0], x[j][1], e, bad, r, u, base, cols);
+            const unsigned all = max(max((unsigned)row_value((int)m, 0), (unsigned)row_value((int)m, 1)),
+                                     max((unsigned)row_value((int)m, 2), (unsigned)row_value((int)m, 3)));
+            const int slot = j * kW4Waves + wave_id();
+            if (lane_id() == 0) most[slot] = more ? max(most[slot], all) : all;
+            if (u >= padded) continue;
+            const int e = fit(m);
+            put(x[0], x[1], e, r, u, base, cols);
+            if ((u & 15) == 0) bexp[(u >> 4) * 4 + r] = (int16_t)(e == kBadRow ? 0 : e);
         }
     }
 
-    static TL_DEV void put(v4f x0, v4f x1, int e, bool bad, int r, int u, char* base, int cols) {
+    // the power of two that brings a largest magnitude (its bits) to [2^29, 2^30); of zeros
+    // one above all others, so that a block of them counts by little
+    static TL_DEV int fit(unsigned m) {
+        return m >= 0x7F800000u ? kBadRow : m == 0 ? 255 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
+    }
+
+    // that of a whole row, its slots' maxima being n words
+    static TL_DEV int fit_row(const unsigned* most, int n) {
+        unsigned m = 0;
+        for (int i = 0; i < n; i += 4) {
+            const v4i v = *(const v4i*)(most + i);
+            m = max(max(m, (unsigned)v[0]), max(max((unsigned)v[1], (unsigned)v[2]), (unsigned)v[3]));
+        }
+        return fit(m);
+    }
+
+    static TL_DEV void put(v4f x0, v4f x1, int e, int r, int u, char* base, int cols) {
+        const bool bad = e == kBadRow;
         int v[8];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -128,42 +146,19 @@ struct RowUnits {
 };
 
 __global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
-    __shared__ unsigned mx[1];
-    const int row = blockIdx.x, tid = threadIdx.x;
+    __shared__ __align__(16) unsigned most[kW4Slots * kW4Waves];
+    const int row = blockIdx.x, padded = w4_blocks(a.k) * 16;
     char* s = (char*)a.scratch;
     // one row at its place among its four
-    char* base = s + w4_digit_off(a.m) + (row >> 2) * w4_frag_bytes(a.k, 16) + (row & 3) * 64;
-    if (tid == 0) mx[0] = 0u;
-    RowUnits x;
-    if (w4_slots(1, a.k) <= kW4Slots) {
-        x.load(a, row, 1);
-        __syncthreads();
-        x.digits(a, 1, base, 16, mx, (int*)s + row);
-        return;
+    char* base = s + w4_digit_off(a.m, a.k) + (row >> 2) * w4_frag_bytes(a.k, 16) + (row & 3) * 64;
+    int16_t* bexp = (int16_t*)(s + w4_bexp_off(a.m) + (row >> 2) * w4_bexp_bytes(a.k)) + (row & 3);
+    for (int u0 = 0; u0 < padded; u0 += kW4Slots * kW4Threads) {
+        RowUnits x;
+        x.load(a, row, 1, kW4Slots, u0);
+        x.digits(a, 1, kW4Slots, u0, base, 16, bexp, most, u0 > 0);
     }
-    // longer rows are read twice
     __syncthreads();
-    const int units = a.k >> 3, padded = w4_blocks(a.k) * 16;
-    unsigned m = 0;
-    for (int u = tid; u < units; u += kW4Threads) {
-        const v4f x0 = load4(a.x, row * a.x_stride + 8 * u, a.act), x1 = load4(a.x, row * a.x_stride + 8 * u + 4, a.act);
-#pragma unroll
-        for (int j = 0; j < 4; j++) m = max(m, max(__float_as_uint(fabsf(x0[j])), __float_as_uint(fabsf(x1[j]))));
-    }
-    atomicMax(&mx[0], m);
-    __syncthreads();
-    m = mx[0];
-    const bool bad = m >= 0x7F800000u;
-    const int e = bad || m == 0 ? 0 : 30 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
-    if (tid == 0) ((int*)s)[row] = bad ? kBadRow : e;
-    for (int u = tid; u < padded; u += kW4Threads) {
-        v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
-        if (u < units) {
-            x0 = load4(a.x, row * a.x_stride + 8 * u, a.act);
-            x1 = load4(a.x, row * a.x_stride + 8 * u + 4, a.act);
-        }
-        RowUnits::put(x0, x1, e, bad, 0, u, base, 16);
-    }
+    if (threadIdx.x == 0) ((int*)s)[row] = RowUnits::fit_row(most, kW4Slots * kW4Waves);
 }
 
 struct W4Shape {
@@ -191,7 +186,15 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     // everything the workgroup starts with, on its way at once: its rows of x, the first
     // scales, the first weights
     RowUnits x;
-    if constexpr (!COPY) x.load(a, m0, min(4, a.m - m0));
+    const int slots = w4_slots(1, a.k);   // of a row
+    if constexpr (!COPY) x.load(a, m0, min(4, a.m - m0), slots, 0);
+    // COPY: exponents of the row blocks' blocks, [nblk][CB] fours
+    auto block_exps = [&](int i) {
+        const int c = i % CB, blk = min(i / CB, nblk - 1);
+        return ((const v2i*)((const char*)a.scratch + w4_bexp_off(a.m) + w4_row_block(blockIdx.y, CB, c, a.m) * w4_bexp_bytes(a.k)))[blk];
+    };
+    v2i bexp0 = {0, 0};
+    if constexpr (COPY) bexp0 = block_exps(threadIdx.x);
 
     // scales of the workgroup's tiles as float32 [tile][group][16 rows]
     float* s_scale = (float*)lds;
@@ -225,11 +228,13 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     char* next = lds + (size_t)per * groups * 64;
     float* red = (float*)next;                     // [wave][16 rows][4 CB]
     next += kW4Waves * 16 * 4 * CB * 4;
-    unsigned* s_mx = (unsigned*)next;
-    int* s_exp = (int*)next + 16;
-    next += 128;
+    int* s_exp = (int*)next;                       // [4 CB]
+    unsigned* s_most = (unsigned*)next + 16;       // [kW4Slots][wave]
+    next += 192;
+    int16_t* s_bexp = (int16_t*)next;              // [nblk][CB][4]
+    next += (CB * w4_bexp_bytes(a.k) + 15) / 16 * 16;
     char* digits = next;
-    const char* scr = (const char*)a.scratch + w4_digit_off(a.m);
+    const char* scr = (const char*)a.scratch + w4_digit_off(a.m, a.k);
 
     // COPY: a chunk's digits, [CB][blocks] of 2 KiB; a thread's share of the next one
     constexpr int kBlockBytes = 128 * 16, kShare = kW4Chunk * kBlockBytes / (kW4Threads * 16);
@@ -256,27 +261,40 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
         if (threadIdx.x < 4 * CB) s_exp[threadIdx.x] = m0 + (int)threadIdx.x < a.m ? ((const int*)a.scratch)[m0 + threadIdx.x] : 0;
         fetch(0);
     } else {
-        if (threadIdx.x < 4) s_mx[threadIdx.x] = 0u;
-        __syncthreads();
-        x.digits(a, min(4, a.m - m0), digits, sh.cols, s_mx, s_exp);
+        x.digits(a, min(4, a.m - m0), slots, 0, digits, sh.cols, s_bexp, s_most, false);
     }
 #pragma unroll
     for (int j = 0; j < kFirst; j++)
         if ((int)threadIdx.x + j * kW4Threads < n4) put_scales(first[j], threadIdx.x + j * kW4Threads);
     for (int i = threadIdx.x + kFirst * kW4Threads; i < n4; i += kW4Threads)
         put_scales(wide ? ((const v4i*)sc)[i] : v4i{((const v2i*)sc)[i][0], ((const v2i*)sc)[i][1], 0, 0}, i);
-    if constexpr (COPY) put(0);
+    if constexpr (COPY) {
+        if ((int)threadIdx.x < CB * nblk) ((v2i*)s_bexp)[threadIdx.x] = bexp0;
+#pragma unroll 1
+        for (int i = threadIdx.x + kW4Threads; i < CB * nblk; i += kW4Threads) ((v2i*)s_bexp)[i] = block_exps(i);
+        put(0);
+    }
     __syncthreads();
 
     v4f acc[CB];
 #pragma unroll
     for (int c = 0; c < CB; c++) acc[c] = v4f{0, 0, 0, 0};
-    // A digit's sums enter times 256^(digit - 3) and 2^-32: 2^-22 of the result for rows
-    // around 1, so that no partial sum overflows whose result does not
+    // A digit's sums enter times 256^(digit - 3), 2^-32 and what their block's exponent is less
+    // than the row's: 2^-22 of the result for rows around 1, so that no partial sum
+    // overflows whose result does not
     const float place = __builtin_amdgcn_ldexpf(1.0f, 8 * (col & 3) - 56);
     const int mine = (nblk - part + sh.split - 1) / sh.split;   // blocks of this wavefront
     const float* scale = s_scale + (wave / sh.split) * groups * 16 + 4 * g;
     const int frag = w4_frag(0, g, col & (sh.cols - 1), sh.cols);
+    const int xrow = (col & (sh.cols - 1)) >> 2;   // this lane's row of a row block
+    int rexp[CB];                                  // the rows' exponents (not finite: any, the result is NaN)
+#pragma unroll
+    for (int c = 0; c < CB; c++) {
+        rexp[c] = COPY ? s_exp[4 * c + xrow] : RowUnits::fit_row(s_most + xrow * slots * kW4Waves, slots * kW4Waves);
+        if (!COPY && wave == 0 && g == 0 && (col & 3) == 0) s_exp[col >> 2] = rexp[c];   // read behind the next barrier
+        rexp[c] = max(rexp[c], -1000);
+    }
+    const int16_t* bexp = s_bexp + xrow;
     const int f64 = 4 * sh.cols * 16;              // bytes of 64 columns' digits
 
     auto block = [&](v4i q, int blk, const char* base) {
@@ -284,9 +302,12 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
         v4f sc[Q];
 #pragma unroll
         for (int j = 0; j < Q; j++) sc[j] = *(const v4f*)(scale + ((blk << LQ) + j) * 16);
+        int at = blk * CB * 4;
+        asm volatile("" : "+s"(at));   // (or every step of the loop holds an address of its own, 30 registers)
 #pragma unroll
         for (int c = 0; c < CB; c++) {
             const char* f = base + c * fcb + frag;
+            const float by = __builtin_amdgcn_ldexpf(place, rexp[c] - bexp[at + c * 4]);
             v4i t = {0, 0, 0, 0};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -298,7 +319,7 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
                     if (LQ == 1 || h == 1)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            acc[c][i] = __builtin_fmaf((float)t[i] * place, sc[LQ == 1 ? h : 0][i], acc[c][i]);
+                            acc[c][i] = __builtin_fmaf((float)t[i] * by, sc[LQ == 1 ? h : 0][i], acc[c][i]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
@@ -307,7 +328,7 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
                         const v4i u = __builtin_amdgcn_mfma_i32_16x16x32_i8(aa, bb, v4i{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            acc[c][i] = __builtin_fmaf((float)u[i] * place, sc[(2 * h + e) & (Q - 1)][i], acc[c][i]);
+                            acc[c][i] = __builtin_fmaf((float)u[i] * by, sc[(2 * h + e) & (Q - 1)][i], acc[c][i]);
                     }
                 }
             }

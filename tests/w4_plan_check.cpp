@@ -29,14 +29,15 @@ static void one(int m, int n, int k, int group) {
     }
     CHECK(p.cols == 16);
     const int64_t scratch = (int64_t)w4_scratch(m, k);
-    CHECK(w4_digit_off(m) >= 4ll * m && w4_digit_off(m) % 16 == 0);
+    CHECK(w4_bexp_off(m) >= 4ll * m && w4_bexp_off(m) % 16 == 0 && w4_digit_off(m, k) % 16 == 0);
     spare += p.grid_y * p.cb != cbs;
     // the workgroup rows at both ends, every row block of theirs
     for (int y : {0, p.grid_y - 2, p.grid_y - 1})
         for (int c = 0; c < p.cb && y >= 0; c++) {
             const int b = w4_row_block(y, p.cb, c, m);
             CHECK(b >= 0 && b < cbs && (b == y * p.cb + c || y * p.cb + c >= cbs));
-            CHECK(w4_digit_off(m) + (b + 1) * w4_frag_bytes(k, 16) <= scratch);
+            CHECK(w4_bexp_off(m) + (b + 1) * w4_bexp_bytes(k) <= w4_digit_off(m, k));
+            CHECK(w4_digit_off(m, k) + (b + 1) * w4_frag_bytes(k, 16) <= scratch);
         }
 }
 

@@ -286,8 +286,9 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
 /* Attention of one query row per token: row r of q [rows][n_heads * head_dim]
  * (dev, type act) attends keys 0 .. row_pos[r] of sequence row_seq[r] (NULL: r),
  * out[r] = softmax(scale q . k) . v in q's type; query head h reads KV head
- * h / (n_heads / n_kv_heads).  Scores, probabilities and sums are float32 (not
- * the INT8 probabilities of tl_attention).  A negative position has no keys: its
+ * h / (n_heads / n_kv_heads).  Scores and sums are float32; probabilities and q enter
+ * the products whole over a bfloat16 cache, over others within 2^-23 of themselves (or
+ * 2^-38 of the row's largest; not the INT8 probabilities of tl_attention).  A negative position has no keys: its
  * row is zero.  A negative row_seq is a padded row, left as it was.  Keys of a
  * page out of range are left out.  Several rows of one sequence at rising
  * positions are causal attention.  The keys are shared out evenly over the GPU

@@ -110,11 +110,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
 //
 // Precision: only 8 of the 16 columns are needed (up to 8 query heads of a KV
 // head per workgroup), so each head has two: one with the leading bits of q or
-// p in the 16-bit type, one with the rest.  Their sums restore about 22 bits
-// (float16) or 16 bits (bfloat16), where an exact 16-bit q uses the second
-// column for nothing.  A bfloat16 cache under float32 activations takes a
-// second product with the third part (X2).  INT8 keys and values are float16
-// integers, exactly.
+// p in the 16-bit type, one with the rest.  Two float16 parts, each rounded to
+// nearest, are within 2^-23 of a float32 number (or, far below the row's largest,
+// within 2^-38 of that); an exact 16-bit q uses the second column for nothing.  Two
+// bfloat16 parts hold 16 bits: probabilities over a bfloat16 cache take a second
+// product with the third part, which makes them whole, and so does q of other
+// activations (X2).  INT8 keys and values are float16 integers, exactly.
 // ---------------------------------------------------------------------------
 template <bool BF>
 TL_DEV v4f mfma32(v4i a, v4i b, v4f c) {
@@ -131,11 +132,11 @@ TL_DEV int i8_pair_f16(unsigned halves) {
     return __builtin_bit_cast(int, v - h2{(_Float16)1152.0f, (_Float16)1152.0f});
 }
 
-// truncating pack of two floats to the 16-bit type
+// two floats to the 16-bit type: bfloat16 truncated, float16 to nearest
 template <bool BF>
 TL_DEV int pack2(float a, float b) {
     if constexpr (BF) return (int)__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-    else return __builtin_bit_cast(int, __builtin_amdgcn_cvt_pkrtz(a, b));
+    else return __builtin_bit_cast(int, h2{(_Float16)a, (_Float16)b});
 }
 
 // W dwords read once
@@ -188,7 +189,8 @@ struct PagedTile {
     static constexpr int LDS = 32 * ROW > 8 * (HD + 4) * 4 ? 32 * ROW : 8 * (HD + 4) * 4;   // a wavefront's bytes
     static constexpr int VD = HD / 16;                   // dimensions of V per lane: O products
     static constexpr int VW = VD * ES / 4;               // dwords of a V row per lane
-    static constexpr int PARTS = X2 ? 2 : 1;
+    static constexpr int QP = X2 ? 2 : 1;                // products of q's parts
+    static constexpr int PP = BF ? 2 : 1;                // and of the probabilities'
 
     // first dimension of the 8 that lane group g multiplies in S product c
     TL_DEV static int q_dim(int c, int g) { return DT == DT_I8 ? (c >> 1) * 64 + 16 * g + 8 * (c & 1) : (c * 4 + g) * 8; }
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
             };
             fetch(kb);   // (a wavefront without keys: the last ones)
             // the query head's parts, scaled by a power of two so that float16 holds them
-            v4i qf[T::PARTS][T::KC];
+            v4i qf[T::QP][T::KC];
             float cs = a.scale * kLog2e;
             if constexpr (DT == DT_I8) cs *= a.c.ks[kvh];
             {
@@ -575,7 +577,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                 }
 #pragma unroll
                 for (int c = 0; c < T::KC; c++) {
-                    float part[T::PARTS][8];
+                    float part[T::QP][8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const float x = q[c][j] * up;
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                         if constexpr (X2) part[1][j] = lo ? 0.0f : x - hi - mid;
                     }
 #pragma unroll
-                    for (int p = 0; p < T::PARTS; p++)
+                    for (int p = 0; p < T::QP; p++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const float x = part[p][2 * j], y = part[p][2 * j + 1];
@@ -604,7 +606,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
             v4f o[T::VD];
 #pragma unroll
             for (int j = 0; j < T::VD; j++) o[j] = v4f{0, 0, 0, 0};
-            const unsigned lo_mask = lo ? (BF ? 0xFFFF0000u : 0xFFFFE000u) : 0u;
+            const unsigned lo_mask = lo ? 0xFFFFFFFFu : 0u;
 
             while (kb < end) {
 #pragma unroll
@@ -625,7 +627,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                             kk = *(const v4i*)(my_lds + T::slot(t, col, c * 4 + g));
                         }
 #pragma unroll
-                        for (int p = 0; p < T::PARTS; p++) s[t] = mfma32<BF>(kk, qf[p][c], s[t]);
+                        for (int p = 0; p < T::QP; p++) s[t] = mfma32<BF>(kk, qf[p][c], s[t]);
                     }
                 __builtin_amdgcn_wave_barrier();
 
@@ -660,22 +662,23 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                 }
                 // p 2^14, so that the float16 parts of small probabilities stay normal
                 const float off = m == -__builtin_inff() ? 0.0f : (BF ? m : m - 14.0f);
-                v4i pf[T::PARTS];
+                v4i pf[T::PP];
                 {
-                    float part[T::PARTS][8];
+                    float part[T::PP][8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const float p = __builtin_amdgcn_exp2f(x[j] - off);
                         l += p;
-                        const float r = p - __uint_as_float(__float_as_uint(p) & lo_mask);
-                        part[0][j] = r;
-                        if constexpr (X2) {
-                            const float hi = __uint_as_float(__float_as_uint(p) & 0xFFFF0000u), rest = p - hi;
+                        // the leading part (the pack rounds it off), or what it leaves
+                        const float hi = BF ? __uint_as_float(__float_as_uint(p) & 0xFFFF0000u) : (float)(_Float16)p;
+                        part[0][j] = p - __uint_as_float(__float_as_uint(hi) & lo_mask);
+                        if constexpr (BF) {
+                            const float rest = p - hi;
                             part[1][j] = lo ? 0.0f : rest - __uint_as_float(__float_as_uint(rest) & 0xFFFF0000u);
                         }
                     }
 #pragma unroll
-                    for (int p = 0; p < T::PARTS; p++)
+                    for (int p = 0; p < T::PP; p++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) pf[p][j] = pack2<BF>(part[p][2 * j], part[p][2 * j + 1]);
                 }
@@ -691,7 +694,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                             vv[r] = (int)__builtin_amdgcn_perm(vf[2 * r + 1][d >> 1], vf[2 * r][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
                     }
 #pragma unroll
-                    for (int p = 0; p < T::PARTS; p++) o[d] = mfma32<BF>(vv, pf[p], o[d]);
+                    for (int p = 0; p < T::PP; p++) o[d] = mfma32<BF>(vv, pf[p], o[d]);
                 }
                 // the registers' next rows
                 kb += kPagedTile;

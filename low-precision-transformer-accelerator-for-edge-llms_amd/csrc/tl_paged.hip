@@ -477,7 +477,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
     const int key_slot = (lane ^ T::swizzle(lane / T::KC_LINE)) * 16;
     const int me = blockIdx.x;
 
-    const bool few = a.rows <= 64;
+    const bool few = a.rows <= kPagedFewRows;
     RowScan first = {};
     LaneRows lr = {};
     int32_t total;
@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
     if (a.fault && bad) *a.fault = 1;
 }
 
-// the parts of one (row, head) joined, W of them side by side
+// the parts of one (row, head) joined, W of them side by side (paged_join_grid)
 template <int HD>
 __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(PagedAttnArgs a, int workgroups) {
     constexpr int Q = HD / 4, W = kAttnThreads / Q;   // quads of a row; parts taken side by side
@@ -775,30 +775,38 @@ __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(PagedAttnArgs 
     __shared__ float s_l[W], s_m[kAttnWaves];
     __shared__ ScanShared s_scan;
     const PagedGeom& geo = a.c.g;
-    const int head = blockIdx.y, row = blockIdx.x;
     const int rep = a.n_heads / geo.n_kv, blocks = (rep + 7) >> 3, hbs = geo.n_kv * blocks;
-    const int seq = a.row_seq ? a.row_seq[row] : row;
-    const int pos = a.row_pos[row];
-    if (paged_row_kind(geo, seq, pos) != PAGED_ROW_OK || pos < 0) return;
-    // the tiles before this row, and all
-    unsigned all;
-    int32_t before = 0, total = 0;
-    if (a.rows <= 64) {
+    int row, head, tiles;
+    int32_t unit;
+    PagedShare share;
+    if (a.rows <= kPagedFewRows) {
+        row = blockIdx.x;
+        head = blockIdx.y;
+        const int pos = a.row_pos[row];
+        if (paged_row_kind(geo, a.row_seq ? a.row_seq[row] : row, pos) != PAGED_ROW_OK || pos < 0) return;
+        unsigned all;
         const LaneRows l = lane_rows(a, all);
-        total = (int32_t)all;
-        before = __builtin_amdgcn_readlane((int)(l.upto - l.tiles), row);
+        share = paged_share((int32_t)all * hbs, workgroups);
+        tiles = paged_tiles(pos + 1);
+        const int kvh = head / rep, hb = kvh * blocks + ((head - kvh * rep) >> 3);
+        unit = __builtin_amdgcn_readlane((int)(l.upto - l.tiles), row) * hbs + hb * tiles;
+    } else {
+        const int w = blockIdx.x + 1;
+        RowScan first;
+        const int32_t total = __builtin_amdgcn_readfirstlane(count_tiles(a, s_scan, first));
+        share = paged_share(total * hbs, workgroups);
+        const int32_t at = share.start(w);
+        if (at >= total * hbs || at == share.start(w - 1)) return;
+        int32_t before;
+        find_row(a, s_scan, (unsigned)at / (unsigned)hbs, first, row, before);
+        tiles = paged_tiles(a.row_pos[row] + 1);
+        const int32_t in = at - before * hbs;
+        const int hb = (int)((unsigned)in / (unsigned)tiles), kvh = hb / blocks, h = (hb - kvh * blocks) * 8 + (int)blockIdx.y;
+        unit = before * hbs + hb * tiles;
+        if (h >= rep || !paged_joins_at(share, w, unit)) return;
+        head = kvh * rep + h;
     }
-    for (int64_t r0 = 0; r0 < a.rows && a.rows > 64; r0 += kAttnThreads) {
-        const unsigned v = row_tiles(a, r0 + threadIdx.x);
-        block_scan(v, s_scan, all);
-        total += (int32_t)all;
-        block_scan(r0 + threadIdx.x < row ? v : 0u, s_scan, all);
-        before += (int32_t)all;
-    }
-    const PagedShare share = paged_share(total * hbs, workgroups);
-    const int kvh = head / rep, h = head - kvh * rep, hb = kvh * blocks + (h >> 3);
-    const int tiles = paged_tiles(pos + 1);
-    const int32_t unit = before * hbs + hb * tiles;
+    const int h = head % rep;
     const int w0 = share.owner(unit), w1 = share.owner(unit + tiles - 1);
     if (w0 == w1) return;   // one workgroup had all of it
     const int ml_at = 2 * (h & 7);
@@ -873,6 +881,7 @@ hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& args) {
     const bool one_tile = ((int64_t)a.c.g.max_pages << a.c.g.page_shift) <= kPagedTile;   // nothing is split
     if (one_tile) a.counters = nullptr;
     const dim3 grid(wgs), block(kAttnThreads);
+    const PagedJoinGrid join = paged_join_grid(a.rows, a.n_heads, a.c.g.n_kv, wgs);
     const bool x2 = a.c.dtype == DT_BF16 && a.act != DT_BF16;
     auto go = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
@@ -880,7 +889,7 @@ hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& args) {
         else if (a.c.dtype == DT_F16) TL_KLAUNCH((paged_attention_kernel<HD, DT_F16, false>), grid, block, 0, s, a);
         else if (x2) TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, true>), grid, block, 0, s, a);
         else TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, false>), grid, block, 0, s, a);
-        if (!a.counters && !one_tile) TL_KLAUNCH((paged_join_kernel<HD>), dim3(a.rows, a.n_heads), block, 0, s, a, wgs);
+        if (!a.counters && !one_tile) TL_KLAUNCH((paged_join_kernel<HD>), dim3(join.x, join.y), block, 0, s, a, wgs);
     };
     if (a.c.g.head_dim == 64) go(std::integral_constant<int, 64>{});
     else go(std::integral_constant<int, 128>{});

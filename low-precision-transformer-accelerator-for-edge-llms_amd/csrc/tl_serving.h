@@ -79,6 +79,24 @@ TL_HD inline PagedShare paged_share(int32_t tiles, int32_t workgroups) {
 TL_HD inline int32_t paged_part(const PagedShare& s, int32_t w, int32_t unit_start) {
     return 2 * w + (unit_start > s.start(w) ? 1 : 0);
 }
+// Whether the parts of the unit (row, head block) that starts at tile `unit` and holds
+// tile start(w) are joined at the boundary in front of workgroup w's run: of a unit's
+// boundaries, the first inside it.  Units that one workgroup has whole have none.
+TL_HD inline bool paged_joins_at(const PagedShare& s, int32_t w, int32_t unit) {
+    return s.start(w) > unit && s.start(w - 1) <= unit;
+}
+// The joining kernel's workgroups.  Up to 64 rows it has one per row and head; more
+// rows than that each would have to be looked for, though only workgroups - 1 (row, head
+// block)s can be split, so there it has one per boundary and head of a block.
+constexpr int32_t kPagedFewRows = 64;
+struct PagedJoinGrid {
+    int32_t x, y;
+};
+inline PagedJoinGrid paged_join_grid(int32_t rows, int32_t n_heads, int32_t n_kv, int32_t workgroups) {
+    if (rows <= kPagedFewRows) return {rows, n_heads};
+    const int32_t rep = n_heads / n_kv;
+    return {workgroups - 1, rep < 8 ? rep : 8};
+}
 // whether a call's tiles can be counted in 31 bits, were every row as long as the
 // table allows
 inline bool paged_countable(const PagedGeom& g, int32_t rows, int32_t head_blocks) {

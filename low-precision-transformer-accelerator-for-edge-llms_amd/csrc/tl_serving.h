@@ -151,6 +151,13 @@ inline size_t w4_scratch(int32_t m, int32_t k) {
     return m <= 0 ? 0 : (size_t)(w4_digit_off(m, k) + w4_row_blocks(m) * w4_frag_bytes(k, 16));
 }
 
+// workgroups of 256 threads that quantize units of 8 weights: a launch holds fewer than
+// 2^32 threads, which 2^35 weights would be
+inline uint32_t w4_quantize_grid(int64_t units) {
+    const int64_t all = (units + 255) / 256;
+    return (uint32_t)(all < 1 << 23 ? all : 1 << 23);
+}
+
 struct W4Plan {
     bool convert;          // one kernel that turns x into digits itself (up to four rows)
     int32_t cb;            // row blocks of a workgroup: 1, 2 or 4

@@ -430,32 +430,34 @@ __global__ __launch_bounds__(256) void pack_w4_kernel(const uint8_t* q, const vo
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void quantize_w4_kernel(const float* w, int64_t total8, int k, int group, int dt,
                                                           uint8_t* q, void* scales) {
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t at = min(u, total8 - 1) * 8;         // idle lanes repeat the last unit
-    const v4f x0 = *(const v4f*)(w + at), x1 = *(const v4f*)(w + at + 4);
-    float mx = 0.0f;
+    for (int64_t u0 = (int64_t)blockIdx.x * 256; u0 < total8; u0 += (int64_t)gridDim.x * 256) {
+        const int64_t u = u0 + threadIdx.x;
+        const int64_t at = min(u, total8 - 1) * 8;         // idle lanes repeat the last unit
+        const v4f x0 = *(const v4f*)(w + at), x1 = *(const v4f*)(w + at + 4);
+        float mx = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) mx = fmaxf(mx, fmaxf(fabsf(x0[j]), fabsf(x1[j])));
-    mx = fmaxf(mx, lane_xor<1>(mx));
-    mx = fmaxf(mx, lane_xor<2>(mx));
-    if (group >= 64) mx = fmaxf(mx, lane_xor<4>(mx));
-    if (group >= 128) mx = fmaxf(mx, lane_xor<8>(mx));
-    float s = __fdiv_rn(mx, 7.0f);
-    if (dt == DT_BF16) s = bf16_bits(to_bf16(s));
-    if (dt == DT_F16) s = f16_bits(to_f16(fminf(s, 65504.0f)));
-    const bool zero = s == 0.0f;
-    if (zero) s = 1.0f;
-    unsigned out = 0;
+        for (int j = 0; j < 4; j++) mx = fmaxf(mx, fmaxf(fabsf(x0[j]), fabsf(x1[j])));
+        mx = fmaxf(mx, lane_xor<1>(mx));
+        mx = fmaxf(mx, lane_xor<2>(mx));
+        if (group >= 64) mx = fmaxf(mx, lane_xor<4>(mx));
+        if (group >= 128) mx = fmaxf(mx, lane_xor<8>(mx));
+        float s = __fdiv_rn(mx, 7.0f);
+        if (dt == DT_BF16) s = bf16_bits(to_bf16(s));
+        if (dt == DT_F16) s = f16_bits(to_f16(fminf(s, 65504.0f)));
+        const bool zero = s == 0.0f;
+        if (zero) s = 1.0f;
+        unsigned out = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        float v = zero ? 0.0f : __builtin_rintf(__fdiv_rn(j < 4 ? x0[j & 3] : x1[j & 3], s));
-        v = v > 7.0f ? 7.0f : v;
-        v = v >= -8.0f ? v : -8.0f;
-        out |= ((unsigned)(int)v & 15u) << (4 * j);
+        for (int j = 0; j < 8; j++) {
+            float v = zero ? 0.0f : __builtin_rintf(__fdiv_rn(j < 4 ? x0[j & 3] : x1[j & 3], s));
+            v = v > 7.0f ? 7.0f : v;
+            v = v >= -8.0f ? v : -8.0f;
+            out |= ((unsigned)(int)v & 15u) << (4 * j);
+        }
+        if (u >= total8) continue;
+        *(unsigned*)(q + (at >> 1)) = out;
+        if (at % group == 0) store1(scales, at / group, dt, s);
     }
-    if (u >= total8) return;
-    *(unsigned*)(q + (at >> 1)) = out;
-    if (at % group == 0) store1(scales, at / group, dt, s);
 }
 
 int log2_groups(int32_t group) { return group == 128 ? 0 : group == 64 ? 1 : 2; }
@@ -506,7 +508,7 @@ hipError_t launch_quantize_w4(hipStream_t s, const float* w, int32_t rows, int32
                               uint8_t* q, void* scales) {
     const int64_t total8 = (int64_t)rows * k / 8;
     if (total8 <= 0) return hipSuccess;
-    TL_KLAUNCH(quantize_w4_kernel, dim3((unsigned)((total8 + 255) / 256)), dim3(256), 0, s, w, total8, k, group, scale_dtype, q,
+    TL_KLAUNCH(quantize_w4_kernel, dim3(w4_quantize_grid(total8)), dim3(256), 0, s, w, total8, k, group, scale_dtype, q,
                scales);
     return hipGetLastError();
 }

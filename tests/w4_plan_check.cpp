@@ -55,6 +55,11 @@ int main() {
     const int m = 0, n = 0, k = 0, group = 0;
     one(3, 20, 131072, 128);
     one(9, 20, 131072, 128);
+    // the quantizer's launch, at the most weights there may be
+    for (int64_t units : {1ll, 256ll, 257ll, 1ll << 31, (1ll << 32) - 255, (1ll << 32) - 4}) {
+        CHECK(w4_quantize_grid(units) >= 1 && (uint64_t)w4_quantize_grid(units) * 256 < 1ull << 32);
+        CHECK(units > 1 << 30 || (int64_t)w4_quantize_grid(units) * 256 >= units);
+    }
     CHECK(spare > 100);   // the case is among them
     std::printf("%d wrong\n", wrong);
     return wrong ? 1 : 0;

@@ -171,16 +171,16 @@ class Engine:
         its distribution and the ``top`` most probable next tokens.  NumPy
         arrays ``logprob``, ``entropy`` [n], ``top_ids``, ``top_logprobs`` [n][top]."""
         import torch
-        t = _np(tokens, np.int32)
-        n, vocab = int(t.size), int(self.cfg["vocab"])
+        t = _np(tokens, np.int32).reshape(-1)
+        n, vocab, top = int(t.size), int(self.cfg["vocab"]), int(top)
         dev = torch.device("cuda", self.rt.device)
         follow = torch.from_numpy(np.append(t[1:], np.int32(-1))).to(dev)
         logits = torch.empty((n, vocab), dtype=torch.float32, device=dev)
         self.rt.call("tl_prefill_logits", int(seq), t, n, logits)
         shapes = {"logprob": ((n,), torch.float32), "entropy": ((n,), torch.float32),
-                  "top_ids": ((n, int(top)), torch.int32), "top_logprobs": ((n, int(top)), torch.float32)}
+                  "top_ids": ((n, top), torch.int32), "top_logprobs": ((n, top), torch.float32)}
         got = {name: torch.empty(shape, dtype=dt, device=dev) for name, (shape, dt) in shapes.items()}
-        self.rt.call("tl_token_logprobs", logits, vocab, _native.TL_F32, n, vocab, follow, int(top), *got.values())
+        self.rt.call("tl_token_logprobs", logits, vocab, _native.TL_F32, n, vocab, follow, top, *got.values())
         return {name: x.cpu().numpy() for name, x in got.items()}
 
     def decode(self, max_new: int, seq: int = 0, eos_id: int = -1, abort_flag=None):

@@ -17,7 +17,7 @@ from types import SimpleNamespace
 import numpy as np
 
 from . import _native
-from ._native import TL_MEM_DEVICE, TL_MEM_HOST, Runtime
+from ._native import TL_MEM_DEVICE, TL_MEM_HOST, Runtime, TlValueError
 from .tinyllama import build_rope_cache
 
 WEIGHT_ORDER = ("q_w", "k_w", "v_w", "o_w", "gate_w", "up_w", "down_w")
@@ -173,6 +173,8 @@ class Engine:
         import torch
         t = _np(tokens, np.int32).reshape(-1)
         n, vocab, top = int(t.size), int(self.cfg["vocab"]), int(top)
+        if not 0 <= top <= min(32, vocab):   # before the prompt changes the sequence
+            raise TlValueError(_native.TL_ERR_BAD_DESCRIPTOR, "top must be 0 .. 32 and at most the vocabulary")
         dev = torch.device("cuda", self.rt.device)
         follow = torch.from_numpy(np.append(t[1:], np.int32(-1))).to(dev)
         logits = torch.empty((n, vocab), dtype=torch.float32, device=dev)

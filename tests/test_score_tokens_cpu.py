@@ -1,5 +1,5 @@
 """Engine.score_tokens' arguments, with a stand-in for the library's handle: what the kernels are given holds a value for
-each position."""
+each position, and a call that is refused has not touched the sequence."""
 import numpy as np
 import pytest
 import torch
@@ -34,3 +34,10 @@ def test_a_target_for_each_position(engine, shape):
     assert tokens.tolist() == list(range(6)) and logits.shape == (6, 50) and (rows, vocab, width, top) == (6, 50, 50, 3)
     assert targets.tolist() == [1, 2, 3, 4, 5, -1]
     assert [tuple(o.shape) for o in out] == [(6,), (6,), (6, 3), (6, 3)] and got["top_ids"].shape == (6, 3)
+
+
+@pytest.mark.parametrize("top", [-1, 33, 51])
+def test_refused_before_the_prompt_runs(engine, top):
+    with pytest.raises(ValueError, match="top"):
+        engine.score_tokens([1, 2, 3], top=top)
+    assert engine.rt.calls == []

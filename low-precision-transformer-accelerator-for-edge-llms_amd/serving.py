@@ -262,6 +262,8 @@ def quantize_w4(w, group: int = 128, scale_dtype=torch.float16, rt: Runtime | No
     if group not in (32, 64, 128) or k == 0 or k % group:
         raise _bad("group must be 32, 64 or 128 and divide k")
     rt = rt or _runtime(w.device)
+    if rt.device != w.device.index:
+        raise _bad("the handle belongs to another device")
     q = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, k // group), dtype=scale_dtype, device=w.device)
     with _COMPLETING:

@@ -286,14 +286,17 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
 /* Attention of one query row per token: row r of q [rows][n_heads * head_dim]
  * (dev, type act) attends keys 0 .. row_pos[r] of sequence row_seq[r] (NULL: r),
  * out[r] = softmax(scale q . k) . v in q's type; query head h reads KV head
- * h / (n_heads / n_kv_heads).  Scores and sums are float32; probabilities and q enter
- * the products whole over a bfloat16 cache, over others within 2^-23 of themselves (or
- * 2^-38 of the row's largest; not the INT8 probabilities of tl_attention).  A negative position has no keys: its
- * row is zero.  A negative row_seq is a padded row, left as it was.  Keys of a
- * page out of range are left out.  Several rows of one sequence at rising
- * positions are causal attention.  The keys are shared out evenly over the GPU
- * whatever the rows' lengths; the parts of a row that was split are joined, in the
- * order of its keys.  out may be q. */
+ * h / (n_heads / n_kv_heads).  Scores and sums are float32; probabilities and q (not
+ * INT8 as tl_attention's are) enter the products whole over a bfloat16 cache, over
+ * others within 2^-23 of themselves or 2^-38 of the row's largest.  A negative position
+ * has no keys: its row is zero.  A negative row_seq is a padded row, left as it was.
+ * Keys of a page out of range are left out; a row left without any is NaN, as a softmax
+ * over nothing is.  A key that is attended and not finite leaves the results of its KV
+ * head's query heads undefined, such a value its dimension of them infinite or NaN.
+ * Several rows of one sequence at rising positions are causal attention; each reads
+ * its keys for itself.  The keys are shared out evenly over the GPU whatever the rows'
+ * lengths; the parts of a row that was split are joined, in the order of its keys.  out
+ * may be q. */
 int32_t tl_paged_attention(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride, int32_t act,
                            int32_t rows, int32_t n_heads, const int32_t *row_seq, const int32_t *row_pos, float scale,
                            void *out, int64_t out_stride);
@@ -326,8 +329,9 @@ int32_t tl_pack_w4(tl_handle *h, const uint8_t *q, const void *scales, int32_t s
  * taken as integers of 2^-30 of their largest magnitude, products are exact, sums
  * float32: a value far below another of its 128 has fewer bits than float32, one 3000
  * times smaller some 18.  An infinity or NaN in a row of x makes its whole row of y
- * NaN.  Few rows (a decoding step) are what it is made for; up to 2^17 are right.  n at
- * most 2^24, n k below 2^35. */
+ * NaN; a scale that is not finite leaves its column of y infinite or NaN.  Few rows (a
+ * decoding step) are what it is made for; up to 2^17 are right.  n at most 2^24, n k
+ * below 2^35. */
 int32_t tl_linear_w4(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
                      int32_t scale_dtype, int32_t group, int32_t n, int32_t k, const void *residual,
                      int64_t res_stride, void *y, int64_t y_stride);

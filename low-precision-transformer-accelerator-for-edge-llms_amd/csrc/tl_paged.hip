@@ -22,7 +22,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 // read twice from memory; the row's cos and sin are shared by its heads through
 // the cache.  What bounds it: from one row to some hundreds the chain of loads and
 // the launch (3.5 us for 1 row as for 61); 2048 rows of 32 + 2 x 8 heads of 128 in
-// float16 take 11.5 us (3.0 TB/s).  A row's values are loaded before its place is
+// float16, 51 MB, take 11.5 us (4.5 TB/s).  A row's values are loaded before its place is
 // known, and the activations' type is the compiler's: with the type looked at per
 // load, loads wait for each other, 12.7 us.
 // ---------------------------------------------------------------------------
@@ -116,6 +116,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
 // bfloat16 parts hold 16 bits: probabilities over a bfloat16 cache take a second
 // product with the third part, which makes them whole, and so does q of other
 // activations (X2).  INT8 keys and values are float16 integers, exactly.
+//
+// What bounds it: memory where the cache is long (40 ragged rows of up to 8192 keys,
+// 32 / 8 heads of 128: bfloat16 120 us, 5.6 TB/s; float32 rows over bfloat16 121, over
+// float16 118), else the chain of loads and the join of the parts.  The third parts
+// cost 1 us of the first.
 // ---------------------------------------------------------------------------
 template <bool BF>
 TL_DEV v4f mfma32(v4i a, v4i b, v4f c) {
@@ -857,9 +862,9 @@ hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a) {
 
 // Workgroups of a call, no more than there can be tiles: two on each of 256 CUs, so
 // that one works while the other changes rows (40 ragged rows of up to 8192 keys, 8
-// KV heads: 118 us against 131 with one on each); one where at most 64 (row, head
-// block)s are split into long runs (8 rows of 16384: 88.7 us against 91.1; one row of
-// 131072, 4 KV heads: 52.8 against 55.6).
+// KV heads: 120 us against 133 with one on each; 32 INT8 rows of 1984, 4 KV heads of
+// 64: 15.6, 17.1); one where at most 64 (row, head block)s are split into long runs (8
+// rows of 16384: 90.0 us against 91.5; one row of 131072, 4 KV heads: 51.1, 53.4).
 int32_t paged_attention_workgroups(const PagedCache& c, int32_t rows, int32_t n_heads) {
     const int64_t units = (int64_t)rows * c.g.n_kv * head_blocks(n_heads, c.g.n_kv);
     const int64_t cap = (((int64_t)c.g.max_pages << c.g.page_shift) + kPagedTile - 1) / kPagedTile;

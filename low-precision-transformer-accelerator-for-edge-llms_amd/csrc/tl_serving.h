@@ -167,10 +167,10 @@ struct W4Plan {
     int64_t lds;           // bytes of a workgroup
 };
 
-// LDS of a workgroup: scales, sums, exponents of rows and blocks, digits
+// LDS of a workgroup: scales, sums, exponents, a word per row and block, digits
 inline int64_t w4_lds(int32_t k, int32_t group, int32_t split, int32_t cb, int64_t digits) {
     return (int64_t)(kW4Waves / split) * w4_groups(k, group) * 64 + kW4Waves * 16 * 4 * cb * 4 + 192 +
-           (cb * w4_bexp_bytes(k) + 15) / 16 * 16 + digits;
+           cb * w4_blocks(k) * 16 + digits;
 }
 
 inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {

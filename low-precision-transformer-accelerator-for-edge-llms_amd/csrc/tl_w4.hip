@@ -22,7 +22,7 @@
 // power of two for a row, and a barrier before its digits, four rows by 5632 x 2048
 // took 8.5 us, now 7.9).  Queued back to back, one row by 5632 x 2048 takes 7.8 us (5.8
 // in a graph), by 32000 x 2048 (group 32, float32 scales) 11.8, by 14336 x 8192 14.5
-// (4.1 TB/s); 13 rows by 2048 x 5632 14.5, 16 by 32000 x 2048 20.8.  With the weights
+// (4.1 TB/s); 13 rows by 2048 x 5632 14.4, 16 by 32000 x 2048 20.5.  With the weights
 // in the rows' own order, where a load's pieces lie k / 2 bytes apart, the second took
 // 20.9.
 #include <algorithm>
@@ -161,6 +161,13 @@ __global__ __launch_bounds__(kW4Threads) void w4_digits_kernel(W4Args a) {
     if (threadIdx.x == 0) ((int*)s)[row] = RowUnits::fit_row(most, kW4Slots * kW4Waves);
 }
 
+// What the sums of a block's digits count by: 2^-32, less what the block was scaled by
+// beyond its row.  2^-22 of the result then for rows around 1, so that no partial sum
+// overflows whose result does not.
+TL_DEV float count_by(int row, int block) {
+    return __builtin_amdgcn_ldexpf(1.0f, max(row, -1000) - block - 32);   // (a row that is not finite: any, its result is NaN)
+}
+
 struct W4Shape {
     int32_t split;       // wavefronts that share a tile of 16 weight rows: 1, 2, 4 or 8
     int32_t cols;        // columns of a product in use by the digits' layout
@@ -188,13 +195,23 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     RowUnits x;
     const int slots = w4_slots(1, a.k);   // of a row
     if constexpr (!COPY) x.load(a, m0, min(4, a.m - m0), slots, 0);
-    // COPY: exponents of the row blocks' blocks, [nblk][CB] fours
-    auto block_exps = [&](int i) {
-        const int c = i % CB, blk = min(i / CB, nblk - 1);
-        return ((const v2i*)((const char*)a.scratch + w4_bexp_off(a.m) + w4_row_block(blockIdx.y, CB, c, a.m) * w4_bexp_bytes(a.k)))[blk];
+    // COPY: what the row blocks' blocks count by, from the exponents of rows and blocks, [nblk][CB] fours
+    struct Exps {
+        v4i row;
+        v2i block;   // int16
     };
-    v2i bexp0 = {0, 0};
-    if constexpr (COPY) bexp0 = block_exps(threadIdx.x);
+    auto block_exps = [&](int i) {
+        const int b = w4_row_block(blockIdx.y, CB, i % CB, a.m), blk = min(i / CB, nblk - 1);
+        return Exps{((const v4i*)a.scratch)[b], ((const v2i*)((const char*)a.scratch + w4_bexp_off(a.m) + b * w4_bexp_bytes(a.k)))[blk]};
+    };
+    auto counts = [&](Exps e) {
+        v4f f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[j] = count_by(e.row[j], (int16_t)(e.block[j >> 1] >> (16 * (j & 1))));
+        return f;
+    };
+    Exps exps0 = {};
+    if constexpr (COPY) exps0 = block_exps(threadIdx.x);
 
     // scales of the workgroup's tiles as float32 [tile][group][16 rows]
     float* s_scale = (float*)lds;
@@ -231,8 +248,9 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     int* s_exp = (int*)next;                       // [4 CB]
     unsigned* s_most = (unsigned*)next + 16;       // [kW4Slots][wave]
     next += 192;
-    int16_t* s_bexp = (int16_t*)next;              // [nblk][CB][4]
-    next += (CB * w4_bexp_bytes(a.k) + 15) / 16 * 16;
+    float* s_by = (float*)next;                    // COPY: [nblk][CB][4]
+    int16_t* s_bexp = (int16_t*)next;              // else [nblk][4]
+    next += CB * nblk * 16;
     char* digits = next;
     const char* scr = (const char*)a.scratch + w4_digit_off(a.m, a.k);
 
@@ -269,9 +287,9 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     for (int i = threadIdx.x + kFirst * kW4Threads; i < n4; i += kW4Threads)
         put_scales(wide ? ((const v4i*)sc)[i] : v4i{((const v2i*)sc)[i][0], ((const v2i*)sc)[i][1], 0, 0}, i);
     if constexpr (COPY) {
-        if ((int)threadIdx.x < CB * nblk) ((v2i*)s_bexp)[threadIdx.x] = bexp0;
+        if ((int)threadIdx.x < CB * nblk) ((v4f*)s_by)[threadIdx.x] = counts(exps0);
 #pragma unroll 1
-        for (int i = threadIdx.x + kW4Threads; i < CB * nblk; i += kW4Threads) ((v2i*)s_bexp)[i] = block_exps(i);
+        for (int i = threadIdx.x + kW4Threads; i < CB * nblk; i += kW4Threads) ((v4f*)s_by)[i] = counts(block_exps(i));
         put(0);
     }
     __syncthreads();
@@ -279,22 +297,15 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
     v4f acc[CB];
 #pragma unroll
     for (int c = 0; c < CB; c++) acc[c] = v4f{0, 0, 0, 0};
-    // A digit's sums enter times 256^(digit - 3), 2^-32 and what their block's exponent is less
-    // than the row's: 2^-22 of the result for rows around 1, so that no partial sum
-    // overflows whose result does not
-    const float place = __builtin_amdgcn_ldexpf(1.0f, 8 * (col & 3) - 56);
     const int mine = (nblk - part + sh.split - 1) / sh.split;   // blocks of this wavefront
     const float* scale = s_scale + (wave / sh.split) * groups * 16 + 4 * g;
     const int frag = w4_frag(0, g, col & (sh.cols - 1), sh.cols);
     const int xrow = (col & (sh.cols - 1)) >> 2;   // this lane's row of a row block
-    int rexp[CB];                                  // the rows' exponents (not finite: any, the result is NaN)
-#pragma unroll
-    for (int c = 0; c < CB; c++) {
-        rexp[c] = COPY ? s_exp[4 * c + xrow] : RowUnits::fit_row(s_most + xrow * slots * kW4Waves, slots * kW4Waves);
-        if (!COPY && wave == 0 && g == 0 && (col & 3) == 0) s_exp[col >> 2] = rexp[c];   // read behind the next barrier
-        rexp[c] = max(rexp[c], -1000);
+    int rexp = 0;
+    if constexpr (!COPY) {
+        rexp = RowUnits::fit_row(s_most + xrow * slots * kW4Waves, slots * kW4Waves);
+        if (wave == 0 && g == 0 && (col & 3) == 0) s_exp[col >> 2] = rexp;   // read behind the next barrier
     }
-    const int16_t* bexp = s_bexp + xrow;
     const int f64 = 4 * sh.cols * 16;              // bytes of 64 columns' digits
 
     auto block = [&](v4i q, int blk, const char* base) {
@@ -307,7 +318,7 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
 #pragma unroll
         for (int c = 0; c < CB; c++) {
             const char* f = base + c * fcb + frag;
-            const float by = __builtin_amdgcn_ldexpf(place, rexp[c] - bexp[at + c * 4]);
+            const float by = COPY ? s_by[at + c * 4 + xrow] : count_by(rexp, s_bexp[at + xrow]);
             v4i t = {0, 0, 0, 0};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -371,12 +382,14 @@ __global__ __launch_bounds__(kW4Threads, CB < 4 ? 4 : 2) void w4_kernel(W4Args a
         }
     }
 
-    // a row of x: its digits' columns; then the wavefronts of a tile
+    // a row of x: its digits' columns, each 256^(digit - 3) of the result; then the wavefronts
+    // of a tile
+    const float place = __builtin_amdgcn_ldexpf(1.0f, 8 * (col & 3) - 24);
 #pragma unroll
     for (int c = 0; c < CB; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v = acc[c][i];
+            float v = acc[c][i] * place;
             v += lane_xor<1>(v);
             v += lane_xor<2>(v);
             if ((col & 3) == 0) red[(wave * 16 + 4 * g + i) * (4 * CB) + 4 * c + (col >> 2)] = v;

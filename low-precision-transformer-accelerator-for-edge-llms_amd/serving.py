@@ -279,7 +279,8 @@ class W4Linear:
     scales[n][k // group].  q [n][k / 2] uint8 holds two weights of -8 .. 7 (two's
     complement) in a byte, the even column in the low nibble; scales [n][k / group] are
     float32, bfloat16 or float16; group is 32, 64 or 128.  Both are packed here, once, into
-    the order the kernels read, and not kept."""
+    the order the kernels read, and not kept.  x is taken to 2^-30 of the largest of each
+    128 of its columns (tl_linear_w4)."""
 
     def __init__(self, q, scales, rt: Runtime | None = None):
         if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.uint8 or q.dim() != 2 or not q.is_contiguous():

@@ -21,7 +21,7 @@
  *     that stream first.
  *   - A handle is not thread safe: one host thread per handle, but for the calls
  *     whose name ends in _async and those that give the sizes of their buffers
- *     (_scratch, tl_w4_packed_bytes), which any number may make meanwhile.
+ *     (_scratch, tl_w4_packed_bytes, tl_w8_packed_bytes), which any number may make meanwhile.
  *     tl_last_error gives the calling thread's copy of the latest message, good
  *     until the thread asks again.
  *   - Matrices are row-major; weights are [N][K] int8 (one output channel per
@@ -239,7 +239,7 @@ int32_t tl_lm_head_argmax(tl_handle *h, const float *x, int32_t *token, float *l
  * What a call finds wrong on the device (a sequence, position, page or token id
  * out of its range) is left out: nothing is read or written outside the buffers.
  * tl_x then returns TL_ERR_BAD_DESCRIPTOR after completing; tl_x_async sets *fault
- * to 1 (and never clears it).  Up to 2^24 - 1 rows (tl_linear_w4: 2^17). */
+ * to 1 (and never clears it).  Up to 2^24 - 1 rows (tl_linear_w4, tl_linear_w8: 2^17). */
 #define TL_OP_COUNTERS 16384
 typedef enum tl_dtype { TL_F32 = 0, TL_BF16 = 1, TL_F16 = 2, TL_I8 = 3 } tl_dtype;
 
@@ -283,6 +283,20 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
                               const int32_t *row_pos, const float *cos, const float *sin, int32_t n_pos, void *q_out,
                               int64_t q_stride, int32_t *fault);
 
+/* tl_paged_append with q and k of each head normed before they are rotated: x f gain, f =
+ * 1 / sqrt(mean of the head's x^2 + eps) in 64 bits and rounded once, both products rounded to
+ * float32; q_gain, k_gain [head_dim] float32 (dev, 16-byte aligned; NULL: that one is not
+ * normed), eps from 0 on.  Values stay as they are. */
+int32_t tl_paged_append_norm(tl_handle *h, const tl_paged_cache *cache, const void *qkv, int64_t qkv_stride,
+                             int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
+                             const int32_t *row_pos, const float *cos, const float *sin, int32_t n_pos,
+                             const float *q_gain, const float *k_gain, double eps, void *q_out, int64_t q_stride);
+int32_t tl_paged_append_norm_async(tl_handle *h, void *stream, const tl_paged_cache *cache, const void *qkv,
+                                   int64_t qkv_stride, int32_t act, int32_t rows, int32_t n_heads,
+                                   const int32_t *row_seq, const int32_t *row_pos, const float *cos, const float *sin,
+                                   int32_t n_pos, const float *q_gain, const float *k_gain, double eps, void *q_out,
+                                   int64_t q_stride, int32_t *fault);
+
 /* Attention of one query row per token: row r of q [rows][n_heads * head_dim]
  * (dev, type act) attends keys 0 .. row_pos[r] of sequence row_seq[r] (NULL: r),
  * out[r] = softmax(scale q . k) . v in q's type; query head h reads KV head
@@ -306,6 +320,48 @@ int32_t tl_paged_attention_async(tl_handle *h, void *stream, const tl_paged_cach
                                  int64_t scratch_bytes, int32_t *counters, int32_t *fault);
 int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
                                    int64_t *bytes);
+
+/* tl_paged_attention of rows whose first prefix_len positions are those of sequence
+ * prefix_seq (a prompt that many sequences share): key t of row r is position t of
+ * prefix_seq for t < prefix_len, of row_seq[r] from there on, whose table entries before
+ * that are not used.  The shared keys are read once for all rows and multiplied as a
+ * matrix; what is said of tl_paged_attention holds, but that probabilities of 16-bit rows
+ * enter the products over the prefix in two 16-bit parts.  A row before the prefix's
+ * last position attends the prefix's keys up to its own.  prefix_len 0: tl_paged_attention. */
+int32_t tl_paged_attention_shared(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride,
+                                  int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
+                                  const int32_t *row_pos, int32_t prefix_seq, int32_t prefix_len, float scale,
+                                  void *out, int64_t out_stride);
+int32_t tl_paged_attention_shared_async(tl_handle *h, void *stream, const tl_paged_cache *cache, const void *q,
+                                        int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads,
+                                        const int32_t *row_seq, const int32_t *row_pos, int32_t prefix_seq,
+                                        int32_t prefix_len, float scale, void *out, int64_t out_stride, void *scratch,
+                                        int64_t scratch_bytes, int32_t *counters, int32_t *fault);
+int32_t tl_paged_attention_shared_scratch(tl_handle *h, const tl_paged_cache *cache, int32_t rows, int32_t n_heads,
+                                          int32_t prefix_len, int64_t *bytes);
+
+/* Projections with 8-bit weights q [n][k] and float32 scales [n] (tl_quantize_weight_rows
+ * makes them), in the order the kernels read, packed (dev, 16-byte aligned) once per weight
+ * matrix into tl_w8_packed_bytes.  With up_q and up_scales (else NULL) the pair is a gate
+ * and an up projection of one shape, packed with gated = 1.  Any n and k: k at most 2^17, n at
+ * most 2^24, n k below 2^35. */
+int32_t tl_w8_packed_bytes(tl_handle *h, int32_t n, int32_t k, int32_t gated, int64_t *bytes);
+int32_t tl_pack_w8(tl_handle *h, const int8_t *q, const float *scales, const int8_t *up_q, const float *up_scales,
+                   int32_t n, int32_t k, void *packed);
+/* y[m][n] = residual[m][n] + (sum_k x8[m][k] w8[n][k]) sw[n] sx[m], x, residual and y of
+ * type act (TL_F32, TL_BF16, TL_F16); x8 and sx are x quantized per row as GI:36-42 does, in
+ * float32: sx = max|x| / 127 (1 where that is 0), x8 = clip(rne(x / sx), +-127).  Sums are exact.
+ * gated: y = silu(gate) up, silu(g) = g / (1 + e^-g) (-0 below -80), no residual (GI:212).  An infinity or NaN in
+ * a row of x makes its whole row of y NaN.  Rows of x, residual and y may start anywhere
+ * (16-byte aligned ones are read and written faster), strides in elements; residual may be
+ * NULL or y, x and y must not overlap.  m from 0 to 2^17. */
+int32_t tl_linear_w8(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
+                     int32_t gated, int32_t n, int32_t k, const void *residual, int64_t res_stride, void *y,
+                     int64_t y_stride);
+int32_t tl_linear_w8_async(tl_handle *h, void *stream, const void *x, int64_t x_stride, int32_t act, int32_t m,
+                           const void *packed, int32_t gated, int32_t n, int32_t k, const void *residual,
+                           int64_t res_stride, void *y, int64_t y_stride, void *scratch, int64_t scratch_bytes);
+int32_t tl_linear_w8_scratch(tl_handle *h, int32_t m, int32_t k, int64_t *bytes);
 
 /* Projections with 4-bit weights: w[n][k] = q s[n][k / group], q from -8 to 7.  q
  * [n][k / 2] bytes: column 2 j of a row is the low nibble of byte j, 2 j + 1 the

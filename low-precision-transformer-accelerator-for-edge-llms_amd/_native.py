@@ -93,8 +93,11 @@ _f32 = C.c_float
 _cachep = C.POINTER(TlPagedCache)
 _append = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i64]
 _w4 = [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64]
+_append_norm = [*_append[:-2], _vp, _vp, C.c_double, *_append[-2:]]
+_w8 = [_vp, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _vp, _i64]
 _logprobs = [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp, _vp]
 _attend = [_cachep, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _vp, _i64]
+_shared = [*_attend[:-3], _i32, _i32, *_attend[-3:]]
 
 SIGNATURES = {
     "tl_create": (_i32, [C.POINTER(TlConfig), _i32, C.POINTER(_vp)]),
@@ -146,6 +149,16 @@ SIGNATURES = {
     "tl_paged_attention": (_i32, [_vp, *_attend]),
     "tl_paged_attention_async": (_i32, [_vp, _vp, *_attend, _vp, _i64, _vp, _vp]),
     "tl_paged_attention_scratch": (_i32, [_vp, _cachep, _i32, _i32, C.POINTER(_i64)]),
+    "tl_paged_append_norm": (_i32, [_vp, *_append_norm]),
+    "tl_paged_append_norm_async": (_i32, [_vp, _vp, *_append_norm, _vp]),
+    "tl_paged_attention_shared": (_i32, [_vp, *_shared]),
+    "tl_paged_attention_shared_async": (_i32, [_vp, _vp, *_shared, _vp, _i64, _vp, _vp]),
+    "tl_paged_attention_shared_scratch": (_i32, [_vp, _cachep, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "tl_linear_w8": (_i32, [_vp, *_w8]),
+    "tl_linear_w8_async": (_i32, [_vp, _vp, *_w8, _vp, _i64]),
+    "tl_linear_w8_scratch": (_i32, [_vp, _i32, _i32, C.POINTER(_i64)]),
+    "tl_w8_packed_bytes": (_i32, [_vp, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "tl_pack_w8": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
     "tl_linear_w4": (_i32, [_vp, *_w4]),
     "tl_linear_w4_async": (_i32, [_vp, _vp, *_w4, _vp, _i64]),
     "tl_linear_w4_scratch": (_i32, [_vp, _i32, _i32, C.POINTER(_i64)]),

@@ -2,15 +2,10 @@
 // one query row per token over it.
 #include <algorithm>
 
-#include "tl_rows.h"
+#include "tl_attn.h"
 
 namespace tl {
 namespace {
-
-typedef float v2f __attribute__((ext_vector_type(2)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------------------
 // append: q and k of each row rotated at its position (TL:69-80, the steps of
@@ -20,7 +15,10 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 // A workgroup takes 256 units of one row: a unit is four rotated pairs (d ..
 // d + 3 and their partners half a head on), or eight values of v.  Nothing is
 // read twice from memory; the row's cos and sin are shared by its heads through
-// the cache.  What bounds it: from one row to some hundreds the chain of loads and
+// the cache.  With gains, q and k of each head are normed first: f = 1 / sqrt(mean x^2 +
+// eps) in 64 bits, rounded once, so that neither the order of the sum nor a square root's
+// last bit shows in an INT8 row; then (x f) gain, each product rounded to float32.  A head's
+// pairs lie in 8 or 16 neighbouring lanes, which add up their squares with DPP moves.  What bounds it: from one row to some hundreds the chain of loads and
 // the launch (3.5 us for 1 row as for 61); 2048 rows of 32 + 2 x 8 heads of 128 in
 // float16, 51 MB, take 11.5 us (4.5 TB/s).  A row's values are loaded before its place is
 // known, and the activations' type is the compiler's: with the type looked at per
@@ -37,7 +35,22 @@ TL_DEV void cache_store4(void* base, int64_t i, int dt, v4f v, float s) {
     *(unsigned*)((int8_t*)base + i) = w;
 }
 
-template <int ACT>
+// sum over the 8 or 16 lanes that hold a head's rotated pairs, in every one of them
+TL_DEV double head_sum(double v, int quads) {
+    auto add = [&](auto ctrl) {
+        constexpr int CTRL = decltype(ctrl)::value;
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const unsigned lo = (unsigned)dpp<CTRL>((int)(unsigned)u), hi = (unsigned)dpp<CTRL>((int)(unsigned)(u >> 32));
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    add(std::integral_constant<int, kDppXor1>{});
+    add(std::integral_constant<int, kDppXor2>{});
+    add(std::integral_constant<int, kDppHalfMirror>{});
+    if (quads == 16) add(std::integral_constant<int, kDppRowMirror>{});
+    return v;
+}
+
+template <int ACT, bool NORM>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     const PagedGeom& g = a.c.g;
     const int row = blockIdx.x;
@@ -51,7 +64,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     if (head < a.n_heads && !a.q_out) return;
     // the values, on their way while the row's place is looked up
     const int64_t at = (int64_t)row * a.qkv_stride + (int64_t)head * hd + d;
-    const v4f x1 = load4(a.qkv, at, ACT), x2 = load4(a.qkv, at + (rotate ? half : 4), ACT);
+    v4f x1 = load4(a.qkv, at, ACT), x2 = load4(a.qkv, at + (rotate ? half : 4), ACT);
     const int seq = a.row_seq ? a.row_seq[row] : row;
     const int pos = a.row_pos[row];
     const PagedRow kind = paged_row_kind(g, seq, pos);
@@ -63,6 +76,18 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         return;
     }
     if (rotate) {
+        if constexpr (NORM) {
+            const float* gain = head < a.n_heads ? a.q_gain : a.k_gain;
+            if (gain) {
+                const v4f g1 = *(const v4f*)(gain + d), g2 = *(const v4f*)(gain + d + half);
+                double sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) sum += (double)x1[j] * x1[j] + (double)x2[j] * x2[j];
+                const float f = (float)(1.0 / __builtin_sqrt(head_sum(sum, quads) / hd + a.eps));
+                x1 = x1 * f * g1;
+                x2 = x2 * f * g2;
+            }
+        }
         const float* c = a.cos + (int64_t)pos * hd + d;
         const float* s = a.sin + (int64_t)pos * hd + d;
         const v4f c1 = *(const v4f*)c, c2 = *(const v4f*)(c + half), s1 = *(const v4f*)s, s2 = *(const v4f*)(s + half);
@@ -122,28 +147,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
 // float16 118), else the chain of loads and the join of the parts.  The third parts
 // cost 1 us of the first.
 // ---------------------------------------------------------------------------
-template <bool BF>
-TL_DEV v4f mfma32(v4i a, v4i b, v4f c) {
-    if constexpr (BF)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-
-// two INT8 values (one in each 16-bit half, zero extended) as float16: 0x6400 | u
-// is 1024 + u for u < 1024, and u = x ^ 0x80 is x + 128, so 1152 less is x exactly
-TL_DEV int i8_pair_f16(unsigned halves) {
-    const h2 v = __builtin_bit_cast(h2, halves ^ 0x64806480u);
-    return __builtin_bit_cast(int, v - h2{(_Float16)1152.0f, (_Float16)1152.0f});
-}
-
-// two floats to the 16-bit type: bfloat16 truncated, float16 to nearest
-template <bool BF>
-TL_DEV int pack2(float a, float b) {
-    if constexpr (BF) return (int)__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-    else return __builtin_bit_cast(int, h2{(_Float16)a, (_Float16)b});
-}
-
 // W dwords read once
 template <int W>
 TL_DEV void load_row(const char* p, unsigned v[W]) {
@@ -157,16 +160,6 @@ TL_DEV void load_row(const char* p, unsigned v[W]) {
     }
 }
 
-TL_DEV float pair_max(float v) {   // maximum over the four 16-lane groups
-    const unsigned u = __float_as_uint(v);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float w = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-    const unsigned x = __float_as_uint(w);
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
 constexpr int kJoinParts = 16;   // parts per (row, head block) up to which they are joined in place
@@ -209,12 +202,39 @@ TL_DEV float* part_ml(const PagedAttnArgs& a, int32_t part, int32_t workgroups) 
     return a.scratch + (int64_t)2 * workgroups * 8 * HD + (int64_t)part * 16;
 }
 
+// tiles of a row at pos
+template <bool PRE>
+TL_DEV unsigned tiles_at(const PagedAttnArgs& a, int pos) {
+    return (unsigned)(PRE ? shared_tiles(a.prefix.len, pos) : paged_tiles(pos + 1));
+}
+
+// What a row takes besides its own keys: the parts that the prefix left, added to m, l
+// and the sums O of four dimensions.
+template <int HD>
+TL_DEV void add_prefix(const PagedAttnArgs& a, int row, int head, int d, float m, float& l, v4f& acc) {
+    float mm = m;
+    for (int s = 0; s < a.prefix.splits; s++) mm = fmaxf(mm, a.prefix.ml[2 * prefix_part(a, s, row, head)]);
+    const float off = mm == -__builtin_inff() ? 0.0f : mm;
+    const float e0 = __builtin_amdgcn_exp2f(m - off);
+    l *= e0;
+    acc *= e0;
+#pragma unroll 4
+    for (int s = 0; s < a.prefix.splits; s++) {
+        const int64_t part = prefix_part(a, s, row, head);
+        const v2f ml = *(const v2f*)(a.prefix.ml + 2 * part);
+        const float e = __builtin_amdgcn_exp2f(ml[0] - off);
+        l += e * ml[1];
+        acc += e * *(const v4f*)(a.prefix.o + part * HD + d);
+    }
+}
+
 // this thread's row of the rows scanned together (kAttnThreads at a time), its tiles
+template <bool PRE>
 TL_DEV unsigned row_tiles(const PagedAttnArgs& a, int64_t row) {
     if (row >= a.rows) return 0u;
     const int seq = a.row_seq ? a.row_seq[row] : (int)row;
     const int pos = a.row_pos[row];
-    return paged_row_kind(a.c.g, seq, pos) == PAGED_ROW_OK ? (unsigned)paged_tiles(pos + 1) : 0u;
+    return paged_row_kind(a.c.g, seq, pos) == PAGED_ROW_OK ? tiles_at<PRE>(a, pos) : 0u;
 }
 
 struct ScanShared {
@@ -246,9 +266,10 @@ TL_DEV unsigned block_scan(unsigned v, ScanShared& sh, unsigned& all) {
 struct RowScan {
     unsigned mine, upto, all;
 };
+template <bool PRE>
 TL_DEV RowScan scan_rows(const PagedAttnArgs& a, ScanShared& sh, int64_t r0) {
     RowScan r;
-    r.mine = row_tiles(a, r0 + threadIdx.x);
+    r.mine = row_tiles<PRE>(a, r0 + threadIdx.x);
     r.upto = block_scan(r.mine, sh, r.all);
     return r;
 }
@@ -259,13 +280,14 @@ struct LaneRows {
     int seq, pos;
     unsigned tiles, upto;
 };
+template <bool PRE>
 TL_DEV LaneRows lane_rows(const PagedAttnArgs& a, unsigned& all) {
     const int r = min(lane_id(), a.rows - 1);
     LaneRows l;
     l.seq = a.row_seq ? a.row_seq[r] : r;
     l.pos = a.row_pos[r];
     const bool use = lane_id() < a.rows && paged_row_kind(a.c.g, l.seq, l.pos) == PAGED_ROW_OK;
-    l.tiles = use ? (unsigned)paged_tiles(l.pos + 1) : 0u;
+    l.tiles = use ? tiles_at<PRE>(a, l.pos) : 0u;
     unsigned v = l.tiles;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -278,18 +300,20 @@ TL_DEV LaneRows lane_rows(const PagedAttnArgs& a, unsigned& all) {
 }
 
 // the call's tiles per head block; first: the first scan's
+template <bool PRE>
 TL_DEV int32_t count_tiles(const PagedAttnArgs& a, ScanShared& sh, RowScan& first) {
-    first = scan_rows(a, sh, 0);
+    first = scan_rows<PRE>(a, sh, 0);
     int32_t total = (int32_t)first.all;
     for (int64_t r0 = kAttnThreads; r0 < a.rows; r0 += kAttnThreads) {
         unsigned all;
-        block_scan(row_tiles(a, r0 + threadIdx.x), sh, all);
+        block_scan(row_tiles<PRE>(a, r0 + threadIdx.x), sh, all);
         total += (int32_t)all;
     }
     return total;
 }
 
 // the row that holds tile `at` (of one head block, at < total) and the tiles before that row
+template <bool PRE>
 TL_DEV void find_row(const PagedAttnArgs& a, ScanShared& sh, int32_t at, RowScan r, int& row, int32_t& before) {
     int32_t base = 0;
     for (int64_t r0 = 0;;) {
@@ -301,7 +325,7 @@ TL_DEV void find_row(const PagedAttnArgs& a, ScanShared& sh, int32_t at, RowScan
         base += (int32_t)r.all;
         r0 += kAttnThreads;
         if (at < base || r0 >= a.rows) break;
-        r = scan_rows(a, sh, r0);
+        r = scan_rows<PRE>(a, sh, r0);
     }
     __syncthreads();
     row = __builtin_amdgcn_readfirstlane(sh.row);
@@ -334,7 +358,7 @@ struct JoinShared {
     float e[kJoinStep][8], l[kJoinStep][8];   // 2^(m - M) (first m) and l of each part
     float m[8], sum[8], keep[8];              // M and the sum so far, what the parts before are scaled by
 };
-template <int HD>
+template <int HD, bool PRE>
 TL_DEV void join_parts(const PagedAttnArgs& a, const PagedShare& share, int w0, int w1, int32_t unit, int row,
                        int64_t head0, int heads, JoinShared& sh) {
     const int h = threadIdx.x / (HD / 4), d = (threadIdx.x - h * (HD / 4)) * 4;   // this thread's four values
@@ -384,7 +408,13 @@ TL_DEV void join_parts(const PagedAttnArgs& a, const PagedShare& share, int w0, 
         }
         __syncthreads();
     }
-    if (h < heads) store4(a.out, (int64_t)row * a.out_stride + (head0 + h) * HD + d, a.act, acc / sh.sum[h]);
+    if (h < heads) {
+        float l = sh.sum[h];
+        if constexpr (PRE) {
+            if (shared_adds(a.prefix.len, a.row_pos[row])) add_prefix<HD>(a, row, (int)head0 + h, d, sh.m[h], l, acc);
+        }
+        store4(a.out, (int64_t)row * a.out_stride + (head0 + h) * HD + d, a.act, acc / l);
+    }
 }
 
 // The pages of the four groups of 8 keys of 32, each in one page; groups behind the
@@ -404,11 +434,20 @@ TL_DEV unsigned pick_page(PagedPlace p, int i) {
     return a ^ ((a ^ b) & high);
 }
 
-TL_DEV PagedPlace place_rows(const PagedGeom& geo, scalar_table row, int kb, int last8) {
+// Groups of 8 keys that a row has: none looked up or read behind the last key's, nor (behind
+// a prefix) before the first one's
+template <bool PRE>
+struct Eights {
+    int first, last;
+    TL_DEV int at(int key) const { return min(PRE ? max(key, first) : key, last); }
+};
+
+template <bool PRE>
+TL_DEV PagedPlace place_rows(const PagedGeom& geo, scalar_table row, int kb, Eights<PRE> has) {
     PagedPlace p;
     p.bad = 0;
     auto look = [&](int j) {
-        const unsigned page = (unsigned)row[min(kb + 8 * j, last8) >> geo.page_shift];
+        const unsigned page = (unsigned)row[has.at(kb + 8 * j) >> geo.page_shift];
         const bool in = page < (unsigned)geo.n_pages;
         p.bad |= in ? 0u : 1u << j;
         return in ? page : 0u;
@@ -433,14 +472,14 @@ TL_DEV const char* group_row(const char* base, const PagedGeom& geo, unsigned pa
 }
 
 // Key rows of S^T: row m of tile t is key 8 (m / 4) + 4 t + m % 4 of the 32
-template <int HD, int DT, bool X2>
-TL_DEV void load_keys(const PagedGeom& geo, const char* base, unsigned page_bytes, int kb, int last8, int lane,
+template <int HD, int DT, bool X2, bool PRE>
+TL_DEV void load_keys(const PagedGeom& geo, const char* base, unsigned page_bytes, int kb, Eights<PRE> has, int lane,
                       PagedPlace p, v4i kf[PagedTile<HD, DT, X2>::KN]) {
     using T = PagedTile<HD, DT, X2>;
 #pragma unroll
     for (int rb = 0; rb < 32 / T::KR; rb++) {
         const int r = rb * T::KR + lane / T::KC_LINE, m = r & 15, t = r >> 4, grp = m >> 2;
-        const char* kr = group_row<T::ROW>(base, geo, page_bytes, pick_page(p, grp), min(kb + 8 * grp, last8)) +
+        const char* kr = group_row<T::ROW>(base, geo, page_bytes, pick_page(p, grp), has.at(kb + 8 * grp)) +
                          (4 * t + (m & 3)) * T::ROW + 16 * (lane % T::KC_LINE);
 #pragma unroll
         for (int i = 0; i < T::KLINES; i++)
@@ -448,11 +487,11 @@ TL_DEV void load_keys(const PagedGeom& geo, const char* base, unsigned page_byte
     }
 }
 
-template <int HD, int DT, bool X2>
-TL_DEV void load_values(const PagedGeom& geo, const char* base, unsigned page_bytes, int kb, int last8, int col, int g,
+template <int HD, int DT, bool X2, bool PRE>
+TL_DEV void load_values(const PagedGeom& geo, const char* base, unsigned page_bytes, int kb, Eights<PRE> has, int col, int g,
                         PagedPlace p, unsigned vf[8][PagedTile<HD, DT, X2>::VW]) {
     using T = PagedTile<HD, DT, X2>;
-    const char* vr = group_row<HD * T::ES>(base, geo, page_bytes, pick_page(p, g), min(kb + 8 * g, last8)) + col * (T::VW * 4);
+    const char* vr = group_row<HD * T::ES>(base, geo, page_bytes, pick_page(p, g), has.at(kb + 8 * g)) + col * (T::VW * 4);
 #pragma unroll
     for (int j = 0; j < 8; j++) load_row<T::VW>(vr + j * HD * T::ES, vf[j]);
 }
@@ -462,7 +501,9 @@ TL_DEV void load_values(const PagedGeom& geo, const char* base, unsigned page_by
 // 32 keys with their own m, l and O, joined through LDS; a whole one is finished,
 // of the others a part is left in scratch.  With counters the workgroup that
 // leaves the last part of a (row, head block) joins them, else a second kernel.
-template <int HD, int DT, bool X2>
+// PRE: rows from the prefix's last position on take their own keys from there on, and the
+// prefix's parts with them; rows before it are rows of the prefix's sequence.
+template <int HD, int DT, bool X2, bool PRE>
 __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedAttnArgs a) {
     using T = PagedTile<HD, DT, X2>;
     constexpr bool BF = T::BF;
@@ -488,10 +529,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
     int32_t total;
     if (few) {
         unsigned all;
-        lr = lane_rows(a, all);
+        lr = lane_rows<PRE>(a, all);
         total = (int32_t)all;
     } else {
-        total = count_tiles(a, s_scan, first);
+        total = count_tiles<PRE>(a, s_scan, first);
     }
     if (me == 0 && a.fault)
         for (int64_t r = threadIdx.x; r < a.rows; r += kAttnThreads)
@@ -507,18 +548,22 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
         row = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tile < lr.upto));
         before = __builtin_amdgcn_readlane((int)(lr.upto - lr.tiles), row);
     } else {
-        find_row(a, s_scan, (unsigned)at / (unsigned)hbs, first, row, before);
+        find_row<PRE>(a, s_scan, (unsigned)at / (unsigned)hbs, first, row, before);
     }
     // tile `at` of all lies `in` tiles into its row's head blocks
     int32_t in = at - before * hbs;
     bool bad = false;
 
     for (; at < stop; row++) {
-        const int seq = few ? __builtin_amdgcn_readlane(lr.seq, row) : a.row_seq ? a.row_seq[row] : row;
+        int seq = few ? __builtin_amdgcn_readlane(lr.seq, row) : a.row_seq ? a.row_seq[row] : row;
         const int pos = few ? __builtin_amdgcn_readlane(lr.pos, row) : a.row_pos[row];
         if (paged_row_kind(geo, seq, pos) != PAGED_ROW_OK) continue;
         const int n = __builtin_amdgcn_readfirstlane(max(pos + 1, 0));
-        const int tiles = paged_tiles(n);
+        const int tiles = (int)tiles_at<PRE>(a, pos);
+        const bool adds = PRE && shared_adds(a.prefix.len, pos);
+        // the first key and the place it is counted from, whole 32s of keys before it
+        const int key0 = adds ? a.prefix.len : 0, base = key0 & ~31;
+        if constexpr (PRE) seq = adds ? seq : a.prefix.seq;
         for (int hb = (int)((unsigned)in / (unsigned)tiles); hb < hbs && at < stop; hb++) {
             const int t0 = in - hb * tiles;
             const int t1 = min(tiles, t0 + (stop - at));
@@ -528,14 +573,22 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
             const int kvh = hb / blocks, h0 = (hb - kvh * blocks) * 8;
             const int heads = min(8, rep - h0);
             const int64_t head0 = (int64_t)kvh * rep + h0;
-            if (n == 0) {   // no keys: zeros
-                for (int i = threadIdx.x; i < heads * HD / 4; i += kAttnThreads)
-                    store4(a.out, (int64_t)row * a.out_stride + head0 * HD + 4 * i, a.act, v4f{0, 0, 0, 0});
+            if (n <= key0) {   // no keys: zeros, or all that the prefix has
+                for (int i = threadIdx.x; i < heads * HD / 4; i += kAttnThreads) {
+                    v4f acc = {0, 0, 0, 0};
+                    if (adds) {
+                        const int h = i / (HD / 4);
+                        float l = 0.0f;
+                        add_prefix<HD>(a, row, (int)head0 + h, (i - h * (HD / 4)) * 4, -__builtin_inff(), l, acc);
+                        acc = acc / l;
+                    }
+                    store4(a.out, (int64_t)row * a.out_stride + head0 * HD + 4 * i, a.act, acc);
+                }
                 continue;
             }
-            const int end = min(n, t1 * kPagedTile);
-            const int last8 = (n - 1) & ~7;
-            int kb = t0 * kPagedTile + 32 * wave;
+            const int end = min(n, base + t1 * kPagedTile);
+            const Eights<PRE> has = {key0 & ~7, (n - 1) & ~7};
+            int kb = base + t0 * kPagedTile + 32 * wave;
             const scalar_table table = (scalar_table)(geo.table + (int64_t)seq * geo.table_stride);
             const unsigned page_bytes = (unsigned)(geo.page_stride * T::ES);
             const unsigned head_bytes = ((unsigned)kvh << geo.page_shift) * (HD * T::ES);
@@ -546,10 +599,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
             unsigned vf[8][T::VW];
             unsigned pages_bad = 0;
             auto fetch = [&](int key) {
-                const PagedPlace place = place_rows(geo, table, key, last8);
+                const PagedPlace place = place_rows<PRE>(geo, table, key, has);
                 pages_bad = place.bad;
-                load_keys<HD, DT, X2>(geo, kbase, page_bytes, key, last8, lane, place, kf);
-                load_values<HD, DT, X2>(geo, vbase, page_bytes, key, last8, col, g, place, vf);
+                load_keys<HD, DT, X2, PRE>(geo, kbase, page_bytes, key, has, lane, place, kf);
+                load_values<HD, DT, X2, PRE>(geo, vbase, page_bytes, key, has, col, g, place, vf);
             };
             fetch(kb);   // (a wavefront without keys: the last ones)
             // the query head's parts, scaled by a power of two so that float16 holds them
@@ -638,7 +691,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
 
                 // lane: keys kb + 8 g + 4 t + i of its head, both parts' products added
                 float x[8], mt = -__builtin_inff();
-                const bool whole = kb + 32 <= n && pages_bad == 0;
+                const bool whole = kb + 32 <= n && (!PRE || kb >= key0) && pages_bad == 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float d = s[j >> 2][j & 3];
@@ -648,7 +701,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                     bad |= pages_bad != 0;
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const bool in = !(pages_bad >> g & 1) && kb + 8 * g + j < n;
+                        const int key = kb + 8 * g + j;
+                        const bool in = !(pages_bad >> g & 1) && key < n && (!PRE || key >= key0);
                         x[j] = in ? x[j] : -__builtin_inff();
 #pragma unroll
                         for (int w = 0; w < T::VW; w++) vf[j][w] = in ? vf[j][w] : 0u;   // 0 x NaN of a stale row is NaN
@@ -740,6 +794,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                 }
                 acc *= sv;
                 if (all) {
+                    if constexpr (PRE) {
+                        if (adds) add_prefix<HD>(a, row, (int)head0 + h, d, mm, ll, acc);
+                    }
                     store4(a.out, (int64_t)row * a.out_stride + (head0 + h) * HD + d, a.act, acc / ll);
                 } else {
                     part_store4(part_o<HD>(a, part) + h * HD + d, acc);
@@ -762,7 +819,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
                 }
                 __syncthreads();
                 if (s_last) {
-                    join_parts<HD>(a, share, w0, w1, unit, row, head0, heads, s_join);
+                    join_parts<HD, PRE>(a, share, w0, w1, unit, row, head0, heads, s_join);
                 }
             }
             __syncthreads();
@@ -773,7 +830,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void paged_attention_kernel(PagedA
 }
 
 // the parts of one (row, head) joined, W of them side by side (paged_join_grid)
-template <int HD>
+template <int HD, bool PRE>
 __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(PagedAttnArgs a, int workgroups) {
     constexpr int Q = HD / 4, W = kAttnThreads / Q;   // quads of a row; parts taken side by side
     __shared__ float s_acc[W][HD];
@@ -790,21 +847,21 @@ __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(PagedAttnArgs 
         const int pos = a.row_pos[row];
         if (paged_row_kind(geo, a.row_seq ? a.row_seq[row] : row, pos) != PAGED_ROW_OK || pos < 0) return;
         unsigned all;
-        const LaneRows l = lane_rows(a, all);
+        const LaneRows l = lane_rows<PRE>(a, all);
         share = paged_share((int32_t)all * hbs, workgroups);
-        tiles = paged_tiles(pos + 1);
+        tiles = (int)tiles_at<PRE>(a, pos);
         const int kvh = head / rep, hb = kvh * blocks + ((head - kvh * rep) >> 3);
         unit = __builtin_amdgcn_readlane((int)(l.upto - l.tiles), row) * hbs + hb * tiles;
     } else {
         const int w = blockIdx.x + 1;
         RowScan first;
-        const int32_t total = __builtin_amdgcn_readfirstlane(count_tiles(a, s_scan, first));
+        const int32_t total = __builtin_amdgcn_readfirstlane(count_tiles<PRE>(a, s_scan, first));
         share = paged_share(total * hbs, workgroups);
         const int32_t at = share.start(w);
         if (at >= total * hbs || at == share.start(w - 1)) return;
         int32_t before;
-        find_row(a, s_scan, (unsigned)at / (unsigned)hbs, first, row, before);
-        tiles = paged_tiles(a.row_pos[row] + 1);
+        find_row<PRE>(a, s_scan, (unsigned)at / (unsigned)hbs, first, row, before);
+        tiles = (int)tiles_at<PRE>(a, a.row_pos[row]);
         const int32_t in = at - before * hbs;
         const int hb = (int)((unsigned)in / (unsigned)tiles), kvh = hb / blocks, h = (hb - kvh * blocks) * 8 + (int)blockIdx.y;
         unit = before * hbs + hb * tiles;
@@ -843,6 +900,9 @@ __global__ __launch_bounds__(kAttnThreads) void paged_join_kernel(PagedAttnArgs 
         acc += *(const v4f*)&s_acc[i][4 * q];
         ll += s_l[i];
     }
+    if constexpr (PRE) {
+        if (shared_adds(a.prefix.len, a.row_pos[row])) add_prefix<HD>(a, row, head, 4 * q, mm, ll, acc);
+    }
     store4(a.out, (int64_t)row * a.out_stride + (int64_t)head * HD + 4 * q, a.act, acc / ll);
 }
 
@@ -854,9 +914,14 @@ hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a) {
     if (a.rows <= 0) return hipSuccess;
     const int units = (a.n_heads + a.c.g.n_kv) * (a.c.g.head_dim / 8) + a.c.g.n_kv * a.c.g.head_dim / 8;
     const dim3 grid(a.rows, (units + 255) / 256), block(256);
-    if (a.act == DT_F32) TL_KLAUNCH((paged_append_kernel<DT_F32>), grid, block, 0, s, a);
-    else if (a.act == DT_BF16) TL_KLAUNCH((paged_append_kernel<DT_BF16>), grid, block, 0, s, a);
-    else TL_KLAUNCH((paged_append_kernel<DT_F16>), grid, block, 0, s, a);
+    auto go = [&](auto norm) {
+        constexpr bool NORM = decltype(norm)::value;
+        if (a.act == DT_F32) TL_KLAUNCH((paged_append_kernel<DT_F32, NORM>), grid, block, 0, s, a);
+        else if (a.act == DT_BF16) TL_KLAUNCH((paged_append_kernel<DT_BF16, NORM>), grid, block, 0, s, a);
+        else TL_KLAUNCH((paged_append_kernel<DT_F16, NORM>), grid, block, 0, s, a);
+    };
+    if (a.q_gain || a.k_gain) go(std::true_type{});
+    else go(std::false_type{});
     return hipGetLastError();
 }
 
@@ -888,16 +953,26 @@ hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& args) {
     const dim3 grid(wgs), block(kAttnThreads);
     const PagedJoinGrid join = paged_join_grid(a.rows, a.n_heads, a.c.g.n_kv, wgs);
     const bool x2 = a.c.dtype == DT_BF16 && a.act != DT_BF16;
-    auto go = [&](auto hd) {
+    auto go = [&](auto hd, auto pre) {
         constexpr int HD = decltype(hd)::value;
-        if (a.c.dtype == DT_I8) TL_KLAUNCH((paged_attention_kernel<HD, DT_I8, false>), grid, block, 0, s, a);
-        else if (a.c.dtype == DT_F16) TL_KLAUNCH((paged_attention_kernel<HD, DT_F16, false>), grid, block, 0, s, a);
-        else if (x2) TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, true>), grid, block, 0, s, a);
-        else TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, false>), grid, block, 0, s, a);
-        if (!a.counters && !one_tile) TL_KLAUNCH((paged_join_kernel<HD>), dim3(join.x, join.y), block, 0, s, a, wgs);
+        constexpr bool PRE = decltype(pre)::value;
+        if (a.c.dtype == DT_I8) TL_KLAUNCH((paged_attention_kernel<HD, DT_I8, false, PRE>), grid, block, 0, s, a);
+        else if (a.c.dtype == DT_F16) TL_KLAUNCH((paged_attention_kernel<HD, DT_F16, false, PRE>), grid, block, 0, s, a);
+        else if (x2) TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, true, PRE>), grid, block, 0, s, a);
+        else TL_KLAUNCH((paged_attention_kernel<HD, DT_BF16, false, PRE>), grid, block, 0, s, a);
+        if (!a.counters && !one_tile) TL_KLAUNCH((paged_join_kernel<HD, PRE>), dim3(join.x, join.y), block, 0, s, a, wgs);
     };
-    if (a.c.g.head_dim == 64) go(std::integral_constant<int, 64>{});
-    else go(std::integral_constant<int, 128>{});
+    using std::integral_constant;
+    if (a.prefix.len > 0) {
+        const hipError_t e = launch_paged_prefix(s, a);
+        if (e != hipSuccess) return e;
+        if (a.c.g.head_dim == 64) go(integral_constant<int, 64>{}, std::true_type{});
+        else go(integral_constant<int, 128>{}, std::true_type{});
+    } else if (a.c.g.head_dim == 64) {
+        go(integral_constant<int, 64>{}, std::false_type{});
+    } else {
+        go(integral_constant<int, 128>{}, std::false_type{});
+    }
     return hipGetLastError();
 }
 

@@ -1278,6 +1278,8 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
     if ((e = init_gemm_pk_kernels())) return bad(e);
     if ((e = init_skinny_kernels())) return bad(e);
     if ((e = init_w4_kernels())) return bad(e);
+    if ((e = init_w8_kernels())) return bad(e);
+    if ((e = init_prefix_kernels())) return bad(e);
     if (const char* env = std::getenv("TL_BATCH_O_FUSE")) h->o_fuse = env[0] != '0';
     if (const char* env = std::getenv("TL_BATCH_KSLICE")) h->batch_kslice = env[0] != '0';
     if (const char* env = std::getenv("TL_BATCH_QKV_KSLICE")) h->qkv_kslice = env[0] != '0';
@@ -2416,12 +2418,15 @@ int32_t check_paged_rows(tl_handle* h, int32_t act, int32_t rows, const int32_t*
 
 int32_t append_args(tl_handle* h, const tl_paged_cache* cache, const void* qkv, int64_t qkv_stride, int32_t act,
                     int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, const float* cos,
-                    const float* sin, int32_t n_pos, void* q_out, int64_t q_stride, PagedAppendArgs* a) {
+                    const float* sin, int32_t n_pos, const float* q_gain, const float* k_gain, double eps, void* q_out,
+                    int64_t q_stride, PagedAppendArgs* a) {
     int32_t r = paged_cache_arg(h, cache, &a->c);
     if (r || (r = check_paged_rows(h, act, rows, row_pos))) return r;
     TL_REQ(h, n_heads >= 0 && n_heads <= 65536, "query head count out of range");
     TL_REQ(h, cos && sin && n_pos >= 1 && aligned16(cos) && aligned16(sin), "RoPE tables missing or not 16-byte aligned");
     TL_REQ(h, qkv || rows == 0, "null qkv");
+    TL_REQ(h, aligned16(q_gain) && aligned16(k_gain), "gains must be 16-byte aligned");
+    TL_REQ(h, (!q_gain && !k_gain) || (eps >= 0.0 && eps <= 1e30), "eps must be a number from 0 on");
     const int64_t hd = cache->head_dim;
     if ((r = check_rows(h, qkv, qkv_stride, (n_heads + 2 * (int64_t)cache->n_kv_heads) * hd, act, "qkv"))) return r;
     if (q_out && (r = check_rows(h, q_out, q_stride, n_heads * hd, act, "q_out"))) return r;
@@ -2431,25 +2436,38 @@ int32_t append_args(tl_handle* h, const tl_paged_cache* cache, const void* qkv, 
     a->qkv = qkv; a->qkv_stride = qkv_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
     a->row_seq = row_seq; a->row_pos = row_pos; a->cos = cos; a->sin = sin; a->n_pos = n_pos;
     a->q_out = q_out; a->q_stride = q_stride;
+    a->q_gain = q_gain; a->k_gain = k_gain; a->eps = eps;
+    return TL_OK;
+}
+
+// the shape of an attention call over a cache: rows, heads and the shared prefix
+int32_t attention_shape(tl_handle* h, const PagedCache& c, int32_t rows, int32_t n_heads, int32_t prefix_len) {
+    TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % c.g.n_kv == 0, "query heads must be a multiple of the KV heads");
+    TL_REQ(h, rows >= 0 && rows < 1 << 24, "row count outside 0 .. 2^24 - 1");
+    TL_REQ(h, prefix_len >= 0 && prefix_len <= (int64_t)c.g.max_pages << c.g.page_shift,
+           "the prefix must lie in its sequence's pages");
+    if (prefix_len > 0 && (int64_t)rows * n_heads >= (int64_t)1 << 30)
+        return fail(h, TL_ERR_UNSUPPORTED, "2^30 or more query heads over a shared prefix");
+    if (!paged_countable(c.g, rows, (n_heads / c.g.n_kv + 7) / 8 * c.g.n_kv))
+        return fail(h, TL_ERR_UNSUPPORTED, "2^31 or more tiles of 128 keys over all rows and KV heads, as long as the table allows");
     return TL_OK;
 }
 
 int32_t attention_args(tl_handle* h, const tl_paged_cache* cache, const void* q, int64_t q_stride, int32_t act,
-                       int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, float scale,
-                       void* out, int64_t out_stride, PagedAttnArgs* a) {
+                       int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos, int32_t prefix_seq,
+                       int32_t prefix_len, float scale, void* out, int64_t out_stride, PagedAttnArgs* a) {
     int32_t r = paged_cache_arg(h, cache, &a->c);
     if (r || (r = check_paged_rows(h, act, rows, row_pos))) return r;
-    TL_REQ(h, n_heads >= 1 && n_heads <= 65535 && n_heads % cache->n_kv_heads == 0,
-           "query heads must be a multiple of the KV heads");
+    if ((r = attention_shape(h, a->c, rows, n_heads, prefix_len))) return r;
+    TL_REQ(h, prefix_len == 0 || (prefix_seq >= 0 && prefix_seq < cache->n_seqs), "the prefix's sequence is out of range");
     TL_REQ(h, (q && out) || rows == 0, "null q or out");
-    if (!paged_countable(a->c.g, rows, (n_heads / cache->n_kv_heads + 7) / 8 * cache->n_kv_heads))
-        return fail(h, TL_ERR_UNSUPPORTED, "2^31 or more tiles of 128 keys over all rows and KV heads, as long as the table allows");
     const int64_t width = (int64_t)n_heads * cache->head_dim;
     if ((r = check_rows(h, q, q_stride, width, act, "q"))) return r;
     if ((r = check_rows(h, out, out_stride, width, act, "out"))) return r;
     if ((r = check_apart(h, q, q_stride, width, out, out_stride, width, act, rows, true, "q and out"))) return r;
     a->q = q; a->q_stride = q_stride; a->act = act; a->rows = rows; a->n_heads = n_heads;
     a->row_seq = row_seq; a->row_pos = row_pos; a->scale = scale; a->out = out; a->out_stride = out_stride;
+    a->prefix.seq = prefix_seq; a->prefix.len = prefix_len;
     return TL_OK;
 }
 
@@ -2484,6 +2502,36 @@ int32_t w4_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int3
     return TL_OK;
 }
 
+// the shape of 8-bit weights
+int32_t w8_shape(tl_handle* h, int32_t n, int32_t k) {
+    TL_REQ(h, n >= 1 && k >= 1, "empty weights");
+    TL_REQ(h, n <= 1 << 24 && (int64_t)n * k < (int64_t)1 << 35, "more than 2^24 rows or 2^35 weights");
+    if (k > kW8MaxK) return fail(h, TL_ERR_UNSUPPORTED, "more than 2^17 columns, whose sums could pass 32 bits");
+    return TL_OK;
+}
+
+int32_t w8_args(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const void* packed, int32_t gated,
+                int32_t n, int32_t k, const void* residual, int64_t res_stride, void* y, int64_t y_stride, W8Args* a) {
+    int32_t r = w8_shape(h, n, k);
+    if (r) return r;
+    TL_REQ(h, act_type(act), "rows must be float32, bfloat16 or float16");
+    TL_REQ(h, m >= 0 && m <= 1 << 17, "row count outside 0 .. 2^17");
+    if ((int64_t)m * n >= (int64_t)1 << 38) return fail(h, TL_ERR_UNSUPPORTED, "2^38 or more results");
+    TL_REQ(h, packed && aligned16(packed), "packed weights missing or misaligned");
+    TL_REQ(h, (x && y) || m == 0, "null x or y");
+    TL_REQ(h, !gated || !residual, "gated weights take no residual");
+    TL_REQ(h, x_stride >= k && (uintptr_t)x % type_size(act) == 0, "x: rows must not overlap and must be aligned");
+    TL_REQ(h, y_stride >= n && (uintptr_t)y % type_size(act) == 0, "y: rows must not overlap and must be aligned");
+    TL_REQ(h, !residual || (res_stride >= n && (uintptr_t)residual % type_size(act) == 0),
+           "residual: rows must not overlap and must be aligned");
+    if ((r = check_apart(h, x, x_stride, k, y, y_stride, n, act, m, false, "x and y"))) return r;
+    if (residual && (r = check_apart(h, residual, res_stride, n, y, y_stride, n, act, m, true, "residual and y"))) return r;
+    a->x = x; a->x_stride = x_stride; a->act = act; a->m = m; a->n = n; a->k = k;
+    a->packed = packed; a->glu = gated != 0;
+    a->residual = residual; a->res_stride = res_stride; a->y = y; a->y_stride = y_stride;
+    return TL_OK;
+}
+
 int32_t logprobs_args(tl_handle* h, const void* logits, int64_t stride, int32_t dtype, int32_t rows, int32_t vocab,
                       const int32_t* targets, int32_t top, float* logprob, float* entropy, int32_t* top_ids,
                       float* top_logprobs, LogprobsArgs* a) {
@@ -2512,8 +2560,8 @@ int32_t tl_paged_append(tl_handle* h, const tl_paged_cache* cache, const void* q
                         const float* cos, const float* sin, int32_t n_pos, void* q_out, int64_t q_stride) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     PagedAppendArgs a{};
-    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_out,
-                                  q_stride, &a);
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos,
+                                  nullptr, nullptr, 0.0, q_out, q_stride, &a);
     if (r) return r;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
@@ -2527,8 +2575,8 @@ int32_t tl_paged_append_async(tl_handle* h, void* stream, const tl_paged_cache* 
                               int64_t q_stride, int32_t* fault) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     PagedAppendArgs a{};
-    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_out,
-                                  q_stride, &a);
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos,
+                                  nullptr, nullptr, 0.0, q_out, q_stride, &a);
     if (r) return r;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
@@ -2541,7 +2589,7 @@ int32_t tl_paged_attention(tl_handle* h, const tl_paged_cache* cache, const void
                            void* out, int64_t out_stride) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     PagedAttnArgs a{};
-    int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
+    int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, 0, 0, scale, out, out_stride, &a);
     if (r) return r;
     const OnDevice on(h->device);
     TL_HIP(h, on.err);
@@ -2558,7 +2606,7 @@ int32_t tl_paged_attention_async(tl_handle* h, void* stream, const tl_paged_cach
                                  int64_t scratch_bytes, int32_t* counters, int32_t* fault) {
     if (!h) return TL_ERR_BAD_DESCRIPTOR;
     PagedAttnArgs a{};
-    const int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, scale, out, out_stride, &a);
+    const int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, 0, 0, scale, out, out_stride, &a);
     if (r) return r;
     const int32_t bad = check_scratch(h, scratch, scratch_bytes, attention_scratch_bytes(a));
     if (bad) return bad;
@@ -2581,6 +2629,143 @@ int32_t tl_paged_attention_scratch(tl_handle* h, const tl_paged_cache* cache, in
            "query heads must be a multiple of the KV heads");
     *bytes = rows > 0 ? (int64_t)paged_attention_scratch(c, rows, n_heads) : 0;
     return TL_OK;
+}
+
+int32_t tl_paged_append_norm(tl_handle* h, const tl_paged_cache* cache, const void* qkv, int64_t qkv_stride, int32_t act,
+                             int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos,
+                             const float* cos, const float* sin, int32_t n_pos, const float* q_gain, const float* k_gain,
+                             double eps, void* q_out, int64_t q_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAppendArgs a{};
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_gain,
+                                  k_gain, eps, q_out, q_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.fault = h->fault_dev;
+    return complete(h, TL_K_OTHER, "tl_paged_append_norm", [&] { return launch_paged_append(h->stream, a); });
+}
+
+int32_t tl_paged_append_norm_async(tl_handle* h, void* stream, const tl_paged_cache* cache, const void* qkv,
+                                   int64_t qkv_stride, int32_t act, int32_t rows, int32_t n_heads, const int32_t* row_seq,
+                                   const int32_t* row_pos, const float* cos, const float* sin, int32_t n_pos,
+                                   const float* q_gain, const float* k_gain, double eps, void* q_out, int64_t q_stride,
+                                   int32_t* fault) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAppendArgs a{};
+    const int32_t r = append_args(h, cache, qkv, qkv_stride, act, rows, n_heads, row_seq, row_pos, cos, sin, n_pos, q_gain,
+                                  k_gain, eps, q_out, q_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.fault = fault;
+    return check_launch(h, launch_paged_append((hipStream_t)stream, a), "tl_paged_append_norm_async");
+}
+
+int32_t tl_paged_attention_shared(tl_handle* h, const tl_paged_cache* cache, const void* q, int64_t q_stride, int32_t act,
+                                  int32_t rows, int32_t n_heads, const int32_t* row_seq, const int32_t* row_pos,
+                                  int32_t prefix_seq, int32_t prefix_len, float scale, void* out, int64_t out_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAttnArgs a{};
+    int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, prefix_seq, prefix_len, scale,
+                               out, out_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    if ((r = ensure_op_scratch(h, paged_shared_scratch(a.c, rows, n_heads, prefix_len)))) return r;
+    a.scratch = (float*)h->op_scratch;
+    a.counters = h->op_counters;
+    a.fault = h->fault_dev;
+    paged_shared_places(a);
+    return complete(h, TL_K_ATTN, "tl_paged_attention_shared", [&] { return launch_paged_attention(h->stream, a); });
+}
+
+int32_t tl_paged_attention_shared_async(tl_handle* h, void* stream, const tl_paged_cache* cache, const void* q,
+                                        int64_t q_stride, int32_t act, int32_t rows, int32_t n_heads,
+                                        const int32_t* row_seq, const int32_t* row_pos, int32_t prefix_seq,
+                                        int32_t prefix_len, float scale, void* out, int64_t out_stride, void* scratch,
+                                        int64_t scratch_bytes, int32_t* counters, int32_t* fault) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    PagedAttnArgs a{};
+    int32_t r = attention_args(h, cache, q, q_stride, act, rows, n_heads, row_seq, row_pos, prefix_seq, prefix_len, scale,
+                               out, out_stride, &a);
+    if (r || (r = check_scratch(h, scratch, scratch_bytes, paged_shared_scratch(a.c, rows, n_heads, prefix_len)))) return r;
+    TL_REQ(h, !counters || ((uintptr_t)counters & 3) == 0, "counters misaligned");
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.scratch = (float*)scratch;
+    a.counters = counters;
+    a.fault = fault;
+    paged_shared_places(a);
+    return check_launch(h, launch_paged_attention((hipStream_t)stream, a), "tl_paged_attention_shared_async");
+}
+
+int32_t tl_paged_attention_shared_scratch(tl_handle* h, const tl_paged_cache* cache, int32_t rows, int32_t n_heads,
+                                          int32_t prefix_len, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes, "null pointer");
+    PagedCache c;
+    int32_t r = paged_cache_arg(h, cache, &c);
+    if (r || (r = attention_shape(h, c, rows, n_heads, prefix_len))) return r;
+    *bytes = (int64_t)paged_shared_scratch(c, rows, n_heads, prefix_len);
+    return TL_OK;
+}
+
+int32_t tl_linear_w8(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const void* packed,
+                     int32_t gated, int32_t n, int32_t k, const void* residual, int64_t res_stride, void* y,
+                     int64_t y_stride) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    W8Args a{};
+    int32_t r = w8_args(h, x, x_stride, act, m, packed, gated, n, k, residual, res_stride, y, y_stride, &a);
+    if (r) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    if ((r = ensure_op_scratch(h, w8_scratch(m, k)))) return r;
+    a.scratch = h->op_scratch;
+    return complete(h, TL_K_OTHER, "tl_linear_w8", [&] { return launch_linear_w8(h->stream, a); });
+}
+
+int32_t tl_linear_w8_async(tl_handle* h, void* stream, const void* x, int64_t x_stride, int32_t act, int32_t m,
+                           const void* packed, int32_t gated, int32_t n, int32_t k, const void* residual,
+                           int64_t res_stride, void* y, int64_t y_stride, void* scratch, int64_t scratch_bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    W8Args a{};
+    int32_t r = w8_args(h, x, x_stride, act, m, packed, gated, n, k, residual, res_stride, y, y_stride, &a);
+    if (r || (r = check_scratch(h, scratch, scratch_bytes, w8_scratch(m, k)))) return r;
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    a.scratch = scratch;
+    return check_launch(h, launch_linear_w8((hipStream_t)stream, a), "tl_linear_w8_async");
+}
+
+int32_t tl_linear_w8_scratch(tl_handle* h, int32_t m, int32_t k, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes && m >= 0 && m <= 1 << 17 && k >= 1 && k <= kW8MaxK, "bad scratch arguments");
+    *bytes = (int64_t)w8_scratch(m, k);
+    return TL_OK;
+}
+
+int32_t tl_w8_packed_bytes(tl_handle* h, int32_t n, int32_t k, int32_t gated, int64_t* bytes) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    TL_REQ(h, bytes, "null pointer");
+    const int32_t r = w8_shape(h, n, k);
+    if (r) return r;
+    *bytes = w8_packed_bytes(n, k, gated != 0);
+    return TL_OK;
+}
+
+int32_t tl_pack_w8(tl_handle* h, const int8_t* q, const float* scales, const int8_t* up_q, const float* up_scales,
+                   int32_t n, int32_t k, void* packed) {
+    if (!h) return TL_ERR_BAD_DESCRIPTOR;
+    const int32_t r = w8_shape(h, n, k);
+    if (r) return r;
+    TL_REQ(h, q && scales && packed && aligned16(packed) && ((uintptr_t)scales & 3) == 0, "null or misaligned pointer");
+    TL_REQ(h, (up_q != nullptr) == (up_scales != nullptr) && ((uintptr_t)up_scales & 3) == 0,
+           "gated weights need both matrices and both scales");
+    const OnDevice on(h->device);
+    TL_HIP(h, on.err);
+    return complete(h, TL_K_OTHER, "tl_pack_w8",
+                    [&] { return launch_pack_w8(h->stream, q, scales, up_q, up_scales, n, k, packed); });
 }
 
 int32_t tl_linear_w4(tl_handle* h, const void* x, int64_t x_stride, int32_t act, int32_t m, const void* packed,

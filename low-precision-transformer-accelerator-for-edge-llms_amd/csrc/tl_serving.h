@@ -1,6 +1,6 @@
-// tl_serving.h -- declarations of the serving operators (paged KV cache, 4-bit
+// tl_serving.h -- declarations of the serving operators (paged KV cache, 4-bit and 8-bit
 // projections, token log probabilities), shared by their kernels (tl_paged.hip,
-// tl_w4.hip, tl_score.hip) and the C++ runtime (tl_runtime.hip).  The index
+// tl_prefix.hip, tl_w4.hip, tl_w8.hip, tl_score.hip) and the C++ runtime (tl_runtime.hip).  The index
 // arithmetic at the top is host code too: a CPU test compiles it by itself.
 #pragma once
 
@@ -85,6 +85,39 @@ TL_HD inline int32_t paged_part(const PagedShare& s, int32_t w, int32_t unit_sta
 TL_HD inline bool paged_joins_at(const PagedShare& s, int32_t w, int32_t unit) {
     return s.start(w) > unit && s.start(w - 1) <= unit;
 }
+// Rows that share the first `len` positions of one sequence.  A row at pos from len - 1 on
+// adds the parts that the prefix's kernel left to its own keys, len .. pos, whose tiles
+// count from the last multiple of 32 up to len; a row before that is a row of the prefix's
+// sequence at pos and has all its keys from there.
+TL_HD inline bool shared_adds(int32_t len, int32_t pos) { return pos >= 0 && pos + 1 >= len; }
+TL_HD inline int32_t shared_tiles(int32_t len, int32_t pos) {
+    if (!shared_adds(len, pos)) return paged_tiles(pos + 1);
+    return paged_tiles(pos + 1 > len ? pos + 1 - (len & ~31) : 0);
+}
+
+// The kernel over a shared prefix: workgroups of 32 qw columns (rows times the query heads
+// of a KV head), the keys of each split so that the whole GPU has some.
+struct PrefixPlan {
+    int32_t qw;        // 1 or 4
+    int32_t qblocks;   // column blocks
+    int32_t splits;
+    int32_t grid;
+};
+constexpr int32_t kPrefixSplitKeys = 256;   // a split's keys, at least
+constexpr int32_t kPrefixWorkgroups = 512;
+inline PrefixPlan prefix_plan(int32_t rows, int32_t n_heads, int32_t n_kv, int32_t len) {
+    const int64_t columns = (int64_t)rows * (n_heads / n_kv);
+    PrefixPlan p;
+    p.qw = columns <= 64 ? 1 : 4;
+    p.qblocks = (int32_t)((columns + 32 * p.qw - 1) / (32 * p.qw));
+    const int64_t units = (int64_t)p.qblocks * n_kv;
+    const int64_t most = (len + kPrefixSplitKeys - 1) / kPrefixSplitKeys, want = (kPrefixWorkgroups + units - 1) / units;
+    p.splits = (int32_t)(want < most ? want : most);
+    if (p.splits < 1) p.splits = 1;
+    p.grid = (int32_t)(units * p.splits);
+    return p;
+}
+
 // The joining kernel's workgroups.  Up to 64 rows it has one per row and head; more
 // rows than that each would have to be looked for, though only workgroups - 1 (row, head
 // block)s can be split, so there it has one per boundary and head of a block.
@@ -224,6 +257,89 @@ inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {
     return p;
 }
 
+// Projections with 8-bit weights and activations: sizes and the plan of a call.
+//
+// Weights and quantized rows of x come in tiles of 16 rows and blocks of 64 columns, an
+// even number of blocks to a tile.  The tiles of gated weights take turns, gate and up.
+// Scratch of a call (w8_scratch() bytes): the scales of its rows, then their blocks.
+constexpr int32_t kW8Waves = 8, kW8Threads = 64 * kW8Waves;
+constexpr int32_t kW8MaxK = 1 << 17;     // 127 * 128 * 2^17 is below 2^31
+constexpr int64_t kW8Lds = 152 * 1024;   // of a workgroup's 160 KiB
+constexpr int32_t kW8Slots = 8;          // units of 8 columns of x that a thread keeps in registers
+
+TL_HD inline int32_t w8_blocks(int32_t k) { return (k + 127) / 128 * 2; }
+TL_HD inline int32_t w8_tiles(int32_t n, bool glu) { return (n + 15) / 16 * (glu ? 2 : 1); }
+TL_HD inline int64_t w8_rows_off(int32_t m) { return ((int64_t)m * 4 + 1023) / 1024 * 1024; }
+inline int64_t w8_packed_bytes(int32_t n, int32_t k, bool glu) { return (int64_t)w8_tiles(n, glu) * (w8_blocks(k) * 1024ll + 64); }
+// units of all of m rows that a thread takes
+TL_HD inline int32_t w8_slots(int32_t m, int32_t k) { return m * ((w8_blocks(k) * 8 + kW8Threads - 1) / kW8Threads); }
+TL_HD inline bool w8_in_rows(int32_t m, int32_t k) { return m <= 4 && w8_slots(m, k) <= kW8Slots; }
+inline size_t w8_scratch(int32_t m, int32_t k) {
+    return m <= 0 || w8_in_rows(m, k) ? 0 : (size_t)(w8_rows_off(m) + (int64_t)((m + 15) / 16) * w8_blocks(k) * 1024);
+}
+
+// Which tile a workgroup of the tiled form takes.  Workgroups go to the 8 XCDs in turn, so
+// each XCD gets a run of tiles of its own (its L2 then serves a run's operands again), in
+// columns of `tall` tiles of tokens.
+struct W8Grid {
+    int32_t n, m;      // tiles of y
+    int32_t tall;
+    TL_HD void tile(int32_t b, int32_t& tn, int32_t& tm) const {
+        const int32_t all = n * m, per = all / 8, rem = all % 8, xcd = b % 8, at = b / 8;
+        const int32_t i = xcd * per + (xcd < rem ? xcd : rem) + at;
+        const int32_t group = i / (tall * n), first = group * tall;
+        const int32_t h = m - first < tall ? m - first : tall;
+        const int32_t in = i - group * tall * n;
+        tn = in / h;
+        tm = first + in - tn * h;
+    }
+};
+
+enum W8Kind : int32_t { W8_ROW = 0, W8_SPLIT = 1, W8_TILE128 = 2, W8_TILE256 = 3 };
+struct W8Plan {
+    W8Kind kind;
+    int32_t split;         // W8_ROW: wavefronts that share a tile of weights
+    int32_t nt, mt;        // W8_SPLIT: tiles of a workgroup
+    int32_t quant_waves;   // wavefronts that quantize a row of x: 1, 2, 4 or 8
+    int32_t grid_x, grid_y;
+    int64_t lds;
+    W8Grid tiles;          // W8_TILE*
+};
+
+inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
+    const int32_t tiles = w8_tiles(n, glu), mbs = (m + 15) / 16;
+    W8Plan p{};
+    if (w8_in_rows(m, k)) {
+        p.kind = W8_ROW;
+        const int32_t units = (n + 15) / 16;
+        p.split = 1;
+        while (p.split < kW8Waves && (int64_t)units * p.split < 2048) p.split *= 2;
+        const int32_t per = kW8Waves / p.split;
+        p.grid_x = (units + per - 1) / per;
+        p.grid_y = 1;
+        p.lds = (int64_t)w8_blocks(k) * 64 * m + kW8Waves * (glu ? 2 : 1) * 64 * m;
+        return p;
+    }
+    p.quant_waves = 8;
+    while (p.quant_waves > 1 && (int64_t)m * p.quant_waves > 4096) p.quant_waves /= 2;
+    if (m <= 256) {
+        p.kind = W8_SPLIT;
+        p.mt = mbs == 1 ? 1 : mbs == 2 ? 2 : 4;
+        p.nt = p.mt == 4 ? 4 : 2;
+        p.grid_x = (tiles + p.nt - 1) / p.nt;
+        p.grid_y = (mbs + p.mt - 1) / p.mt;
+        return p;
+    }
+    const int64_t big = (int64_t)((tiles + 15) / 16) * ((mbs + 15) / 16);
+    const int32_t side = big >= 192 ? 16 : 8;
+    p.kind = side == 16 ? W8_TILE256 : W8_TILE128;
+    p.tiles = W8Grid{(tiles + side - 1) / side, (mbs + side - 1) / side, 8};
+    p.grid_x = p.tiles.n * p.tiles.m;
+    p.grid_y = 1;
+    p.lds = (int64_t)2 * 2 * (2 * side) * 1024;
+    return p;
+}
+
 }  // namespace tl
 
 #if defined(__HIPCC__)
@@ -256,12 +372,24 @@ struct PagedAppendArgs {
     int32_t n_pos;
     void* q_out;               // [rows][n_heads * head_dim], stride q_stride, or null
     int64_t q_stride;
+    const float* q_gain;       // [head_dim], 16-byte aligned: q, or k, is normed first; or null
+    const float* k_gain;
+    double eps;
     int32_t* fault;            // set to 1 where a row names no place in the cache, or null
 };
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a);
 
+// The first `len` positions of sequence `seq`, shared by all rows (len 0: none), and what
+// the kernel over them leaves: O [splits][rows][n_heads][head_dim], m and l [...][2]
+struct PagedPrefix {
+    int32_t seq, len, splits;
+    float* o;
+    float* ml;
+};
+
 struct PagedAttnArgs {
     PagedCache c;
+    PagedPrefix prefix;
     const void* q;             // [rows][n_heads * head_dim], stride q_stride
     int64_t q_stride;
     int32_t act;
@@ -279,6 +407,11 @@ constexpr int32_t kOpCounters = 16384;
 int32_t paged_attention_workgroups(const PagedCache& c, int32_t rows, int32_t n_heads);
 size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads);
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
+// with a shared prefix: scratch of both kernels, and its places from a.scratch
+size_t paged_shared_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, int32_t len);
+void paged_shared_places(PagedAttnArgs& a);
+hipError_t launch_paged_prefix(hipStream_t s, const PagedAttnArgs& a);
+hipError_t init_prefix_kernels();
 
 // Projections with 4-bit weights.  Packed weights (launch_pack_w4) hold, for each
 // 16 rows and 128 columns, 1 KiB in the order a wavefront's lanes take it, rows and
@@ -307,6 +440,27 @@ hipError_t launch_pack_w4(hipStream_t s, const uint8_t* q, const void* scales, i
 hipError_t launch_quantize_w4(hipStream_t s, const float* w, int32_t rows, int32_t k, int32_t group, int32_t scale_dtype,
                               uint8_t* q, void* scales);
 hipError_t init_w4_kernels();
+
+// Projections with 8-bit weights (launch_pack_w8) and rows quantized on the way
+struct W8Args {
+    const void* x;             // [m][k] of act, stride x_stride, any alignment of the type
+    int64_t x_stride;
+    int32_t act;
+    int32_t m, n, k;
+    const void* packed;
+    bool glu;                  // packed holds gate and up: y = silu(gate) up
+    bool x_aligned, y_aligned; // set by the launch: rows may be read 16 bytes, written 4 values at once
+    const void* residual;      // [m][n] of act, stride res_stride, or null
+    int64_t res_stride;
+    void* y;                   // [m][n] of act, stride y_stride
+    int64_t y_stride;
+    void* scratch;             // w8_scratch() bytes, 16-byte aligned
+};
+hipError_t launch_linear_w8(hipStream_t s, const W8Args& a);
+// q [n][k] and scales [n]; with q2 and scales2, gate and up
+hipError_t launch_pack_w8(hipStream_t s, const int8_t* q, const float* scales, const int8_t* q2, const float* scales2,
+                          int32_t n, int32_t k, void* packed);
+hipError_t init_w8_kernels();
 
 // log probabilities, entropy and top alternatives of rows of logits
 struct LogprobsArgs {

@@ -10,7 +10,7 @@ can be captured into a ``torch.cuda.CUDAGraph`` (but the first on a device).  Sc
 memory is torch's, kept for each stream, and a captured graph has its own, so calls
 on different streams and graphs share none; threads may call at the same time.  A
 captured call joins the parts of a long row in another order than a queued one does,
-so attention may differ between them in the last place.  A ``PagedCache`` or ``W4Linear``
+so attention may differ between them in the last place.  A ``PagedCache``, ``W4Linear`` or ``W8Linear``
 is kept until the calls made with it on other streams than the one it was made on are
 done, and as long as a graph that holds such calls.  Tensors are CUDA tensors of one
 device; float types are float32, bfloat16 and float16.  Nothing here is differentiable:
@@ -165,28 +165,43 @@ class PagedCache:
             table.stride(0) if table.shape[0] > 1 else table.shape[1], k.stride(0) if n_pages > 1 else n_kv * page * hd,
             _CACHE[k.dtype], n_pages, page, n_kv, hd, table.shape[0], table.shape[1])
         self._desc = C.byref(self.desc)
-        self._scratch: dict[tuple[int, int], int] = {}
+        self._scratch: dict[tuple[int, int, int], int] = {}
         self._scratch_bytes(0, n_kv)   # the descriptor's own checks
 
-    def _scratch_bytes(self, rows: int, n_heads: int) -> int:
-        got = self._scratch.get((rows, n_heads))
+    def _scratch_bytes(self, rows: int, n_heads: int, prefix_len: int = 0) -> int:
+        got = self._scratch.get((rows, n_heads, prefix_len))
         if got is None:
             n = C.c_int64()
-            self.rt.check(self.rt.lib.tl_paged_attention_scratch(self.rt.h, self._desc, rows, n_heads, C.byref(n)),
-                          "tl_paged_attention_scratch")
-            got = self._scratch[(rows, n_heads)] = n.value
+            if prefix_len:
+                self.rt.check(self.rt.lib.tl_paged_attention_shared_scratch(self.rt.h, self._desc, rows, n_heads, prefix_len,
+                                                                            C.byref(n)), "tl_paged_attention_shared_scratch")
+            else:
+                self.rt.check(self.rt.lib.tl_paged_attention_scratch(self.rt.h, self._desc, rows, n_heads, C.byref(n)),
+                              "tl_paged_attention_scratch")
+            got = self._scratch[(rows, n_heads, prefix_len)] = n.value
         return got
+
+    def _gain(self, name: str, t):
+        """Address of a head's norm gains, or None."""
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != self.device \
+                or t.shape != (self.head_dim,) or not t.is_contiguous():
+            raise _bad(f"{name} must be [{self.head_dim}] float32 on {self.device}")
+        return t.data_ptr()
 
     def _row_ids(self, row_seq, row_pos, rows: int):
         if row_seq is None:
             return None, _ints("row_pos", row_pos, self.device, rows)
         return _ints("row_seq", row_seq, self.device, rows), _ints("row_pos", row_pos, self.device, rows)
 
-    def append(self, qkv, row_seq, row_pos, out=None):
+    def append(self, qkv, row_seq, row_pos, out=None, norm=None, eps: float = 1e-5):
         """Rows of Q|K|V projections [rows][(n_heads + 2 n_kv_heads) * head_dim]: q and k rotated at
         row_pos, k and v written to the cache at row_pos of sequence row_seq (None: row r
         is sequence r; negative: a padded row, skipped).  Returns the rotated q (``out`` if
-        given; it may be the q part of qkv); a padded row of a new tensor is undefined."""
+        given; it may be the q part of qkv); a padded row of a new tensor is undefined.
+        ``norm``: gains (q, k), [head_dim] float32 each or None, with which q and k of every
+        head are normed first: x / sqrt(mean x^2 + eps) * gain."""
         dev, hd = self.device, self.head_dim
         _rows("qkv", qkv, dev)
         if self.rope is None:
@@ -202,16 +217,26 @@ class PagedCache:
             _rows("out", out, dev, n_heads * hd, qkv.dtype)
             if out.shape[0] != rows:
                 raise _bad("out must have a row for each of qkv's")
+        if norm is not None:
+            q_gain, k_gain = self._gain("the q gains", norm[0]), self._gain("the k gains", norm[1])
+            if not 0.0 <= eps <= 1e30:
+                raise _bad("eps must be a number from 0 on")
         if rows == 0:
             return out
         cos, sin = self.rope
         stride = _stride(qkv)
         q_stride = stride if out.data_ptr() == qkv.data_ptr() and rows == 1 else _stride(out)
         rt = self.rt
-        st = rt.lib.tl_paged_append_async(
-            rt.h, _stream(dev), self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
-            rows, n_heads, seq, pos, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-            out.data_ptr() if n_heads else None, q_stride, self.fault.data_ptr())
+        q_out = out.data_ptr() if n_heads else None
+        if norm is None:
+            st = rt.lib.tl_paged_append_async(
+                rt.h, _stream(dev), self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
+                rows, n_heads, seq, pos, cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out, q_stride, self.fault.data_ptr())
+        else:
+            st = rt.lib.tl_paged_append_norm_async(
+                rt.h, _stream(dev), self._desc, qkv.data_ptr(), stride, _ACT[qkv.dtype],
+                rows, n_heads, seq, pos, cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_gain, k_gain, eps, q_out, q_stride,
+                self.fault.data_ptr())
         if st:
             rt.check(st, "append")
         return out
@@ -221,6 +246,21 @@ class PagedCache:
         (rotated) over keys 0 .. row_pos[r] of sequence row_seq[r] (None: r); a
         negative position gives zeros, a negative sequence leaves its row of ``out`` as it
         was (undefined in a new tensor).  ``out`` may be q.  ``scale``: 1 / sqrt(head_dim) unless given."""
+        return self._attend("attend", q, row_seq, row_pos, 0, 0, scale, out)
+
+    def attend_shared(self, q, row_seq, row_pos, prefix_seq: int, prefix_len: int, scale: float | None = None, out=None):
+        """``attend`` of rows whose first ``prefix_len`` positions are those of sequence
+        ``prefix_seq``, a prompt that all of them begin with: its keys are read once for all
+        rows, key t of row r is position t of prefix_seq for t < prefix_len and of
+        row_seq[r] from there on (table entries of row_seq before that are not used).
+        Several prompts in a batch: one call each into one ``out``, the other rows' row_seq
+        negative.  In a captured graph the prefix is the one it was captured with."""
+        if not 0 <= prefix_len <= self.desc.max_pages * self.desc.page_size or (
+                prefix_len and not 0 <= prefix_seq < self.n_seqs):
+            raise _bad("the prefix must lie in the pages of a sequence of the table")
+        return self._attend("attend_shared", q, row_seq, row_pos, int(prefix_seq), int(prefix_len), scale, out)
+
+    def _attend(self, what, q, row_seq, row_pos, prefix_seq, prefix_len, scale, out):
         dev, hd = self.device, self.head_dim
         _rows("q", q, dev)
         rows, width = q.shape
@@ -236,15 +276,20 @@ class PagedCache:
                 raise _bad("out must have a row for each of q's")
         if rows == 0:
             return out
-        need = self._scratch_bytes(rows, n_heads)
+        need = self._scratch_bytes(rows, n_heads, prefix_len)
         rt, stream = self.rt, _stream(dev)
         scratch, counters, keep = _workspace(dev, stream, need)
-        st = rt.lib.tl_paged_attention_async(
-            rt.h, stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows,
-            n_heads, seq, pos, 1.0 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), _stride(out),
-            scratch, need, counters, self.fault.data_ptr())
+        scale = 1.0 / math.sqrt(hd) if scale is None else scale
+        if prefix_len:
+            st = rt.lib.tl_paged_attention_shared_async(
+                rt.h, stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows, n_heads, seq, pos, prefix_seq,
+                prefix_len, scale, out.data_ptr(), _stride(out), scratch, need, counters, self.fault.data_ptr())
+        else:
+            st = rt.lib.tl_paged_attention_async(
+                rt.h, stream, self._desc, q.data_ptr(), _stride(q), _ACT[q.dtype], rows, n_heads, seq, pos, scale,
+                out.data_ptr(), _stride(out), scratch, need, counters, self.fault.data_ptr())
         if st:
-            rt.check(st, "attend")
+            rt.check(st, what)
         return out
 
     def check(self) -> None:
@@ -342,6 +387,116 @@ class W4Linear:
         if st:
             rt.check(st, "W4Linear")
         return out
+
+
+def quantize_w8(w, rt: Runtime | None = None):
+    """8-bit weights of float32 ones [n][k] (tl_quantize_weight_rows): (q int8, scales
+    [n] float32) for ``W8Linear`` and ``W8GatedLinear``."""
+    if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype != torch.float32 or w.dim() != 2 or 0 in w.shape:
+        raise _bad("w must be a CUDA tensor [n][k] of float32")
+    rt = rt or _runtime(w.device)
+    if rt.device != w.device.index:
+        raise _bad("the handle belongs to another device")
+    q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+    scales = torch.empty(w.shape[0], dtype=torch.float32, device=w.device)
+    with _COMPLETING:
+        rt.call("tl_quantize_weight_rows", w.contiguous(), w.shape[0], w.shape[1], q, scales)
+    return q, scales
+
+
+class _W8:
+    """Packed 8-bit weights, of one projection or of a gate and an up projection."""
+
+    def __init__(self, pairs, rt: Runtime | None):
+        q = pairs[0][0]
+        for w, s in pairs:
+            if not isinstance(w, torch.Tensor) or not w.is_cuda or w.dtype != torch.int8 or w.dim() != 2 \
+                    or not w.is_contiguous() or w.shape != q.shape or w.device != q.device:
+                raise _bad("weights must be contiguous CUDA tensors [n][k] of int8, of one shape and device")
+            if not isinstance(s, torch.Tensor) or s.device != q.device or s.dtype != torch.float32 \
+                    or s.shape != (q.shape[0],) or not s.is_contiguous():
+                raise _bad(f"scales must be [n] float32 on {q.device}")
+        self.device = q.device
+        self.n, self.k = q.shape
+        self.gated = len(pairs) == 2
+        self.rt = rt = rt or _runtime(q.device)
+        if rt.device != q.device.index:
+            raise _bad("the handle belongs to another device")
+        n = C.c_int64()
+        rt.check(rt.lib.tl_w8_packed_bytes(rt.h, self.n, self.k, int(self.gated), C.byref(n)), type(self).__name__)
+        self.packed = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+        with _COMPLETING:
+            rt.call("tl_pack_w8", *pairs[0], *(pairs[1] if self.gated else (None, None)), self.n, self.k, self.packed)
+        self._scratch: dict[int, int] = {}
+
+    def _scratch_bytes(self, rows: int) -> int:
+        got = self._scratch.get(rows)
+        if got is None:
+            n = C.c_int64()
+            self.rt.check(self.rt.lib.tl_linear_w8_scratch(self.rt.h, rows, self.k, C.byref(n)), "tl_linear_w8_scratch")
+            got = self._scratch[rows] = n.value
+        return got
+
+    def _call(self, x, residual, out):
+        dev = self.device
+        _rows("x", x, dev, self.k)
+        rows = x.shape[0]
+        if out is None:
+            out = torch.empty((rows, self.n), dtype=x.dtype, device=dev)
+        else:
+            _rows("out", out, dev, self.n, x.dtype)
+        if residual is not None:
+            _rows("residual", residual, dev, self.n, x.dtype)
+        if out.shape[0] != rows or (residual is not None and residual.shape[0] != rows):
+            raise _bad("out and residual must have a row for each of x's")
+        if rows == 0:
+            return out
+        need = self._scratch_bytes(rows)
+        rt, stream = self.rt, _stream(dev)
+        scratch, _, keep = _workspace(dev, stream, need)
+        st = rt.lib.tl_linear_w8_async(
+            rt.h, stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows, self.packed.data_ptr(), int(self.gated), self.n,
+            self.k, None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),
+            out.data_ptr(), _stride(out), scratch, need)
+        if st:
+            rt.check(st, type(self).__name__)
+        return out
+
+
+class W8Linear(_W8):
+    """A projection in 8-bit integers: y = x w^T (+ residual), with w[n][k] = q[n][k] *
+    scales[n] and each row of x quantized on the way, x8 = rne(x / s), s = max |x| / 127.
+    q [n][k] int8 and scales [n] float32 (``quantize_w8``) are packed here, once, and not
+    kept.  Any n and any k up to 2^17; sums are exact (tl_linear_w8)."""
+
+    def __init__(self, q, scales, rt: Runtime | None = None):
+        super().__init__([(q, scales)], rt)
+
+    @classmethod
+    def from_float(cls, w, rt: Runtime | None = None) -> "W8Linear":
+        """Quantize and pack float32 weights [n][k]."""
+        return cls(*quantize_w8(w, rt), rt)
+
+    def __call__(self, x, residual=None, out=None):
+        """x [rows][k] -> [rows][n] in x's type; ``out`` may be ``residual``, not x."""
+        return self._call(x, residual, out)
+
+
+class W8GatedLinear(_W8):
+    """The first half of a gated feed-forward block in 8-bit integers, in one product:
+    y = silu(x gate^T) * (x up^T), both projections as ``W8Linear``'s."""
+
+    def __init__(self, gate, gate_scales, up, up_scales, rt: Runtime | None = None):
+        super().__init__([(gate, gate_scales), (up, up_scales)], rt)
+
+    @classmethod
+    def from_float(cls, gate, up, rt: Runtime | None = None) -> "W8GatedLinear":
+        """Quantize and pack float32 weights [n][k]."""
+        return cls(*quantize_w8(gate, rt), *quantize_w8(up, rt), rt)
+
+    def __call__(self, x, out=None):
+        """x [rows][k] -> [rows][n] in x's type; ``out`` is apart from x."""
+        return self._call(x, None, out)
 
 
 class TokenLogprobs(NamedTuple):

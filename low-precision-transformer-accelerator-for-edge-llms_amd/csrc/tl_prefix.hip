@@ -19,8 +19,9 @@ namespace {
 // once, turned to 16 bits and, the values, on their side, and lie in LDS in the order of
 // the products' operands.
 //
-// The keys are split over workgroups; each leaves O, m and l of its columns in scratch,
-// which the kernel of the rows' own keys adds to those (paged_attention_kernel).
+// The keys are split over workgroups; each leaves O, m and l of its columns in scratch.  In
+// the same launch other workgroups take the rows' own keys as paged_attention_kernel does
+// (attention_run); a second kernel joins what both left.
 //
 // Precision: q enters in QP 16-bit parts and the probabilities in PP, as many as it takes:
 // of 16-bit rows q is exact in one (float16 holds a bfloat16 scaled to its row); float32 rows
@@ -28,6 +29,7 @@ namespace {
 // two parts, as one bfloat16 or float16 rounding of each would weigh as much as the result's own.
 // ---------------------------------------------------------------------------
 constexpr int kPrefixThreads = 256;
+constexpr float kPrefixSlack = 4.0f;
 
 template <int HD, int DT, int QP, int PP, int QW>
 struct Prefix {
@@ -67,6 +69,30 @@ struct Prefix {
 
 typedef const __attribute__((address_space(4))) int32_t* scalar_table;
 
+// two floats to the 16-bit type, each to nearest
+template <bool BF>
+TL_DEV int round2(float a, float b) {
+    const v2f v = {a, b};
+    if constexpr (BF) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(int, __builtin_convertvector(v, b2));
+    } else {
+        return __builtin_bit_cast(int, __builtin_convertvector(v, h2));
+    }
+}
+// what a pair of 16-bit values leaves of a and b
+template <bool BF>
+TL_DEV void less2(int w, float& a, float& b) {
+    if constexpr (BF) {
+        a -= __uint_as_float((unsigned)w << 16);
+        b -= __uint_as_float((unsigned)w & 0xFFFF0000u);
+    } else {
+        const h2 h = __builtin_bit_cast(h2, w);
+        a = __builtin_fmaf(-1.0f, (float)h[0], a);
+        b = __builtin_fmaf(-1.0f, (float)h[1], b);
+    }
+}
+
 // W bytes times 8 rows to registers
 template <int BYTES>
 struct Piece {
@@ -86,11 +112,9 @@ struct Piece {
 };
 
 template <int HD, int DT, int QP, int PP, int QW>
-__global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_kernel(PagedAttnArgs a, int qblocks) {
+TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroups, const int qblocks, char* lds, float (*s_ml)[32][2]) {
     using P = Prefix<HD, DT, QP, PP, QW>;
     constexpr bool BF = P::BF;
-    extern __shared__ __align__(16) char lds[];
-    __shared__ float s_ml[4][32][2];
     const PagedGeom& geo = a.c.g;
     const int rep = a.n_heads / geo.n_kv;
     const int lane = lane_id(), wave = wave_id(), col = lane & 15, g = lane >> 4;
@@ -98,12 +122,13 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
 
     // workgroup: (KV head, split, column block), column blocks that read the same keys side by
     // side on one XCD
-    const int all = gridDim.x, xcd = blockIdx.x % 8, per = all / 8, rem = all % 8;
-    const int at = xcd * per + min(xcd, rem) + blockIdx.x / 8;
+    const int xcd = me % 8, per = workgroups / 8, rem = workgroups % 8;
+    const int at = xcd * per + min(xcd, rem) + me / 8;
     const int qb = at % qblocks, split = at / qblocks % a.prefix.splits, kvh = at / qblocks / a.prefix.splits;
     const int len = a.prefix.len;
     const int steps_all = (len + P::KT * P::KG - 1) / (P::KT * P::KG);
-    const int s0 = (int)((int64_t)steps_all * split / a.prefix.splits), s1 = (int)((int64_t)steps_all * (split + 1) / a.prefix.splits);
+    const PagedShare share = paged_share(steps_all, a.prefix.splits);
+    const int s0 = share.start(split), s1 = share.start(split + 1);
 
     const scalar_table table = (scalar_table)(geo.table + (int64_t)a.prefix.seq * geo.table_stride);
     const int last8 = (len - 1) & ~7;
@@ -116,12 +141,12 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
     // columns of this lane: query head and row
     int64_t q_at[2];
     int rows_of[2], head_of[2];
-    const int64_t columns = (int64_t)a.rows * rep;
+    const int columns = a.rows * rep;   // (below 2^30)
 #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
-        const int64_t c = std::min<int64_t>((int64_t)qb * P::COLS + wq * 32 + ct * 16 + col, columns - 1);
-        rows_of[ct] = (int)(c / rep);
-        head_of[ct] = kvh * rep + (int)(c - (int64_t)rows_of[ct] * rep);
+        const int c = min(qb * P::COLS + wq * 32 + ct * 16 + col, columns - 1);
+        rows_of[ct] = (int)((unsigned)c / (unsigned)rep);
+        head_of[ct] = kvh * rep + c - rows_of[ct] * rep;
         q_at[ct] = (int64_t)rows_of[ct] * a.q_stride + (int64_t)head_of[ct] * HD;
     }
     v4i qf[QP][2][P::KC];
@@ -153,6 +178,10 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
             up = __builtin_amdgcn_ldexpf(up, e);
             s = __builtin_amdgcn_ldexpf(s, -e);
         }
+        if (s == 0.0f) {   // all scores alike: products of 0, so that a masked one stays minus infinity
+            up = 0.0f;
+            s = 1.0f;
+        }
         cs[ct] = s;
 #pragma unroll
         for (int c = 0; c < P::KC; c++) {
@@ -163,13 +192,8 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
             for (int p = 0; p < QP; p++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    unsigned w[2];
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        w[i] = BF ? to_bf16(rest[2 * j + i]) : to_f16(rest[2 * j + i]);
-                        rest[2 * j + i] -= BF ? bf16_bits(w[i]) : f16_bits(w[i]);
-                    }
-                    qf[p][ct][c][j] = (int)(w[0] | w[1] << 16);
+                    qf[p][ct][c][j] = round2<BF>(rest[2 * j], rest[2 * j + 1]);
+                    less2<BF>(qf[p][ct][c][j], rest[2 * j], rest[2 * j + 1]);
                 }
         }
     }
@@ -177,44 +201,47 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
     // a tile's pieces on their way: KN times 8 dimensions of a key, VN dimensions of 8 keys
     Piece<8 * P::ES> kr[P::KN];
     Piece<P::VN * P::ES> vr[8];
-    int32_t pages[P::KT / 8];      // of the next tile to be read
-    unsigned bad = 0;              // octets of the tile in registers whose page is out of range
-    bool any_bad = false;
+    // Pages of the next tile to be read, of each of this thread's pieces; those of the keys
+    // are the wavefront's, as its keys of one load lie in one group of 8.  They are vector
+    // loads: a scalar load in flight makes every LDS read wait for it.
+    int32_t k_page[P::KN], v_page;
+    int zero;
+    asm("v_mov_b32 %0, 0" : "=v"(zero));
+    const int32_t* pages = geo.table + (int64_t)a.prefix.seq * geo.table_stride;
+    auto k_octet = [&](int j) { return (j * P::T + wq * 64) / P::UK >> 3; };
+    const int v_octet = tid / P::UV, v_d = tid % P::UV * P::VN;
     auto look_up = [&](int step) {
         const int key0 = (step * P::KG + group) * P::KT;
 #pragma unroll
-        for (int o = 0; o < P::KT / 8; o++) pages[o] = table[min(key0 + 8 * o, last8) >> geo.page_shift];
+        for (int j = 0; j < P::KN; j++) k_page[j] = pages[(min(key0 + 8 * k_octet(j), last8) >> geo.page_shift) + zero];
+        v_page = pages[min(key0 + 8 * v_octet, last8) >> geo.page_shift];
     };
-    const int v_octet = tid / P::UV, v_d = tid % P::UV * P::VN;
+    auto in_pool = [&](int32_t page) { return (unsigned)page < (unsigned)geo.n_pages ? page : 0; };
     auto fetch = [&](int step) {
         const int key0 = (step * P::KG + group) * P::KT;
-        bad = 0;
-#pragma unroll
-        for (int o = 0; o < P::KT / 8; o++)
-            if ((unsigned)pages[o] >= (unsigned)geo.n_pages) {
-                bad |= 1u << o;
-                pages[o] = 0;
-            }
         // rows behind the last key are read where its eight are
 #pragma unroll
         for (int j = 0; j < P::KN; j++) {
             const int i = j * P::T + tid, key = i / P::UK, u = i % P::UK;
-            const int octet = __builtin_amdgcn_readfirstlane(key >> 3);   // the wavefront's keys lie in one
-            int32_t page = pages[0];
-#pragma unroll
-            for (int o = 1; o < P::KT / 8; o++) page = octet == o ? pages[o] : page;
-            const int k = min(key0 + 8 * octet, last8) + (key & 7);
-            kr[j].load(kbase + page * page_bytes + ((k & page_mask) * HD + 8 * u) * P::ES);
+            const int k = (min(key0 + 8 * k_octet(j), last8) & page_mask) + (key & 7);
+            kr[j].load(kbase + in_pool(__builtin_amdgcn_readfirstlane(k_page[j])) * page_bytes + (k * HD + 8 * u) * P::ES);
         }
-        int32_t page = pages[0];
-#pragma unroll
-        for (int o = 1; o < P::KT / 8; o++) page = v_octet == o ? pages[o] : page;
-        const char* v = vbase + page * page_bytes + ((min(key0 + 8 * v_octet, last8) & page_mask) * HD + v_d) * P::ES;
+        const char* v = vbase + in_pool(v_page) * page_bytes + ((min(key0 + 8 * v_octet, last8) & page_mask) * HD + v_d) * P::ES;
 #pragma unroll
         for (int r = 0; r < 8; r++) vr[r].load(v + r * HD * P::ES);
     };
+    // groups of 8 of a tile whose page is out of range
+    auto lost_of = [&](int step) {
+        const int key0 = (step * P::KG + group) * P::KT;
+        unsigned bad = 0;
+        for (int o = 0; o < P::KT / 8; o++) {
+            const int32_t page = table[min(key0 + 8 * o, last8) >> geo.page_shift];
+            bad |= (unsigned)page >= (unsigned)geo.n_pages ? 1u << o : 0u;
+        }
+        return bad;
+    };
     char* const k_lds = lds + group * (P::BUF * 2 * P::TILE);
-    auto keep = [&](int step) {
+    auto keep = [&](int step, bool whole, unsigned bad) {
         char* kl = k_lds + (P::BUF == 2 ? (step & 1) * 2 * P::TILE : 0);
         char* vl = kl + P::TILE;
 #pragma unroll
@@ -230,20 +257,22 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
             }
             *(v4i*)(kl + P::key_at(key, u)) = w;
         }
-        // values of keys behind the last one and of pages out of range are zero, as 0 x NaN is NaN
-        const int left = len - ((step * P::KG + group) * P::KT + 8 * v_octet);
-        const bool lost = bad >> v_octet & 1;
+        if (!whole) {   // values of keys behind the last one and of lost pages are zero, as 0 x NaN is NaN
+            asm volatile("");
+            const int left = bad >> v_octet & 1 ? 0 : len - ((step * P::KG + group) * P::KT + 8 * v_octet);
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+#pragma unroll
+                for (unsigned& w : vr[r].w) w = r < left ? w : 0u;
+        }
 #pragma unroll
         for (int i = 0; i < P::VN; i++) {
             v4i w;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const unsigned x = vr[2 * r].w[i * P::ES / 4], y = vr[2 * r + 1].w[i * P::ES / 4];
-                unsigned pair;
-                if constexpr (DT == DT_I8) pair = (unsigned)i8_pair_f16(__builtin_amdgcn_perm(y, x, 0x0C040C00u + 0x00010001u * (unsigned)(i & 3)));
-                else pair = __builtin_amdgcn_perm(y, x, i & 1 ? 0x07060302u : 0x05040100u);
-                if (left < 2 * r + 2) pair = left == 2 * r + 1 ? pair & 0xFFFFu : 0u;
-                w[r] = lost ? 0 : (int)pair;
+                if constexpr (DT == DT_I8) w[r] = i8_pair_f16(__builtin_amdgcn_perm(y, x, 0x0C040C00u + 0x00010001u * (unsigned)(i & 3)));
+                else w[r] = (int)__builtin_amdgcn_perm(y, x, i & 1 ? 0x07060302u : 0x05040100u);
             }
             *(v4i*)(vl + P::value_at(v_octet, v_d + i)) = w;
         }
@@ -254,6 +283,13 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
 #pragma unroll
     for (int j = 0; j < P::VD; j++) o[j][0] = o[j][1] = v4f{0, 0, 0, 0};
 
+    // whether a page of this split is out of range: looked at once, so that no tile has to
+    bool any_lost = false;
+    {
+        const int first = (s0 * P::KG * P::KT) >> geo.page_shift, last = (min(s1 * P::KG * P::KT, len) - 1) >> geo.page_shift;
+        for (int p = first + lane; p <= last; p += 64) any_lost |= (unsigned)table[p] >= (unsigned)geo.n_pages;
+        any_lost = __builtin_amdgcn_ballot_w64(any_lost) != 0;
+    }
     if (s0 < s1) {
         look_up(s0);
         fetch(s0);
@@ -261,8 +297,11 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
     }
     for (int step = s0; step < s1; step++) {
         if constexpr (P::BUF == 1) __builtin_amdgcn_wave_barrier();
-        keep(step);
-        const unsigned bad_now = bad;
+        const int key0 = (step * P::KG + group) * P::KT;
+        unsigned bad_now = 0;
+        if (any_lost) bad_now = lost_of(step);
+        const bool whole = key0 + P::KT <= len && bad_now == 0;
+        keep(step, whole, bad_now);
         if constexpr (P::BUF == 2) __syncthreads();
         else __builtin_amdgcn_wave_barrier();
         if (step + 1 < s1) {
@@ -271,7 +310,6 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
         }
         const char* kl = k_lds + (P::BUF == 2 ? (step & 1) * 2 * P::TILE : 0);
         const char* vl = kl + P::TILE;
-        const int key0 = (step * P::KG + group) * P::KT;
         v4f s[P::SUB][2][2];
 #pragma unroll
         for (int sub = 0; sub < P::SUB; sub++)
@@ -288,11 +326,9 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
                         for (int ct = 0; ct < 2; ct++) s[sub][t][ct] = mfma32<BF>(kk, qf[p][ct][c], s[sub][t][ct]);
                 }
             }
-        const bool whole = key0 + P::KT <= len && bad_now == 0;
-        any_bad |= bad_now != 0;
-        unsigned in = 0xFFFFu;   // keys 32 sub + 8 g + j: bit 8 sub + j
         if (!whole) {
-            in = 0;
+            asm volatile("");    // a branch, no selects in every tile
+            unsigned in = 0;     // keys 32 sub + 8 g + j: bit 8 sub + j
 #pragma unroll
             for (int sub = 0; sub < P::SUB; sub++) {
                 const int left = len - (key0 + 32 * sub + 8 * g);
@@ -316,7 +352,10 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
 #pragma unroll
                 for (int j = 0; j < 8; j++) mt = fmaxf(mt, s[sub][j >> 2][ct][j & 3]);
             mt = pair_max(mt);
-            if (__builtin_amdgcn_ballot_w64(mt > m[ct]) != 0) {
+            // sums are scaled anew only where a score leaves them by kPrefixSlack: a fresh maximum,
+            // of which most tiles have one among 16 columns, alone does not
+            if (__builtin_amdgcn_ballot_w64(mt * cs[ct] > m[ct] * cs[ct] + kPrefixSlack) != 0) {
+                asm volatile("");
                 const float mn = fmaxf(m[ct], mt);
                 const float al = m[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * cs[ct]);
                 m[ct] = mn;
@@ -324,28 +363,23 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
 #pragma unroll
                 for (int j = 0; j < P::VD; j++) o[j][ct] *= al;
             }
-            // p 2^14, so that the float16 parts of small probabilities stay normal
-            const float off = (m[ct] == -__builtin_inff() ? 0.0f : m[ct] * cs[ct]) - (BF ? 0.0f : 14.0f);
+            // p 2^14 over float16, so that the parts of small probabilities stay normal; 2^10 of it
+            // here, as a score may lie kPrefixSlack above m
+            const float off = (m[ct] == -__builtin_inff() ? 0.0f : m[ct] * cs[ct]) - (BF ? 0.0f : 14.0f - kPrefixSlack);
 #pragma unroll
             for (int sub = 0; sub < P::SUB; sub++) {
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][j >> 2][ct][j & 3], cs[ct], -off));
-                    if (!whole) p[j] = in >> (8 * sub + j) & 1 ? p[j] : 0.0f;
                     l[ct] += p[j];
                 }
 #pragma unroll
                 for (int part = 0; part < PP; part++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        unsigned w[2];
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            w[i] = BF ? to_bf16(p[2 * j + i]) : to_f16(p[2 * j + i]);
-                            if (part + 1 < PP) p[2 * j + i] -= BF ? bf16_bits(w[i]) : f16_bits(w[i]);
-                        }
-                        pf[sub][part][ct][j] = (int)(w[0] | w[1] << 16);
+                        pf[sub][part][ct][j] = round2<BF>(p[2 * j], p[2 * j + 1]);
+                        if (part + 1 < PP) less2<BF>(pf[sub][part][ct][j], p[2 * j], p[2 * j + 1]);
                     }
             }
         }
@@ -360,20 +394,21 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
                     for (int ct = 0; ct < 2; ct++) o[j][ct] = mfma32<BF>(vv, pf[sub][part][ct], o[j][ct]);
             }
     }
-    if (a.fault && any_bad) *a.fault = 1;
+    if (a.fault && any_lost) *a.fault = 1;
 
     // m in units of the exponent, l over the lane groups, values' scale
     const float sv = DT == DT_I8 ? a.c.vs[kvh] : 1.0f;
 #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
-        m[ct] = m[ct] == -__builtin_inff() ? m[ct] : m[ct] * cs[ct];
+        // (2^14 of the probabilities over float16, as the other kernel's parts)
+        m[ct] = m[ct] == -__builtin_inff() ? m[ct] : m[ct] * cs[ct] + (BF ? 0.0f : kPrefixSlack);
         l[ct] += lane_xor<16>(l[ct]);
         l[ct] += lane_xor<32>(l[ct]);
     }
     if constexpr (P::KG == 1) {
 #pragma unroll
         for (int ct = 0; ct < 2; ct++) {
-            if ((int64_t)qb * P::COLS + wq * 32 + ct * 16 + col >= columns) continue;
+            if (qb * P::COLS + wq * 32 + ct * 16 + col >= columns) continue;
             const int64_t part = prefix_part(a, split, rows_of[ct], head_of[ct]);
             if (g == 0) *(v2f*)(a.prefix.ml + 2 * part) = v2f{m[ct], l[ct]};
 #pragma unroll
@@ -394,7 +429,7 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * HD / 4; i += kPrefixThreads) {
             const int c = i / (HD / 4), d = (i - c * (HD / 4)) * 4;
-            const int64_t column = (int64_t)qb * P::COLS + c;
+            const int column = qb * P::COLS + c;
             if (column >= columns) continue;
             float mm = s_ml[0][c][0];
 #pragma unroll
@@ -408,19 +443,107 @@ __global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void paged_prefix_
                 ll += e * s_ml[w][c][1];
                 acc += e * *(const v4f*)((const float*)(lds + w * (32 * (HD + 4) * 4)) + c * (HD + 4) + d);
             }
-            const int row = (int)(column / rep);
-            const int64_t part = prefix_part(a, split, row, kvh * rep + (int)(column - (int64_t)row * rep));
+            const int row = (int)((unsigned)column / (unsigned)rep);
+            const int64_t part = prefix_part(a, split, row, kvh * rep + column - row * rep);
             if (d == 0) *(v2f*)(a.prefix.ml + 2 * part) = v2f{mm, ll};
             *(v4f*)(a.prefix.o + part * HD + d) = acc * sv;
         }
     }
 }
 
+template <int HD, int DT, int QP, int PP, int QW>
+__global__ __launch_bounds__(kPrefixThreads, QP == 3 ? 1 : 2) void shared_attention_kernel(PagedAttnArgs a, SharedRoles roles, int qblocks) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ float s_ml[4][32][2];
+    int at;
+    if (roles.is_own(blockIdx.x, at)) attention_run<HD, DT, QP == 3, true>(a, at, roles.own, *(AttnShared<HD, DT, QP == 3>*)lds);
+    else prefix_run<HD, DT, QP, PP, QW>(a, at, roles.prefix, qblocks, lds, s_ml);
+}
+
+// What the rows' own keys and the prefix left of a query head, joined: workgroup (row, head,
+// or several heads where there are few parts), `lanes` parts of a head side by side.
+template <int HD>
+__global__ __launch_bounds__(kPrefixThreads) void shared_join_kernel(PagedAttnArgs a, int own_workgroups, int lanes) {
+    constexpr int Q = HD / 4, W = kPrefixThreads / Q, AHEAD = 4;
+    __shared__ float s_acc[W][HD], s_l[W], s_m[W];
+    const PagedGeom& geo = a.c.g;
+    const int rep = a.n_heads / geo.n_kv, blocks = (rep + 7) >> 3;
+    const int q = threadIdx.x % Q, slot = threadIdx.x / Q, s = slot % lanes;
+    const int row = blockIdx.x, head = blockIdx.y * (W / lanes) + slot / lanes;
+    const int pos = a.row_pos[row];
+    if (paged_row_kind(geo, a.row_seq ? a.row_seq[row] : row, pos) != PAGED_ROW_OK) return;
+    const bool adds = shared_adds(a.prefix.len, pos);
+    const int tiles = shared_tiles(a.prefix.len, pos);
+    const PagedShare share = paged_share(a.prefix.starts[a.rows], own_workgroups);
+    const int kvh = min(head, a.n_heads - 1) / rep, h = min(head, a.n_heads - 1) - kvh * rep;
+    const int32_t unit = a.prefix.starts[row] + (kvh * blocks + (h >> 3)) * tiles;
+    const int w0 = share.owner(unit), w1 = share.owner(unit + tiles - 1);
+    // the prefix's parts, then the own keys': whole, of no keys none, or in parts
+    const int slots = adds ? a.prefix.splits + (w0 == w1 && pos + 1 > a.prefix.len) : 0;
+    const int parts = head < a.n_heads ? slots + (w0 == w1 ? 0 : w1 - w0 + 1) : 0;
+    float m = -__builtin_inff(), l = 0.0f;
+    v4f acc = {0, 0, 0, 0};
+    for (int p0 = s; p0 < parts; p0 += AHEAD * lanes) {
+        v2f ml[AHEAD];
+        v4f o[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const int p = min(p0 + j * lanes, parts - 1);
+            const float *from_o, *from_ml;
+            if (p < slots) {
+                const int64_t part = prefix_part(a, p, row, head);
+                from_o = a.prefix.o + part * HD;
+                from_ml = a.prefix.ml + 2 * part;
+            } else {
+                const int part = paged_part(share, w0 + p - slots, unit);
+                from_o = part_o<HD>(a, part) + (h & 7) * HD;
+                from_ml = part_ml<HD>(a, part, own_workgroups) + 2 * (h & 7);
+            }
+            o[j] = *(const v4f*)(from_o + 4 * q);
+            ml[j] = *(const v2f*)from_ml;
+            if (p0 + j * lanes >= parts) ml[j][0] = -__builtin_inff();
+        }
+        float mm = m;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) mm = fmaxf(mm, ml[j][0]);
+        const float off = mm == -__builtin_inff() ? 0.0f : mm;
+        const float keep = __builtin_amdgcn_exp2f(m - off);
+        m = mm;
+        l *= keep;
+        acc *= keep;
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            const float e = __builtin_amdgcn_exp2f(ml[j][0] - off);
+            l += e * ml[j][1];
+            acc += e * o[j];
+        }
+    }
+    *(v4f*)&s_acc[slot][4 * q] = acc;
+    if (q == 0) {
+        s_l[slot] = l;
+        s_m[slot] = m;
+    }
+    __syncthreads();
+    if (s != 0 || parts == 0) return;
+    float mm = m;
+    for (int i = 1; i < lanes; i++) mm = fmaxf(mm, s_m[slot + i]);
+    const float off = mm == -__builtin_inff() ? 0.0f : mm;
+    const float keep = __builtin_amdgcn_exp2f(m - off);
+    l *= keep;
+    acc *= keep;
+    for (int i = 1; i < lanes; i++) {
+        const float e = __builtin_amdgcn_exp2f(s_m[slot + i] - off);
+        l += e * s_l[slot + i];
+        acc += e * *(const v4f*)&s_acc[slot + i][4 * q];
+    }
+    store4(a.out, (int64_t)row * a.out_stride + (int64_t)head * HD + 4 * q, a.act, acc / l);
+}
+
 // Calls f(instance) with the instance for a's types: parts of q and of the probabilities
 template <int HD, int DT, int QP, int PP, int QW>
 struct Instance {
-    using P = Prefix<HD, DT, QP, PP, QW>;
-    static constexpr auto kernel = paged_prefix_kernel<HD, DT, QP, PP, QW>;
+    static constexpr auto kernel = shared_attention_kernel<HD, DT, QP, PP, QW>;
+    static constexpr int LDS = std::max<int>(Prefix<HD, DT, QP, PP, QW>::LDS, sizeof(AttnShared<HD, DT, QP == 3>));
 };
 template <int HD, int QW, typename F>
 hipError_t with_types(int dtype, int act, F f) {
@@ -437,13 +560,21 @@ hipError_t with_instance(int hd, int qw, int dtype, int act, F f) {
 
 }  // namespace
 
-hipError_t launch_paged_prefix(hipStream_t s, const PagedAttnArgs& a) {
+hipError_t launch_shared_attention(hipStream_t s, const PagedAttnArgs& a) {
     const PrefixPlan p = prefix_plan(a.rows, a.n_heads, a.c.g.n_kv, a.prefix.len);
-    return with_instance(a.c.g.head_dim, p.qw, a.c.dtype, a.act, [&](auto i) {
+    const SharedRoles roles{p.grid, paged_attention_workgroups(a.c, a.rows, a.n_heads)};
+    const hipError_t e = with_instance(a.c.g.head_dim, p.qw, a.c.dtype, a.act, [&](auto i) {
         using I = decltype(i);
-        TL_KLAUNCH(I::kernel, dim3(p.grid), dim3(kPrefixThreads), I::P::LDS, s, a, p.qblocks);
+        TL_KLAUNCH(I::kernel, dim3(roles.prefix + roles.own), dim3(kPrefixThreads), I::LDS, s, a, roles, p.qblocks);
         return hipGetLastError();
     });
+    if (e != hipSuccess) return e;
+    const int side = kPrefixThreads / (a.c.g.head_dim / 4);   // parts that a workgroup takes side by side
+    const int lanes = shared_join_lanes(side, p.splits, roles.own, (int64_t)a.rows * a.n_heads);
+    const dim3 grid(a.rows, (a.n_heads + side / lanes - 1) / (side / lanes));
+    if (a.c.g.head_dim == 64) TL_KLAUNCH((shared_join_kernel<64>), grid, dim3(kPrefixThreads), 0, s, a, roles.own, lanes);
+    else TL_KLAUNCH((shared_join_kernel<128>), grid, dim3(kPrefixThreads), 0, s, a, roles.own, lanes);
+    return hipGetLastError();
 }
 
 hipError_t init_prefix_kernels() {
@@ -455,7 +586,7 @@ hipError_t init_prefix_kernels() {
                     if (e == hipSuccess)
                         e = with_instance(hd, qw, dtype, act, [](auto i) {
                             using I = decltype(i);
-                            return hipFuncSetAttribute((const void*)I::kernel, hipFuncAttributeMaxDynamicSharedMemorySize, I::P::LDS);
+                            return hipFuncSetAttribute((const void*)I::kernel, hipFuncAttributeMaxDynamicSharedMemorySize, I::LDS);
                         });
     return e;
 }
@@ -465,7 +596,7 @@ size_t paged_shared_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, 
     const size_t own = paged_attention_scratch(c, rows, n_heads);
     if (len <= 0) return own;
     const PrefixPlan p = prefix_plan(rows, n_heads, c.g.n_kv, len);
-    return (own + 15) / 16 * 16 + (size_t)p.splits * rows * n_heads * (c.g.head_dim + 4) * sizeof(float);
+    return (own + 15) / 16 * 16 + ((size_t)(p.splits + 1) * rows * n_heads * (c.g.head_dim + 2) + rows + 1) * sizeof(float);
 }
 
 void paged_shared_places(PagedAttnArgs& a) {
@@ -473,7 +604,8 @@ void paged_shared_places(PagedAttnArgs& a) {
     const PrefixPlan p = prefix_plan(a.rows, a.n_heads, a.c.g.n_kv, a.prefix.len);
     a.prefix.splits = p.splits;
     a.prefix.o = (float*)((char*)a.scratch + (paged_attention_scratch(a.c, a.rows, a.n_heads) + 15) / 16 * 16);
-    a.prefix.ml = a.prefix.o + (int64_t)p.splits * a.rows * a.n_heads * a.c.g.head_dim;
+    a.prefix.ml = a.prefix.o + (int64_t)(p.splits + 1) * a.rows * a.n_heads * a.c.g.head_dim;
+    a.prefix.starts = (int32_t*)(a.prefix.ml + (int64_t)(p.splits + 1) * a.rows * a.n_heads * 2);
 }
 
 }  // namespace tl

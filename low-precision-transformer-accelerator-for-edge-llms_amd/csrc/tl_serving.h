@@ -118,6 +118,33 @@ inline PrefixPlan prefix_plan(int32_t rows, int32_t n_heads, int32_t n_kv, int32
     return p;
 }
 
+// Which workgroups of the kernel of a shared prefix take its keys and which the rows' own:
+// they take turns 256 at a time, one of each on every CU, as the ones multiply while the
+// others wait for memory; what is left of either kind follows.
+struct SharedRoles {
+    int32_t prefix, own;   // workgroups of each kind
+    TL_HD bool is_own(int32_t b, int32_t& at) const {
+        const int32_t k = (prefix < own ? prefix : own) >> 8;
+        if (b < k << 9) {
+            at = (b >> 9 << 8) + (b & 255);
+            return b >> 8 & 1;
+        }
+        at = b - (k << 8);
+        if (at < prefix) return false;
+        at = b - prefix;
+        return true;
+    }
+};
+
+// Parts of a query head that the join takes side by side, of the `side` that a workgroup can:
+// about four to each thread (the prefix's splits and what the own keys may be split into).
+inline int32_t shared_join_lanes(int32_t side, int32_t splits, int32_t own_workgroups, int64_t heads) {
+    const int64_t parts = splits + 1 + 8 * (int64_t)own_workgroups / (heads > 0 ? heads : 1);
+    int32_t lanes = 1;
+    while (lanes < side && 4 * lanes < parts) lanes *= 2;
+    return lanes;
+}
+
 // The joining kernel's workgroups.  Up to 64 rows it has one per row and head; more
 // rows than that each would have to be looked for, though only workgroups - 1 (row, head
 // block)s can be split, so there it has one per boundary and head of a block.
@@ -380,11 +407,13 @@ struct PagedAppendArgs {
 hipError_t launch_paged_append(hipStream_t s, const PagedAppendArgs& a);
 
 // The first `len` positions of sequence `seq`, shared by all rows (len 0: none), and what
-// the kernel over them leaves: O [splits][rows][n_heads][head_dim], m and l [...][2]
+// the kernel leaves to the join: O [splits + 1][rows][n_heads][head_dim], m and l [...][2],
+// and the first tile of each row's own keys [rows], then the number of all
 struct PagedPrefix {
     int32_t seq, len, splits;
     float* o;
     float* ml;
+    int32_t* starts;
 };
 
 struct PagedAttnArgs {
@@ -407,10 +436,10 @@ constexpr int32_t kOpCounters = 16384;
 int32_t paged_attention_workgroups(const PagedCache& c, int32_t rows, int32_t n_heads);
 size_t paged_attention_scratch(const PagedCache& c, int32_t rows, int32_t n_heads);
 hipError_t launch_paged_attention(hipStream_t s, const PagedAttnArgs& a);
-// with a shared prefix: scratch of both kernels, and its places from a.scratch
+// with a shared prefix (launch_paged_attention calls it): its scratch, and the places in it
 size_t paged_shared_scratch(const PagedCache& c, int32_t rows, int32_t n_heads, int32_t len);
 void paged_shared_places(PagedAttnArgs& a);
-hipError_t launch_paged_prefix(hipStream_t s, const PagedAttnArgs& a);
+hipError_t launch_shared_attention(hipStream_t s, const PagedAttnArgs& a);
 hipError_t init_prefix_kernels();
 
 // Projections with 4-bit weights.  Packed weights (launch_pack_w4) hold, for each

@@ -69,6 +69,25 @@ static void prefix(int rows, int heads, int n_kv, int len) {
     CHECK((int64_t)p.qblocks * 32 * p.qw >= columns && (int64_t)(p.qblocks - 1) * 32 * p.qw < columns);
     CHECK(p.splits >= 1 && p.splits <= len && (int64_t)p.grid == (int64_t)p.qblocks * n_kv * p.splits);
     CHECK((int64_t)p.grid * 256 < 1ll << 32);
+    // the workgroups of both kinds, each once
+    if (p.grid > 100000) return;
+    for (int own : {1, 7, 255, 256, 257, 512}) {
+        const SharedRoles roles{p.grid, own};
+        std::vector<char> seen(p.grid + own);
+        for (int b = 0; b < p.grid + own; b++) {
+            int at = -1;
+            const bool mine = roles.is_own(b, at);
+            CHECK(at >= 0 && at < (mine ? own : p.grid));
+            if (at < 0 || at >= (mine ? own : p.grid)) return;
+            CHECK(!seen[mine ? p.grid + at : at]);
+            seen[mine ? p.grid + at : at] = 1;
+        }
+    }
+    for (int side : {8, 16})
+        for (int own : {1, 512}) {
+            const int lanes = shared_join_lanes(side, p.splits, own, (int64_t)rows * heads);
+            CHECK(lanes >= 1 && lanes <= side && side % lanes == 0);
+        }
 }
 
 static void rows_behind(int len, int pos) {

@@ -363,7 +363,6 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
     p.tiles = W8Grid{(tiles + side - 1) / side, (mbs + side - 1) / side, 8};
     p.grid_x = p.tiles.n * p.tiles.m;
     p.grid_y = 1;
-    p.lds = (int64_t)2 * 2 * (2 * side) * 1024;
     return p;
 }
 

@@ -388,86 +388,146 @@ __global__ __launch_bounds__(kW8Threads, NT * MT > 8 ? 2 : 4) void w8_split_kern
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup has a tile of WN TN x WM TM blocks, both operands through LDS,
-// 128 columns at a time in two buffers; wavefront (wn, wm) multiplies TN x TM blocks.
+// Many rows: a workgroup has a tile of WN TN x WM TM blocks; wavefront (wn, wm) multiplies TN
+// x TM of them.  Both operands come into LDS by global -> LDS loads, a block of 64 columns
+// (a stage) at a time, kStages - 1 stages ahead in a ring.  Stage s + 1's operands are read
+// from LDS to registers while stage s is multiplied.  The ring's buffers are arrays of
+// their own, so that the compiler sees that a read does not wait for the loads into the
+// others, and the loop goes once around the ring.
 // ---------------------------------------------------------------------------
+typedef __attribute__((address_space(1))) const char W8Global;
+typedef __attribute__((address_space(3))) void W8Lds;
+constexpr int kStages = 4;
+
+// At most N of the wavefront's loads left, or all of its LDS reads done.  By the builtin,
+// which the compiler counts with: it adds no wait of its own for what this one covers.
+template <int N>
+TL_DEV void wait_loads() {
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
+TL_DEV void wait_reads() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+TL_DEV void meet() { asm volatile("s_barrier" ::: "memory"); }
+
 template <int WN, int WM, int TN, int TM, bool GLU>
-__global__ __launch_bounds__(64 * WN * WM) void w8_tile_kernel(W8Args a, W8Grid grid) {
+__global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Grid grid) {
     constexpr int NB = WN * TN, MB = WM * TM, WAVES = WN * WM;
-    constexpr int FR = (NB + MB) * 2, PW = FR / WAVES;   // blocks of a stage, of which a wavefront brings
-    static_assert(FR % WAVES == 0 && PW % 2 == 0, "whole pairs of blocks");
-    extern __shared__ __align__(16) char lds[];
+    constexpr int FR = NB + MB, PW = FR / WAVES;   // blocks of a stage, of which a wavefront brings
+    static_assert(FR % WAVES == 0, "whole blocks");
+    constexpr int ROW = TN * 64 + 16;              // bytes of a token's sums, on their way to y
+    static_assert(16 * ROW * ((WAVES + kStages - 1) / kStages) <= FR * 1024, "sums fit the ring");
+    __shared__ __align__(16) char ring0[FR * 1024], ring1[FR * 1024], ring2[FR * 1024], ring3[FR * 1024];
     const int lane = lane_id(), wave = wave_id(), wn = wave % WN, wm = wave / WN;
     const int blocks = w8_blocks(a.k), tiles = w8_tiles(a.n, a.glu), mbs = (a.m + 15) >> 4;
     int tn, tm;
     grid.tile(blockIdx.x, tn, tm);
     const int tile0 = tn * NB, mb0 = tm * MB;
 
-    const char* src[PW / 2];
+    const char* src[PW];
 #pragma unroll
-    for (int j = 0; j < PW / 2; j++) {
-        const int b = wave * (PW / 2) + j;
+    for (int j = 0; j < PW; j++) {
+        const int b = wave * PW + j;
         src[j] = (b < NB ? (const char*)a.packed + (int64_t)min(tile0 + b, tiles - 1) * blocks * 1024
                          : w8_rows_at(a) + (int64_t)min(mb0 + b - NB, mbs - 1) * blocks * 1024) + lane * 16;
     }
-    v4i r[PW];
-    auto fetch = [&]() {
+    auto bring = [&](char* ring) {
 #pragma unroll
-        for (int j = 0; j < PW / 2; j++) {
-            r[2 * j] = *(const v4i*)src[j];
-            r[2 * j + 1] = *(const v4i*)(src[j] + 1024);
-            src[j] += 2048;
+        for (int j = 0; j < PW; j++) {
+            __builtin_amdgcn_global_load_lds((W8Global*)src[j], (W8Lds*)(ring + (wave * PW + j) * 1024), 16, 0, 0);
+            src[j] += 1024;
         }
     };
-    auto keep = [&](int buf) {
-        char* to = lds + (buf * FR + wave * PW) * 1024 + lane * 16;
+    v4i wf[2][TN], xf[2][TM];
+    auto read = [&](int set, const char* ring) {
 #pragma unroll
-        for (int j = 0; j < PW; j++) *(v4i*)(to + j * 1024) = r[j];
+        for (int i = 0; i < TN; i++) wf[set][i] = *(const v4i*)(ring + (wn * TN + i) * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < TM; j++) xf[set][j] = *(const v4i*)(ring + (NB + wm * TM + j) * 1024 + lane * 16);
+        __builtin_amdgcn_sched_barrier(0);   // reads stay in front of the products that they are to hide behind
     };
     v4i acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; i++)
 #pragma unroll
         for (int j = 0; j < TM; j++) acc[i][j] = v4i{0, 0, 0, 0};
-    const int stages = blocks >> 1;
-    fetch();
-    keep(0);
-    __syncthreads();
-    for (int s = 0; s < stages; s++) {
-        if (s + 1 < stages) fetch();
-        const char* wl = lds + ((s & 1) * FR + wn * TN * 2) * 1024 + lane * 16;
-        const char* xl = lds + ((s & 1) * FR + (NB + wm * TM) * 2) * 1024 + lane * 16;
+    auto multiply = [&](int set) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            v4i wf[TN], xf[TM];
+        for (int i = 0; i < TN; i++)
 #pragma unroll
-            for (int i = 0; i < TN; i++) wf[i] = *(const v4i*)(wl + (2 * i + h) * 1024);
-#pragma unroll
-            for (int j = 0; j < TM; j++) xf[j] = *(const v4i*)(xl + (2 * j + h) * 1024);
-#pragma unroll
-            for (int i = 0; i < TN; i++)
-#pragma unroll
-                for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[set][i], xf[set][j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Stage s, whose operands are in registers: stage s + 1 has arrived when at most the loads
+    // of s + 2 and s + 3 are left; behind the barrier it is there for every wavefront, and
+    // every wavefront has stage s in registers, whose buffer takes s + 4.
+    auto stage = [&](int set, char* here, const char* next) {
+        wait_loads<2 * PW>();
+        wait_reads();
+        meet();
+        bring(here);
+        read(set ^ 1, next);
+        multiply(set);
+    };
+    // one of the last stages, `left` of them and it left
+    auto late = [&](int left, int set, char* here, const char* next) {
+        if (left <= 0) return;
+        if (left > 1) {
+            if (left > 3) wait_loads<2 * PW>();
+            else if (left > 2) wait_loads<PW>();
+            else wait_loads<0>();
+            wait_reads();
+            meet();
+            if (left > 4) bring(here);
+            read(set ^ 1, next);
         }
-        if (s + 1 < stages) keep((s + 1) & 1);
-        __syncthreads();
+        multiply(set);
+    };
+    bring(ring0);
+    bring(ring1);   // (blocks is even)
+    if (blocks > 2) {
+        bring(ring2);
+        bring(ring3);
+        wait_loads<3 * PW>();
+    } else {
+        wait_loads<PW>();
     }
-    const float* scales = w8_scales(a);
-    const int g = lane >> 4;
+    meet();
+    read(0, ring0);
+    int left = blocks;
+    for (; left >= 2 * kStages; left -= kStages) {
+        stage(0, ring0, ring1);
+        stage(1, ring1, ring2);
+        stage(0, ring2, ring3);
+        stage(1, ring3, ring0);
+    }
+    late(left, 0, ring0, ring1);
+    late(left - 1, 1, ring1, ring2);
+    late(left - 2, 0, ring2, ring3);
+    late(left - 3, 1, ring3, ring0);
+    late(left - 4, 0, ring0, ring1);
+    late(left - 5, 1, ring1, ring2);
+    // sums of 16 tokens at a time through this wavefront's part of the ring, a token's side by
+    // side, so that its results are written together
+    __syncthreads();
+    char* mine = (wave % kStages == 0 ? ring0 : wave % kStages == 1 ? ring1 : wave % kStages == 2 ? ring2 : ring3) + wave / kStages * 16 * ROW;
+    constexpr int Q = (GLU ? TN / 2 : TN) * 4, STEP = 64 / Q;   // fours of a token; tokens of a pass
+    const int q = lane % Q, t = tile0 + wn * TN + (q >> 2) * (GLU ? 2 : 1);
+    const float* scales = w8_scales(a) + min(t, tiles - 1 - GLU) * 16 + 4 * (q & 3);
+    const v4f sw = *(const v4f*)scales, su = *(const v4f*)(scales + (GLU ? 16 : 0));
+    const int n = (GLU ? t >> 1 : t) * 16 + 4 * (q & 3);
 #pragma unroll
     for (int j = 0; j < TM; j++) {
-        const int m = (mb0 + wm * TM + j) * 16 + (lane & 15);
-        if (m >= a.m) continue;
-        const float sx = w8_row_scales(a)[m];
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int i = 0; i < TN; i += GLU ? 2 : 1) {
-            const int t = tile0 + wn * TN + i;
-            if (t >= tiles) break;
-            const float* sw = scales + t * 16 + 4 * g;
-            if constexpr (GLU)
-                w8_put(a, m, (t >> 1) * 16 + 4 * g, w8_glu(acc[i][j], acc[i + 1][j], *(const v4f*)sw, *(const v4f*)(sw + 16), sx));
-            else
-                w8_put(a, m, t * 16 + 4 * g, w8_scaled(acc[i][j], *(const v4f*)sw, sx));
+        for (int i = 0; i < TN; i++) *(v4i*)(mine + (lane & 15) * ROW + i * 64 + (lane >> 4) * 16) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+        const int m0 = (mb0 + wm * TM + j) * 16;
+#pragma unroll 1
+        for (int r = lane / Q; r < 16; r += STEP) {
+            if (m0 + r >= a.m || t >= tiles) continue;
+            const float sx = w8_row_scales(a)[m0 + r];
+            const char* from = mine + r * ROW + (q >> 2) * (GLU ? 128 : 64) + (q & 3) * 16;
+            if constexpr (GLU) w8_put(a, m0 + r, n, w8_glu(*(const v4i*)from, *(const v4i*)(from + 64), sw, su, sx));
+            else w8_put(a, m0 + r, n, w8_scaled(*(const v4i*)from, sw, sx));
         }
     }
 }
@@ -529,11 +589,11 @@ hipError_t launch_linear_w8(hipStream_t s, const W8Args& args) {
         return hipGetLastError();
     }
     if (p.kind == W8_TILE128) {
-        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, true>), grid, dim3(256), p.lds, s, a, p.tiles);
-        else TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, false>), grid, dim3(256), p.lds, s, a, p.tiles);
+        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, true>), grid, dim3(256), 0, s, a, p.tiles);
+        else TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, false>), grid, dim3(256), 0, s, a, p.tiles);
     } else {
-        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, true>), grid, block, p.lds, s, a, p.tiles);
-        else TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, false>), grid, block, p.lds, s, a, p.tiles);
+        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, true>), grid, block, 0, s, a, p.tiles);
+        else TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, false>), grid, block, 0, s, a, p.tiles);
     }
     return hipGetLastError();
 }
@@ -548,9 +608,7 @@ hipError_t launch_pack_w8(hipStream_t s, const int8_t* q, const float* scales, c
 
 hipError_t init_w8_kernels() {
     hipError_t e = hipSuccess;
-    for (const void* f : {(const void*)w8_row_kernel<false>, (const void*)w8_row_kernel<true>,
-                          (const void*)w8_tile_kernel<2, 2, 4, 4, false>, (const void*)w8_tile_kernel<2, 2, 4, 4, true>,
-                          (const void*)w8_tile_kernel<2, 4, 8, 4, false>, (const void*)w8_tile_kernel<2, 4, 8, 4, true>})
+    for (const void* f : {(const void*)w8_row_kernel<false>, (const void*)w8_row_kernel<true>})
         if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kW8Lds);
     return e;
 }

@@ -414,13 +414,15 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
     constexpr int FR = NB + MB, PW = FR / WAVES;   // blocks of a stage, of which a wavefront brings
     static_assert(FR % WAVES == 0, "whole blocks");
     constexpr int ROW = TN * 64 + 16;              // bytes of a token's sums, on their way to y
-    static_assert(16 * ROW * ((WAVES + kStages - 1) / kStages) <= FR * 1024, "sums fit the ring");
+    static_assert((16 * ROW + TM * 64) * ((WAVES + kStages - 1) / kStages) <= FR * 1024, "sums and scales fit the ring");
     __shared__ __align__(16) char ring0[FR * 1024], ring1[FR * 1024], ring2[FR * 1024], ring3[FR * 1024];
     const int lane = lane_id(), wave = wave_id(), wn = wave % WN, wm = wave / WN;
     const int blocks = w8_blocks(a.k), tiles = w8_tiles(a.n, a.glu), mbs = (a.m + 15) >> 4;
     int tn, tm;
     grid.tile(blockIdx.x, tn, tm);
     const int tile0 = tn * NB, mb0 = tm * MB;
+    static_assert(TM <= 4, "a scale to each lane");
+    const float my_scale = w8_row_scales(a)[min((mb0 + wm * TM) * 16 + min(lane, TM * 16 - 1), a.m - 1)];
 
     const char* src[PW];
 #pragma unroll
@@ -442,7 +444,6 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
         for (int i = 0; i < TN; i++) wf[set][i] = *(const v4i*)(ring + (wn * TN + i) * 1024 + lane * 16);
 #pragma unroll
         for (int j = 0; j < TM; j++) xf[set][j] = *(const v4i*)(ring + (NB + wm * TM + j) * 1024 + lane * 16);
-        __builtin_amdgcn_sched_barrier(0);   // reads stay in front of the products that they are to hide behind
     };
     v4i acc[TN][TM];
 #pragma unroll
@@ -454,7 +455,6 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
         for (int i = 0; i < TN; i++)
 #pragma unroll
             for (int j = 0; j < TM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[set][i], xf[set][j], acc[i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
     };
     // Stage s, whose operands are in registers: stage s + 1 has arrived when at most the loads
     // of s + 2 and s + 3 are left; behind the barrier it is there for every wavefront, and
@@ -463,9 +463,21 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
         wait_loads<2 * PW>();
         wait_reads();
         meet();
-        bring(here);
+        __builtin_amdgcn_sched_barrier(0);
         read(set ^ 1, next);
+        bring(here);
         multiply(set);
+        // LDS takes 8 cycles or more for a read and 8 wavefronts ask at once: the reads are
+        // spread between the products, or these would wait until all are taken
+        constexpr int READS = TN + TM, EACH = TN * TM / READS;
+#pragma unroll
+        for (int i = 0; i < READS; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            if (i < PW) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, TN * TM - EACH * READS, 0);
+        __builtin_amdgcn_sched_barrier(0);
     };
     // one of the last stages, `left` of them and it left
     auto late = [&](int left, int set, char* here, const char* next) {
@@ -508,12 +520,14 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
     // sums of 16 tokens at a time through this wavefront's part of the ring, a token's side by
     // side, so that its results are written together
     __syncthreads();
-    char* mine = (wave % kStages == 0 ? ring0 : wave % kStages == 1 ? ring1 : wave % kStages == 2 ? ring2 : ring3) + wave / kStages * 16 * ROW;
+    char* mine = (wave % kStages == 0 ? ring0 : wave % kStages == 1 ? ring1 : wave % kStages == 2 ? ring2 : ring3) + wave / kStages * (16 * ROW + TM * 64);
     constexpr int Q = (GLU ? TN / 2 : TN) * 4, STEP = 64 / Q;   // fours of a token; tokens of a pass
     const int q = lane % Q, t = tile0 + wn * TN + (q >> 2) * (GLU ? 2 : 1);
     const float* scales = w8_scales(a) + min(t, tiles - 1 - GLU) * 16 + 4 * (q & 3);
     const v4f sw = *(const v4f*)scales, su = *(const v4f*)(scales + (GLU ? 16 : 0));
     const int n = (GLU ? t >> 1 : t) * 16 + 4 * (q & 3);
+    float* row_scales = (float*)(mine + 16 * ROW);
+    if (lane < TM * 16) row_scales[lane] = my_scale;
 #pragma unroll
     for (int j = 0; j < TM; j++) {
         __builtin_amdgcn_wave_barrier();
@@ -521,10 +535,10 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
         for (int i = 0; i < TN; i++) *(v4i*)(mine + (lane & 15) * ROW + i * 64 + (lane >> 4) * 16) = acc[i][j];
         __builtin_amdgcn_wave_barrier();
         const int m0 = (mb0 + wm * TM + j) * 16;
-#pragma unroll 1
+#pragma unroll 2
         for (int r = lane / Q; r < 16; r += STEP) {
             if (m0 + r >= a.m || t >= tiles) continue;
-            const float sx = w8_row_scales(a)[m0 + r];
+            const float sx = row_scales[j * 16 + r];
             const char* from = mine + r * ROW + (q >> 2) * (GLU ? 128 : 64) + (q & 3) * 16;
             if constexpr (GLU) w8_put(a, m0 + r, n, w8_glu(*(const v4i*)from, *(const v4i*)(from + 64), sw, su, sx));
             else w8_put(a, m0 + r, n, w8_scaled(*(const v4i*)from, sw, sx));

@@ -293,6 +293,7 @@ constexpr int32_t kW8Waves = 8, kW8Threads = 64 * kW8Waves;
 constexpr int32_t kW8MaxK = 1 << 17;     // 127 * 128 * 2^17 is below 2^31
 constexpr int64_t kW8Lds = 152 * 1024;   // of a workgroup's 160 KiB
 constexpr int32_t kW8Slots = 8;          // units of 8 columns of x that a thread keeps in registers
+constexpr int32_t kW8Keep = 4;           // and where x is quantized by a kernel of its own
 
 TL_HD inline int32_t w8_blocks(int32_t k) { return (k + 127) / 128 * 2; }
 TL_HD inline int32_t w8_tiles(int32_t n, bool glu) { return (n + 15) / 16 * (glu ? 2 : 1); }
@@ -322,7 +323,10 @@ struct W8Grid {
     }
 };
 
-enum W8Kind : int32_t { W8_ROW = 0, W8_SPLIT = 1, W8_TILE128 = 2, W8_TILE256 = 3 };
+enum W8Kind : int32_t { W8_ROW = 0, W8_SPLIT = 1, W8_TILE = 2 };
+// Tiles of 16 weight rows by tiles of 16 tokens of a workgroup of the tiled form
+enum W8Shape : int32_t { W8_8x8 = 0, W8_14x16, W8_16x14, W8_16x16, W8_SHAPES };
+constexpr int32_t kW8Sides[W8_SHAPES][2] = {{8, 8}, {14, 16}, {16, 14}, {16, 16}};
 struct W8Plan {
     W8Kind kind;
     int32_t split;         // W8_ROW: wavefronts that share a tile of weights
@@ -330,7 +334,8 @@ struct W8Plan {
     int32_t quant_waves;   // wavefronts that quantize a row of x: 1, 2, 4 or 8
     int32_t grid_x, grid_y;
     int64_t lds;
-    W8Grid tiles;          // W8_TILE*
+    W8Shape shape;         // W8_TILE
+    W8Grid tiles;
 };
 
 inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
@@ -347,20 +352,45 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
         p.lds = (int64_t)w8_blocks(k) * 64 * m + kW8Waves * (glu ? 2 : 1) * 64 * m;
         return p;
     }
+    // wavefronts to a row of x, as few as hold it in registers while there are rows enough
     p.quant_waves = 8;
-    while (p.quant_waves > 1 && (int64_t)m * p.quant_waves > 4096) p.quant_waves /= 2;
-    if (m <= 256) {
+    while (p.quant_waves > 1 && (int64_t)m * p.quant_waves > 4096 && w8_blocks(k) * 8 <= kW8Keep * 64 * (p.quant_waves / 2))
+        p.quant_waves /= 2;
+    // Without LDS (tiles of nt by mt, K split over a workgroup) while 64 x 64 tiles are at most
+    // 400: 128 rows by 5632 x 2048 take 11.4 us, in the tiled form 18.2, 256 rows 17.6 and 18.9,
+    // 512 rows by 2048 x 5632 20.7 and 33.9; but 384 rows by 5632 x 2048 (528 tiles) 23.8 and
+    // 20.3, 128 rows by 14336 x 4096 (448) 29.9 and 25.8.
+    auto wgs = [&](int32_t nt, int32_t mt) { return (int64_t)((tiles + nt - 1) / nt) * ((mbs + mt - 1) / mt); };
+    if (wgs(4, 4) <= 400) {
         p.kind = W8_SPLIT;
-        p.mt = mbs == 1 ? 1 : mbs == 2 ? 2 : 4;
+        // A 4 x 4 workgroup takes as long as 3.5 of the others, and fewer than 200 no less: 32
+        // rows by 14336 x 4096 take 15.5 us as 2 x 2, 22.1 as 2 x 1; 48 rows 22.7 as 2 x 2, 18.5
+        // as 4 x 4; 128 rows by 2048 x 5632 13.5, 12.2, 16.3; 64 by 5632 x 2048 10.7, 10.4, 11.0.
+        const int64_t one = wgs(2, 1), two = wgs(2, 2), w4 = wgs(4, 4), four = (w4 > 200 ? w4 : 200) * 7 / 2;
+        p.mt = one <= two && one <= four ? 1 : two <= four ? 2 : 4;
         p.nt = p.mt == 4 ? 4 : 2;
         p.grid_x = (tiles + p.nt - 1) / p.nt;
         p.grid_y = (mbs + p.mt - 1) / p.mt;
         return p;
     }
-    const int64_t big = (int64_t)((tiles + 15) / 16) * ((mbs + 15) / 16);
-    const int32_t side = big >= 192 ? 16 : 8;
-    p.kind = side == 16 ? W8_TILE256 : W8_TILE128;
-    p.tiles = W8Grid{(tiles + side - 1) / side, (mbs + side - 1) / side, 8};
+    // The shape with the least work on the busiest CU, in units of a product of two tiles: a
+    // 16 x 16 workgroup at a time on each of 256 CUs, of 8 x 8 two, which read a quarter more
+    // for their products (8192^3: 472 us, 589; 1024 rows by 4096 x 4096, 64 workgroups or 256:
+    // 53, 33).  One side of 14 where that saves a round (2001 rows of 14336 x 4096 pairs: 227
+    // us, 241).
+    p.kind = W8_TILE;
+    int64_t best = INT64_MAX;
+    for (int32_t i = W8_SHAPES - 1; i >= 0; i--) {
+        const int32_t sn = kW8Sides[i][0], sm = kW8Sides[i][1];
+        if (glu && i == W8_14x16) continue;   // a wavefront has 7 tiles of weights there: no pairs
+        const int32_t at_once = i == W8_8x8 ? 512 : 256, weight = i == W8_8x8 ? 250 : i == W8_16x16 ? 100 : 106;
+        const int64_t all = (int64_t)((tiles + sn - 1) / sn) * ((mbs + sm - 1) / sm);
+        const int64_t cost = (all + at_once - 1) / at_once * sn * sm * weight;
+        if (cost >= best) continue;
+        best = cost;
+        p.shape = (W8Shape)i;
+        p.tiles = W8Grid{(tiles + sn - 1) / sn, (mbs + sm - 1) / sm, 8};
+    }
     p.grid_x = p.tiles.n * p.tiles.m;
     p.grid_y = 1;
     return p;

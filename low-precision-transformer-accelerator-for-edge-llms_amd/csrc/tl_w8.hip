@@ -136,22 +136,20 @@ TL_DEV v4f w8_glu(v4i gate, v4i up, v4f sg, v4f su, float sx) {
 // ---------------------------------------------------------------------------
 // Rows of x to INT8 blocks and scales in scratch, `waves` wavefronts to a row.
 // ---------------------------------------------------------------------------
-constexpr int kQuantKeep = 4;   // units of a row that a thread keeps between its two passes
-
 __global__ __launch_bounds__(kW8Threads) void w8_quantize_kernel(W8Args a, int waves) {
     __shared__ unsigned s_most[kW8Waves];
     const int wave = wave_id(), part = wave % waves;
     const int row = blockIdx.x * (kW8Waves / waves) + wave / waves;
     const int blocks = w8_blocks(a.k), units = blocks * 8, step = 64 * waves;
     const bool in = row < a.m;
-    Unit x[kQuantKeep];
+    Unit x[kW8Keep];
     unsigned most = 0;
     if (in) {
 #pragma unroll
-        for (int j = 0; j < kQuantKeep; j++) x[j].load(a, row, part * 64 + lane_id() + j * step);
+        for (int j = 0; j < kW8Keep; j++) x[j].load(a, row, part * 64 + lane_id() + j * step);
 #pragma unroll
-        for (int j = 0; j < kQuantKeep; j++) most = max(most, x[j].most(a.act));
-        for (int u = part * 64 + lane_id() + kQuantKeep * step; u < units; u += step) {
+        for (int j = 0; j < kW8Keep; j++) most = max(most, x[j].most(a.act));
+        for (int u = part * 64 + lane_id() + kW8Keep * step; u < units; u += step) {
             Unit y;
             y.load(a, row, u);
             most = max(most, y.most(a.act));
@@ -175,8 +173,8 @@ __global__ __launch_bounds__(kW8Threads) void w8_quantize_kernel(W8Args a, int w
             *(v2i*)(to + (int64_t)(u >> 3) * 1024 + (u >> 1 & 3) * 256 + (u & 1) * 8) = finite ? y.quantized(a.act, d) : v2i{0, 0};
     };
 #pragma unroll
-    for (int j = 0; j < kQuantKeep; j++) put(x[j], part * 64 + lane_id() + j * step);
-    for (int u = part * 64 + lane_id() + kQuantKeep * step; u < units; u += step) {
+    for (int j = 0; j < kW8Keep; j++) put(x[j], part * 64 + lane_id() + j * step);
+    for (int u = part * 64 + lane_id() + kW8Keep * step; u < units; u += step) {
         Unit y;
         y.load(a, row, u);
         put(y, u);
@@ -411,8 +409,7 @@ TL_DEV void meet() { asm volatile("s_barrier" ::: "memory"); }
 template <int WN, int WM, int TN, int TM, bool GLU>
 __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Grid grid) {
     constexpr int NB = WN * TN, MB = WM * TM, WAVES = WN * WM;
-    constexpr int FR = NB + MB, PW = FR / WAVES;   // blocks of a stage, of which a wavefront brings
-    static_assert(FR % WAVES == 0, "whole blocks");
+    constexpr int PW = (NB + MB + WAVES - 1) / WAVES, FR = PW * WAVES;   // blocks of a stage (NB + MB in use), a wavefront's
     constexpr int ROW = TN * 64 + 16;              // bytes of a token's sums, on their way to y
     static_assert((16 * ROW + TM * 64) * ((WAVES + kStages - 1) / kStages) <= FR * 1024, "sums and scales fit the ring");
     __shared__ __align__(16) char ring0[FR * 1024], ring1[FR * 1024], ring2[FR * 1024], ring3[FR * 1024];
@@ -421,13 +418,15 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
     int tn, tm;
     grid.tile(blockIdx.x, tn, tm);
     const int tile0 = tn * NB, mb0 = tm * MB;
-    static_assert(TM <= 4, "a scale to each lane");
-    const float my_scale = w8_row_scales(a)[min((mb0 + wm * TM) * 16 + min(lane, TM * 16 - 1), a.m - 1)];
+    constexpr int SL = (TM * 16 + 63) / 64;        // scales of this wavefront's tokens, in each lane
+    float my_scale[SL];
+#pragma unroll
+    for (int i = 0; i < SL; i++) my_scale[i] = w8_row_scales(a)[min((mb0 + wm * TM) * 16 + 64 * i + lane, a.m - 1)];
 
     const char* src[PW];
 #pragma unroll
     for (int j = 0; j < PW; j++) {
-        const int b = wave * PW + j;
+        const int b = min(wave * PW + j, NB + MB - 1);
         src[j] = (b < NB ? (const char*)a.packed + (int64_t)min(tile0 + b, tiles - 1) * blocks * 1024
                          : w8_rows_at(a) + (int64_t)min(mb0 + b - NB, mbs - 1) * blocks * 1024) + lane * 16;
     }
@@ -527,7 +526,9 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
     const v4f sw = *(const v4f*)scales, su = *(const v4f*)(scales + (GLU ? 16 : 0));
     const int n = (GLU ? t >> 1 : t) * 16 + 4 * (q & 3);
     float* row_scales = (float*)(mine + 16 * ROW);
-    if (lane < TM * 16) row_scales[lane] = my_scale;
+#pragma unroll
+    for (int i = 0; i < SL; i++)
+        if (64 * i + lane < TM * 16) row_scales[64 * i + lane] = my_scale[i];
 #pragma unroll
     for (int j = 0; j < TM; j++) {
         __builtin_amdgcn_wave_barrier();
@@ -602,12 +603,23 @@ hipError_t launch_linear_w8(hipStream_t s, const W8Args& args) {
         else go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
         return hipGetLastError();
     }
-    if (p.kind == W8_TILE128) {
-        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, true>), grid, dim3(256), 0, s, a, p.tiles);
-        else TL_KLAUNCH((w8_tile_kernel<2, 2, 4, 4, false>), grid, dim3(256), 0, s, a, p.tiles);
-    } else {
-        if (a.glu) TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, true>), grid, block, 0, s, a, p.tiles);
-        else TL_KLAUNCH((w8_tile_kernel<2, 4, 8, 4, false>), grid, block, 0, s, a, p.tiles);
+    auto tile = [&](auto wn, auto wm, auto tn, auto tm) {
+        constexpr int WN = decltype(wn)::value, WM = decltype(wm)::value, TN = decltype(tn)::value, TM = decltype(tm)::value;
+        if constexpr (TN % 2 == 0) {
+            if (a.glu) {
+                TL_KLAUNCH((w8_tile_kernel<WN, WM, TN, TM, true>), grid, dim3(64 * WN * WM), 0, s, a, p.tiles);
+                return;
+            }
+        }
+        TL_KLAUNCH((w8_tile_kernel<WN, WM, TN, TM, false>), grid, dim3(64 * WN * WM), 0, s, a, p.tiles);
+    };
+    integral_constant<int, 2> two;
+    integral_constant<int, 4> four;
+    switch (p.shape) {
+        case W8_8x8: tile(two, two, four, four); break;
+        case W8_14x16: tile(two, four, integral_constant<int, 7>{}, four); break;
+        case W8_16x14: tile(four, two, four, integral_constant<int, 7>{}); break;
+        default: tile(two, four, integral_constant<int, 8>{}, four); break;
     }
     return hipGetLastError();
 }

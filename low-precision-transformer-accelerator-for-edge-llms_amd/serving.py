@@ -453,7 +453,9 @@ class _W8:
             return out
         need = self._scratch_bytes(rows)
         rt, stream = self.rt, _stream(dev)
-        scratch, _, keep = _workspace(dev, stream, need)
+        scratch = keep = None
+        if need:
+            scratch, _, keep = _workspace(dev, stream, need)
         st = rt.lib.tl_linear_w8_async(
             rt.h, stream, x.data_ptr(), _stride(x), _ACT[x.dtype], rows, self.packed.data_ptr(), int(self.gated), self.n,
             self.k, None if residual is None else residual.data_ptr(), 0 if residual is None else _stride(residual),

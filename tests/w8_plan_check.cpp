@@ -15,7 +15,7 @@ static int wrong;
         if (!(c) && ++wrong < 20) std::printf("line %d, m %d n %d k %d glu %d: %s\n", __LINE__, m, n, k, glu, #c); \
     } while (0)
 
-static int kinds[8];
+static int kinds[8], shapes_seen[W8_SHAPES];
 
 static void one(int m, int n, int k, bool glu) {
     const W8Plan p = w8_plan(m, n, k, glu);
@@ -46,8 +46,12 @@ static void one(int m, int n, int k, bool glu) {
         CHECK(p.nt * p.mt * 1024 <= 65536);
         return;
     }
-    const int side_n = p.tiles.n ? (tiles + p.tiles.n - 1) / p.tiles.n : 0;
-    CHECK(side_n >= 1 && (int64_t)p.grid_x == (int64_t)p.tiles.n * p.tiles.m);
+    const int sn = kW8Sides[p.shape][0], sm = kW8Sides[p.shape][1];
+    CHECK((int64_t)p.tiles.n * sn >= tiles && (int64_t)(p.tiles.n - 1) * sn < tiles);
+    CHECK((int64_t)p.tiles.m * sm >= mbs && (int64_t)(p.tiles.m - 1) * sm < mbs);
+    CHECK(!glu || p.shape != W8_14x16);
+    shapes_seen[p.shape]++;
+    CHECK((int64_t)p.grid_x == (int64_t)p.tiles.n * p.tiles.m);
     CHECK((int64_t)p.grid_x * 512 < 1ll << 32);
     if (p.grid_x > 3000000) return;
     std::vector<char> seen(p.grid_x);
@@ -116,7 +120,8 @@ int main() {
             for (int glu = 0; glu < 2; glu++)
                 if ((int64_t)m * s[0] < 1ll << 38) one(m, s[0], s[1], glu);
     const int m = 0, n = 0, k = 0, glu = 0;
-    for (int kind = W8_ROW; kind <= W8_TILE256; kind++) CHECK(kinds[kind] > 5);
+    for (int kind = W8_ROW; kind <= W8_TILE; kind++) CHECK(kinds[kind] > 5);
+    for (int shape = 0; shape < W8_SHAPES; shape++) CHECK(shapes_seen[shape] > 0);
     const int heads[][2] = {{32, 4}, {8, 8}, {5, 1}, {40, 8}, {1, 1}, {128, 1}, {1024, 1024}};
     for (auto& h : heads)
         for (int r : {1, 2, 3, 8, 16, 17, 33, 64, 257, 4096, 1 << 20})

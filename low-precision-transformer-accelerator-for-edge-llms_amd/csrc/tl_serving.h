@@ -292,7 +292,7 @@ inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {
 constexpr int32_t kW8Waves = 8, kW8Threads = 64 * kW8Waves;
 constexpr int32_t kW8MaxK = 1 << 17;     // 127 * 128 * 2^17 is below 2^31
 constexpr int64_t kW8Lds = 152 * 1024;   // of a workgroup's 160 KiB
-constexpr int32_t kW8Slots = 8;          // units of 8 columns of x that a thread keeps in registers
+constexpr int32_t kW8Slots = 4;          // units of 8 columns of x that a thread keeps in registers
 constexpr int32_t kW8Keep = 4;           // and where x is quantized by a kernel of its own
 
 TL_HD inline int32_t w8_blocks(int32_t k) { return (k + 127) / 128 * 2; }
@@ -344,8 +344,13 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
     if (w8_in_rows(m, k)) {
         p.kind = W8_ROW;
         const int32_t units = (n + 15) / 16;
+        // Wavefronts to a tile: enough for four on each CU, and for eight where each still has 8
+        // blocks (one row by 14336 x 4096: 448 workgroups 12.6 us in a graph, 224 13.4; by 32000 x
+        // 2048 13.0, 14.5; but by 5632 x 2048, with 4 blocks each, 7.2, and 6.3 with 8).
         p.split = 1;
-        while (p.split < kW8Waves && (int64_t)units * p.split < 2048) p.split *= 2;
+        while (p.split < kW8Waves && ((int64_t)units * p.split < 1024 ||
+                                      ((int64_t)units * p.split < 2048 && w8_blocks(k) >= 16 * p.split)))
+            p.split *= 2;
         const int32_t per = kW8Waves / p.split;
         p.grid_x = (units + per - 1) / per;
         p.grid_y = 1;

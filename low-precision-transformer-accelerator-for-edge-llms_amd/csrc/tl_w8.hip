@@ -100,20 +100,30 @@ TL_DEV float glu(float g, float u) {
     return __fdiv_rn(g >= 0.0f ? g : g * t, 1.0f + t) * u;
 }
 
-// four neighbours of a row of y from column n on
-TL_DEV void w8_put(const W8Args& a, int64_t m, int n, v4f v) {
+// four neighbours of a row of the residual from column n on, zeros behind the last column
+TL_DEV v4f w8_residual(const W8Args& a, int64_t m, int n) {
+    const int64_t at = m * a.res_stride + n;
+    if (a.y_aligned && n + 4 <= a.n) return load4(a.residual, at, a.act);
+    v4f v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (n + i < a.n) v[i] = load1(a.residual, at + i, a.act);
+    return v;
+}
+// and of y
+TL_DEV void w8_store(const W8Args& a, int64_t m, int n, v4f v) {
     const int64_t at = m * a.y_stride + n;
     if (a.y_aligned && n + 4 <= a.n) {
-        if (a.residual) v += load4(a.residual, m * a.res_stride + n, a.act);
         store4(a.y, at, a.act, v);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (n + i < a.n) {
-            const float r = a.residual ? load1(a.residual, m * a.res_stride + n + i, a.act) : 0.0f;
-            store1(a.y, at + i, a.act, a.residual ? v[i] + r : v[i]);
-        }
+        if (n + i < a.n) store1(a.y, at + i, a.act, v[i]);
+}
+TL_DEV void w8_put(const W8Args& a, int64_t m, int n, v4f v) {
+    if (a.residual) v += w8_residual(a, m, n);
+    w8_store(a, m, n, v);
 }
 
 // results of 4 rows of a weight tile (from row 4 g of it) for token m: sums to y
@@ -136,7 +146,9 @@ TL_DEV v4f w8_glu(v4i gate, v4i up, v4f sg, v4f su, float sx) {
 // ---------------------------------------------------------------------------
 // Rows of x to INT8 blocks and scales in scratch, `waves` wavefronts to a row.
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(kW8Threads) void w8_quantize_kernel(W8Args a, int waves) {
+template <int ACT>
+__global__ __launch_bounds__(kW8Threads, 8) void w8_quantize_kernel(W8Args a, int waves) {
+    a.act = ACT;
     __shared__ unsigned s_most[kW8Waves];
     const int wave = wave_id(), part = wave % waves;
     const int row = blockIdx.x * (kW8Waves / waves) + wave / waves;
@@ -182,7 +194,11 @@ __global__ __launch_bounds__(kW8Threads) void w8_quantize_kernel(W8Args a, int w
 }
 
 // ---------------------------------------------------------------------------
-// Up to four rows: every workgroup quantizes them itself, into LDS.
+// Up to four rows whose columns its registers hold: every workgroup quantizes them itself,
+// into LDS.  Rows, first weights, scales and residual are asked for together; what bounds
+// it is that chain (load, maximum, quotients, products, sums: one row by 2048 x 5632 7.3 us in a
+// graph, by 5632 x 2048 6.3, the gated pair 8.6) and then the weights (14336 x 4096: 12.6
+// us, 4.7 TB/s; the pair 22.1, 5.3 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kRowAhead = 8;   // weight blocks in flight per wavefront
 
@@ -216,6 +232,17 @@ __global__ __launch_bounds__(kW8Threads, 4) void w8_row_kernel(W8Args a, int spl
     for (int j = 0; j < AHEAD; j++)
 #pragma unroll
         for (int s = 0; s < S; s++) wf[j][s] = __builtin_nontemporal_load((const v4i*)(w[s] + (int64_t)min(j, last) * split * 1024));
+
+    // what this thread finishes: four columns of y of a token
+    static_assert(kW8Waves * 4 * 4 <= kW8Threads, "one item to a thread");
+    const int fr = (int)threadIdx.x / (per * 4), fq = (int)threadIdx.x - fr * (per * 4), ft = blockIdx.x * per + (fq >> 2);
+    const bool finishes = fr < m && ft < tiles;
+    v4f sw[S], res = {0, 0, 0, 0};
+    if (finishes) {
+#pragma unroll
+        for (int s = 0; s < S; s++) sw[s] = *(const v4f*)(w8_scales(a) + (ft * S + s) * 16 + 4 * (fq & 3));
+        if (a.residual) res = w8_residual(a, fr, ft * 16 + 4 * (fq & 3));
+    }
 
     unsigned most[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -277,27 +304,23 @@ __global__ __launch_bounds__(kW8Threads, 4) void w8_row_kernel(W8Args a, int spl
 #pragma unroll
         for (int s = 0; s < S; s++) *(v4i*)(red + (((wave * S + s) * 4 + g) * m + col) * 16) = acc[s];
     __syncthreads();
-    const float* scales = w8_scales(a);
-    for (int i = threadIdx.x; i < per * 4 * m; i += kW8Threads) {
-        const int r = i / (per * 4), q = i - r * (per * 4);   // token, four columns of y
-        const int t = blockIdx.x * per + (q >> 2);
-        if (t >= tiles) continue;
-        v4i sum[S];
-        v4f sw[S];
+    if (!finishes) return;
+    v4i sum[S];
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            sum[s] = v4i{0, 0, 0, 0};
-            for (int p = 0; p < split; p++)
-                sum[s] += *(const v4i*)(red + (((((q >> 2) * split + p) * S + s) * 4 + (q & 3)) * m + r) * 16);
-            sw[s] = *(const v4f*)(scales + (t * S + s) * 16 + 4 * (q & 3));
-        }
-        unsigned mr = most[0];
-#pragma unroll
-        for (int j = 1; j < 4; j++) mr = j == r ? most[j] : mr;
-        const float sx = row_scale(mr);
-        if constexpr (GLU) w8_put(a, r, t * 16 + 4 * (q & 3), w8_glu(sum[0], sum[1], sw[0], sw[1], sx));
-        else w8_put(a, r, t * 16 + 4 * (q & 3), w8_scaled(sum[0], sw[0], sx));
+    for (int s = 0; s < S; s++) {
+        sum[s] = v4i{0, 0, 0, 0};
+        for (int p = 0; p < split; p++)
+            sum[s] += *(const v4i*)(red + (((((fq >> 2) * split + p) * S + s) * 4 + (fq & 3)) * m + fr) * 16);
     }
+    unsigned mr = most[0];
+#pragma unroll
+    for (int j = 1; j < 4; j++) mr = j == fr ? most[j] : mr;
+    const float sx = row_scale(mr);
+    v4f v;
+    if constexpr (GLU) v = w8_glu(sum[0], sum[1], sw[0], sw[1], sx);
+    else v = w8_scaled(sum[0], sw[0], sx);
+    if (a.residual) v += res;
+    w8_store(a, fr, ft * 16 + 4 * (fq & 3), v);
 }
 
 // Sums of NB tiles of 16 weight rows and 16 MB tokens in LDS, [MB][NB][lane] fours as a
@@ -589,7 +612,10 @@ hipError_t launch_linear_w8(hipStream_t s, const W8Args& args) {
         return hipGetLastError();
     }
     const int per = kW8Waves / p.quant_waves;
-    TL_KLAUNCH(w8_quantize_kernel, dim3((a.m + per - 1) / per), dim3(kW8Threads), 0, s, a, p.quant_waves);
+    const dim3 rows((a.m + per - 1) / per), threads(kW8Threads);
+    if (a.act == DT_F32) TL_KLAUNCH((w8_quantize_kernel<DT_F32>), rows, threads, 0, s, a, p.quant_waves);
+    else if (a.act == DT_BF16) TL_KLAUNCH((w8_quantize_kernel<DT_BF16>), rows, threads, 0, s, a, p.quant_waves);
+    else TL_KLAUNCH((w8_quantize_kernel<DT_F16>), rows, threads, 0, s, a, p.quant_waves);
     const dim3 grid(p.grid_x, p.grid_y), block(kW8Threads);
     using std::integral_constant;
     if (p.kind == W8_SPLIT) {

@@ -354,7 +354,7 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
         const int32_t per = kW8Waves / p.split;
         p.grid_x = (units + per - 1) / per;
         p.grid_y = 1;
-        p.lds = (int64_t)w8_blocks(k) * 64 * m + kW8Waves * (glu ? 2 : 1) * 64 * m;
+        p.lds = (int64_t)w8_blocks(k) * 64 * m + kW8Waves * (glu ? 2 : 1) * 1024;
         return p;
     }
     // wavefronts to a row of x, as few as hold it in registers while there are rows enough

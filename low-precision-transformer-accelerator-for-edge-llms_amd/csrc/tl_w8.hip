@@ -143,6 +143,29 @@ TL_DEV v4f w8_glu(v4i gate, v4i up, v4f sg, v4f su, float sx) {
     return v;
 }
 
+// Steps 0 .. count - 1 of which the first AHEAD have been fetched into sets 0 .. AHEAD - 1:
+// multiply(set, step), fetch(set, step).  No step is fetched behind the last one, and in the
+// loop none under a condition, which would have the compiler wait for all that are on their way.
+template <int AHEAD, typename Multiply, typename Fetch>
+TL_DEV void in_flight(int count, Multiply multiply, Fetch fetch) {
+    int i0 = 0;
+    for (; i0 + 2 * AHEAD <= count; i0 += AHEAD) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            multiply(j, i0 + j);
+            fetch(j, i0 + j + AHEAD);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) {
+        if (i0 + j < count) multiply(j, i0 + j);
+        if (j + 1 < AHEAD && i0 + j + AHEAD < count) fetch(j, i0 + j + AHEAD);
+    }
+#pragma unroll
+    for (int j = 0; j + 1 < AHEAD; j++)
+        if (i0 + j + AHEAD < count) multiply(j, i0 + j + AHEAD);
+}
+
 // ---------------------------------------------------------------------------
 // Rows of x to INT8 blocks and scales in scratch, `waves` wavefronts to a row.
 // ---------------------------------------------------------------------------
@@ -285,24 +308,20 @@ __global__ __launch_bounds__(kW8Threads, 4) void w8_row_kernel(W8Args a, int spl
 #pragma unroll
     for (int s = 0; s < S; s++) acc[s] = v4i{0, 0, 0, 0};
     const char* xl = lds + (g * m + min(col, m - 1)) * 16;
-    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+    auto multiply = [&](int j, int i) {
+        const v4i xf = *(const v4i*)(xl + (int64_t)(part + i * split) * 64 * m);
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) {
-            if (i0 + j < count) {
-                const v4i xf = *(const v4i*)(xl + (int64_t)(part + (i0 + j) * split) * 64 * m);
+        for (int s = 0; s < S; s++) acc[s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][s], xf, acc[s], 0, 0, 0);
+    };
+    auto fetch = [&](int j, int i) {
 #pragma unroll
-                for (int s = 0; s < S; s++) acc[s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][s], xf, acc[s], 0, 0, 0);
-            }
-#pragma unroll
-            for (int s = 0; s < S; s++)
-                wf[j][s] = __builtin_nontemporal_load((const v4i*)(w[s] + (int64_t)min(i0 + j + AHEAD, last) * split * 1024));
-        }
-    }
-    // parts of a tile meet in LDS: [wave][s][4 g][row] fours
+        for (int s = 0; s < S; s++) wf[j][s] = __builtin_nontemporal_load((const v4i*)(w[s] + (int64_t)i * split * 1024));
+    };
+    in_flight<AHEAD>(count, multiply, fetch);
+    // parts of a tile meet in LDS: [wave][s][4 g][16 columns] fours
     char* red = lds + (int64_t)blocks * 64 * m;
-    if (col < m)
 #pragma unroll
-        for (int s = 0; s < S; s++) *(v4i*)(red + (((wave * S + s) * 4 + g) * m + col) * 16) = acc[s];
+    for (int s = 0; s < S; s++) *(v4i*)(red + (wave * S + s) * 1024 + lane * 16) = acc[s];
     __syncthreads();
     if (!finishes) return;
     v4i sum[S];
@@ -310,7 +329,7 @@ __global__ __launch_bounds__(kW8Threads, 4) void w8_row_kernel(W8Args a, int spl
     for (int s = 0; s < S; s++) {
         sum[s] = v4i{0, 0, 0, 0};
         for (int p = 0; p < split; p++)
-            sum[s] += *(const v4i*)(red + (((((fq >> 2) * split + p) * S + s) * 4 + (fq & 3)) * m + fr) * 16);
+            sum[s] += *(const v4i*)(red + (((fq >> 2) * split + p) * S + s) * 1024 + ((fq & 3) * 16 + fr) * 16);
     }
     unsigned mr = most[0];
 #pragma unroll
@@ -353,7 +372,7 @@ TL_DEV void w8_finish(const W8Args& a, const char* sums, int tile0, int m0, int 
 // ---------------------------------------------------------------------------
 template <int NT, int MT, bool GLU>
 __global__ __launch_bounds__(kW8Threads, NT * MT > 8 ? 2 : 4) void w8_split_kernel(W8Args a) {
-    constexpr int AHEAD = 8 / (NT + MT) > 2 ? 8 / (NT + MT) : 2;
+    constexpr int AHEAD = 4;
     __shared__ __align__(16) int sums[NT * MT * 256];
     const int lane = lane_id(), wave = wave_id();
     const int blocks = w8_blocks(a.k), tiles = w8_tiles(a.n, a.glu), mbs = (a.m + 15) >> 4;
@@ -383,19 +402,15 @@ __global__ __launch_bounds__(kW8Threads, NT * MT > 8 ? 2 : 4) void w8_split_kern
 #pragma unroll
         for (int j = 0; j < MT; j++) acc[i][j] = v4i{0, 0, 0, 0};
     __syncthreads();
-    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+    in_flight<AHEAD>(
+        count,
+        [&](int s, int) {
 #pragma unroll
-        for (int s = 0; s < AHEAD; s++) {
-            if (i0 + s < count) {
+            for (int i = 0; i < NT; i++)
 #pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int j = 0; j < MT; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s][i], xf[s][j], acc[i][j], 0, 0, 0);
-            }
-            fetch(s, i0 + s + AHEAD);
-        }
-    }
+                for (int j = 0; j < MT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s][i], xf[s][j], acc[i][j], 0, 0, 0);
+        },
+        fetch);
     if (count > 0) {
 #pragma unroll
         for (int i = 0; i < NT; i++)

@@ -31,7 +31,7 @@ static void one(int m, int n, int k, bool glu) {
         CHECK(p.split == 1 || p.split == 2 || p.split == 4 || p.split == 8);
         const int per = kW8Waves / p.split, units = (n + 15) / 16;
         CHECK((int64_t)p.grid_x * per >= units && (int64_t)(p.grid_x - 1) * per < units);
-        CHECK(p.lds >= (int64_t)blocks * 64 * m + kW8Waves * (glu ? 2 : 1) * 64 * m);
+        CHECK(p.lds >= (int64_t)blocks * 64 * m + kW8Waves * (glu ? 2 : 1) * 1024);
         // the threads hold every unit of every row
         CHECK((int64_t)w8_slots(1, k) * kW8Threads >= blocks * 8);
         return;

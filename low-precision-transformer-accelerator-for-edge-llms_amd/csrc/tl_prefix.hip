@@ -26,7 +26,14 @@ namespace {
 // Precision: q enters in QP 16-bit parts and the probabilities in PP, as many as it takes:
 // of 16-bit rows q is exact in one (float16 holds a bfloat16 scaled to its row); float32 rows
 // take two float16 parts (within 2^-23) or three bfloat16 ones (whole).  Probabilities of 16-bit rows take
-// two parts, as one bfloat16 or float16 rounding of each would weigh as much as the result's own.
+// two parts, as one bfloat16 or float16 rounding of each would weigh as much as the result's
+// own (64 rows over 32768 bfloat16 keys: 95 us and an error of 0.0017 of the result, which is
+// that rounding; with one part 85 us and 0.0023).
+//
+// What bounds it: a short prefix the chain page, keys, products, parts (4 rows over 500 INT8
+// keys 8.3 us and 3.8 of the join); a long one the products and the exponentials, neither of which hides
+// behind the other well (64 rows over 131072 bfloat16 keys of 8 heads of 128: per 64 keys and 32 columns
+// of a wavefront 1536 cycles of products, some 1900 of vector instructions, 4200 in all).
 // ---------------------------------------------------------------------------
 constexpr int kPrefixThreads = 256;
 constexpr float kPrefixSlack = 4.0f;

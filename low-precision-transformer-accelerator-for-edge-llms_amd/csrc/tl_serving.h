@@ -103,15 +103,22 @@ struct PrefixPlan {
     int32_t splits;
     int32_t grid;
 };
-constexpr int32_t kPrefixSplitKeys = 256;   // a split's keys, at least
-constexpr int32_t kPrefixWorkgroups = 512;
+// Two workgroups to a CU where each still has 2048 keys (64 rows over 131072 keys of 8 heads
+// of 128 259 us, one to a CU 311), else one, which leaves half the parts (8 rows over 16000
+// keys of 8 heads of 64 16.3 us and 20.2), each of one or four tiles' keys at least (4 rows over
+// 500 keys 11.6 us, with 256 keys each 12.4; 32 rows over 1536 17.1, with 128 18.1).
+constexpr int32_t kPrefixWorkgroups = 256;
+constexpr int64_t kPrefixManyKeys = 2048;
+TL_HD inline int32_t prefix_split_keys(int32_t qw) { return qw == 1 ? 128 : 256; }
 inline PrefixPlan prefix_plan(int32_t rows, int32_t n_heads, int32_t n_kv, int32_t len) {
     const int64_t columns = (int64_t)rows * (n_heads / n_kv);
     PrefixPlan p;
     p.qw = columns <= 64 ? 1 : 4;
     p.qblocks = (int32_t)((columns + 32 * p.qw - 1) / (32 * p.qw));
     const int64_t units = (int64_t)p.qblocks * n_kv;
-    const int64_t most = (len + kPrefixSplitKeys - 1) / kPrefixSplitKeys, want = (kPrefixWorkgroups + units - 1) / units;
+    const int32_t least = prefix_split_keys(p.qw);
+    const int64_t most = ((int64_t)len + least - 1) / least, all = (int64_t)len * units >= 2 * kPrefixWorkgroups * kPrefixManyKeys ? 2 * kPrefixWorkgroups : kPrefixWorkgroups,
+                  want = (all + units - 1) / units;
     p.splits = (int32_t)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
     p.grid = (int32_t)(units * p.splits);

@@ -327,7 +327,8 @@ int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, in
  * that are not used.  The shared keys are read once for all rows and multiplied as a
  * matrix; what is said of tl_paged_attention holds, but that probabilities of 16-bit rows
  * enter the products over the prefix in two 16-bit parts.  A row before the prefix's
- * last position attends the prefix's keys up to its own.  prefix_len 0: tl_paged_attention. */
+ * last position attends the prefix's keys up to its own.  A page of the prefix out of range
+ * is a fault whichever rows attend it.  prefix_len 0: tl_paged_attention. */
 int32_t tl_paged_attention_shared(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride,
                                   int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
                                   const int32_t *row_pos, int32_t prefix_seq, int32_t prefix_len, float scale,

@@ -171,6 +171,8 @@ class PagedCache:
     def _scratch_bytes(self, rows: int, n_heads: int, prefix_len: int = 0) -> int:
         got = self._scratch.get((rows, n_heads, prefix_len))
         if got is None:
+            if len(self._scratch) > 4096:   # prefixes of ever new lengths
+                self._scratch.clear()
             n = C.c_int64()
             if prefix_len:
                 self.rt.check(self.rt.lib.tl_paged_attention_shared_scratch(self.rt.h, self._desc, rows, n_heads, prefix_len,
@@ -218,6 +220,8 @@ class PagedCache:
             if out.shape[0] != rows:
                 raise _bad("out must have a row for each of qkv's")
         if norm is not None:
+            if len(norm) != 2:
+                raise _bad("norm must be the gains of q and of k")
             q_gain, k_gain = self._gain("the q gains", norm[0]), self._gain("the k gains", norm[1])
             if not 0.0 <= eps <= 1e30:
                 raise _bad("eps must be a number from 0 on")

@@ -168,7 +168,7 @@ def test_completing_form_graph_and_refusals(serving):
         assert torch.equal(c.append(x, seq, pos, norm=gains), replayed[0]) and torch.equal(c.k, replayed[1])
     c.check()
     for bad in ((gains[0].double(), None), (None, gains[0][:32]), (gains[0].cpu(), None), (gains[0].expand(1, 64), None),
-                (torch.zeros(128, device="cuda")[::2], None), (torch.zeros(65, device="cuda")[1:], None)):
+                (torch.zeros(128, device="cuda")[::2], None), (torch.zeros(65, device="cuda")[1:], None), (gains[0],), (*gains, None)):
         with pytest.raises(ValueError):
             c.append(x, seq, pos, norm=bad)
     for eps in (-1.0, float("nan"), float("inf")):

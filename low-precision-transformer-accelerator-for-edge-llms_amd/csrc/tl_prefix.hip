@@ -225,15 +225,22 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
         for (int j = 0; j < P::KN; j++) k_page[j] = pages[(min(key0 + 8 * k_octet(j), last8) >> geo.page_shift) + zero];
         v_page = pages[min(key0 + 8 * v_octet, last8) >> geo.page_shift];
     };
+    uint32_t k_off[P::KN];
+#pragma unroll
+    for (int j = 0; j < P::KN; j++) {
+        const int i = j * P::T + tid;
+        k_off[j] = (uint32_t)((i / P::UK % 8) * HD + i % P::UK * 8) * P::ES;
+    }
     auto in_pool = [&](int32_t page) { return (unsigned)page < (unsigned)geo.n_pages ? page : 0; };
     auto fetch = [&](int step) {
         const int key0 = (step * P::KG + group) * P::KT;
         // rows behind the last key are read where its eight are
 #pragma unroll
         for (int j = 0; j < P::KN; j++) {
-            const int i = j * P::T + tid, key = i / P::UK, u = i % P::UK;
-            const int k = (min(key0 + 8 * k_octet(j), last8) & page_mask) + (key & 7);
-            kr[j].load(kbase + in_pool(__builtin_amdgcn_readfirstlane(k_page[j])) * page_bytes + (k * HD + 8 * u) * P::ES);
+            // a base of the wavefront's and a place in its eight rows
+            const char* eight = kbase + in_pool(__builtin_amdgcn_readfirstlane(k_page[j])) * page_bytes +
+                                (min(key0 + 8 * k_octet(j), last8) & page_mask) * (HD * P::ES);
+            kr[j].load(eight + k_off[j]);
         }
         const char* v = vbase + in_pool(v_page) * page_bytes + ((min(key0 + 8 * v_octet, last8) & page_mask) * HD + v_d) * P::ES;
 #pragma unroll

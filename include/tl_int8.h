@@ -353,9 +353,9 @@ int32_t tl_pack_w8(tl_handle *h, const int8_t *q, const float *scales, const int
  * type act (TL_F32, TL_BF16, TL_F16); x8 and sx are x quantized per row as GI:36-42 does, in
  * float32: sx = max|x| / 127 (1 where that is 0), x8 = clip(rne(x / sx), +-127).  Sums are exact.
  * gated: y = silu(gate) up, silu(g) = g / (1 + e^-g) (-0 below -80), no residual (GI:212).  An infinity or NaN in
- * a row of x makes its whole row of y NaN.  Rows of x, residual and y may start anywhere
- * (16-byte aligned ones are read and written faster), strides in elements; residual may be
- * NULL or y, x and y must not overlap.  m from 0 to 2^17. */
+ * a row of x makes its whole row of y NaN.  Rows of x, residual and y may start
+ * anywhere their type may, strides in elements; residual may be NULL or y, x and y must not
+ * overlap.  m from 0 to 2^17. */
 int32_t tl_linear_w8(tl_handle *h, const void *x, int64_t x_stride, int32_t act, int32_t m, const void *packed,
                      int32_t gated, int32_t n, int32_t k, const void *residual, int64_t res_stride, void *y,
                      int64_t y_stride);

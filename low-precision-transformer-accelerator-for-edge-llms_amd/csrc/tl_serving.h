@@ -519,7 +519,6 @@ struct W8Args {
     int32_t m, n, k;
     const void* packed;
     bool glu;                  // packed holds gate and up: y = silu(gate) up
-    bool x_aligned, y_aligned; // set by the launch: rows may be read 16 bytes, written 4 values at once
     const void* residual;      // [m][n] of act, stride res_stride, or null
     int64_t res_stride;
     void* y;                   // [m][n] of act, stride y_stride

@@ -19,6 +19,11 @@
 namespace tl {
 namespace {
 
+// Rows may start anywhere their type may: wide loads and stores need no more than that of
+// the address.
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int v2i_any __attribute__((ext_vector_type(2), aligned(2)));
+
 // Eight columns of a row of x, as they lie in memory; zeros behind column k.
 struct Unit {
     v4i raw[2];
@@ -28,12 +33,12 @@ struct Unit {
         const int left = a.k - 8 * u;
         if (left <= 0) return;
         const int64_t at = row * a.x_stride + 8 * (int64_t)u;
-        if (a.x_aligned && left >= 8) {
+        if (left >= 8) {
             if (a.act == DT_F32) {
-                raw[0] = *(const v4i*)((const float*)a.x + at);
-                raw[1] = *(const v4i*)((const float*)a.x + at + 4);
+                raw[0] = *(const v4i_any*)((const float*)a.x + at);
+                raw[1] = *(const v4i_any*)((const float*)a.x + at + 4);
             } else {
-                raw[0] = *(const v4i*)((const uint16_t*)a.x + at);
+                raw[0] = *(const v4i_any*)((const uint16_t*)a.x + at);
             }
             return;
         }
@@ -103,7 +108,10 @@ TL_DEV float glu(float g, float u) {
 // four neighbours of a row of the residual from column n on, zeros behind the last column
 TL_DEV v4f w8_residual(const W8Args& a, int64_t m, int n) {
     const int64_t at = m * a.res_stride + n;
-    if (a.y_aligned && n + 4 <= a.n) return load4(a.residual, at, a.act);
+    if (n + 4 <= a.n) {
+        if (a.act == DT_F32) return __builtin_bit_cast(v4f, (v4i)*(const v4i_any*)((const float*)a.residual + at));
+        return unpack4(*(const v2i_any*)((const uint16_t*)a.residual + at), a.act);
+    }
     v4f v = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -113,8 +121,14 @@ TL_DEV v4f w8_residual(const W8Args& a, int64_t m, int n) {
 // and of y
 TL_DEV void w8_store(const W8Args& a, int64_t m, int n, v4f v) {
     const int64_t at = m * a.y_stride + n;
-    if (a.y_aligned && n + 4 <= a.n) {
-        store4(a.y, at, a.act, v);
+    if (n + 4 <= a.n) {
+        if (a.act == DT_F32) {
+            *(v4i_any*)((float*)a.y + at) = __builtin_bit_cast(v4i, v);
+            return;
+        }
+        v2i w;
+        store4(&w, 0, a.act, v);
+        *(v2i_any*)((uint16_t*)a.y + at) = w;
         return;
     }
 #pragma unroll
@@ -602,23 +616,22 @@ __global__ __launch_bounds__(256) void pack_w8_kernel(const int8_t* q, const flo
         const int c = (int)(b - tile * blocks) * 64 + 16 * (lane >> 4);
         const int64_t row = (two == 2 ? tile >> 1 : tile) * 16 + (lane & 15);
         const int8_t* from = two == 2 && (tile & 1) ? q2 : q;
-        unsigned v[4] = {0, 0, 0, 0};
-        if (row < n)
+        typedef int v4i_bytes __attribute__((ext_vector_type(4), aligned(1)));
+        v4i v = {0, 0, 0, 0};
+        if (row < n && c + 16 <= k) {
+            v = *(const v4i_bytes*)(from + row * k + c);
+        } else if (row < n) {
             for (int j = 0; j < 16; j++)
-                if (c + j < k) v[j >> 2] |= (unsigned)(uint8_t)from[row * k + c + j] << (8 * (j & 3));
-        *(v4i*)(packed + i * 16) = v4i{(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+                if (c + j < k) v[j >> 2] |= (int)((unsigned)(uint8_t)from[row * k + c + j] << (8 * (j & 3)));
+        }
+        *(v4i*)(packed + i * 16) = v;
     }
 }
 
 }  // namespace
 
-hipError_t launch_linear_w8(hipStream_t s, const W8Args& args) {
-    if (args.m <= 0 || args.n <= 0) return hipSuccess;
-    W8Args a = args;
-    const int es = a.act == DT_F32 ? 4 : 2;
-    a.x_aligned = (uintptr_t)a.x % 16 == 0 && a.x_stride * es % 16 == 0;
-    a.y_aligned = (uintptr_t)a.y % (4 * es) == 0 && a.y_stride % 4 == 0 &&
-                  (!a.residual || ((uintptr_t)a.residual % (4 * es) == 0 && a.res_stride % 4 == 0));
+hipError_t launch_linear_w8(hipStream_t s, const W8Args& a) {
+    if (a.m <= 0 || a.n <= 0) return hipSuccess;
     const W8Plan p = w8_plan(a.m, a.n, a.k, a.glu);
     if (p.kind == W8_ROW) {
         const dim3 grid(p.grid_x), block(kW8Threads);

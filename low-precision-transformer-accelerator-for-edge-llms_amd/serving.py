@@ -10,9 +10,9 @@ can be captured into a ``torch.cuda.CUDAGraph`` (but the first on a device).  Sc
 memory is torch's, kept for each stream, and a captured graph has its own, so calls
 on different streams and graphs share none; threads may call at the same time.  A
 captured call joins the parts of a long row in another order than a queued one does,
-so attention may differ between them in the last place.  A ``PagedCache``, ``W4Linear`` or ``W8Linear``
-is kept until the calls made with it on other streams than the one it was made on are
-done, and as long as a graph that holds such calls.  Tensors are CUDA tensors of one
+so attention may differ between them in the last place.  A ``PagedCache``, ``W4Linear``,
+``W8Linear`` or ``W8GatedLinear`` is kept until the calls made with it on other streams than
+the one it was made on are done, and as long as a graph that holds such calls.  Tensors are CUDA tensors of one
 device; float types are float32, bfloat16 and float16.  Nothing here is differentiable:
 results carry no gradient.
 

@@ -589,7 +589,7 @@ __global__ __launch_bounds__(64 * WN * WM, 1) void w8_tile_kernel(W8Args a, W8Gr
         __builtin_amdgcn_wave_barrier();
         const int m0 = (mb0 + wm * TM + j) * 16;
 #pragma unroll 2
-        for (int r = lane / Q; r < 16; r += STEP) {
+        for (int r = lane < Q * STEP ? lane / Q : 16; r < 16; r += STEP) {   // (7 tiles: lanes 56 on would write again)
             if (m0 + r >= a.m || t >= tiles) continue;
             const float sx = row_scales[j * 16 + r];
             const char* from = mine + r * ROW + (q >> 2) * (GLU ? 128 : 64) + (q & 3) * 16;

@@ -204,6 +204,24 @@ def test_strides(serving, act, m, n, k):
         assert torch.equal(y, lin(x.contiguous(), residual=plain))
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(2, 40, 64), (20, 100, 200), (200, 130, 70),       # registers, K split
+                                   (513, 4000, 64), (1000, 14000, 40), (1000, 14001, 130),   # tiles of 8 x 8, 14 x 16
+                                   (1100, 9000, 64), (256, 65536, 40)])               # 16 x 14, 16 x 16
+def test_out_is_residual(serving, act, m, n, k):
+    """Every result takes its residual once, where it is written over it too."""
+    g = torch.Generator().manual_seed(m + n)
+    w, s = weights(g, n, k)
+    lin = serving.W8Linear(w.cuda(), s.cuda())
+    x = torch.randn(m, k, generator=g).to(DT[act]).cuda()
+    r = torch.randn(m, n, generator=g).to(DT[act]).cuda()
+    want = lin(x, residual=r)
+    for _ in range(2):
+        y = r.clone()
+        assert lin(x, residual=y, out=y) is y
+        assert torch.equal(y, want)
+
+
 def test_packing_of_few_columns_and_quantizer(serving):
     g = torch.Generator().manual_seed(3)
     w = torch.randn(50, 70, generator=g)

@@ -149,7 +149,7 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
 
     // columns of this lane: query head and row
     int64_t q_at[2];
-    int rows_of[2], head_of[2];
+    int rows_of[2], head_of[2], pos_of[2];
     const int columns = a.rows * rep;   // (below 2^30)
 #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
@@ -157,6 +157,7 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
         rows_of[ct] = (int)((unsigned)c / (unsigned)rep);
         head_of[ct] = kvh * rep + c - rows_of[ct] * rep;
         q_at[ct] = (int64_t)rows_of[ct] * a.q_stride + (int64_t)head_of[ct] * HD;
+        pos_of[ct] = a.row_pos[rows_of[ct]];
     }
     v4i qf[QP][2][P::KC];
     float cs[2];
@@ -187,7 +188,10 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
             up = __builtin_amdgcn_ldexpf(up, e);
             s = __builtin_amdgcn_ldexpf(s, -e);
         }
-        if (s == 0.0f) {   // all scores alike: products of 0, so that a masked one stays minus infinity
+        // All scores alike: products of 0, so that a masked one stays minus infinity.  So are those
+        // of rows that take nothing from here, whose q may meanwhile be written over by their
+        // results: when the other columns' sums are scaled anew must not depend on that.
+        if (s == 0.0f || !shared_adds(len, pos_of[ct])) {
             up = 0.0f;
             s = 1.0f;
         }

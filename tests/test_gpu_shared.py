@@ -181,6 +181,24 @@ def test_rows_of_every_kind(serving, rows, cache):
         check(got, want[short], tol[short])
 
 
+@pytest.mark.parametrize("act,cache", [("f32", "i8"), ("bf16", "bf16"), ("f32", "f16")])
+def test_in_place_and_apart_are_the_same(serving, act, cache):
+    """Rows shorter than the prefix, whose results may lie where the prefix's workgroups read q, change nothing in the
+    other rows' last bits."""
+    kv, hd, page, plen, b = 2, 64, 16, 3000, 60
+    built = shared(cache, kv, hd, page, plen, [i % 40 + 1 for i in range(b)], seed=9)
+    c = make(serving, built)
+    seq = torch.arange(1, b + 1, dtype=torch.int32, device="cuda")
+    pos = torch.tensor([i * 7 % 90 if i % 2 else plen + i % 40 for i in range(b)], dtype=torch.int32, device="cuda")
+    q = (3 * torch.randn(b, 8 * kv * hd, generator=built[4])).to(DT[act]).cuda()
+    want = c.attend_shared(q, seq, pos, 0, plen)
+    for _ in range(20):
+        out = q.clone()
+        c.attend_shared(out, seq, pos, 0, plen, out=out)
+        assert torch.equal(out, want)
+    c.check()
+
+
 def test_equals_attend(serving):
     """Where the sequences' tables hold the prompt's pages, as a server's do, the result is attend's."""
     plen, page, kv, heads, b = 1000, 16, 2, 16, 24

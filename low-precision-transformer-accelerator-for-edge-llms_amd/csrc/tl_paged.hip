@@ -83,9 +83,20 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
                 double sum = 0.0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) sum += (double)x1[j] * x1[j] + (double)x2[j] * x2[j];
-                const float f = (float)(1.0 / __builtin_sqrt(head_sum(sum, quads) / hd + a.eps));
-                x1 = x1 * f * g1;
-                x2 = x2 * f * g2;
+                const double wide = 1.0 / __builtin_sqrt(head_sum(sum, quads) / hd + a.eps);
+                const float f = (float)wide;
+                if (f >= 0x1p-126f && f < __builtin_inff()) {
+                    x1 *= f;
+                    x2 *= f;
+                } else {   // a factor that float32 does not hold whole: heads near either end of its range
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x1[j] = (float)(x1[j] * wide);
+                        x2[j] = (float)(x2[j] * wide);
+                    }
+                }
+                x1 *= g1;
+                x2 *= g2;
             }
         }
         const float* c = a.cos + (int64_t)pos * hd + d;

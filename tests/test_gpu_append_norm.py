@@ -136,6 +136,25 @@ def test_zeros_and_extremes(serving):
     assert torch.allclose(q[0, 128:192].double().pow(2).mean(), torch.tensor(1.0, dtype=torch.float64, device="cuda"), rtol=1e-5)
 
 
+@pytest.mark.parametrize("act,size", [("f32", 2e38), ("bf16", 3e38), ("f32", 1e-40), ("bf16", 1e-39), ("f32", 1e-44)])
+def test_ends_of_the_range(serving, act, size):
+    """Heads whose factor leaves float32's normal numbers, without eps."""
+    cos, sin = tables(4, 64)
+    k = torch.zeros(2, 1, 16, 64, dtype=torch.float16, device="cuda")
+    c = serving.PagedCache(k, k.clone(), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), rope=(cos.cuda(), sin.cuda()))
+    x = ((torch.rand(1, 4 * 64, generator=torch.Generator().manual_seed(1)) * 1.0 + 0.1) / 1.1 * size).to(DT[act])
+    gain = torch.ones(64, device="cuda")
+    ids = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2)]   # position 0: no rotation
+    q = c.append(x.cuda(), *ids, norm=(gain, gain), eps=0.0)
+    c.check()
+    xd = x.double()[:, :128].view(2, 64)
+    want = (xd / xd.pow(2).mean(dim=1, keepdim=True).sqrt()).view(1, 128)
+    # the factor and its product round to float32, then the result to its type
+    tol = 2.01 * 2.0 ** -24 * want.abs()
+    tol = tol + STEP[act] * (want.abs() + tol)
+    assert ((q.cpu().double() - want).abs() <= tol).all()
+
+
 def test_completing_form_graph_and_refusals(serving):
     import ctypes as C
     g = torch.Generator().manual_seed(4)

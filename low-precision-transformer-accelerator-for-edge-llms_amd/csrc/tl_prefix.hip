@@ -147,9 +147,10 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
     const char* kbase = (const char*)a.c.k + head_bytes;
     const char* vbase = (const char*)a.c.v + head_bytes;
 
-    // columns of this lane: query head and row
+    // columns of this lane: query head and row (rows that take nothing from here among them, whose q
+    // may meanwhile be written over by their results)
     int64_t q_at[2];
-    int rows_of[2], head_of[2], pos_of[2];
+    int rows_of[2], head_of[2];
     const int columns = a.rows * rep;   // (below 2^30)
 #pragma unroll
     for (int ct = 0; ct < 2; ct++) {
@@ -157,7 +158,6 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
         rows_of[ct] = (int)((unsigned)c / (unsigned)rep);
         head_of[ct] = kvh * rep + c - rows_of[ct] * rep;
         q_at[ct] = (int64_t)rows_of[ct] * a.q_stride + (int64_t)head_of[ct] * HD;
-        pos_of[ct] = a.row_pos[rows_of[ct]];
     }
     v4i qf[QP][2][P::KC];
     float cs[2];
@@ -188,10 +188,8 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
             up = __builtin_amdgcn_ldexpf(up, e);
             s = __builtin_amdgcn_ldexpf(s, -e);
         }
-        // All scores alike: products of 0, so that a masked one stays minus infinity.  So are those
-        // of rows that take nothing from here, whose q may meanwhile be written over by their
-        // results: when the other columns' sums are scaled anew must not depend on that.
-        if (s == 0.0f || !shared_adds(len, pos_of[ct])) {
+        // all scores alike: products of 0, so that a masked one stays minus infinity
+        if (s == 0.0f) {
             up = 0.0f;
             s = 1.0f;
         }
@@ -385,12 +383,14 @@ TL_DEV void prefix_run(const PagedAttnArgs& a, const int me, const int workgroup
 #pragma unroll
                 for (int j = 0; j < 8; j++) mt = fmaxf(mt, s[sub][j >> 2][ct][j & 3]);
             mt = pair_max(mt);
-            // sums are scaled anew only where a score leaves them by kPrefixSlack: a fresh maximum,
-            // of which most tiles have one among 16 columns, alone does not
-            if (__builtin_amdgcn_ballot_w64(mt * cs[ct] > m[ct] * cs[ct] + kPrefixSlack) != 0) {
+            // A column's sums are scaled anew only where a score leaves them by kPrefixSlack: a fresh
+            // maximum, of which most tiles have one among 16 columns, alone does not.  The other
+            // columns take a factor of 1: a row's bits do not depend on what stands in the others.
+            const bool leaves = mt * cs[ct] > m[ct] * cs[ct] + kPrefixSlack;
+            if (__builtin_amdgcn_ballot_w64(leaves) != 0) {
                 asm volatile("");
-                const float mn = fmaxf(m[ct], mt);
-                const float al = m[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * cs[ct]);
+                const float mn = leaves ? mt : m[ct];
+                const float al = !leaves ? 1.0f : m[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[ct] - mn) * cs[ct]);
                 m[ct] = mn;
                 l[ct] *= al;
 #pragma unroll

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import threading
 from typing import NamedTuple
 
@@ -259,10 +260,14 @@ class PagedCache:
         row_seq[r] from there on (table entries of row_seq before that are not used).
         Several prompts in a batch: one call each into one ``out``, the other rows' row_seq
         negative.  In a captured graph the prefix is the one it was captured with."""
+        try:
+            prefix_seq, prefix_len = operator.index(prefix_seq), operator.index(prefix_len)
+        except TypeError:
+            raise _bad("the prefix's sequence and length must be whole numbers") from None
         if not 0 <= prefix_len <= self.desc.max_pages * self.desc.page_size or (
                 prefix_len and not 0 <= prefix_seq < self.n_seqs):
             raise _bad("the prefix must lie in the pages of a sequence of the table")
-        return self._attend("attend_shared", q, row_seq, row_pos, int(prefix_seq), int(prefix_len), scale, out)
+        return self._attend("attend_shared", q, row_seq, row_pos, prefix_seq, prefix_len, scale, out)
 
     def _attend(self, what, q, row_seq, row_pos, prefix_seq, prefix_len, scale, out):
         dev, hd = self.device, self.head_dim

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import numbers
 import operator
 import threading
 from typing import NamedTuple
@@ -221,10 +222,12 @@ class PagedCache:
             if out.shape[0] != rows:
                 raise _bad("out must have a row for each of qkv's")
         if norm is not None:
-            if len(norm) != 2:
-                raise _bad("norm must be the gains of q and of k")
-            q_gain, k_gain = self._gain("the q gains", norm[0]), self._gain("the k gains", norm[1])
-            if not 0.0 <= eps <= 1e30:
+            try:
+                q_gain, k_gain = norm
+            except (TypeError, ValueError):
+                raise _bad("norm must be the gains of q and of k") from None
+            q_gain, k_gain = self._gain("the q gains", q_gain), self._gain("the k gains", k_gain)
+            if not isinstance(eps, numbers.Real) or not 0.0 <= eps <= 1e30:
                 raise _bad("eps must be a number from 0 on")
         if rows == 0:
             return out

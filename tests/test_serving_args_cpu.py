@@ -36,3 +36,18 @@ def test_prefixes_that_are():
     for prefix in ((0, -1), (0, 129), (3, 1), (-1, 1), (0, 1 << 70)):
         with pytest.raises(TlValueError, match="pages of a sequence"):
             c.attend_shared(*rows(4), *prefix)
+
+
+def test_norms():
+    c = cache()
+    gain = torch.ones(64)
+    for norm in ((gain, gain), [None, gain], (gain, None), torch.ones(2, 64), (None, None)):
+        for eps in (0, 0.0, 1e-6, np.float32(1e-5), 1e30):
+            assert c.append(*rows(8), norm=norm, eps=eps).shape == (0, 256)
+    for norm in (5, gain, (gain,), (gain, gain, gain), (gain, 1.0), (gain, gain[:32]), (gain.double(), gain), "qk", torch.tensor(1.0),
+                 (torch.ones(128)[::2], gain), {"q": gain, "k": gain}):
+        with pytest.raises(TlValueError):
+            c.append(*rows(8), norm=norm)
+    for eps in (-1e-9, float("nan"), float("inf"), 2e30, "1e-5", None, torch.tensor(1e-5), 1j):
+        with pytest.raises(TlValueError, match="eps"):
+            c.append(*rows(8), norm=(gain, gain), eps=eps)

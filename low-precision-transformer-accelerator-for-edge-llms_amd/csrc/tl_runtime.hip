@@ -1278,7 +1278,6 @@ int32_t tl_create(const tl_config* cfg, int32_t max_seqs, tl_handle** out) {
     if ((e = init_gemm_pk_kernels())) return bad(e);
     if ((e = init_skinny_kernels())) return bad(e);
     if ((e = init_w4_kernels())) return bad(e);
-    if ((e = init_w8_kernels())) return bad(e);
     if ((e = init_prefix_kernels())) return bad(e);
     if (const char* env = std::getenv("TL_BATCH_O_FUSE")) h->o_fuse = env[0] != '0';
     if (const char* env = std::getenv("TL_BATCH_KSLICE")) h->batch_kslice = env[0] != '0';

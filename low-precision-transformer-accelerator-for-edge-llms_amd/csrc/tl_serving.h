@@ -298,9 +298,12 @@ inline W4Plan w4_plan(int32_t m, int32_t n, int32_t k, int32_t group) {
 // Scratch of a call (w8_scratch() bytes): the scales of its rows, then their blocks.
 constexpr int32_t kW8Waves = 8, kW8Threads = 64 * kW8Waves;
 constexpr int32_t kW8MaxK = 1 << 17;     // 127 * 128 * 2^17 is below 2^31
-constexpr int64_t kW8Lds = 152 * 1024;   // of a workgroup's 160 KiB
 constexpr int32_t kW8Slots = 4;          // units of 8 columns of x that a thread keeps in registers
 constexpr int32_t kW8Keep = 4;           // and where x is quantized by a kernel of its own
+// LDS of a workgroup of single rows: what any launch may have; their columns and the partial
+// sums of gated weights take half of it at most
+constexpr int64_t kW8Lds = 64 * 1024;
+static_assert(kW8Slots * kW8Threads * 8 + kW8Waves * 2 * 1024 <= kW8Lds, "rows and sums fit");
 
 TL_HD inline int32_t w8_blocks(int32_t k) { return (k + 127) / 128 * 2; }
 TL_HD inline int32_t w8_tiles(int32_t n, bool glu) { return (n + 15) / 16 * (glu ? 2 : 1); }
@@ -529,7 +532,6 @@ hipError_t launch_linear_w8(hipStream_t s, const W8Args& a);
 // q [n][k] and scales [n]; with q2 and scales2, gate and up
 hipError_t launch_pack_w8(hipStream_t s, const int8_t* q, const float* scales, const int8_t* q2, const float* scales2,
                           int32_t n, int32_t k, void* packed);
-hipError_t init_w8_kernels();
 
 // log probabilities, entropy and top alternatives of rows of logits
 struct LogprobsArgs {

@@ -686,11 +686,4 @@ hipError_t launch_pack_w8(hipStream_t s, const int8_t* q, const float* scales, c
     return hipGetLastError();
 }
 
-hipError_t init_w8_kernels() {
-    hipError_t e = hipSuccess;
-    for (const void* f : {(const void*)w8_row_kernel<false>, (const void*)w8_row_kernel<true>})
-        if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kW8Lds);
-    return e;
-}
-
 }  // namespace tl

@@ -170,7 +170,9 @@ int32_t tl_gemm_i8(tl_handle *h, const int8_t *a, const int8_t *w, int32_t m, in
 int32_t tl_gemm_i8_noalloc(tl_handle *h, const int8_t *a, const int8_t *w, int32_t m, int32_t n, int32_t k,
                            int32_t *c);
 /* GEMM + GI:45-46 dequantization per row/channel, optional residual (GI:266):
- * y[m][n] = residual[m][n] + f32(acc) * f32(a_scales[m] * w_scales[n]). */
+ * y[m][n] = residual[m][n] + f32(acc) * f32(a_scales[m] * w_scales[n]).  Bit for bit the
+ * golden's, of rows quantized before, complete when it returns; tl_linear_w8 quantizes rows
+ * of any float type on the way, from weights packed once, and can be queued and captured. */
 int32_t tl_gemm_i8_dequant(tl_handle *h, const int8_t *a, const double *a_scales, const int8_t *w,
                            const float *w_scales, int32_t m, int32_t n, int32_t k,
                            const float *residual, float *y);
@@ -285,7 +287,8 @@ int32_t tl_paged_append_async(tl_handle *h, void *stream, const tl_paged_cache *
 
 /* tl_paged_append with q and k of each head normed before they are rotated: x f gain, f =
  * 1 / sqrt(mean of the head's x^2 + eps) in 64 bits and rounded once, both products rounded to
- * float32; q_gain, k_gain [head_dim] float32 (dev, 16-byte aligned; NULL: that one is not
+ * float32.  A factor that is no normal float32 number (heads near either end of the range)
+ * is not rounded: x f is a 64-bit product, rounded once.  q_gain, k_gain [head_dim] float32 (dev, 16-byte aligned; NULL: that one is not
  * normed), eps from 0 on.  Values stay as they are. */
 int32_t tl_paged_append_norm(tl_handle *h, const tl_paged_cache *cache, const void *qkv, int64_t qkv_stride,
                              int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
@@ -328,7 +331,13 @@ int32_t tl_paged_attention_scratch(tl_handle *h, const tl_paged_cache *cache, in
  * matrix; what is said of tl_paged_attention holds, but that probabilities of 16-bit rows
  * enter the products over the prefix in two 16-bit parts.  A row before the prefix's
  * last position attends the prefix's keys up to its own.  A page of the prefix out of range
- * is a fault whichever rows attend it.  prefix_len 0: tl_paged_attention. */
+ * is a fault whichever rows attend it.  prefix_len 0: tl_paged_attention.
+ * What it costs: the prefix's products for every row given, padded ones and ones that end
+ * before the prefix does among them, and a second kernel.  Rows of several prefixes are
+ * better given prefix by prefix, each call its own rows, than all to every call with the
+ * others padded.  Over a short prefix tl_paged_attention, on tables that hold its pages, is as
+ * fast or faster (up to some 1500 positions with heads of 64, or behind hundreds of a row's
+ * own); from some 4000 on this one is for four rows or more. */
 int32_t tl_paged_attention_shared(tl_handle *h, const tl_paged_cache *cache, const void *q, int64_t q_stride,
                                   int32_t act, int32_t rows, int32_t n_heads, const int32_t *row_seq,
                                   const int32_t *row_pos, int32_t prefix_seq, int32_t prefix_len, float scale,
@@ -342,7 +351,8 @@ int32_t tl_paged_attention_shared_scratch(tl_handle *h, const tl_paged_cache *ca
                                           int32_t prefix_len, int64_t *bytes);
 
 /* Projections with 8-bit weights q [n][k] and float32 scales [n] (tl_quantize_weight_rows
- * makes them), in the order the kernels read, packed (dev, 16-byte aligned) once per weight
+ * makes them; the product of the dense path, whose rows are quantized before, is
+ * tl_gemm_i8_dequant), in the order the kernels read, packed (dev, 16-byte aligned) once per weight
  * matrix into tl_w8_packed_bytes.  With up_q and up_scales (else NULL) the pair is a gate
  * and an up projection of one shape, packed with gated = 1.  Any n and k: k at most 2^17, n at
  * most 2^24, n k below 2^35. */

@@ -16,7 +16,8 @@ namespace {
 // d + 3 and their partners half a head on), or eight values of v.  Nothing is
 // read twice from memory; the row's cos and sin are shared by its heads through
 // the cache.  With gains, q and k of each head are normed first: f = 1 / sqrt(mean x^2 +
-// eps) in 64 bits, rounded once, so that neither the order of the sum nor a square root's
+// eps) in 64 bits, rounded once (or, where float32 holds it as no normal number, not
+// rounded), so that neither the order of the sum nor a square root's
 // last bit shows in an INT8 row; then (x f) gain, each product rounded to float32.  A head's
 // pairs lie in 8 or 16 neighbouring lanes, which add up their squares with DPP moves.  What bounds it: from one row to some hundreds the chain of loads and
 // the launch (3.5 us for 1 row as for 61); 2048 rows of 32 + 2 x 8 heads of 128 in

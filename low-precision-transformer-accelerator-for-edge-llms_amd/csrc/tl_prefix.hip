@@ -31,9 +31,12 @@ namespace {
 // that rounding; with one part 85 us and 0.0023).
 //
 // What bounds it: a short prefix the chain page, keys, products, parts (4 rows over 500 INT8
-// keys 8.3 us and 3.8 of the join); a long one the products and the exponentials, neither of which hides
+// keys 7.1 us and 3.7 of the join); a long one the products and the exponentials, neither of which hides
 // behind the other well (64 rows over 131072 bfloat16 keys of 8 heads of 128: per 64 keys and 32 columns
 // of a wavefront 1536 cycles of products, some 1900 of vector instructions, 4200 in all).
+// 64 rows over 32768 keys and 350 of their own, 32 / 8 heads of 128: bfloat16 over bfloat16 94 us,
+// over INT8 90, float16 95; float32 over INT8 98, float16 105 (15 registers spilled), bfloat16
+// 147 (one wavefront per SIMD).
 // ---------------------------------------------------------------------------
 constexpr int kPrefixThreads = 256;
 constexpr float kPrefixSlack = 4.0f;

@@ -355,8 +355,8 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
         p.kind = W8_ROW;
         const int32_t units = (n + 15) / 16;
         // Wavefronts to a tile: enough for four on each CU, and for eight where each still has 8
-        // blocks (one row by 14336 x 4096: 448 workgroups 12.6 us in a graph, 224 13.4; by 32000 x
-        // 2048 13.0, 14.5; but by 5632 x 2048, with 4 blocks each, 7.2, and 6.3 with 8).
+        // blocks (one row by 14336 x 4096: 448 workgroups 11.2 us in a graph, 224 12.7; by 32000 x
+        // 2048 12.1, 13.5; but by 5632 x 2048, with 4 blocks each, 7.2, and 6.2 with 8).
         p.split = 1;
         while (p.split < kW8Waves && ((int64_t)units * p.split < 1024 ||
                                       ((int64_t)units * p.split < 2048 && w8_blocks(k) >= 16 * p.split)))
@@ -372,15 +372,18 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
     while (p.quant_waves > 1 && (int64_t)m * p.quant_waves > 4096 && w8_blocks(k) * 8 <= kW8Keep * 64 * (p.quant_waves / 2))
         p.quant_waves /= 2;
     // Without LDS (tiles of nt by mt, K split over a workgroup) while 64 x 64 tiles are at most
-    // 400: 128 rows by 5632 x 2048 take 11.4 us, in the tiled form 18.2, 256 rows 17.6 and 18.9,
-    // 512 rows by 2048 x 5632 20.7 and 33.9; but 384 rows by 5632 x 2048 (528 tiles) 23.8 and
-    // 20.3, 128 rows by 14336 x 4096 (448) 29.9 and 25.8.
+    // 400: 128 rows by 5632 x 2048 take 11.4 us, in the tiled form 17.2, 256 rows 18.1 and 18.2,
+    // 512 rows by 2048 x 5632 19.8 and 32.2; but 384 rows by 5632 x 2048 (528 tiles) 21.7 and
+    // 19.7, 128 rows by 14336 x 4096 (448) 26.8 and 25.6, 48 rows of pairs of them (448) 27.5 and
+    // 27.3, 100 rows (896) 50 and 30.  The rule goes by the tiles alone: up to some 32 rows of
+    // still more channels the tiled form loses (8 rows of those pairs 24.3, without LDS 22.2, 32
+    // rows 26.1, 23.2; by 32000 x 2048 17.6, 14.8 and 19.0, 15.8, but 64 rows 20.9, 22.0).
     auto wgs = [&](int32_t nt, int32_t mt) { return (int64_t)((tiles + nt - 1) / nt) * ((mbs + mt - 1) / mt); };
     if (wgs(4, 4) <= 400) {
         p.kind = W8_SPLIT;
         // A 4 x 4 workgroup takes as long as 3.5 of the others, and fewer than 200 no less: 32
-        // rows by 14336 x 4096 take 15.5 us as 2 x 2, 22.1 as 2 x 1; 48 rows 22.7 as 2 x 2, 18.5
-        // as 4 x 4; 128 rows by 2048 x 5632 13.5, 12.2, 16.3; 64 by 5632 x 2048 10.7, 10.4, 11.0.
+        // rows by 14336 x 4096 take 14.6 us as 2 x 2, 20.8 as 2 x 1; 48 rows 21.5 as 2 x 2, 16.2
+        // as 4 x 4; 128 rows by 2048 x 5632 12.4, 11.4, 15.8; 64 by 5632 x 2048 10.4, 9.4, 11.0.
         const int64_t one = wgs(2, 1), two = wgs(2, 2), w4 = wgs(4, 4), four = (w4 > 200 ? w4 : 200) * 7 / 2;
         p.mt = one <= two && one <= four ? 1 : two <= four ? 2 : 4;
         p.nt = p.mt == 4 ? 4 : 2;
@@ -390,9 +393,10 @@ inline W8Plan w8_plan(int32_t m, int32_t n, int32_t k, bool glu) {
     }
     // The shape with the least work on the busiest CU, in units of a product of two tiles: a
     // 16 x 16 workgroup at a time on each of 256 CUs, of 8 x 8 two, which read a quarter more
-    // for their products (8192^3: 472 us, 589; 1024 rows by 4096 x 4096, 64 workgroups or 256:
-    // 53, 33).  One side of 14 where that saves a round (2001 rows of 14336 x 4096 pairs: 227
-    // us, 241).
+    // for their products (8192^3: 450 us, 564; 1024 rows by 4096 x 4096, 64 workgroups or 256:
+    // 51, 32).  One side of 14 where rounds of 256 are fuller by it: tokens' (2001 rows of 14336 x
+    // 4096 pairs, 896 workgroups of 16 x 16 or 1008: 232 us, 214) or channels' (4096 rows by 14336
+    // x 4096, 896 or 1024: 219 us, 212).
     p.kind = W8_TILE;
     int64_t best = INT64_MAX;
     for (int32_t i = W8_SHAPES - 1; i >= 0; i--) {

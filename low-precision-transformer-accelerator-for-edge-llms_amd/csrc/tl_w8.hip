@@ -233,9 +233,9 @@ __global__ __launch_bounds__(kW8Threads, 8) void w8_quantize_kernel(W8Args a, in
 // ---------------------------------------------------------------------------
 // Up to four rows whose columns its registers hold: every workgroup quantizes them itself,
 // into LDS.  Rows, first weights, scales and residual are asked for together; what bounds
-// it is that chain (load, maximum, quotients, products, sums: one row by 2048 x 5632 7.3 us in a
-// graph, by 5632 x 2048 6.3, the gated pair 8.6) and then the weights (14336 x 4096: 12.6
-// us, 4.7 TB/s; the pair 22.1, 5.3 TB/s).
+// it is that chain (load, maximum, quotients, products, sums: one row by 2048 x 5632 7.1 us in a
+// graph, by 5632 x 2048 6.2, the gated pair 8.2) and then the weights (two sets in turn, 14336 x
+// 4096: 11.2 us, 5.2 TB/s; the pair 20.3, 5.8 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kRowAhead = 8;   // weight blocks in flight per wavefront
 

@@ -84,3 +84,28 @@ def test_two_prompts_in_place(serving, act, cache):
     c.attend_shared(x, second, pos, b, lens[1], out=x)
     c.check()
     assert torch.equal(x, want) and torch.isfinite(x).all()
+
+
+@pytest.mark.parametrize("plen", [700, 704])
+def test_prompts_by_slices(serving, plen):
+    """Prompts whose rows stand together, one call each on slices of the batch's tensors, give what the padded calls give,
+    but for the order in which sums are split.  The second prompt's own page holds NaN in front of position 700, which its
+    rows attend: they are NaN, and no other row is."""
+    kv, hd, page, b, cut = 2, 64, 16, 23, 5
+    built = shared("f16", kv, hd, page, plen, [plen + i for i in range(b)], seed=8)
+    c = make(serving, built)
+    c.table[b, :plen // page] = c.table[0, :plen // page]
+    wide = torch.randn(b, 4 * kv * hd + 16, generator=built[4]).cuda()
+    q, pos = wide[:, :4 * kv * hd], vector([2 * plen - 1 + i for i in range(b)])
+    seq = vector(list(range(1, b + 1)))
+    prompts = [(slice(0, cut), 0, plen), (slice(cut, b), b, plen + 7)]
+    want, got = torch.zeros(b, 4 * kv * hd, device="cuda"), torch.zeros(b, 4 * kv * hd, device="cuda")
+    for rows, prefix, n in prompts:
+        others = torch.full_like(seq, -1)
+        others[rows] = seq[rows]
+        c.attend_shared(q, others, pos, prefix, n, out=want)
+        c.attend_shared(q[rows], seq[rows], pos[rows], prefix, n, out=got[rows])
+    c.check()
+    whole = b if plen % page == 0 else cut
+    assert (got - want)[:whole].abs().max() < 2e-6 and (want[:whole] != 0).any(1).all()
+    assert torch.isnan(got[whole:]).all() and torch.isnan(want[whole:]).all()
